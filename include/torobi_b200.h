@@ -410,6 +410,73 @@ int tq_cross_entropy_bwd(const void* logits, const int64_t* targets, const float
                          int64_t rows, int64_t vocab, int64_t ld, const float* dloss, float scale,
                          void* dlogits, void* stream);
 
+/* ------------------------------------------------- scores, distillation --- */
+/*
+ * What a scorer and a distilling trainer read off the logits [rows, vocab]
+ * (bf16 or f32: dtype TQ_DTYPE_*; row pitch ld elements, ld >= vocab; any
+ * alignment of the type).  No counterpart in the reference, whose loss node
+ * is the cross-entropy above; sums are f32.  temperature T > 0:
+ * q = softmax(z[r] / T).  A -inf logit has probability 0; a row of nothing
+ * else has no distribution (log probabilities -inf, entropy 0, gradient 0);
+ * a NaN or +inf makes its row's outputs NaN.
+ *
+ * tq_token_logprobs_fwd:
+ *   logprobs[r] = ln q[tokens[r]]; 0 where the token is outside [0, vocab)
+ *                 (a position without one)
+ *   entropy[r]  = -sum_j q[j] ln q[j]
+ *   top_logprobs, top_ids [rows, top]: the top largest logits' ln q and
+ *                 indices, largest first, ties to the lowest index (NaN above
+ *                 everything); top 0 to 128 and at most vocab (and vocab at
+ *                 most 2^20 with f32 or 2^21 with bf16 logits when top > 0);
+ *                 both may be NULL when top is 0
+ *   stats       [rows, 4] f32, 16-byte aligned, what the backward reads; may
+ *               be NULL
+ */
+int tq_token_logprobs_fwd(const void* logits, int dtype, const int64_t* tokens, int64_t rows,
+                          int64_t vocab, int64_t ld, float temperature, int64_t top,
+                          float* logprobs, float* entropy, float* stats, float* top_logprobs,
+                          int64_t* top_ids, void* stream);
+
+/*
+ * Its VJP through logprobs and entropy (dlogprobs, dentropy [rows] f32, NULL
+ * for none), in the logits' type, row pitch ld_out:
+ *   dlogits[r, j] = (dlogprobs[r] ([j == tokens[r]] - q[j])
+ *                    - dentropy[r] q[j] (ln q[j] + entropy[r])) / T
+ * dlogits may be the logits buffer itself (then ld_out == ld).  A row whose
+ * upstream gradients are 0 gets zeros, whatever its logits hold.
+ */
+int tq_token_logprobs_bwd(const void* logits, int dtype, const int64_t* tokens,
+                          const float* stats, int64_t rows, int64_t vocab, int64_t ld,
+                          float temperature, const float* dlogprobs, const float* dentropy,
+                          void* dlogits, int64_t ld_out, void* stream);
+
+/*
+ * Distillation from a teacher's top logits: per row, k alternatives (1 to
+ * 128) with their ids (ids_bits 32 or 64) and logits or log probabilities
+ * (teacher_dtype TQ_DTYPE_*), dense [rows, k]; an id outside [0, vocab) is no
+ * alternative.  p = softmax(teacher_logits[r] / T) over the row's alternatives.
+ *   kl[r] = sum_i p[i] (ln p[i] - ln q[ids[i]]); 0 for a row without any
+ *   ce[r] = ln sum_j exp(z[j]) - z[targets[r]] (temperature 1); 0 where the
+ *           target is outside [0, vocab).  targets and ce: both or neither.
+ * The same id may be given twice: its shares add.  stats as above.
+ */
+int tq_distill_fwd(const void* logits, int dtype, const void* teacher_ids, int ids_bits,
+                   const void* teacher_logits, int teacher_dtype, int64_t k,
+                   const int64_t* targets, int64_t rows, int64_t vocab, int64_t ld,
+                   float temperature, float* kl, float* ce, float* stats, void* stream);
+
+/*
+ * Its VJP with respect to the logits (dkl, dce [rows] f32, NULL for none):
+ *   dlogits[r, j] = dkl[r] / T (q[j] - sum_{i: ids[i] == j} p[i])
+ *                   + dce[r] (softmax(z[r])[j] - [j == targets[r]])
+ * dlogits may be the logits buffer itself (then ld_out == ld).
+ */
+int tq_distill_bwd(const void* logits, int dtype, const void* teacher_ids, int ids_bits,
+                   const void* teacher_logits, int teacher_dtype, int64_t k,
+                   const int64_t* targets, const float* stats, int64_t rows, int64_t vocab,
+                   int64_t ld, float temperature, const float* dkl, const float* dce,
+                   void* dlogits, int64_t ld_out, void* stream);
+
 /* ------------------------------------------------------ data parallel ---- */
 /*
  * NCCL communicator for the data-parallel step (no reference counterpart:

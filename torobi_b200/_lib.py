@@ -104,6 +104,14 @@ SIGNATURES = {
                        _vp], _i32),
     "tq_cross_entropy_fwd": ([_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp], _i32),
     "tq_cross_entropy_bwd": ([_vp, _vp, _vp, _i64, _i64, _i64, _vp, _f32, _vp, _vp], _i32),
+    "tq_token_logprobs_fwd": ([_vp, _i32, _vp, _i64, _i64, _i64, _f32, _i64, _vp, _vp, _vp, _vp,
+                               _vp, _vp], _i32),
+    "tq_token_logprobs_bwd": ([_vp, _i32, _vp, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _i64,
+                               _vp], _i32),
+    "tq_distill_fwd": ([_vp, _i32, _vp, _i32, _vp, _i32, _i64, _vp, _i64, _i64, _i64, _f32, _vp,
+                        _vp, _vp, _vp], _i32),
+    "tq_distill_bwd": ([_vp, _i32, _vp, _i32, _vp, _i32, _i64, _vp, _vp, _i64, _i64, _i64, _f32,
+                        _vp, _vp, _vp, _i64, _vp], _i32),
     "tq_dp_unique_id": ([_vp], _i32),
     "tq_dp_comm_init": ([ctypes.POINTER(_vp), _vp, _i32, _i32], _i32),
     "tq_dp_allreduce_sum": ([_vp, _vp, _i64, _i32, _vp], _i32),

@@ -1,5 +1,8 @@
 """Fused decoder glue as differentiable ops: RMSNorm, rotary embedding and
-SwiGLU, each one sm_100a kernel forward and one backward (csrc/glue.cu).
+SwiGLU, each one sm_100a kernel forward and one backward (csrc/glue.cu), and
+what is read off the logits: the cross-entropy (csrc/loss.cu), the log
+probabilities of given tokens with entropy and alternatives, and the
+distillation from a teacher's alternatives (csrc/logits.cu).
 
 RMSNorm is ``x * rsqrt(mean(x^2) + eps) * w`` (engine/src/interp.rs:312-319),
 with a frozen gain; RoPE rotates the first half of each head against the
@@ -9,11 +12,14 @@ second (engine/src/interp.rs:350-388); SwiGLU is ``(g * sigmoid(g)) * u``
 from __future__ import annotations
 
 import ctypes
+import math
+from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .ops import _launch, _need_cuda, _ptr, _stream
-from ._lib import check, lib
+from ._lib import TQ_DTYPE_BF16, TQ_DTYPE_F32, check, lib
 
 
 def _bf16_contig(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -271,3 +277,254 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor,
     ``inplace=True`` writes the gradient over the logits in backward (no
     second [rows, vocab] buffer); the graph then cannot be run backward twice."""
     return _CrossEntropy.apply(logits, targets, inplace)
+
+
+_LOGIT_DTYPES = {torch.bfloat16: TQ_DTYPE_BF16, torch.float32: TQ_DTYPE_F32}
+
+
+def _one_device(op: str, **tensors) -> None:
+    """Every tensor on the first one's device, and that one current (the
+    kernels launch on its current stream)."""
+    _need_cuda(op, **tensors)
+    first = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if first is None:
+            first = t.device
+        elif t.device != first:
+            raise ValueError(f"[{op}] {name} is on {t.device}, the others on {first}")
+
+
+def _logit_rows(op: str, z: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
+    """``(z, rows, vocab, pitch)``: the logits as rows of one pitch, read in
+    place when their strides allow it (a slice of padded rows), else copied."""
+    if z.dtype not in _LOGIT_DTYPES:
+        raise ValueError(f"[{op}] logits must be bfloat16 or float32, got {z.dtype}")
+    if z.dim() < 1 or z.shape[-1] == 0:
+        raise ValueError(f"[{op}] logits need a non-empty last axis, got {tuple(z.shape)}")
+    vocab = z.shape[-1]
+    rows = z.numel() // vocab
+    if z.is_contiguous():
+        return z, rows, vocab, vocab
+    pitch = None
+    span = 1  # rows below the axis looked at
+    if z.stride(-1) == 1 or vocab == 1:
+        for size, stride in zip(reversed(z.shape[:-1]), reversed(z.stride()[:-1])):
+            if size == 1:
+                continue
+            if pitch is None:
+                pitch = stride
+            elif stride != pitch * span:
+                pitch = 0
+                break
+            span *= size
+    if pitch is None:
+        pitch = vocab  # one row
+        if z.stride(-1) != 1 and vocab != 1:
+            pitch = 0
+    if rows and pitch < vocab:
+        return z.contiguous(), rows, vocab, vocab
+    return z, rows, vocab, max(pitch, vocab)
+
+
+def _gradient_like(z: torch.Tensor, rows: int, vocab: int, pitch: int) -> torch.Tensor:
+    """Room for a gradient of logits, with their rows' pitch."""
+    if pitch == vocab:
+        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    wide = torch.empty(rows, pitch, dtype=z.dtype, device=z.device)
+    return wide.view(*z.shape[:-1], pitch)[..., :vocab]
+
+
+def _positions(op: str, name: str, t: torch.Tensor, z: torch.Tensor) -> torch.Tensor:
+    if t.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"[{op}] {name} must be int64 or int32, got {t.dtype}")
+    if t.shape != z.shape[:-1]:
+        raise ValueError(f"[{op}] {name} {tuple(t.shape)} must match the logits' positions "
+                         f"{tuple(z.shape[:-1])}")
+    return t.to(torch.int64).contiguous()
+
+
+def _temperature(op: str, temperature: float) -> float:
+    t = float(temperature)
+    if not (t > 0.0 and math.isfinite(t)):
+        raise ValueError(f"[{op}] temperature must be positive and finite, got {temperature}")
+    return t
+
+
+def _upstream(g: torch.Tensor | None) -> torch.Tensor | None:
+    return None if g is None else g.float().contiguous()
+
+
+class TokenLogprobs(NamedTuple):
+    """What ``token_logprobs`` answers, per position."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+def _token_logprobs(z, rows, vocab, pitch, tokens, top, temperature, want_stats):
+    dev = z.device
+    lead = z.shape[:-1]
+    logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
+    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
+    top_logprobs = torch.empty(*lead, top, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_stats else None
+    with torch.cuda.device(dev):
+        _launch("token_logprobs", lambda: lib().tq_token_logprobs_fwd(
+            _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), rows, vocab, pitch, temperature, top,
+            _ptr(logprobs), _ptr(entropy), _ptr(stats), _ptr(top_logprobs), _ptr(top_ids),
+            _stream()))
+    return logprobs, entropy, top_logprobs, top_ids, stats
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, tokens, top, temperature, inplace):
+        z, rows, vocab, pitch = _logit_rows("token_logprobs", z)
+        *out, stats = _token_logprobs(z, rows, vocab, pitch, tokens, top, temperature, True)
+        ctx.save_for_backward(z, tokens, stats)
+        ctx.shape, ctx.temperature, ctx.inplace = (rows, vocab, pitch), temperature, inplace
+        ctx.spent = False
+        ctx.mark_non_differentiable(out[2], out[3])
+        ctx.set_materialize_grads(False)
+        return tuple(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogprobs, dentropy, _top, _ids):
+        z, tokens, stats = ctx.saved_tensors
+        dz = _gradient_room(ctx, "token_logprobs", z)
+        rows, vocab, pitch = ctx.shape
+        dlogprobs, dentropy = _upstream(dlogprobs), _upstream(dentropy)
+        with torch.cuda.device(z.device):
+            _launch("token_logprobs", lambda: lib().tq_token_logprobs_bwd(
+                _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), _ptr(stats), rows, vocab, pitch,
+                ctx.temperature, _ptr(dlogprobs), _ptr(dentropy), _ptr(dz), pitch, _stream()))
+        return dz, None, None, None, None
+
+
+def _gradient_room(ctx, op: str, z: torch.Tensor) -> torch.Tensor:
+    if not ctx.inplace:
+        return _gradient_like(z, *ctx.shape)
+    if ctx.spent:
+        raise RuntimeError(f"[{op}] inplace=True wrote the gradient over the logits: this graph "
+                           "cannot be run backward twice")
+    ctx.spent = True
+    return z
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
+                   temperature: float = 1.0, inplace: bool = False) -> TokenLogprobs:
+    """What a model thought of given tokens: ``q = softmax(logits /
+    temperature)`` over the last axis of ``logits`` (bf16 or f32 [..., vocab]),
+    read once, and per position
+
+    ``logprobs`` f32 ``ln q[token]`` (0 where the token is outside [0, vocab):
+    a padding position), ``entropy`` f32 ``-sum q ln q``, and the ``top`` (0 to
+    128) most likely alternatives, most likely first, equal logits by lowest
+    id: ``top_logprobs`` f32 and ``top_ids`` int64 [..., top].
+
+    Differentiable through logprobs and entropy.  ``inplace=True`` writes the
+    gradient over the logits in backward, as ``cross_entropy`` does.  A -inf
+    logit has probability 0; a position of nothing else has no distribution
+    (log probabilities -inf, entropy 0, gradient 0)."""
+    op = "token_logprobs"
+    _one_device(op, logits=logits, tokens=tokens)
+    tokens = _positions(op, "tokens", tokens, logits)
+    temperature = _temperature(op, temperature)
+    if not 0 <= top <= min(128, logits.shape[-1]):
+        raise ValueError(f"[{op}] top must be 0 to 128 and at most the vocabulary "
+                         f"({logits.shape[-1]}), got {top}")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, int(top), temperature,
+                                                   bool(inplace)))
+    z, rows, vocab, pitch = _logit_rows(op, logits)
+    return TokenLogprobs(*_token_logprobs(z, rows, vocab, pitch, tokens, int(top), temperature,
+                                          False)[:4])
+
+
+def _distillation(z, rows, vocab, pitch, teacher, targets, temperature, want_stats):
+    dev = z.device
+    ids, logits = teacher
+    kl = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
+    ce = None if targets is None else torch.empty_like(kl)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_stats else None
+    with torch.cuda.device(dev):
+        _launch("distillation", lambda: lib().tq_distill_fwd(
+            _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
+            _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), rows, vocab, pitch,
+            temperature, _ptr(kl), _ptr(ce), _ptr(stats), _stream()))
+    return kl, ce, stats
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, ids, logits, targets, temperature, inplace):
+        z, rows, vocab, pitch = _logit_rows("distillation", z)
+        kl, ce, stats = _distillation(z, rows, vocab, pitch, (ids, logits), targets, temperature,
+                                      True)
+        ctx.save_for_backward(z, ids, logits, targets, stats)
+        ctx.shape, ctx.temperature, ctx.inplace = (rows, vocab, pitch), temperature, inplace
+        ctx.spent = False
+        ctx.set_materialize_grads(False)
+        return kl if ce is None else (kl, ce)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dkl, dce=None):
+        z, ids, logits, targets, stats = ctx.saved_tensors
+        dz = _gradient_room(ctx, "distillation", z)
+        rows, vocab, pitch = ctx.shape
+        dkl, dce = _upstream(dkl), _upstream(dce)
+        with torch.cuda.device(z.device):
+            _launch("distillation", lambda: lib().tq_distill_bwd(
+                _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
+                _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), _ptr(stats), rows,
+                vocab, pitch, ctx.temperature, _ptr(dkl), _ptr(dce), _ptr(dz), pitch, _stream()))
+        return dz, None, None, None, None, None
+
+
+def distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                 targets: torch.Tensor | None = None, temperature: float = 1.0,
+                 inplace: bool = False):
+    """The divergence from a teacher's top logits, per position and
+    differentiable: ``kl = sum_i p_i (ln p_i - ln q[teacher_ids[i]])`` f32, with
+    ``p = softmax(teacher_logits / temperature)`` over the position's k (1 to
+    128) given alternatives and ``q = softmax(logits / temperature)`` over the
+    whole vocabulary.
+
+    logits bf16 or f32 [..., vocab]; teacher_ids int64 or int32 [..., k], an id
+    outside [0, vocab) being no alternative (kl and its gradient are 0 where a
+    position has none); teacher_logits bf16 or f32 [..., k], logits or log
+    probabilities (``token_logprobs(..., top=k)`` gives both).  No gradient
+    reaches the teacher.  With ``targets`` [...] the answer is ``(kl, ce)``:
+    ``ce`` is the targets' cross-entropy at temperature 1, 0 where a target is
+    outside [0, vocab); both gradients come from one pass.  A loss that mixes
+    them is ``(1 - a) * ce + a * temperature**2 * kl``.  ``inplace=True``
+    writes the gradient over the logits in backward."""
+    op = "distillation"
+    _one_device(op, logits=logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits,
+                targets=targets)
+    if teacher_ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"[{op}] teacher_ids must be int64 or int32, got {teacher_ids.dtype}")
+    if teacher_logits.dtype not in _LOGIT_DTYPES:
+        raise ValueError(f"[{op}] teacher_logits must be bfloat16 or float32, got "
+                         f"{teacher_logits.dtype}")
+    if (teacher_ids.shape != teacher_logits.shape or teacher_ids.dim() != logits.dim()
+            or teacher_ids.shape[:-1] != logits.shape[:-1]):
+        raise ValueError(f"[{op}] teacher_ids {tuple(teacher_ids.shape)} and teacher_logits "
+                         f"{tuple(teacher_logits.shape)} must be [..., k] over the logits' "
+                         f"positions {tuple(logits.shape[:-1])}")
+    temperature = _temperature(op, temperature)
+    ids, given = teacher_ids.contiguous(), teacher_logits.detach().contiguous()
+    if targets is not None:
+        targets = _positions(op, "targets", targets, logits)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Distillation.apply(logits, ids, given, targets, temperature, bool(inplace))
+    z, rows, vocab, pitch = _logit_rows(op, logits)
+    kl, ce, _ = _distillation(z, rows, vocab, pitch, (ids, given), targets, temperature, False)
+    return kl if ce is None else (kl, ce)
