@@ -366,6 +366,43 @@ int tq_attention_bwd(const void* q, const void* k, const void* v, const void* ou
                      void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
                      void* stream);
 
+/*
+ * The same attention for rows that pack several documents: query i of
+ * sequence b sees the keys first[b, i] <= j < last[b, i] (int32 [batch, seq],
+ * taken within [0, seq]) in place of the causal rule.  A query that sees none
+ * gets o = 0, lse = -inf and no gradient.  Layouts, types and determinism as
+ * above; the work of key tiles that no query of a tile sees is not done.
+ * What a query does not see still enters products with 0: k, v, and q and
+ * dout of queries that see nothing, must be finite.  No counterpart in the
+ * reference (its node takes a causal mode or a mask tensor,
+ * engine/src/interp.rs:405-432).
+ * workspace: tq_span_attention_bwd_workspace_bytes() bytes, 256-byte aligned.
+ */
+int tq_span_attention_fwd(const void* q, const void* k, const void* v, const int32_t* first,
+                          const int32_t* last, int64_t batch, int64_t seq, int64_t heads,
+                          int64_t kv_heads, int64_t head_dim, float scale, void* out, float* lse,
+                          void* stream);
+int tq_span_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
+                                          size_t* bytes);
+int tq_span_attention_bwd(const void* q, const void* k, const void* v, const int32_t* first,
+                          const int32_t* last, const void* out, const void* dout,
+                          const float* lse, int64_t batch, int64_t seq, int64_t heads,
+                          int64_t kv_heads, int64_t head_dim, float scale, void* dq, void* dk,
+                          void* dv, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The spans of packed documents, for the three calls above: documents
+ * [batch, seq] holds an id per position (ids_bits 32 or 64); a run of equal
+ * ids is one document, a negative id is padding and sees nothing.
+ *   causal != 0: a position sees its document up to itself, and the first
+ *                prefix[b, i] positions of it whole (prefix int32
+ *                [batch, seq], the document's at each of its positions; NULL
+ *                for none): a prompt seen in both directions
+ *   causal == 0: the whole document (prefix is not read)
+ */
+int tq_document_spans(const void* documents, int ids_bits, const int32_t* prefix, int64_t batch,
+                      int64_t seq, int causal, int32_t* first, int32_t* last, void* stream);
+
 /* --------------------------------------------------------------- export --- */
 
 /*

@@ -1,0 +1,441 @@
+"""span_attention and document_spans (csrc/attn.cu) against their definitions
+in 64 bits.
+
+Tolerances.  The operands are bf16 and the products are summed in f32; what is
+rounded on the way is P (and dS) to bf16 before a product and the result: each
+half a step, 2^-8 of the value at most.  |o| errs by at most
+2^-8 (sum_j p_j |v_j| + |o|), plus the exponentials' 8e-5 and f32 sums, for
+which a tenth of that bound is ample.  For the gradients the same holds with
+the products' magnitudes: dv by 2^-8 (sum_i p_ij |do_i| + |dv|), dq and dk by
+2^-8 times sums of |dS| |k| (or |q|), where dS's own error comes from its
+rounding and from delta = sum do o, whose o is rounded to bf16:
+p_ij 2^-8 sum_d |do o|.  lse: f32, within 1e-4 (a quarter of the
+exponentials are a polynomial of relative error 7.5e-5; log is 1-Lipschitz
+here) plus 4 steps of f32 of its own size and of the scores'.
+"""
+from __future__ import annotations
+
+import pytest
+
+R = 2.0 ** -8 * 1.1
+
+
+def _spans_reference(documents, prefix, causal):
+    """first, last [batch][seq] by walking the runs."""
+    firsts, lasts = [], []
+    for r, row in enumerate(documents):
+        first, last = [0] * len(row), [0] * len(row)
+        i = 0
+        while i < len(row):
+            j = i
+            while j < len(row) and row[j] == row[i]:
+                j += 1
+            for t in range(i, j):
+                first[t] = i
+                if row[i] < 0:
+                    last[t] = i
+                elif not causal:
+                    last[t] = j
+                else:
+                    last[t] = t + 1
+                    if prefix is not None:
+                        last[t] = max(t + 1, min(i + max(prefix[r][t], 0), j))
+            i = j
+        firsts.append(first)
+        lasts.append(last)
+    return firsts, lasts
+
+
+def _random_documents(rnd, batch, seq, mean):
+    rows = []
+    for _ in range(batch):
+        row, n = [], 0
+        while len(row) < seq:
+            length = max(1, int(rnd.expovariate(1 / mean)))
+            ident = -1 if rnd.random() < 0.15 else n
+            row += [ident] * length
+            n += 1
+        rows.append(row[:seq])
+    return rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ids", ["int32", "int64"])
+@pytest.mark.parametrize("seq, mean", [(1, 1), (2, 1), (31, 3), (200, 40), (1025, 1), (4096, 300),
+                                       (4099, 900), (9001, 20000), (12289, 5)])
+def test_document_spans(cuda, seq, mean, ids):
+    import random
+
+    import torch
+
+    from torobi_b200 import glue
+
+    rnd = random.Random(seq * 7 + len(ids))
+    rows = _random_documents(rnd, 3, seq, mean)
+    rows[0] = [0] * seq
+    prefix = [[rnd.choice([-3, 0, 1, 5, 60, 10 ** 9]) for _ in row] for row in rows]
+    d = torch.tensor(rows, dtype=getattr(torch, ids), device=cuda)
+    pre = torch.tensor(prefix, dtype=torch.int32, device=cuda)
+    for causal, use in ((True, None), (True, pre), (False, None)):
+        first, last = glue.document_spans(d, use, causal=causal)
+        f, l = _spans_reference(rows, None if use is None else prefix, causal)
+        assert first.tolist() == f and last.tolist() == l
+
+
+def _reference(q, k, v, first, last, scale, do=None):
+    """o, lse, the gradients and the bounds' sums, in 64 bits, a head at a time."""
+    import torch
+
+    b, s, h, d = q.shape
+    hk = k.shape[2]
+    qd, kd, vd = q.double(), k.double(), v.double()
+    j = torch.arange(s, device=q.device)
+    see = (j >= first[:, :, None].clamp(0, s)) & (j < last[:, :, None].clamp(0, s))
+    o, ob = torch.zeros_like(qd), torch.zeros_like(qd)
+    lse = torch.empty(b, h, s, dtype=torch.float64, device=q.device)
+    g = {n: torch.zeros_like(t) for n, t in (("dq", qd), ("dk", kd), ("dv", vd))}
+    gb = {n: torch.zeros_like(t) for n, t in g.items()}
+    for hi in range(h):
+        kv = hi // (h // hk)
+        x = (qd[:, :, hi] @ kd[:, :, kv].transpose(1, 2)) * scale
+        x = x.masked_fill(~see, float("-inf"))
+        lse[:, hi] = x.logsumexp(2)
+        p = torch.where(see.any(2, keepdim=True), x.softmax(2), 0.0)
+        o[:, :, hi] = p @ vd[:, :, kv]
+        ob[:, :, hi] = p @ vd[:, :, kv].abs()
+        if do is None:
+            continue
+        up = do[:, :, hi].double()
+        dp = up @ vd[:, :, kv].transpose(1, 2)
+        delta = (up * o[:, :, hi]).sum(2, keepdim=True)
+        wide = (up * o[:, :, hi]).abs().sum(2, keepdim=True)
+        ds = p * (dp - delta) * scale
+        dsb = (ds.abs() + p * wide * scale)
+        g["dq"][:, :, hi] = ds @ kd[:, :, kv]
+        gb["dq"][:, :, hi] = dsb @ kd[:, :, kv].abs()
+        g["dk"][:, :, kv] += ds.transpose(1, 2) @ qd[:, :, hi]
+        gb["dk"][:, :, kv] += dsb.transpose(1, 2) @ qd[:, :, hi].abs()
+        g["dv"][:, :, kv] += p.transpose(1, 2) @ up
+        gb["dv"][:, :, kv] += p.transpose(1, 2) @ up.abs()
+    return o, ob, lse, g, gb
+
+
+def _inputs(cuda, seed, b, s, h, hk, d, gain=1.0):
+    import torch
+
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    mk = lambda n, f=1.0: (torch.randn(b, s, n, d, device=cuda, generator=g) * f).bfloat16()  # noqa: E731
+    return mk(h, gain), mk(hk), mk(hk), mk(h)
+
+
+def _check(q, k, v, do, first, last, scale=None):
+    import torch
+
+    from torobi_b200 import device_status, glue
+
+    sc = scale if scale is not None else q.shape[-1] ** -0.5
+    o, lse = glue.span_attention_forward(q, k, v, first, last, scale)
+    ro, ob, rl, g, gb = _reference(q, k, v, first, last, sc, do)
+    none = (last.clamp(0, q.shape[1]) <= first.clamp(0, q.shape[1]))
+    assert ((o.double() - ro).abs() <= R * (ob + ro.abs()) + 1e-30).all()
+    assert (o[none] == 0).all() and (lse.transpose(1, 2)[none] == float("-inf")).all()
+    seen = ~none[:, None, :].expand_as(lse)
+    top = (q.double().abs().amax() * k.double().abs().amax() * q.shape[-1] * sc).item()
+    assert ((lse.double() - rl).abs()[seen]
+            <= 1e-4 + 2.0 ** -22 * (rl.abs()[seen] + top)).all()
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = glue.span_attention(*leaves, first, last, scale)
+    assert torch.equal(out, o)
+    got = torch.autograd.grad(out, leaves, do)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        # 1e-6: where the gradient is zero (one visible key), rounding is left.
+        off = (t.double() - g[name]).abs() - R * (gb[name] + g[name].abs()) - 1e-6 * top
+        assert off.max().item() <= 0, (name, off.max().item())
+    assert (got[0][none] == 0).all()
+    assert device_status() == 0
+    return o, got
+
+
+def _spans(cuda, documents, prefix=None, causal=True):
+    import torch
+
+    from torobi_b200 import glue
+
+    d = torch.tensor(documents, dtype=torch.int32, device=cuda)
+    p = None if prefix is None else torch.tensor(prefix, dtype=torch.int32, device=cuda)
+    return glue.document_spans(d, p, causal=causal)
+
+
+CASES = [
+    # batch, seq, heads, kv_heads, dim, mean document, prefix, causal
+    (1, 1, 2, 1, 64, 1, False, True),
+    (1, 7, 2, 2, 128, 2, False, True),
+    (2, 128, 4, 2, 64, 30, False, True),
+    (2, 129, 4, 1, 128, 30, True, True),
+    (1, 200, 4, 2, 64, 60, False, False),
+    (3, 255, 6, 6, 64, 10, True, True),
+    (1, 300, 8, 1, 128, 500, True, True),
+    (2, 513, 14, 2, 64, 100, False, True),
+    (2, 640, 2, 2, 128, 64, False, False),
+    (1, 1000, 4, 4, 64, 250, True, True),
+    (1, 1537, 8, 2, 128, 700, False, True),
+    (2, 2048, 4, 1, 64, 40, False, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_packed_documents(cuda, case):
+    import random
+
+    b, s, h, hk, d, mean, pre, causal = case
+    rnd = random.Random(s)
+    docs = _random_documents(rnd, b, s, mean)
+    prefix = None
+    if pre:
+        prefix = [[0] * s for _ in range(b)]
+        for r, row in enumerate(docs):
+            for i in range(s):
+                start = i == 0 or row[i] != row[i - 1]
+                prefix[r][i] = rnd.randrange(0, max(2, mean)) if start else prefix[r][i - 1]
+    first, last = _spans(cuda, docs, prefix, causal)
+    _check(*_inputs(cuda, s + d, b, s, h, hk, d), first, last)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("kind", ["window", "padding_tiles", "nothing", "far_apart", "outside",
+                                  "one_key", "random", "sharp"])
+def test_spans_of_other_shapes(cuda, kind, dim):
+    """Spans that no document makes: sliding windows, whole tiles that see
+    nothing, neighbouring tiles far apart, bounds outside the row, one key
+    each, arbitrary ones; and scores that move the running maximum."""
+    import torch
+
+    b, s, h, hk = 2, 777, 4, 2
+    i = torch.arange(s, device=cuda, dtype=torch.int32).expand(b, s).contiguous()
+    gain = 1.0
+    if kind == "window":
+        first, last = (i - 150).clamp(min=0), i + 1
+    elif kind == "padding_tiles":
+        first, last = torch.zeros_like(i), i + 1
+        dead = ((i >= 128) & (i < 400)) | (i >= 650)
+        first, last = torch.where(dead, i, first), torch.where(dead, i, last)
+    elif kind == "nothing":
+        first, last = i.clone(), i.clone()
+        last[1] += 1
+    elif kind == "far_apart":  # neighbouring query tiles at opposite ends
+        even = (i // 128) % 2 == 0
+        first = torch.where(even, 0, s - 100).to(torch.int32)
+        last = torch.where(even, 70, s).to(torch.int32)
+    elif kind == "outside":
+        first, last = i - 2000, i + 2000
+        first[0, ::3] = 5000
+        last[1, ::5] = -7
+    elif kind == "one_key":
+        first = (i * 37) % s
+        last = first + 1
+    elif kind == "random":
+        g = torch.Generator(device=cuda).manual_seed(1)
+        first = torch.randint(0, s, (b, s), device=cuda, generator=g, dtype=torch.int32)
+        last = first + torch.randint(-50, 300, (b, s), device=cuda, generator=g, dtype=torch.int32)
+    else:
+        first, last, gain = (i // 300) * 300, i + 1, 12.0
+    _check(*_inputs(cuda, 5 + dim, b, s, h, hk, dim, gain), first.contiguous(),
+           last.contiguous())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_causal_document_is_causal_attention(cuda, dim):
+    """One document a row: what ``attention`` gives, bit for bit."""
+    import torch
+
+    from torobi_b200 import glue
+
+    q, k, v, do = _inputs(cuda, 3, 2, 400, 8, 2, dim)
+    first, last = _spans(cuda, [[0] * 400] * 2)
+    a = [t.clone().requires_grad_() for t in (q, k, v)]
+    c = [t.clone().requires_grad_() for t in (q, k, v)]
+    x, y = glue.span_attention(*a, first, last), glue.attention(*c, True)
+    assert torch.equal(x, y)
+    for s, t in zip(torch.autograd.grad(x, a, do), torch.autograd.grad(y, c, do)):
+        assert torch.equal(s, t)
+
+
+@pytest.mark.gpu
+def test_a_document_does_not_see_its_neighbours(cuda):
+    """A document's outputs and gradients are the same whatever stands beside
+    it (bit for bit where no warp's 32 rows hold two documents: a warp moves
+    its rows' running maxima together)."""
+    import torch
+
+    from torobi_b200 import glue
+
+    q, k, v, do = _inputs(cuda, 8, 1, 500, 4, 2, 128)
+    docs = [[0] * 128 + [1] * 192 + [2] * 180]
+    first, last = _spans(cuda, docs)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = glue.span_attention(*leaves, first, last)
+    want = [o.detach(), *torch.autograd.grad(o, leaves, do)]
+    for t in (q, k, v, do):
+        t[:, :128] = torch.randn_like(t[:, :128]) * 3
+        t[:, 320:] = 0
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = glue.span_attention(*leaves, first, last)
+    for a, c in zip(want, [o.detach(), *torch.autograd.grad(o, leaves, do)]):
+        assert torch.equal(a[:, 128:320], c[:, 128:320])
+
+
+@pytest.mark.gpu
+def test_span_gradient_against_differences(cuda):
+    """The gradients against central differences of the 64-bit definition
+    along random directions."""
+    import torch
+
+    from torobi_b200 import glue
+
+    q, k, v, do = _inputs(cuda, 9, 1, 60, 2, 1, 64)
+    first, last = _spans(cuda, [[0] * 25 + [-1] * 5 + [1] * 30])
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(glue.span_attention(*leaves, first, last), leaves, do)
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    _, _, _, g, gb = _reference(q, k, v, first, last, 0.125, do)
+    for n, name in enumerate(("dq", "dk", "dv")):
+        way = torch.randn(got[n].shape, device=cuda, generator=gen, dtype=torch.float64)
+        step = 1e-4
+
+        def loss(at):
+            args = [t.double() for t in (q, k, v)]
+            args[n] = args[n] + at * way
+            o, *_ = _reference(*args, first, last, 0.125)
+            return (o * do.double()).sum()
+
+        diff = (loss(step) - loss(-step)) / (2 * step)
+        along = (got[n].double() * way).sum()
+        # Each element errs within its bound; the difference's own error is of
+        # order step^2 and far below.
+        assert (along - diff).abs() <= (R * (gb[name] + g[name].abs()) * way.abs()).sum() + 1e-5
+
+
+@pytest.mark.gpu
+def test_span_attention_repeats_captured_and_on_another_stream(cuda):
+    """The same bits every time: run again, on a side stream, and from two
+    captured graphs replayed on new inputs."""
+    import torch
+
+    from torobi_b200 import glue
+
+    docs = torch.tensor([[0] * 100 + [1] * 300 + [-1] * 13, [5] * 413], device=cuda)
+    sets = [_inputs(cuda, 30 + i, 2, 413, 4, 2, 64) for i in range(3)]
+
+    def work(q, k, v, do):
+        first, last = glue.document_spans(docs)
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        o = glue.span_attention(*leaves, first, last)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do), first, last]
+
+    want = [work(*x) for x in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = work(*sets[0])
+    torch.cuda.current_stream().wait_stream(side)
+    for a, c in zip(other, want[0]):
+        assert torch.equal(a, c)
+    graphs = []
+    for i in range(2):
+        static = [t.clone() for t in sets[i]]
+        with torch.cuda.stream(side):
+            work(*static)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = work(*static)
+        graphs.append((graph, static, out))
+    for turn in range(2):
+        for i, (graph, static, out) in enumerate(graphs):
+            for t, n in zip(static, sets[i + turn]):
+                t.copy_(n)
+            graph.replay()
+        for i, (graph, static, out) in enumerate(graphs):
+            for a, c in zip(out, want[i + turn]):
+                assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_span_refusals(cuda):
+    import torch
+
+    from torobi_b200 import TqError, glue
+
+    q, k, v, _ = _inputs(cuda, 1, 2, 16, 4, 2, 64)
+    f = torch.zeros(2, 16, dtype=torch.int32, device=cuda)
+    for bad in (lambda: glue.span_attention(q, k, v, f.long(), f),
+                lambda: glue.span_attention(q, k, v, f[:1], f),
+                lambda: glue.span_attention(q, k, v, f, f.cpu()),
+                lambda: glue.span_attention(q.float(), k, v, f, f),
+                lambda: glue.span_attention(q, k[:, :8], v[:, :8], f, f),
+                lambda: glue.span_attention(q, k, v[:, :8], f, f),
+                lambda: glue.document_spans(f[0]), lambda: glue.document_spans(f.float()),
+                lambda: glue.document_spans(f, f[:1]),
+                lambda: glue.document_spans(f, f.float()),
+                lambda: glue.document_spans(f, f, causal=False)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TqError, match="scale"):
+        glue.span_attention(q, k, v, f, f, scale=-1.0)
+    with pytest.raises(TqError, match="head dim"):
+        glue.span_attention(q[..., :32], k[..., :32], v[..., :32], f, f)
+    # Strided spans and empty batches are taken.
+    wide = torch.zeros(2, 32, dtype=torch.int32, device=cuda)
+    o, lse = glue.span_attention_forward(q, k, v, wide[:, ::2], wide[:, ::2])
+    assert (o == 0).all() and (lse == float("-inf")).all()
+    o, _ = glue.span_attention_forward(q[:0], k[:0], v[:0], f[:0], f[:0])
+    assert o.shape == (0, 16, 4, 64)
+    assert glue.document_spans(f[:, :0])[0].shape == (2, 0)
+
+
+P = 1 << 20  # an aligned stand-in address; nothing is dereferenced
+
+
+def test_span_entry_points_refuse_on_the_host():
+    import ctypes
+
+    import torobi_b200 as tq
+
+    L = tq.lib()
+
+    def fwd(first=P, last=P, heads=4, kv=2, dim=64, scale=0.1, out=P, batch=2, seq=129):
+        return L.tq_span_attention_fwd(P, P, P, first, last, batch, seq, heads, kv, dim, scale,
+                                       out, P, None)
+
+    def said():
+        return L.tq_last_error().decode()
+
+    assert fwd(first=None) == 1 and "null" in said()
+    assert fwd(last=None) == 1 and "null" in said()
+    assert fwd(first=P + 2) == 3 and "first and last" in said()
+    assert fwd(kv=3) == 1 and fwd(dim=96) == 2 and fwd(scale=0.0) == 1 and fwd(out=P + 8) == 3
+    assert fwd(batch=0, first=None, last=None, out=None) == 0
+
+    need, plain = ctypes.c_size_t(), ctypes.c_size_t()
+    assert L.tq_span_attention_bwd_workspace_bytes(2, 129, 4, ctypes.byref(need)) == 0
+    assert L.tq_attention_bwd_workspace_bytes(2, 129, 4, ctypes.byref(plain)) == 0
+    # Beside the statistics: two ints a padded row, four a 64-row tile.
+    assert need.value == plain.value + 2 * 256 * 8 + 2 * 4 * 16
+
+    def bwd(ws_bytes=need.value, ws=P, first=P):
+        return L.tq_span_attention_bwd(P, P, P, first, P, P, P, P, 2, 129, 4, 2, 64, 0.125, P, P,
+                                       P, ws, ws_bytes, None)
+
+    assert bwd(ws_bytes=plain.value) == 1 and "workspace" in said()
+    assert bwd(ws=P + 16) == 3 and bwd(ws=None) == 1 and bwd(first=None) == 1
+
+    def spans(docs=P, bits=32, prefix=None, batch=2, seq=8, first=P, last=P):
+        return L.tq_document_spans(docs, bits, prefix, batch, seq, 1, first, last, None)
+
+    assert spans(bits=16) == 2 and spans(docs=None) == 1 and spans(last=None) == 1
+    assert spans(docs=P + 2) == 3 and spans(docs=P + 4, bits=64) == 3 and spans(prefix=P + 1) == 3
+    assert spans(seq=-1) == 1 and spans(seq=1 << 31) == 1
+    assert spans(batch=0, docs=None) == 0 and spans(seq=0, docs=None) == 0

@@ -9,6 +9,14 @@
 // the natural-log log-sum-exp of each query row's scaled scores, kept for the
 // backward.  dim is 64 or 128.
 //
+// Each kernel also comes in a SPAN form, for rows that pack several documents
+// (and prompts seen in both directions, and padding): query i of sequence b
+// sees the keys first[b, i] <= j < last[b, i], two ints a row, in place of the
+// causal rule.  Key tiles that no row of a query tile sees are neither loaded
+// nor multiplied (the tile's range is the least first to the greatest last),
+// tiles that every row sees whole take the unmasked code, and a row that sees
+// nothing gets o = 0, lse = -inf and no gradient.
+//
 // The forward and the backward kernels are described where they start below.
 #include <cuda_bf16.h>
 
@@ -96,15 +104,30 @@ struct FwdCfg {
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
+// A query row's keys [lo, hi) within [0, seq); lo = hi = 0 when it sees none.
+struct Span {
+  int lo, hi;
+};
+
+__device__ __forceinline__ Span load_span(const int* first, const int* last, int b, int i,
+                                          int seq) {
+  if (i >= seq) return {0, 0};
+  const size_t at = static_cast<size_t>(b) * seq + i;
+  const int lo = max(first[at], 0), hi = min(last[at], seq);
+  return lo < hi ? Span{lo, hi} : Span{0, 0};
+}
+
 struct FwdParams {
   AttnShape sh;
+  const int* first;  // SPAN: [batch, seq]
+  const int* last;
   int n_pairs;
   uint16_t* out;
   float* lse;
   int* status;
 };
 
-template <int D>
+template <int D, bool SPAN>
 __global__ void __launch_bounds__(384, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
@@ -147,10 +170,15 @@ __global__ void __launch_bounds__(384, 1)
   const int hk = h / sh.group;
   const int t0 = 2 * pair;                             // first query tile
   const bool has1 = t0 + 1 < sh.n_tiles;               // second query tile exists
-  const int n_kv0 = sh.causal ? t0 + 1 : sh.n_tiles;  // key tiles of query tile 0
-  const int n_kv1 = has1 ? (sh.causal ? t0 + 2 : sh.n_tiles) : 0;
-  const int n_kv = n_kv0 > n_kv1 ? n_kv0 : n_kv1;
-  auto nkv_of = [&](int w) { return w == 0 ? n_kv0 : n_kv1; };
+  // Key tiles [kv_lo(w), kv_hi(w)) of query tile w, all within [j0, j0 + n_kv).
+  int lo0 = 0, lo1 = 0;
+  int hi0 = sh.causal ? t0 + 1 : sh.n_tiles;
+  int hi1 = has1 ? (sh.causal ? t0 + 2 : sh.n_tiles) : 0;
+  __shared__ int range[2][2];  // SPAN: the tiles' least first and greatest last
+  if (SPAN && threadIdx.x < 2) {
+    range[threadIdx.x][0] = sh.seq;
+    range[threadIdx.x][1] = 0;
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -182,6 +210,28 @@ __global__ void __launch_bounds__(384, 1)
   griddep_launch_dependents();
   griddep_wait();
 
+  if constexpr (SPAN) {
+    if (threadIdx.x < 2 * kTile) {
+      const int w = threadIdx.x / kTile;
+      const Span sp = load_span(p.first, p.last, b, t0 * kTile + threadIdx.x, sh.seq);
+      const int lo = __reduce_min_sync(0xffffffffu, sp.lo < sp.hi ? sp.lo : sh.seq);
+      const int hi = __reduce_max_sync(0xffffffffu, sp.hi);
+      if (lane == 0) {
+        atomicMin(&range[w][0], lo);
+        atomicMax(&range[w][1], hi);
+      }
+    }
+    __syncthreads();
+    hi0 = (range[0][1] + kTile - 1) / kTile;
+    hi1 = (range[1][1] + kTile - 1) / kTile;
+    lo0 = hi0 ? range[0][0] / kTile : 0;
+    lo1 = hi1 ? range[1][0] / kTile : 0;
+  }
+  const int j0 = !SPAN ? 0 : hi0 == 0 ? lo1 : hi1 == 0 ? lo0 : min(lo0, lo1);
+  const int n_kv = max(hi0, hi1) - j0;
+  auto kv_lo = [&](int w) { return w == 0 ? lo0 : lo1; };
+  auto kv_hi = [&](int w) { return w == 0 ? hi0 : hi1; };
+
   if (warp == 0) {
     // ------------------------------------------------------------- TMA
     if (elect_one_sync()) {
@@ -200,7 +250,8 @@ __global__ void __launch_bounds__(384, 1)
         if (!mbar_wait(k_empty(s), ((j / KST) & 1) ^ 1, p.status)) return false;
         mbar_arrive_expect_tx(k_full(s), C::TILE_BYTES);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(k_s(s) + sl * C::SLAB_BYTES, &tm_k, k_full(s), sl * 64, hk, j * kTile, b);
+          tma_load_4d(k_s(s) + sl * C::SLAB_BYTES, &tm_k, k_full(s), sl * 64, hk,
+                      (j0 + j) * kTile, b);
         ++nk;
         return true;
       };
@@ -211,7 +262,8 @@ __global__ void __launch_bounds__(384, 1)
         if (!mbar_wait(v_empty(s), ((j / VST) & 1) ^ 1, p.status)) break;
         mbar_arrive_expect_tx(v_full(s), C::TILE_BYTES);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(v_s(s) + sl * C::SLAB_BYTES, &tm_v, v_full(s), sl * 64, hk, j * kTile, b);
+          tma_load_4d(v_s(s) + sl * C::SLAB_BYTES, &tm_v, v_full(s), sl * 64, hk,
+                      (j0 + j) * kTile, b);
         ++nv;
       }
       // Never leave a copy in flight.
@@ -227,9 +279,13 @@ __global__ void __launch_bounds__(384, 1)
       constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kTile, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(kTile, D, false, true);
       bool ok = mbar_wait(q_full, 0, p.status);
-      // S_w(j) = Q_w K_j^T into S_w.
-      auto issue_s = [&](int w, int j) {
-        const int s = j % KST;
+      // Key tiles count from j0 here: tile t is key tile j0 + t, and query
+      // tile w takes part in t of [from(w), to(w)).
+      auto from = [&](int w) { return kv_lo(w) - j0; };
+      auto to = [&](int w) { return kv_hi(w) - j0; };
+      // S_w(t) = Q_w K_t^T into S_w.
+      auto issue_s = [&](int w, int t) {
+        const int s = t % KST;
         const uint32_t d = tmem + C::S_COL + w * kTile;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -239,48 +295,50 @@ __global__ void __launch_bounds__(384, 1)
         }
         umma_commit(s_full(w));
       };
-      // O_w += P_w(j) V_j, P_w from the first 64 columns of S_w.
-      auto issue_pv = [&](int w, int j) {
-        const int s = j % VST;
+      // O_w += P_w(t) V_t, P_w from the first 64 columns of S_w.
+      auto issue_pv = [&](int w, int t) {
+        const int s = t % VST;
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
           umma_bf16_ts(tmem + C::O_COL + w * D, tmem + C::S_COL + w * kTile + kk * 8,
                        make_sdesc(v_s(s) + kk * 2048, C::SLAB_BYTES, 1024, kSw128), idesc_o,
-                       (j > 0 || kk > 0) ? 1u : 0u);
+                       (t > from(w) || kk > 0) ? 1u : 0u);
         umma_commit(o_done(w));
       };
-      // Key tile 0: both tiles' scores.
-      if (ok) ok = mbar_wait(k_full(0), 0, p.status);
-      if (ok) {
+      // The first key tile's scores, of both query tiles unless one starts later.
+      if (ok && n_kv > 0) ok = mbar_wait(k_full(0), 0, p.status);
+      if (ok && n_kv > 0) {
         tc_fence_after();
-        issue_s(0, 0);
-        if (n_kv1 > 0) issue_s(1, 0);
+        for (int w = 0; w < 2; ++w)
+          if (from(w) == 0 && to(w) > 0) issue_s(w, 0);
         umma_commit(k_empty(0));
       }
-      for (int j = 0; j < n_kv && ok; ++j) {
-        const int s = j % VST;
-        const bool next = j + 1 < n_kv;
+      for (int t = 0; t < n_kv && ok; ++t) {
+        const int s = t % VST;
+        const bool next = t + 1 < n_kv;
         if (next) {
-          ok = mbar_wait(k_full((j + 1) % KST), ((j + 1) / KST) & 1, p.status);
+          ok = mbar_wait(k_full((t + 1) % KST), ((t + 1) / KST) & 1, p.status);
           if (!ok) break;
         }
-        ok = mbar_wait(v_full(s), (j / VST) & 1, p.status);
+        ok = mbar_wait(v_full(s), (t / VST) & 1, p.status);
         if (!ok) break;
         for (int w = 0; w < 2 && ok; ++w) {
-          if (j >= nkv_of(w)) continue;
-          ok = mbar_wait(p_ready(w), j & 1, p.status);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(w, j);
-          if (j + 1 < nkv_of(w)) issue_s(w, j + 1);
+          if (t >= to(w)) continue;
+          if (t >= from(w)) {
+            ok = mbar_wait(p_ready(w), (t - from(w)) & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(w, t);
+          }
+          if (t + 1 >= from(w) && t + 1 < to(w)) issue_s(w, t + 1);
         }
         if (!ok) break;
         umma_commit(v_empty(s));
-        if (next) umma_commit(k_empty((j + 1) % KST));
+        if (next) umma_commit(k_empty((t + 1) % KST));
       }
       // Nothing may outlive the CTA's TMEM: wait for each tile's last PV.
       for (int w = 0; w < 2; ++w)
-        if (nkv_of(w) > 0) mbar_wait(o_done(w), (nkv_of(w) - 1) & 1, p.status);
+        if (to(w) > from(w)) mbar_wait(o_done(w), (to(w) - from(w) - 1) & 1, p.status);
     }
   } else if (warp >= 4) {
     // --------------------------------------------------------- softmax
@@ -289,7 +347,9 @@ __global__ void __launch_bounds__(384, 1)
     const int row = quad * 32 + lane;
     const int qw0 = (t0 + w) * kTile;
     const int qpos = qw0 + row;
-    const int nk = nkv_of(w);
+    const int jw = kv_lo(w), nk = kv_hi(w) - jw;
+    Span sp{0, 0};
+    if (SPAN) sp = load_span(p.first, p.last, b, qpos, sh.seq);
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t scol = lrow + C::S_COL + w * kTile;
     const uint32_t ocol = lrow + C::O_COL + w * D;
@@ -301,15 +361,28 @@ __global__ void __launch_bounds__(384, 1)
       ok = mbar_wait(s_full(w), j & 1, p.status);
       if (!ok) break;
       tc_fence_after();
-      const int kv0 = j * kTile;
+      const int kv0 = (jw + j) * kTile;
       int lim = kTile - 1;  // last column of this key tile that counts for the row
-      if ((sh.causal && kv0 + kTile - 1 > qw0) || kv0 + kTile > sh.seq) {
-        lim = sh.seq - 1 - kv0;
-        if (sh.causal && qpos - kv0 < lim) lim = qpos - kv0;
+      bool masked;
+      if constexpr (SPAN) {
+        masked = __any_sync(0xffffffffu, sp.lo > kv0 || sp.hi < kv0 + kTile);
+      } else {
+        if ((sh.causal && kv0 + kTile - 1 > qw0) || kv0 + kTile > sh.seq) {
+          lim = sh.seq - 1 - kv0;
+          if (sh.causal && qpos - kv0 < lim) lim = qpos - kv0;
+        }
+        // Only the diagonal key tile (causal) and the one past seq need a mask:
+        // both passes come in a masked and an unmasked form.
+        masked = lim < kTile - 1 || (sh.causal && kv0 + kTile - 1 > qw0);
       }
-      // Only the diagonal key tile (causal) and the one past seq need a mask:
-      // both passes come in a masked and an unmasked form.
-      const bool masked = lim < kTile - 1 || (sh.causal && kv0 + kTile - 1 > qw0);
+      // Whether a column counts for the row (SPAN: lo <= key < hi in one
+      // unsigned comparison).
+      const int col0 = kv0 - sp.lo;
+      const unsigned len = sp.hi - sp.lo;
+      auto counts = [&](int col) {
+        if constexpr (SPAN) return static_cast<unsigned>(col0 + col) < len;
+        return col <= lim;
+      };
       // Pass 1: the row maximum (eight interleaved chains, then a tree).
       float m8[8];
 #pragma unroll
@@ -323,7 +396,7 @@ __global__ void __launch_bounds__(384, 1)
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (!M || c4 * 32 + i <= lim) m8[i & 7] = fmaxf(m8[i & 7], __uint_as_float(r[i]));
+            if (!M || counts(c4 * 32 + i)) m8[i & 7] = fmaxf(m8[i & 7], __uint_as_float(r[i]));
         }
       };
       if (masked)
@@ -379,10 +452,10 @@ __global__ void __launch_bounds__(384, 1)
             float p2 = ex2_approx(fmaf(__uint_as_float(r[i + 2]), c, -mref));
             float p3 = exp2_poly(fmaf(__uint_as_float(r[i + 3]), c, -mref));
             if (M) {
-              if (col > lim) p0 = 0.0f;
-              if (col + 1 > lim) p1 = 0.0f;
-              if (col + 2 > lim) p2 = 0.0f;
-              if (col + 3 > lim) p3 = 0.0f;
+              if (!counts(col)) p0 = 0.0f;
+              if (!counts(col + 1)) p1 = 0.0f;
+              if (!counts(col + 2)) p2 = 0.0f;
+              if (!counts(col + 3)) p3 = 0.0f;
             }
             a4[0] += p0;
             a4[1] += p1;
@@ -407,6 +480,13 @@ __global__ void __launch_bounds__(384, 1)
     }
     if (ok && nk > 0) ok = mbar_wait(o_done(w), (nk - 1) & 1, p.status);
     tc_fence_after();
+    if (SPAN && nk == 0 && qpos < sh.seq) {  // no row of the tile sees anything
+      uint4* dst = reinterpret_cast<uint4*>(
+          p.out + ((static_cast<size_t>(b) * sh.seq + qpos) * sh.heads + h) * D);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+      p.lse[(static_cast<size_t>(b) * sh.heads + h) * sh.seq + qpos] = -INFINITY;
+    }
     if (ok && nk > 0) {
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       const bool valid = qpos < sh.seq;
@@ -466,6 +546,19 @@ __global__ void __launch_bounds__(384, 1)
 
 constexpr int kHalf = 64;  // the streamed tile of the backward kernels
 
+// SPAN: what the prep launch leaves of the spans for the other two, rows padded
+// like the statistics: each row's (lo, hi - lo) (padding rows: 0, 0), and over
+// each 64-row query tile the keys that any row sees, [lo, hi), and those that
+// every row sees, [all_lo, all_hi).
+struct SpanTile {
+  int lo, hi, all_lo, all_hi;
+};
+
+struct SpanWork {
+  int2* rows;       // [batch, seq_pad]
+  SpanTile* tiles;  // [batch, seq_pad / 64]
+};
+
 struct PrepParams {
   const uint16_t* out;
   const uint16_t* dout;
@@ -473,12 +566,40 @@ struct PrepParams {
   float* lse2;
   float* delta;
   int batch, seq, heads, seq_pad, dim;
+  const int* first;  // SPAN
+  const int* last;
+  SpanWork span;
+  unsigned row_blocks;  // SPAN: blocks from here on do the spans, a warp a tile
 };
 
 // Eight lanes per row, dim / 8 elements each.
+template <bool SPAN>
 __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const PrepParams p) {
   griddep_wait();
   griddep_launch_dependents();
+  if (SPAN && blockIdx.x >= p.row_blocks) {
+    const int tiles = p.seq_pad / kHalf;
+    const long long t = static_cast<long long>(blockIdx.x - p.row_blocks) * 8 + (threadIdx.x >> 5);
+    if (t >= static_cast<long long>(p.batch) * tiles) return;
+    const int b = static_cast<int>(t / tiles), i0 = static_cast<int>(t % tiles) * kHalf;
+    SpanTile s{p.seq, 0, 0, p.seq};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = i0 + e * 32 + (threadIdx.x & 31);
+      const Span sp = load_span(p.first, p.last, b, i, p.seq);
+      p.span.rows[static_cast<size_t>(b) * p.seq_pad + i] = make_int2(sp.lo, sp.hi - sp.lo);
+      if (sp.lo < sp.hi) s.lo = min(s.lo, sp.lo);
+      s.hi = max(s.hi, sp.hi);
+      s.all_lo = max(s.all_lo, sp.lo);
+      s.all_hi = min(s.all_hi, sp.hi);
+    }
+    s.lo = __reduce_min_sync(0xffffffffu, s.lo);
+    s.hi = __reduce_max_sync(0xffffffffu, s.hi);
+    s.all_lo = __reduce_max_sync(0xffffffffu, s.all_lo);
+    s.all_hi = __reduce_min_sync(0xffffffffu, s.all_hi);
+    if ((threadIdx.x & 31) == 0) p.span.tiles[t] = s;
+    return;
+  }
   const long long gid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const long long row = gid >> 3;
   const int sub = threadIdx.x & 7;
@@ -521,6 +642,7 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const PrepParams p) 
 
 struct BwdParams {
   AttnShape sh;
+  SpanWork span;  // SPAN
   int seq_pad;
   float scale;
   const float* lse2;
@@ -560,7 +682,7 @@ struct DqCfg {
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
-template <int D>
+template <int D, bool SPAN>
 __global__ void __launch_bounds__(384, 1)
     attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_do,
@@ -603,6 +725,7 @@ __global__ void __launch_bounds__(384, 1)
   const int hk = h / sh.group;
   const int q0 = qt * kTile;
   const int n_half = (sh.seq + kHalf - 1) / kHalf;
+  int kv_first = 0;  // first 64-key tile
   int n_kv = n_half;
   if (sh.causal && (q0 + kTile - 1) / kHalf + 1 < n_kv) n_kv = (q0 + kTile - 1) / kHalf + 1;
 
@@ -637,6 +760,14 @@ __global__ void __launch_bounds__(384, 1)
   griddep_launch_dependents();
   griddep_wait();
 
+  if constexpr (SPAN) {  // the key tiles that either 64-row half of the tile sees
+    const SpanTile* t =
+        p.span.tiles + static_cast<size_t>(b) * (p.seq_pad / kHalf) + 2 * qt;
+    const SpanTile u = t[0], v = t[1];
+    kv_first = min(u.lo, v.lo) / kHalf;
+    n_kv = max((max(u.hi, v.hi) + kHalf - 1) / kHalf - kv_first, 0);
+  }
+
   if (warp == 0) {
     // ------------------------------------------------------------- TMA
     if (elect_one_sync()) {
@@ -655,12 +786,14 @@ __global__ void __launch_bounds__(384, 1)
         if (!mbar_wait(k_empty(ks), ((j / KST) & 1) ^ 1, p.status)) break;
         mbar_arrive_expect_tx(k_full(ks), C::KTILE);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(k_s(ks) + sl * C::KSLAB, &tm_k, k_full(ks), sl * 64, hk, j * kHalf, b);
+          tma_load_4d(k_s(ks) + sl * C::KSLAB, &tm_k, k_full(ks), sl * 64, hk,
+                      (kv_first + j) * kHalf, b);
         ++nk;
         if (!mbar_wait(v_empty(vs), ((j / VST) & 1) ^ 1, p.status)) break;
         mbar_arrive_expect_tx(v_full(vs), C::KTILE);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(v_s(vs) + sl * C::KSLAB, &tm_v, v_full(vs), sl * 64, hk, j * kHalf, b);
+          tma_load_4d(v_s(vs) + sl * C::KSLAB, &tm_v, v_full(vs), sl * 64, hk,
+                      (kv_first + j) * kHalf, b);
         ++nv;
       }
       mbar_wait(q_full, 0, p.status);
@@ -739,6 +872,8 @@ __global__ void __launch_bounds__(384, 1)
     const float lse2 = p.lse2[srow];
     const float dl = p.delta[srow];
     const float c = sh.scale_log2;
+    int2 sp = make_int2(0, 0);  // first key and how many
+    if (SPAN) sp = p.span.rows[static_cast<size_t>(b) * p.seq_pad + qpos];
     bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
       ok = mbar_wait(s_full(j & 1), (j >> 1) & 1, p.status);
@@ -751,20 +886,25 @@ __global__ void __launch_bounds__(384, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free(j & 1));
-      const int kv0 = j * kHalf + half * 32;
+      const int kv0 = (kv_first + j) * kHalf + half * 32;
       int lim = 31;  // last column of this half tile that counts
-      if ((sh.causal && kv0 + 31 > q0) || kv0 + 32 > sh.seq) {
+      if (!SPAN && ((sh.causal && kv0 + 31 > q0) || kv0 + 32 > sh.seq)) {
         lim = sh.seq - 1 - kv0;
         if (sh.causal && qpos - kv0 < lim) lim = qpos - kv0;
       }
+      auto counts = [&](int col) {
+        if constexpr (SPAN)
+          return static_cast<unsigned>(kv0 + col - sp.x) < static_cast<unsigned>(sp.y);
+        return col <= lim;
+      };
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         float p0 = ex2_approx(fmaf(__uint_as_float(sv[i]), c, -lse2));
         float p1 = (i & 2) ? exp2_poly(fmaf(__uint_as_float(sv[i + 1]), c, -lse2))
                            : ex2_approx(fmaf(__uint_as_float(sv[i + 1]), c, -lse2));
-        if (i > lim) p0 = 0.0f;
-        if (i + 1 > lim) p1 = 0.0f;
+        if (!counts(i)) p0 = 0.0f;
+        if (!counts(i + 1)) p1 = 0.0f;
         pk[i / 2] = pack_bf16x2_f32(p0 * (__uint_as_float(dv[i]) - dl),
                                     p1 * (__uint_as_float(dv[i + 1]) - dl));
       }
@@ -784,6 +924,10 @@ __global__ void __launch_bounds__(384, 1)
         uint32_t o[32];
         tmem_ld_32x32b_x32(lrow + C::DQ_COL + c4 * 32, o);
         tmem_ld_wait();
+        if (SPAN && n_kv == 0) {  // no row of the tile sees anything
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -840,7 +984,7 @@ struct DkvCfg {
   static_assert(SMEM > 118784, "one CTA per SM");
 };
 
-template <int D>
+template <int D, bool SPAN>
 __global__ void __launch_bounds__(384, 1)
     attn_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_do,
@@ -882,9 +1026,13 @@ __global__ void __launch_bounds__(384, 1)
   const int hk = bk % sh.kv_heads;
   const int kv0 = jt * kTile;
   const int n_half = (sh.seq + kHalf - 1) / kHalf;
-  const int i0 = sh.causal ? kv0 / kHalf : 0;  // first query tile that sees this key tile
-  const int nq = n_half - i0;
-  const int T = sh.group * nq;
+  int i0 = sh.causal ? kv0 / kHalf : 0;  // first query tile that sees this key tile
+  int nq = n_half - i0;
+  __shared__ int seen[2];  // SPAN: the first and last query tile that see it
+  if (SPAN && threadIdx.x == 0) {
+    seen[0] = n_half;
+    seen[1] = -1;
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -912,6 +1060,27 @@ __global__ void __launch_bounds__(384, 1)
   // kernel's CTA placed on this SM may then wait for it, never hold it.
   griddep_launch_dependents();
   griddep_wait();
+
+  const SpanTile* const tiles =
+      SPAN ? p.span.tiles + static_cast<size_t>(b) * (p.seq_pad / kHalf) : nullptr;
+  if constexpr (SPAN) {
+    int a = n_half, z = -1;
+    for (int i = threadIdx.x; i < n_half; i += 384)
+      if (tiles[i].lo < kv0 + kTile && tiles[i].hi > kv0) {
+        a = min(a, i);
+        z = i;
+      }
+    a = __reduce_min_sync(0xffffffffu, a);
+    z = __reduce_max_sync(0xffffffffu, z);
+    if (lane == 0) {
+      atomicMin(&seen[0], a);
+      atomicMax(&seen[1], z);
+    }
+    __syncthreads();
+    i0 = seen[0];
+    nq = max(seen[1] + 1 - i0, 0);
+  }
+  const int T = sh.group * nq;
 
   if (warp == 0) {
     // ------------------------------------------------------------- TMA
@@ -1031,7 +1200,17 @@ __global__ void __launch_bounds__(384, 1)
       // A key row sees query q only if q >= kvpos (causal); rows past seq
       // carry lse2 = +inf, so their probabilities are 0 already.
       int first = 0;
-      if (sh.causal && qq0 < kvpos) first = kvpos - qq0;
+      if (!SPAN && sh.causal && qq0 < kvpos) first = kvpos - qq0;
+      // SPAN: the rows' spans, unless every row of the query tile sees the
+      // whole key tile (the spans do not fit beside the tiles in shared
+      // memory; all threads read the same few words, from L1).
+      bool whole = true;
+      const int2* spans = nullptr;
+      if constexpr (SPAN) {
+        const SpanTile st4 = tiles[i0 + t % nq];
+        whole = st4.all_lo <= kv0 && st4.all_hi >= kv0 + kTile;
+        spans = p.span.rows + static_cast<size_t>(b) * p.seq_pad + qq0;
+      }
       uint32_t pk[16], dk[16];
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
@@ -1044,7 +1223,14 @@ __global__ void __launch_bounds__(384, 1)
         for (int e = 0; e < 4; ++e) {
           const float x = fmaf(__uint_as_float(sv[i + e]), c, -la[e]);
           float pe = e == 3 ? exp2_poly(x) : ex2_approx(x);
-          if (i + e < first) pe = 0.0f;
+          if constexpr (SPAN) {
+            if (!whole) {
+              const int2 sp = spans[i + e];
+              if (static_cast<unsigned>(kvpos - sp.x) >= static_cast<unsigned>(sp.y)) pe = 0.0f;
+            }
+          } else {
+            if (i + e < first) pe = 0.0f;
+          }
           pv[e] = pe;
           dsv[e] = pe * (__uint_as_float(dv[i + e]) - da[e]);
         }
@@ -1088,6 +1274,10 @@ __global__ void __launch_bounds__(384, 1)
           uint32_t o[32];
           tmem_ld_32x32b_x32(lrow + col + c4 * 32, o);
           tmem_ld_wait();
+          if (SPAN && T == 0) {  // no query sees the key tile
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0;
+          }
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -1157,11 +1347,11 @@ AttnShape make_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads
   return s;
 }
 
-template <int D>
-int launch_fwd(const void* q, const void* k, const void* v, const AttnShape& sh, void* out,
-               float* lse, int* status, cudaStream_t stream) {
+template <int D, bool SPAN>
+int launch_fwd(const void* q, const void* k, const void* v, const int* first, const int* last,
+               const AttnShape& sh, void* out, float* lse, int* status, cudaStream_t stream) {
   using C = FwdCfg<D>;
-  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_fwd_kernel<D>), C::SMEM,
+  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_fwd_kernel<D, SPAN>), C::SMEM,
                              "cudaFuncSetAttribute(attn_fwd)");
   if (rc) return rc;
   CUtensorMap tq_, tk, tv;
@@ -1170,25 +1360,58 @@ int launch_fwd(const void* q, const void* k, const void* v, const AttnShape& sh,
   if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
   FwdParams p{};
   p.sh = sh;
+  p.first = first;
+  p.last = last;
   p.n_pairs = (sh.n_tiles + 1) / 2;
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.status = status;
   const unsigned grid = static_cast<unsigned>(sh.batch) * sh.heads * p.n_pairs;
-  return launch_kernel(attn_fwd_kernel<D>, dim3(grid), dim3(384), C::SMEM, stream, 1,
+  return launch_kernel(attn_fwd_kernel<D, SPAN>, dim3(grid), dim3(384), C::SMEM, stream, 1,
                        "attention forward launch", tq_, tk, tv, p);
 }
 
-template <int D>
-int launch_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
-               const float* lse, const AttnShape& sh, float scale, void* dq, void* dk, void* dv,
-               float* lse2, float* delta, int seq_pad, int* status, cudaStream_t stream) {
+// What the caller's workspace holds: two statistics per query row and, for
+// spans, each row's and each query tile's.
+struct BwdWork {
+  float* lse2;
+  float* delta;
+  SpanWork span;
+  int seq_pad;
+  size_t bytes;
+};
+
+BwdWork bwd_work(void* base, int64_t batch, int64_t seq, int64_t heads, bool span) {
+  const int64_t seq_pad = (seq + kTile - 1) / kTile * kTile;
+  const size_t rows = static_cast<size_t>(batch * seq_pad);
+  BwdWork w{};
+  w.seq_pad = static_cast<int>(seq_pad);
+  w.lse2 = static_cast<float*>(base);
+  w.delta = w.lse2 + rows * heads;
+  w.bytes = 2 * rows * heads * sizeof(float);
+  if (span) {
+    w.span.rows = reinterpret_cast<int2*>(static_cast<uint8_t*>(base) + w.bytes);
+    w.bytes += rows * sizeof(int2);
+    w.span.tiles = reinterpret_cast<SpanTile*>(static_cast<uint8_t*>(base) + w.bytes);
+    w.bytes += rows / kHalf * sizeof(SpanTile);
+  }
+  return w;
+}
+
+template <int D, bool SPAN>
+int launch_bwd(const void* q, const void* k, const void* v, const int* first, const int* last,
+               const void* out, const void* dout, const float* lse, const AttnShape& sh,
+               float scale, void* dq, void* dk, void* dv, const BwdWork& work, int* status,
+               cudaStream_t stream) {
+  float* const lse2 = work.lse2;
+  float* const delta = work.delta;
+  const int seq_pad = work.seq_pad;
   using Q = DqCfg<D>;
   using KV = DkvCfg<D>;
-  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dq_kernel<D>), Q::SMEM,
+  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dq_kernel<D, SPAN>), Q::SMEM,
                              "cudaFuncSetAttribute(attn_bwd_dq)");
   if (rc) return rc;
-  rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dkv_kernel<D>), KV::SMEM,
+  rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dkv_kernel<D, SPAN>), KV::SMEM,
                          "cudaFuncSetAttribute(attn_bwd_dkv)");
   if (rc) return rc;
   PrepParams pp{};
@@ -1203,8 +1426,15 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
   pp.seq_pad = seq_pad;
   pp.dim = D;
   const long long rows = static_cast<long long>(sh.batch) * sh.heads * seq_pad;
-  rc = launch_kernel(attn_bwd_prep_kernel, dim3(static_cast<unsigned>((rows * 8 + 255) / 256)),
-                     dim3(256), 0, stream, 1, "attention backward prep launch", pp);
+  pp.first = first;
+  pp.last = last;
+  pp.span = work.span;
+  pp.row_blocks = static_cast<unsigned>((rows * 8 + 255) / 256);
+  const unsigned span_blocks =
+      SPAN ? static_cast<unsigned>((static_cast<long long>(sh.batch) * (seq_pad / kHalf) + 7) / 8)
+           : 0;
+  rc = launch_kernel(attn_bwd_prep_kernel<SPAN>, dim3(pp.row_blocks + span_blocks), dim3(256), 0,
+                     stream, 1, "attention backward prep launch", pp);
   if (rc) return rc;
   // Query-side maps (128-row boxes for dq, 64-row boxes for dkv) and the
   // key/value maps the other way round.
@@ -1219,6 +1449,7 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
   if ((rc = map_bshd(&v128, v, sh.batch, sh.seq, sh.kv_heads, D, kTile))) return rc;
   BwdParams p{};
   p.sh = sh;
+  p.span = work.span;
   p.seq_pad = seq_pad;
   p.scale = scale;
   p.lse2 = lse2;
@@ -1228,12 +1459,214 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
   p.dv = static_cast<uint16_t*>(dv);
   p.status = status;
   const unsigned grid_q = static_cast<unsigned>(sh.batch) * sh.heads * sh.n_tiles;
-  rc = launch_kernel(attn_bwd_dq_kernel<D>, dim3(grid_q), dim3(384), Q::SMEM, stream, 1,
+  rc = launch_kernel(attn_bwd_dq_kernel<D, SPAN>, dim3(grid_q), dim3(384), Q::SMEM, stream, 1,
                      "attention backward dq launch", q128, do128, k64, v64, p);
   if (rc) return rc;
   const unsigned grid_kv = static_cast<unsigned>(sh.batch) * sh.kv_heads * sh.n_tiles;
-  return launch_kernel(attn_bwd_dkv_kernel<D>, dim3(grid_kv), dim3(384), KV::SMEM, stream, 1,
+  return launch_kernel(attn_bwd_dkv_kernel<D, SPAN>, dim3(grid_kv), dim3(384), KV::SMEM, stream, 1,
                        "attention backward dkv launch", q64, do64, k128, v128, p);
+}
+
+int attention_fwd(const void* q, const void* k, const void* v, const int* first, const int* last,
+                  bool span, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
+                  int64_t head_dim, float scale, int causal, void* out, float* lse,
+                  void* stream) {
+  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
+  if (rc) return rc;
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
+  if (batch == 0 || seq == 0) return TQ_OK;
+  if (!q || !k || !v || !out || !lse || (span && (!first || !last)))
+    return fail(TQ_ERR_INVALID, "attention: null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      !aligned(lse, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: q, k, v and out must be 16-byte aligned");
+  if (!aligned(first, 4) || !aligned(last, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: first and last must be 4-byte aligned");
+  int* status = device_status_ptr(&rc);
+  if (!status) return rc;
+  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
+  auto launch = head_dim == 64 ? (span ? launch_fwd<64, true> : launch_fwd<64, false>)
+                               : (span ? launch_fwd<128, true> : launch_fwd<128, false>);
+  return launch(q, k, v, first, last, sh, out, lse, status, as_stream(stream));
+}
+
+int bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads, bool span, size_t* bytes) {
+  if (!bytes) return fail(TQ_ERR_INVALID, "attention: null bytes pointer");
+  if (batch < 0 || seq < 0 || heads <= 0)
+    return fail(TQ_ERR_INVALID, "attention: batch and seq must be >= 0, heads > 0");
+  *bytes = bwd_work(nullptr, batch, seq, heads, span).bytes;
+  return TQ_OK;
+}
+
+int attention_bwd(const void* q, const void* k, const void* v, const int* first, const int* last,
+                  bool span, const void* out, const void* dout, const float* lse, int64_t batch,
+                  int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
+                  int causal, void* dq, void* dk, void* dv, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
+  if (rc) return rc;
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
+  if (batch == 0 || seq == 0) return TQ_OK;
+  size_t need = 0;
+  rc = bwd_workspace_bytes(batch, seq, heads, span, &need);
+  if (rc) return rc;
+  if (workspace_bytes < need)
+    return fail(TQ_ERR_INVALID, "attention: workspace of %zu bytes, %zu needed", workspace_bytes,
+                need);
+  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace ||
+      (span && (!first || !last)))
+    return fail(TQ_ERR_INVALID, "attention: null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
+      !aligned(workspace, 256) || !aligned(lse, 4))
+    return fail(TQ_ERR_MISALIGNED,
+                "attention: tensors must be 16-byte aligned and the workspace 256-byte aligned");
+  if (!aligned(first, 4) || !aligned(last, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: first and last must be 4-byte aligned");
+  int* status = device_status_ptr(&rc);
+  if (!status) return rc;
+  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
+  const BwdWork work = bwd_work(workspace, batch, seq, heads, span);
+  auto launch = head_dim == 64 ? (span ? launch_bwd<64, true> : launch_bwd<64, false>)
+                               : (span ? launch_bwd<128, true> : launch_bwd<128, false>);
+  return launch(q, k, v, first, last, out, dout, lse, sh, scale, dq, dk, dv, work, status,
+                as_stream(stream));
+}
+
+// --------------------------------------------------------- document spans --
+
+constexpr int kScanThreads = 1024;
+constexpr int kScanItems = 4;
+
+struct DocParams {
+  const void* documents;
+  const int* prefix;  // may be null
+  int ids64, seq, causal;
+  int* first;
+  int* last;
+};
+
+// Inclusive scan over the block's threads (max, or min from the other end) of
+// one int a thread.
+template <bool BACK>
+__device__ __forceinline__ int scan_threads(int v, int* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = BACK ? __shfl_down_sync(0xffffffffu, v, off) : __shfl_up_sync(0xffffffffu, v, off);
+    if (BACK ? lane + off < 32 : lane >= off) v = BACK ? min(v, o) : max(v, o);
+  }
+  __syncthreads();  // the last call's reads of sh
+  if (lane == (BACK ? 0 : 31)) sh[warp] = v;
+  __syncthreads();
+  if (BACK) {
+    for (int i = warp + 1; i < kScanThreads / 32; ++i) v = min(v, sh[i]);
+  } else {
+    for (int i = 0; i < warp; ++i) v = max(v, sh[i]);
+  }
+  return v;
+}
+
+// One CTA per row of ids.  A document is a run of equal ids: its start reaches
+// its positions by a running maximum of the runs' starts from the front, its
+// end by a running minimum from the back, stretch by stretch.
+__global__ void __launch_bounds__(kScanThreads) document_spans_kernel(const DocParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ int sh[kScanThreads / 32];
+  __shared__ int carry;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * p.seq;
+  auto id = [&](int i) -> int64_t {
+    return p.ids64 ? static_cast<const int64_t*>(p.documents)[base + i]
+                   : static_cast<const int*>(p.documents)[base + i];
+  };
+  constexpr int kStretch = kScanThreads * kScanItems;
+  const int stretches = (p.seq + kStretch - 1) / kStretch;
+  const bool ends = !p.causal || p.prefix;
+  int from = 0;  // the start of the run that reaches into the stretch
+  for (int s = 0; s < stretches; ++s) {
+    const int i0 = s * kStretch + threadIdx.x * kScanItems;
+    int start[kScanItems];
+    bool padding[kScanItems];
+    int run = 0;
+    int64_t prev = i0 > 0 && i0 <= p.seq ? id(i0 - 1) : 0;
+#pragma unroll
+    for (int e = 0; e < kScanItems; ++e) {
+      const int i = i0 + e;
+      padding[e] = true;
+      if (i < p.seq) {
+        const int64_t now = id(i);
+        padding[e] = now < 0;
+        if (i == 0 || now != prev) run = i;
+        prev = now;
+      }
+      start[e] = run;
+    }
+    int before = scan_threads<false>(run, sh);
+    if (threadIdx.x == kScanThreads - 1) carry = max(before, from);
+    // The thread before this one's scan is what reaches in here.
+    int in = __shfl_up_sync(0xffffffffu, before, 1);
+    if ((threadIdx.x & 31) == 0) {
+      in = 0;
+      for (int i = 0; i < static_cast<int>(threadIdx.x >> 5); ++i) in = max(in, sh[i]);
+    }
+    in = max(in, from);
+    __syncthreads();
+    from = carry;
+#pragma unroll
+    for (int e = 0; e < kScanItems; ++e) {
+      const int i = i0 + e;
+      if (i >= p.seq) continue;
+      p.first[base + i] = max(start[e], in);
+      if (!ends || padding[e]) p.last[base + i] = padding[e] ? max(start[e], in) : i + 1;
+    }
+  }
+  if (!ends) return;
+  int next = p.seq;  // the start of the run after the stretch's last
+  for (int s = stretches - 1; s >= 0; --s) {
+    const int i0 = s * kStretch + threadIdx.x * kScanItems;
+    int end[kScanItems];
+    bool padding[kScanItems];
+    int run = p.seq;
+    int64_t after = i0 + kScanItems < p.seq ? id(i0 + kScanItems) : 0;
+#pragma unroll
+    for (int e = kScanItems - 1; e >= 0; --e) {
+      const int i = i0 + e;
+      padding[e] = true;
+      if (i < p.seq) {
+        const int64_t now = id(i);
+        padding[e] = now < 0;
+        if (i + 1 < p.seq && now != after) run = i + 1;
+        after = now;
+      }
+      end[e] = run;
+    }
+    int behind = scan_threads<true>(run, sh);
+    if (threadIdx.x == 0) carry = min(behind, next);
+    int in = __shfl_down_sync(0xffffffffu, behind, 1);
+    if ((threadIdx.x & 31) == 31) {
+      in = p.seq;
+      for (int i = static_cast<int>(threadIdx.x >> 5) + 1; i < kScanThreads / 32; ++i)
+        in = min(in, sh[i]);
+    }
+    in = min(in, next);
+    __syncthreads();
+    next = carry;
+#pragma unroll
+    for (int e = 0; e < kScanItems; ++e) {
+      const int i = i0 + e;
+      if (i >= p.seq || padding[e]) continue;
+      const int stop = min(end[e], in);
+      int last = stop;
+      if (p.causal) {
+        const int64_t seen = static_cast<int64_t>(p.first[base + i]) + max(p.prefix[base + i], 0);
+        last = max(i + 1, seen < stop ? static_cast<int>(seen) : stop);
+      }
+      p.last[base + i] = last;
+    }
+  }
 }
 
 }  // namespace
@@ -1242,32 +1675,13 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
 extern "C" int tq_attention_fwd(const void* q, const void* k, const void* v, int64_t batch,
                                 int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                 float scale, int causal, void* out, float* lse, void* stream) {
-  using namespace tq;
-  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
-  if (rc) return rc;
-  if (!(scale > 0.0f) || !std::isfinite(scale))
-    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
-  if (batch == 0 || seq == 0) return TQ_OK;
-  if (!q || !k || !v || !out || !lse) return fail(TQ_ERR_INVALID, "attention: null pointer");
-  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
-      !aligned(lse, 4))
-    return fail(TQ_ERR_MISALIGNED, "attention: q, k, v and out must be 16-byte aligned");
-  int* status = device_status_ptr(&rc);
-  if (!status) return rc;
-  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
-  if (head_dim == 64) return launch_fwd<64>(q, k, v, sh, out, lse, status, as_stream(stream));
-  return launch_fwd<128>(q, k, v, sh, out, lse, status, as_stream(stream));
+  return tq::attention_fwd(q, k, v, nullptr, nullptr, false, batch, seq, heads, kv_heads, head_dim,
+                           scale, causal, out, lse, stream);
 }
 
 extern "C" int tq_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
                                                 size_t* bytes) {
-  using namespace tq;
-  if (!bytes) return fail(TQ_ERR_INVALID, "attention: null bytes pointer");
-  if (batch < 0 || seq < 0 || heads <= 0)
-    return fail(TQ_ERR_INVALID, "attention: batch and seq must be >= 0, heads > 0");
-  const int64_t seq_pad = (seq + kTile - 1) / kTile * kTile;
-  *bytes = static_cast<size_t>(2 * batch * heads * seq_pad) * sizeof(float);
-  return TQ_OK;
+  return tq::bwd_workspace_bytes(batch, seq, heads, false, bytes);
 }
 
 extern "C" int tq_attention_bwd(const void* q, const void* k, const void* v, const void* out,
@@ -1275,34 +1689,56 @@ extern "C" int tq_attention_bwd(const void* q, const void* k, const void* v, con
                                 int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
                                 int causal, void* dq, void* dk, void* dv, void* workspace,
                                 size_t workspace_bytes, void* stream) {
+  return tq::attention_bwd(q, k, v, nullptr, nullptr, false, out, dout, lse, batch, seq, heads,
+                           kv_heads, head_dim, scale, causal, dq, dk, dv, workspace,
+                           workspace_bytes, stream);
+}
+
+extern "C" int tq_span_attention_fwd(const void* q, const void* k, const void* v,
+                                     const int32_t* first, const int32_t* last, int64_t batch,
+                                     int64_t seq, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, float scale, void* out, float* lse,
+                                     void* stream) {
+  return tq::attention_fwd(q, k, v, first, last, true, batch, seq, heads, kv_heads, head_dim,
+                           scale, 0, out, lse, stream);
+}
+
+extern "C" int tq_span_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
+                                                     size_t* bytes) {
+  return tq::bwd_workspace_bytes(batch, seq, heads, true, bytes);
+}
+
+extern "C" int tq_span_attention_bwd(const void* q, const void* k, const void* v,
+                                     const int32_t* first, const int32_t* last, const void* out,
+                                     const void* dout, const float* lse, int64_t batch,
+                                     int64_t seq, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, float scale, void* dq, void* dk, void* dv,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  return tq::attention_bwd(q, k, v, first, last, true, out, dout, lse, batch, seq, heads, kv_heads,
+                           head_dim, scale, 0, dq, dk, dv, workspace, workspace_bytes, stream);
+}
+
+extern "C" int tq_document_spans(const void* documents, int ids_bits, const int32_t* prefix,
+                                 int64_t batch, int64_t seq, int causal, int32_t* first,
+                                 int32_t* last, void* stream) {
   using namespace tq;
-  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
-  if (rc) return rc;
-  if (!(scale > 0.0f) || !std::isfinite(scale))
-    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
+  if (ids_bits != 32 && ids_bits != 64)
+    return fail(TQ_ERR_UNSUPPORTED, "document_spans: document ids must be 32- or 64-bit integers");
+  if (batch < 0 || seq < 0 || batch > (1ll << 31) - 1 || seq > (1ll << 30))
+    return fail(TQ_ERR_INVALID, "document_spans: batch and seq must be >= 0, seq at most 2^30");
   if (batch == 0 || seq == 0) return TQ_OK;
-  size_t need = 0;
-  rc = tq_attention_bwd_workspace_bytes(batch, seq, heads, &need);
-  if (rc) return rc;
-  if (workspace_bytes < need)
-    return fail(TQ_ERR_INVALID, "attention: workspace of %zu bytes, %zu needed", workspace_bytes,
-                need);
-  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace)
-    return fail(TQ_ERR_INVALID, "attention: null pointer");
-  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
-      !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
-      !aligned(workspace, 256) || !aligned(lse, 4))
-    return fail(TQ_ERR_MISALIGNED,
-                "attention: tensors must be 16-byte aligned and the workspace 256-byte aligned");
-  int* status = device_status_ptr(&rc);
-  if (!status) return rc;
-  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
-  const int seq_pad = sh.n_tiles * kTile;
-  float* lse2 = static_cast<float*>(workspace);
-  float* delta = lse2 + static_cast<size_t>(batch * heads) * seq_pad;
-  if (head_dim == 64)
-    return launch_bwd<64>(q, k, v, out, dout, lse, sh, scale, dq, dk, dv, lse2, delta, seq_pad,
-                          status, as_stream(stream));
-  return launch_bwd<128>(q, k, v, out, dout, lse, sh, scale, dq, dk, dv, lse2, delta, seq_pad,
-                         status, as_stream(stream));
+  if (!documents || !first || !last) return fail(TQ_ERR_INVALID, "document_spans: null pointer");
+  if (!aligned(documents, ids_bits / 8) || !aligned(prefix, 4) || !aligned(first, 4) ||
+      !aligned(last, 4))
+    return fail(TQ_ERR_MISALIGNED, "document_spans: a pointer is not aligned to its type");
+  DocParams p{};
+  p.documents = documents;
+  p.prefix = causal ? prefix : nullptr;
+  p.ids64 = ids_bits == 64;
+  p.seq = static_cast<int>(seq);
+  p.causal = causal ? 1 : 0;
+  p.first = first;
+  p.last = last;
+  return launch_kernel(document_spans_kernel, dim3(static_cast<unsigned>(batch)),
+                       dim3(kScanThreads), 0, as_stream(stream), 1, "document_spans launch", p);
 }

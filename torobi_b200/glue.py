@@ -212,6 +212,133 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     return _Attention.apply(q, k, v, causal, scale)
 
 
+def document_spans(documents: torch.Tensor, prefix: torch.Tensor | None = None,
+                   causal: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """The spans ``span_attention`` takes, of rows that pack documents:
+    ``(first, last)`` int32 [batch, seq], position i seeing the positions
+    ``first <= j < last``.
+
+    documents int32 or int64 [batch, seq]: a run of equal ids is one document,
+    a negative id is padding and sees nothing.  A position sees its document up
+    to itself (``causal``) or whole; with ``prefix`` (int32 or int64 [batch,
+    seq], causal only: the document's prompt length, at each of its positions)
+    every position also sees its document's first ``prefix`` positions."""
+    op = "document_spans"
+    _one_device(op, documents=documents, prefix=prefix)
+    if documents.dim() != 2 or documents.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"[{op}] documents must be int32 or int64 [batch, seq], got "
+                         f"{documents.dtype} {tuple(documents.shape)}")
+    if prefix is not None:
+        if not causal:
+            raise ValueError(f"[{op}] a prefix goes with causal=True")
+        if prefix.shape != documents.shape or prefix.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"[{op}] prefix must be int32 or int64 {tuple(documents.shape)}, got "
+                             f"{prefix.dtype} {tuple(prefix.shape)}")
+        prefix = prefix.to(torch.int32).contiguous()
+    documents = documents.contiguous()
+    b, s = documents.shape
+    first = torch.empty(b, s, dtype=torch.int32, device=documents.device)
+    last = torch.empty_like(first)
+    with torch.cuda.device(documents.device):
+        _launch("document_spans", lambda: lib().tq_document_spans(
+            _ptr(documents), 8 * documents.element_size(), _ptr(prefix), b, s, int(bool(causal)),
+            _ptr(first), _ptr(last), _stream()))
+    return first, last
+
+
+def _span_operands(op: str, q, k, v, first, last):
+    q, k, v = (_bf16_contig(n, t) for n, t in (("q", q), ("k", k), ("v", v)))
+    if q.dim() != 4 or k.shape != v.shape or k.dim() != 4:
+        raise ValueError(f"[{op}] q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
+                         "want [batch, seq, heads, dim] and equal k/v")
+    b, s, _, d = q.shape
+    if k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
+        raise ValueError(f"[{op}] k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+    for name, t in (("first", first), ("last", last)):
+        if t.dtype != torch.int32 or t.shape != (b, s):
+            raise ValueError(f"[{op}] {name} must be int32 [{b}, {s}], got {t.dtype} "
+                             f"{tuple(t.shape)}")
+    return q, k, v, first.contiguous(), last.contiguous()
+
+
+def span_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                           first: torch.Tensor, last: torch.Tensor,
+                           scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``attention_forward`` with a span of keys for every query in place of
+    the causal rule: query i of a row sees ``first[b, i] <= j < last[b, i]``
+    (int32 [batch, seq], taken within [0, seq]); one that sees nothing gets o =
+    0 and lse = -inf.  Returns o and lse."""
+    op = "span_attention"
+    _one_device(op, q=q, k=k, v=v, first=first, last=last)
+    q, k, v, first, last = _span_operands(op, q, k, v, first, last)
+    b, s, h, d = q.shape
+    sc = float(scale) if scale is not None else d ** -0.5
+    o = torch.empty_like(q)
+    lse = torch.empty(b, h, s, dtype=torch.float32, device=q.device)
+    with torch.cuda.device(q.device):
+        _launch("attention", lambda: lib().tq_span_attention_fwd(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), b, s, h, k.shape[2], d, sc,
+            _ptr(o), _ptr(lse), _stream()))
+    return o, lse
+
+
+def span_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            first: torch.Tensor, last: torch.Tensor, o: torch.Tensor,
+                            do: torch.Tensor, lse: torch.Tensor, scale: float | None = None):
+    """dq, dk, dv of ``span_attention_forward`` given the upstream gradient do
+    (q's layout) and the forward's o and lse."""
+    op = "span_attention"
+    _one_device(op, q=q, k=k, v=v, first=first, last=last, o=o, do=do, lse=lse)
+    q, k, v, first, last = _span_operands(op, q, k, v, first, last)
+    o, do = _bf16_contig("o", o), _bf16_contig("do", do)
+    if o.shape != q.shape or do.shape != q.shape:
+        raise ValueError(f"[{op}] o and do must have q's shape")
+    b, s, h, d = q.shape
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (b, h, s):
+        raise ValueError(f"[{op}] lse must be f32 [{b}, {h}, {s}]")
+    lse = lse.contiguous()
+    sc = float(scale) if scale is not None else d ** -0.5
+    nbytes = ctypes.c_size_t()
+    check(lib().tq_span_attention_bwd_workspace_bytes(b, s, h, ctypes.byref(nbytes)))
+    ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=q.device)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    with torch.cuda.device(q.device):
+        _launch("attention", lambda: lib().tq_span_attention_bwd(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), _ptr(o), _ptr(do), _ptr(lse), b,
+            s, h, k.shape[2], d, sc, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), nbytes.value,
+            _stream()))
+    return dq, dk, dv
+
+
+class _SpanAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, first, last, scale):
+        o, lse = span_attention_forward(q, k, v, first, last, scale)
+        ctx.save_for_backward(q, k, v, first, last, o, lse)
+        ctx.scale = scale
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, first, last, o, lse = ctx.saved_tensors
+        dq, dk, dv = span_attention_backward(q, k, v, first, last, o, do, lse, ctx.scale)
+        return dq, dk, dv, None, None, None
+
+
+def span_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: torch.Tensor,
+                   last: torch.Tensor, scale: float | None = None) -> torch.Tensor:
+    """Differentiable grouped-query attention in which query i sees the keys
+    ``first[b, i] <= j < last[b, i]``: documents packed into one row, prompts
+    seen in both directions, sliding windows, padding (``document_spans`` makes
+    the first two).  q [batch, seq, heads, dim], k/v [batch, seq, kv_heads,
+    dim] bf16, dim 64 or 128; first/last int32 [batch, seq]; output in q's
+    layout; the scale defaults to dim^-1/2.  A query that sees nothing gets 0
+    and passes no gradient.  What a query does not see still enters products
+    with 0, so k and v, and q of queries that see nothing, must be finite."""
+    return _SpanAttention.apply(q, k, v, first, last, scale)
+
+
 class _SwiGLU(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, u):
