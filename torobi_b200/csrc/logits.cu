@@ -75,6 +75,37 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 
+// Pairs of f32, one instruction for two.
+struct F2 {
+  uint64_t v;
+};
+
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(F2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 // ------------------------------------------------------------------- rows --
 
 template <typename T>
@@ -232,24 +263,29 @@ __device__ __forceinline__ void add_chunks(Sums& v, const uint32_t (&w)[U][8], f
   const float m = max_nan(v.m, mx);
   if (m == -INFINITY) return;
   move_to<M>(v, m, c);
-  float s[2] = {0.0f, 0.0f}, a[2] = {0.0f, 0.0f};
+  F2 s = f2(0.0f, 0.0f), a = s;
+  const F2 minus_m = f2(-m, -m), cc = f2(c, c), c1 = f2(kLog2e, kLog2e);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float f[CH];
     Elem<T>::unpack(w[u], f);
 #pragma unroll
-    for (int e = 0; e < CH; ++e) {
-      const float d = f[e] - m;
-      float x = d * c;
-      if (M == kEntropy) x = max_nan(x, -200.0f);
-      const float p = ex2_approx(x);
-      s[e & 1] += p;
-      if (M == kEntropy) a[e & 1] = fmaf(p, x, a[e & 1]);
-      if (M == kTwo) a[e & 1] += ex2_approx(d * kLog2e);
+    for (int e = 0; e < CH; e += 2) {
+      const F2 d = f2(f[e], f[e + 1]) + minus_m;
+      float2 x = split(d * cc);
+      if (M == kEntropy) x = make_float2(max_nan(x.x, -200.0f), max_nan(x.y, -200.0f));
+      const F2 p = f2(ex2_approx(x.x), ex2_approx(x.y));
+      s = s + p;
+      if (M == kEntropy) a = fma2(p, f2(x.x, x.y), a);
+      if (M == kTwo) {
+        const float2 y = split(d * c1);
+        a = a + f2(ex2_approx(y.x), ex2_approx(y.y));
+      }
     }
   }
-  v.s += s[0] + s[1];
-  if (M != kPlain) v.a += a[0] + a[1];
+  const float2 ss = split(s), aa = split(a);
+  v.s += ss.x + ss.y;
+  if (M != kPlain) v.a += aa.x + aa.y;
 }
 
 // The block's sums, in sh[0] for every thread after the call.
@@ -623,15 +659,26 @@ __device__ __forceinline__ void row_gradient(const T* z, T* dz, int vocab, int p
   if constexpr (SAME) {
     const int lo = max(c0, row.lo), hi = min(c1, row.hi);
     T* const out = dz - row.off;
-#pragma unroll 2
-    for (int c = lo + threadIdx.x; c < hi; c += kThreads) {
-      uint32_t w[8];
+    auto finish = [&](int c, uint32_t(&w)[8]) {
       float f[CH];
-      ld_chunk(row.chunk(c), w);
       Elem<T>::unpack(w, f);
       grad(row.first(c), f);
       Elem<T>::pack(f, w);
       st_chunk(out + static_cast<int64_t>(c) * CH, w);
+    };
+    // Two chunks' loads in flight a thread before either is finished.
+    int c = lo + threadIdx.x;
+    for (; c + kThreads < hi; c += 2 * kThreads) {
+      uint32_t w0[8], w1[8];
+      ld_chunk(row.chunk(c), w0);
+      ld_chunk(row.chunk(c + kThreads), w1);
+      finish(c, w0);
+      finish(c + kThreads, w1);
+    }
+    if (c < hi) {
+      uint32_t w0[8];
+      ld_chunk(row.chunk(c), w0);
+      finish(c, w0);
     }
     // The first and last chunk, where they reach out of the row.
     const int64_t head = c0 == 0 && row.lo == 1 ? min(CH - row.off, vocab) : 0;
@@ -672,7 +719,8 @@ template <typename T, bool SAME>
 __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const LogprobGradParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t r = blockIdx.x / p.parts;
+  // Last row first: the forward's last rows may still be in L2.
+  const int64_t r = gridDim.x / p.parts - 1 - blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x % p.parts);
   const float4 st = p.stats[r];  // m, log2 s, entropy
   const int64_t tok = p.tokens[r];
@@ -883,7 +931,8 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGrad
   __shared__ float off[kMaxTop + 1];
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t r = blockIdx.x / p.parts;
+  // Last row first: the forward's last rows may still be in L2.
+  const int64_t r = gridDim.x / p.parts - 1 - blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x % p.parts);
   const T* const z = static_cast<const T*>(p.z) + r * p.ld;
   T* const dz = static_cast<T*>(p.dz) + r * p.ld_out;

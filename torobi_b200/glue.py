@@ -16,7 +16,6 @@ import math
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .ops import _launch, _need_cuda, _ptr, _stream
 from ._lib import TQ_DTYPE_BF16, TQ_DTYPE_F32, check, lib
@@ -239,10 +238,9 @@ def document_spans(documents: torch.Tensor, prefix: torch.Tensor | None = None,
     b, s = documents.shape
     first = torch.empty(b, s, dtype=torch.int32, device=documents.device)
     last = torch.empty_like(first)
-    with torch.cuda.device(documents.device):
-        _launch("document_spans", lambda: lib().tq_document_spans(
-            _ptr(documents), 8 * documents.element_size(), _ptr(prefix), b, s, int(bool(causal)),
-            _ptr(first), _ptr(last), _stream()))
+    _on(documents.device, "document_spans", lambda stream: lib().tq_document_spans(
+        _ptr(documents), 8 * documents.element_size(), _ptr(prefix), b, s, int(bool(causal)),
+        _ptr(first), _ptr(last), stream))
     return first, last
 
 
@@ -275,10 +273,9 @@ def span_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     sc = float(scale) if scale is not None else d ** -0.5
     o = torch.empty_like(q)
     lse = torch.empty(b, h, s, dtype=torch.float32, device=q.device)
-    with torch.cuda.device(q.device):
-        _launch("attention", lambda: lib().tq_span_attention_fwd(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), b, s, h, k.shape[2], d, sc,
-            _ptr(o), _ptr(lse), _stream()))
+    _on(q.device, "attention", lambda stream: lib().tq_span_attention_fwd(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), b, s, h, k.shape[2], d, sc,
+        _ptr(o), _ptr(lse), stream))
     return o, lse
 
 
@@ -302,11 +299,9 @@ def span_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     check(lib().tq_span_attention_bwd_workspace_bytes(b, s, h, ctypes.byref(nbytes)))
     ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=q.device)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    with torch.cuda.device(q.device):
-        _launch("attention", lambda: lib().tq_span_attention_bwd(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), _ptr(o), _ptr(do), _ptr(lse), b,
-            s, h, k.shape[2], d, sc, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), nbytes.value,
-            _stream()))
+    _on(q.device, "attention", lambda stream: lib().tq_span_attention_bwd(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), _ptr(o), _ptr(do), _ptr(lse), b,
+        s, h, k.shape[2], d, sc, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), nbytes.value, stream))
     return dq, dk, dv
 
 
@@ -319,8 +314,8 @@ class _SpanAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, do):
+        _once("span_attention")
         q, k, v, first, last, o, lse = ctx.saved_tensors
         dq, dk, dv = span_attention_backward(q, k, v, first, last, o, do, lse, ctx.scale)
         return dq, dk, dv, None, None, None
@@ -410,17 +405,34 @@ _LOGIT_DTYPES = {torch.bfloat16: TQ_DTYPE_BF16, torch.float32: TQ_DTYPE_F32}
 
 
 def _one_device(op: str, **tensors) -> None:
-    """Every tensor on the first one's device, and that one current (the
-    kernels launch on its current stream)."""
-    _need_cuda(op, **tensors)
+    """Every tensor (None: none) on one CUDA device."""
     first = None
     for name, t in tensors.items():
         if t is None:
             continue
+        if not (isinstance(t, torch.Tensor) and t.is_cuda):
+            _need_cuda(op, **{name: t})
         if first is None:
             first = t.device
         elif t.device != first:
             raise ValueError(f"[{op}] {name} is on {t.device}, the others on {first}")
+
+
+def _on(dev: torch.device, kind: str, call) -> None:
+    """Launches ``call(stream)`` on the device's current stream.  Small calls
+    wait for the host, so the device is switched only if it is another one and
+    the stream is asked for by its handle."""
+    if torch.cuda.current_device() == dev.index:
+        stream = torch._C._cuda_getCurrentRawStream(dev.index)
+        _launch(kind, lambda: call(stream))
+    else:
+        with torch.cuda.device(dev):
+            _launch(kind, lambda: call(_stream()))
+
+
+def _once(op: str) -> None:
+    if torch.is_grad_enabled():  # in a backward pass: create_graph=True
+        raise RuntimeError(f"[{op}] has no second derivative")
 
 
 def _logit_rows(op: str, z: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
@@ -500,11 +512,9 @@ def _token_logprobs(z, rows, vocab, pitch, tokens, top, temperature, want_stats)
     top_logprobs = torch.empty(*lead, top, dtype=torch.float32, device=dev)
     top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_stats else None
-    with torch.cuda.device(dev):
-        _launch("token_logprobs", lambda: lib().tq_token_logprobs_fwd(
-            _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), rows, vocab, pitch, temperature, top,
-            _ptr(logprobs), _ptr(entropy), _ptr(stats), _ptr(top_logprobs), _ptr(top_ids),
-            _stream()))
+    _on(dev, "token_logprobs", lambda stream: lib().tq_token_logprobs_fwd(
+        _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), rows, vocab, pitch, temperature, top,
+        _ptr(logprobs), _ptr(entropy), _ptr(stats), _ptr(top_logprobs), _ptr(top_ids), stream))
     return logprobs, entropy, top_logprobs, top_ids, stats
 
 
@@ -521,16 +531,15 @@ class _TokenLogprobs(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dlogprobs, dentropy, _top, _ids):
+        _once("token_logprobs")
         z, tokens, stats = ctx.saved_tensors
         dz = _gradient_room(ctx, "token_logprobs", z)
         rows, vocab, pitch = ctx.shape
         dlogprobs, dentropy = _upstream(dlogprobs), _upstream(dentropy)
-        with torch.cuda.device(z.device):
-            _launch("token_logprobs", lambda: lib().tq_token_logprobs_bwd(
-                _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), _ptr(stats), rows, vocab, pitch,
-                ctx.temperature, _ptr(dlogprobs), _ptr(dentropy), _ptr(dz), pitch, _stream()))
+        _on(z.device, "token_logprobs", lambda stream: lib().tq_token_logprobs_bwd(
+            _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), _ptr(stats), rows, vocab, pitch,
+            ctx.temperature, _ptr(dlogprobs), _ptr(dentropy), _ptr(dz), pitch, stream))
         return dz, None, None, None, None
 
 
@@ -580,11 +589,10 @@ def _distillation(z, rows, vocab, pitch, teacher, targets, temperature, want_sta
     kl = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
     ce = None if targets is None else torch.empty_like(kl)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_stats else None
-    with torch.cuda.device(dev):
-        _launch("distillation", lambda: lib().tq_distill_fwd(
-            _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
-            _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), rows, vocab, pitch,
-            temperature, _ptr(kl), _ptr(ce), _ptr(stats), _stream()))
+    _on(dev, "distillation", lambda stream: lib().tq_distill_fwd(
+        _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
+        _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), rows, vocab, pitch,
+        temperature, _ptr(kl), _ptr(ce), _ptr(stats), stream))
     return kl, ce, stats
 
 
@@ -601,17 +609,16 @@ class _Distillation(torch.autograd.Function):
         return kl if ce is None else (kl, ce)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dkl, dce=None):
+        _once("distillation")
         z, ids, logits, targets, stats = ctx.saved_tensors
         dz = _gradient_room(ctx, "distillation", z)
         rows, vocab, pitch = ctx.shape
         dkl, dce = _upstream(dkl), _upstream(dce)
-        with torch.cuda.device(z.device):
-            _launch("distillation", lambda: lib().tq_distill_bwd(
-                _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
-                _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), _ptr(stats), rows,
-                vocab, pitch, ctx.temperature, _ptr(dkl), _ptr(dce), _ptr(dz), pitch, _stream()))
+        _on(z.device, "distillation", lambda stream: lib().tq_distill_bwd(
+            _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
+            _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), _ptr(stats), rows,
+            vocab, pitch, ctx.temperature, _ptr(dkl), _ptr(dce), _ptr(dz), pitch, stream))
         return dz, None, None, None, None, None
 
 
