@@ -17,6 +17,14 @@ norms (each residual add fused into the norm after it), RoPE and SwiGLU
 between them are fused kernels (``glue``); attention is this package's
 tensor-core kernels (``attention="native"``) or PyTorch's fused SDPA
 (``"library"``); the bf16 head is a library GEMM.
+
+Rows may pack several documents: with ``documents`` (an id per position, a run
+of equal ids being one document, a negative id padding) attention stays within
+each document, on this package's kernels whatever ``attention`` is, and only
+targets of the same document count.  Rotary positions run on through the row:
+the rotation enters the scores by differences alone.  With ``prefix`` (the
+document's prompt length, at each of its positions) prompts are seen in both
+directions, and their tokens are not targets.
 The head stays bf16 (a plain library GEMM): QLoRA quantizes the blocks'
 linears and keeps the vocabulary projection in the compute dtype.
 """
@@ -143,6 +151,23 @@ def apply_rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.T
     return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(x.dtype)
 
 
+def _counted(documents: torch.Tensor, prefix: torch.Tensor | None) -> torch.Tensor:
+    """[B, S-1]: whether position t + 1 is a target of position t in packed
+    rows: of the same document, and not in its prompt."""
+    now, nxt = documents[:, :-1], documents[:, 1:]
+    counted = (now == nxt) & (nxt >= 0)
+    if prefix is not None:
+        first, _ = glue.document_spans(documents)
+        index = torch.arange(documents.shape[1], device=documents.device)
+        counted &= (index >= first + prefix)[:, 1:]
+    return counted
+
+
+def _mean_over(loss: torch.Tensor, counted: torch.Tensor) -> torch.Tensor:
+    """The mean where it counts (0 where nothing does)."""
+    return torch.where(counted, loss, 0.0).sum() / counted.sum().clamp(min=1)
+
+
 @dataclass
 class Block:
     input_norm: torch.Tensor
@@ -240,11 +265,15 @@ class QLoRACausalLM:
         return t
 
     def block_forward(self, blk: Block, x: torch.Tensor, h: torch.Tensor,
-                      next_norm: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+                      next_norm: torch.Tensor,
+                      spans: tuple[torch.Tensor, torch.Tensor] | None = None
+                      ) -> tuple[torch.Tensor, torch.Tensor]:
         """One pre-norm block on the residual stream ``x`` whose input norm
         ``h`` is already computed; returns the new stream and its norm under
         ``next_norm`` (the next block's input norm, or the final norm).  Each
-        residual add is fused with the norm that follows it."""
+        residual add is fused with the norm that follows it.  ``spans``: the
+        keys each position sees (``glue.document_spans``) in place of the
+        causal rule."""
         cfg = self.cfg
         B, S, H = x.shape
         cos, sin = self._rope(S)
@@ -254,7 +283,9 @@ class QLoRACausalLM:
         q = glue.rope(q.view(B, S, cfg.heads, cfg.head_dim), cos, sin)
         k = glue.rope(k.view(B, S, cfg.kv_heads, cfg.head_dim), cos, sin)
         v = v.view(B, S, cfg.kv_heads, cfg.head_dim)
-        if self.attention == "native":
+        if spans is not None:
+            att = glue.span_attention(q, k, v, *spans).view(B, S, cfg.heads * cfg.head_dim)
+        elif self.attention == "native":
             # The tensor-core kernels read [B, S, heads, D] as it stands and
             # write the output in the layout o_proj reads.
             att = glue.attention(q, k, v, causal=True).view(B, S, cfg.heads * cfg.head_dim)
@@ -272,30 +303,72 @@ class QLoRACausalLM:
                                                  blk.adapters["down_proj"]),
                                  next_norm, cfg.rms_eps)
 
-    def hidden(self, ids: torch.Tensor) -> torch.Tensor:
+    def hidden(self, ids: torch.Tensor, documents: torch.Tensor | None = None,
+               prefix: torch.Tensor | None = None) -> torch.Tensor:
         """The final-normed hidden states: the blocks' residual stream
         (``x += attn(norm(x)); x += mlp(norm(x))``) and the final norm."""
+        spans = None
+        if documents is not None:
+            if documents.shape != ids.shape:
+                raise ValueError(f"documents {tuple(documents.shape)} must match the ids "
+                                 f"{tuple(ids.shape)}")
+            spans = glue.document_spans(documents, prefix)
+        elif prefix is not None:
+            raise ValueError("a prefix goes with documents")
         x = F.embedding(ids, self.embed)
         if not self.blocks:
             return glue.rms_norm(x, self.final_norm, self.cfg.rms_eps)
         h = glue.rms_norm(x, self.blocks[0].input_norm, self.cfg.rms_eps)
         for i, blk in enumerate(self.blocks):
             nxt = self.blocks[i + 1].input_norm if i + 1 < len(self.blocks) else self.final_norm
-            x, h = self.block_forward(blk, x, h, nxt)
+            x, h = self.block_forward(blk, x, h, nxt, spans)
         return h
 
     def logits(self, h: torch.Tensor) -> torch.Tensor:
         head = self.embed if self.lm_head is None else self.lm_head
         return h @ head.t()
 
-    def loss(self, ids: torch.Tensor) -> torch.Tensor:
-        """Mean next-token cross-entropy (f32) over positions 0..S-2: the
-        fused per-position loss kernel, its gradient written over the bf16
-        logits in backward."""
-        h = self.hidden(ids)[:, :-1]
+    def loss(self, ids: torch.Tensor, documents: torch.Tensor | None = None,
+             prefix: torch.Tensor | None = None) -> torch.Tensor:
+        """Mean next-token cross-entropy (f32) over positions 0..S-2 (of
+        packed documents: over the targets that count): the fused per-position
+        loss kernel, its gradient written over the bf16 logits in backward."""
+        h = self.hidden(ids, documents, prefix)[:, :-1]
         z = self.logits(h)
         tgt = ids[:, 1:]
-        return glue.cross_entropy(z, tgt, inplace=True).mean()
+        loss = glue.cross_entropy(z, tgt, inplace=True)
+        if documents is None:
+            return loss.mean()
+        return _mean_over(loss, _counted(documents, prefix))
+
+    def token_logprobs(self, ids: torch.Tensor, top: int = 0, temperature: float = 1.0,
+                       documents: torch.Tensor | None = None,
+                       prefix: torch.Tensor | None = None) -> glue.TokenLogprobs:
+        """What the model thinks of each next token, positions 0..S-2: its log
+        probability (0 where the target does not count), the entropy and the
+        ``top`` most likely alternatives (``glue.token_logprobs``);
+        differentiable through the first two."""
+        tgt = ids[:, 1:]
+        if documents is not None:
+            tgt = torch.where(_counted(documents, prefix), tgt, -1)
+        z = self.logits(self.hidden(ids, documents, prefix)[:, :-1])
+        return glue.token_logprobs(z, tgt, top=top, temperature=temperature, inplace=True)
+
+    def distill_loss(self, ids: torch.Tensor, teacher_ids: torch.Tensor,
+                     teacher_logits: torch.Tensor, documents: torch.Tensor | None = None,
+                     prefix: torch.Tensor | None = None, temperature: float = 1.0,
+                     alpha: float = 0.5) -> torch.Tensor:
+        """``(1 - alpha) * ce + alpha * temperature**2 * kl``, a mean over the
+        targets that count: the targets' cross-entropy and the divergence from
+        a teacher's top logits [B, S-1, k] (its ``token_logprobs(ids, top=k)``
+        over the same rows gives both; ``glue.distillation``)."""
+        z = self.logits(self.hidden(ids, documents, prefix)[:, :-1])
+        kl, ce = glue.distillation(z, teacher_ids, teacher_logits, targets=ids[:, 1:],
+                                   temperature=temperature, inplace=True)
+        loss = (1.0 - alpha) * ce + alpha * temperature ** 2 * kl
+        if documents is None:
+            return loss.mean()
+        return _mean_over(loss, _counted(documents, prefix))
 
     def base_nbytes(self) -> int:
         return sum(w.nbytes() for blk in self.blocks for w in blk.linears.values())

@@ -219,8 +219,11 @@ class Trainer:
 
     def __init__(self, model, opt: AdamWConfig | None = None, micro_batch: int = 1,
                  reduce: NcclGradReduce | None = None, rank: int = 0, world: int = 1,
-                 graph: bool = False, gate: StepGate | None = None):
+                 graph: bool = False, gate: StepGate | None = None, objective=None):
         self.model = model
+        # objective(ids, *more) -> scalar loss of a micro-batch's rows; the
+        # model's next-token loss unless given (e.g. model.distill_loss).
+        self.objective = objective
         # gate (several ranks): checked on the host before each step's
         # allreduce, so a lost rank raises RankLost instead of hanging NCCL.
         self.gate = gate
@@ -243,47 +246,56 @@ class Trainer:
         self.last_norm = float("nan")
         self._pending: list[float] = []  # grad scales of launched, unsettled steps
 
-    def _gradients(self, ids: torch.Tensor) -> None:
+    def _gradients(self, ids: torch.Tensor, *more: torch.Tensor) -> None:
         """Zeroes the gradient and loss buffers, then accumulates every
         micro-batch's loss and adapter gradients into them."""
         self.store.zero_grad()
         self.loss_buf.zero_()
+        objective = self.objective or self.model.loss
         for a, b in micro_batches(ids.shape[0], self.micro):
-            loss = self.model.loss(ids[a:b])
+            loss = objective(ids[a:b], *[t[a:b] for t in more])
             loss.backward()
             self.loss_buf += loss.detach()
 
-    def _graphed(self, ids: torch.Tensor):
-        key = (tuple(ids.shape), ids.dtype)
+    def _graphed(self, *rows: torch.Tensor):
+        key = tuple((tuple(t.shape), t.dtype) for t in rows)
         hit = self._graphs.get(key)
         if hit is None:
-            static = ids.clone()
+            static = [t.clone() for t in rows]
             # Warm up on a side stream first (first-call set-up, allocator
             # pools), as capture requires, then capture one pass.
-            side = torch.cuda.Stream(device=ids.device)
+            side = torch.cuda.Stream(device=rows[0].device)
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
                 for _ in range(2):
-                    self._gradients(static)
+                    self._gradients(*static)
             torch.cuda.current_stream().wait_stream(side)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, capture_error_mode="thread_local"):
-                self._gradients(static)
+                self._gradients(*static)
             hit = (g, static)
             self._graphs[key] = hit
         return hit
 
-    def step(self, ids: torch.Tensor) -> torch.Tensor:
+    def step(self, ids: torch.Tensor, *more: torch.Tensor) -> torch.Tensor:
         """One optimizer step over this rank's rows ``ids`` [rows, seq] (on
-        the device).  Returns the global mean loss as a device tensor."""
+        the device).  ``more``: further tensors with a row for each (document
+        ids, a teacher's alternatives), handed to the objective beside the
+        micro-batch's ids in this order.  Returns the global mean loss as a
+        device tensor: the mean of the micro-batches' losses, each a mean over
+        what counts in it."""
         st = self.store
+        for t in more:
+            if t.shape[0] != ids.shape[0]:
+                raise ValueError(f"{t.shape[0]} rows beside {ids.shape[0]} rows of ids")
         parts = micro_batches(ids.shape[0], self.micro)
         if self.graph:
-            g, static = self._graphed(ids)
-            static.copy_(ids)
+            g, static = self._graphed(ids, *more)
+            for t, now in zip(static, (ids, *more)):
+                t.copy_(now)
             g.replay()
         else:
-            self._gradients(ids)
+            self._gradients(ids, *more)
         if self.gate is not None:
             try:
                 self.gate.wait(self.steps)
