@@ -383,7 +383,7 @@ int tq_span_attention_fwd(const void* q, const void* k, const void* v, const int
                           int64_t kv_heads, int64_t head_dim, float scale, void* out, float* lse,
                           void* stream);
 int tq_span_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
-                                          size_t* bytes);
+                                          int64_t kv_heads, size_t* bytes);
 int tq_span_attention_bwd(const void* q, const void* k, const void* v, const int32_t* first,
                           const int32_t* last, const void* out, const void* dout,
                           const float* lse, int64_t batch, int64_t seq, int64_t heads,

@@ -180,6 +180,15 @@ CASES = [
     (1, 1000, 4, 4, 64, 250, True, True),
     (1, 1537, 8, 2, 128, 700, False, True),
     (2, 2048, 4, 1, 64, 40, False, True),
+    # Query heads a key/value head: those a tile holds, and rows it leaves over.
+    (1, 200, 3, 1, 64, 50, False, True),
+    (1, 200, 5, 1, 128, 50, True, True),
+    (2, 150, 11, 1, 64, 50, False, True),
+    (1, 300, 12, 1, 128, 90, False, True),
+    (1, 300, 14, 1, 64, 90, True, True),
+    (1, 260, 16, 1, 128, 60, False, False),
+    (1, 130, 34, 2, 64, 60, False, True),
+    (1, 260, 32, 1, 64, 60, True, True),
 ]
 
 
@@ -420,16 +429,20 @@ def test_span_entry_points_refuse_on_the_host():
     assert fwd(batch=0, first=None, last=None, out=None) == 0
 
     need, plain = ctypes.c_size_t(), ctypes.c_size_t()
-    assert L.tq_span_attention_bwd_workspace_bytes(2, 129, 4, ctypes.byref(need)) == 0
-    assert L.tq_attention_bwd_workspace_bytes(2, 129, 4, ctypes.byref(plain)) == 0
-    # Beside the statistics: two ints a padded row, four a 64-row tile.
-    assert need.value == plain.value + 2 * 256 * 8 + 2 * 4 * 16
+    # 4 heads over 2: 64-row tiles of 32 positions, five of them; per tile and
+    # two heads 64 rows of two statistics, per tile 64 spans and four bounds.
+    assert L.tq_span_attention_bwd_workspace_bytes(2, 129, 4, 2, ctypes.byref(need)) == 0
+    assert need.value == 2 * 5 * (2 * 64 * 8 + 64 * 8 + 16)
+    # 11 heads over one: too few rows would be filled, a tile holds one head.
+    assert L.tq_span_attention_bwd_workspace_bytes(1, 65, 11, 1, ctypes.byref(plain)) == 0
+    assert plain.value == 2 * (11 * 64 * 8 + 64 * 8 + 16)
+    assert L.tq_span_attention_bwd_workspace_bytes(2, 129, 4, 3, ctypes.byref(plain)) == 1
 
     def bwd(ws_bytes=need.value, ws=P, first=P):
         return L.tq_span_attention_bwd(P, P, P, first, P, P, P, P, 2, 129, 4, 2, 64, 0.125, P, P,
                                        P, ws, ws_bytes, None)
 
-    assert bwd(ws_bytes=plain.value) == 1 and "workspace" in said()
+    assert bwd(ws_bytes=need.value - 4) == 1 and "workspace" in said()
     assert bwd(ws=P + 16) == 3 and bwd(ws=None) == 1 and bwd(first=None) == 1
 
     def spans(docs=P, bits=32, prefix=None, batch=2, seq=8, first=P, last=P):

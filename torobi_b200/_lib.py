@@ -99,8 +99,8 @@ SIGNATURES = {
                           _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp], _i32),
     "tq_span_attention_fwd": ([_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f32, _vp,
                                _vp, _vp], _i32),
-    "tq_span_attention_bwd_workspace_bytes": ([_i64, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)],
-                                              _i32),
+    "tq_span_attention_bwd_workspace_bytes": ([_i64, _i64, _i64, _i64,
+                                               ctypes.POINTER(ctypes.c_size_t)], _i32),
     "tq_span_attention_bwd": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                _i64, _f32, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp], _i32),
     "tq_document_spans": ([_vp, _i32, _vp, _i64, _i64, _i32, _vp, _vp, _vp], _i32),

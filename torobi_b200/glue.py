@@ -296,7 +296,8 @@ def span_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     lse = lse.contiguous()
     sc = float(scale) if scale is not None else d ** -0.5
     nbytes = ctypes.c_size_t()
-    check(lib().tq_span_attention_bwd_workspace_bytes(b, s, h, ctypes.byref(nbytes)))
+    check(lib().tq_span_attention_bwd_workspace_bytes(b, s, h, k.shape[2],
+                                                       ctypes.byref(nbytes)))
     ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=q.device)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     _on(q.device, "attention", lambda stream: lib().tq_span_attention_bwd(
@@ -470,7 +471,7 @@ def _logit_rows(op: str, z: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
 def _gradient_like(z: torch.Tensor, rows: int, vocab: int, pitch: int) -> torch.Tensor:
     """Room for a gradient of logits, with their rows' pitch."""
     if pitch == vocab:
-        return torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        return torch.empty_like(z, memory_format=torch.contiguous_format)
     wide = torch.empty(rows, pitch, dtype=z.dtype, device=z.device)
     return wide.view(*z.shape[:-1], pitch)[..., :vocab]
 
@@ -481,7 +482,7 @@ def _positions(op: str, name: str, t: torch.Tensor, z: torch.Tensor) -> torch.Te
     if t.shape != z.shape[:-1]:
         raise ValueError(f"[{op}] {name} {tuple(t.shape)} must match the logits' positions "
                          f"{tuple(z.shape[:-1])}")
-    return t.to(torch.int64).contiguous()
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
 def _temperature(op: str, temperature: float) -> float:
@@ -492,25 +493,36 @@ def _temperature(op: str, temperature: float) -> float:
 
 
 def _upstream(g: torch.Tensor | None) -> torch.Tensor | None:
-    return None if g is None else g.float().contiguous()
+    if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+        return g
+    return g.float().contiguous()
+
+
+def _positions_f32(lead: torch.Size, dev: torch.device) -> torch.Tensor:
+    # Sizes one by one: torch parses them in half the time of a torch.Size.
+    return (torch.empty(*lead, dtype=torch.float32, device=dev) if lead else
+            torch.empty((), dtype=torch.float32, device=dev))
 
 
 class TokenLogprobs(NamedTuple):
-    """What ``token_logprobs`` answers, per position."""
+    """What ``token_logprobs`` answers, per position (the alternatives None
+    where none were asked for)."""
 
     logprobs: torch.Tensor
     entropy: torch.Tensor
-    top_logprobs: torch.Tensor
-    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
 
 
 def _token_logprobs(z, rows, vocab, pitch, tokens, top, temperature, want_stats):
     dev = z.device
     lead = z.shape[:-1]
-    logprobs = torch.empty(lead, dtype=torch.float32, device=dev)
-    entropy = torch.empty(lead, dtype=torch.float32, device=dev)
-    top_logprobs = torch.empty(*lead, top, dtype=torch.float32, device=dev)
-    top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
+    logprobs = _positions_f32(lead, dev)
+    entropy = torch.empty_like(logprobs)
+    top_logprobs = top_ids = None
+    if top:
+        top_logprobs = torch.empty(*lead, top, dtype=torch.float32, device=dev)
+        top_ids = torch.empty(*lead, top, dtype=torch.int64, device=dev)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_stats else None
     _on(dev, "token_logprobs", lambda stream: lib().tq_token_logprobs_fwd(
         _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), rows, vocab, pitch, temperature, top,
@@ -526,7 +538,8 @@ class _TokenLogprobs(torch.autograd.Function):
         ctx.save_for_backward(z, tokens, stats)
         ctx.shape, ctx.temperature, ctx.inplace = (rows, vocab, pitch), temperature, inplace
         ctx.spent = False
-        ctx.mark_non_differentiable(out[2], out[3])
+        if top:
+            ctx.mark_non_differentiable(out[2], out[3])
         ctx.set_materialize_grads(False)
         return tuple(out)
 
@@ -562,7 +575,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     ``logprobs`` f32 ``ln q[token]`` (0 where the token is outside [0, vocab):
     a padding position), ``entropy`` f32 ``-sum q ln q``, and the ``top`` (0 to
     128) most likely alternatives, most likely first, equal logits by lowest
-    id: ``top_logprobs`` f32 and ``top_ids`` int64 [..., top].
+    id: ``top_logprobs`` f32 and ``top_ids`` int64 [..., top] (None for none).
 
     Differentiable through logprobs and entropy.  ``inplace=True`` writes the
     gradient over the logits in backward, as ``cross_entropy`` does.  A -inf
@@ -586,7 +599,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
 def _distillation(z, rows, vocab, pitch, teacher, targets, temperature, want_stats):
     dev = z.device
     ids, logits = teacher
-    kl = torch.empty(z.shape[:-1], dtype=torch.float32, device=dev)
+    kl = _positions_f32(z.shape[:-1], dev)
     ce = None if targets is None else torch.empty_like(kl)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=dev) if want_stats else None
     _on(dev, "distillation", lambda stream: lib().tq_distill_fwd(
