@@ -9,79 +9,22 @@
 // the natural-log log-sum-exp of each query row's scaled scores, kept for the
 // backward.  dim is 64 or 128.
 //
-// Each kernel also comes in a SPAN form, for rows that pack several documents
-// (and prompts seen in both directions, and padding): query i of sequence b
-// sees the keys first[b, i] <= j < last[b, i], two ints a row, in place of the
-// causal rule.  Key tiles that no row of a query tile sees are neither loaded
-// nor multiplied (the tile's range is the least first to the greatest last),
-// tiles that every row sees whole take the unmasked code, and a row that sees
-// nothing gets o = 0, lse = -inf and no gradient.  A tile's rows are then the
-// `pack` query heads that share a key/value head at a few positions (row =
-// position * pack + head: the order the box {64 dims, pack heads, positions}
-// lands in), not one head's at 128: the rows of a tile see nearly the same
-// keys, so little of a tile is masked at the borders of short documents.
-// Llama-3-8B heads (4 a key/value head), rows of 2048 packing 6 documents: 22 %
-// fewer tile pairs forward than with one head's 128 positions a tile.
-//
 // The forward and the backward kernels are described where they start below.
 #include <cuda_bf16.h>
 
-#include <climits>
 #include <cmath>
 #include <cstdlib>
 #include <type_traits>
 
-#include "tq_ptx.cuh"
-#include "tq_runtime.h"
+#include "attn.cuh"
 
 namespace tq {
 namespace {
-
-constexpr int kTile = 128;  // query rows and key rows per tile
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kRescaleLog2 = 8.0f;  // move m only when the row max grows by > 2^8
-
-// 2^x on the FMA pipe, for a share of the softmax's exponentials (the MUFU
-// unit alone would take as long as the tile's MMAs).  Range reduction by the
-// round-to-nearest of x + 1.5 * 2^23 (n = nearest integer, f = x - n in
-// [-0.5, 0.5]), 2^f by a cubic least-squares fit in relative error (fitted for
-// this kernel; max relative error 7.5e-5 in f32, below bf16's 2^-9), and n
-// added to the exponent field.  x is clamped at -125 so that the result stays
-// a normal number.
-__device__ __forceinline__ float exp2_poly(float x) {
-  x = fmaxf(x, -125.0f);
-  const float t = __fadd_rn(x, 12582912.0f);
-  const float f = __fsub_rn(x, __fsub_rn(t, 12582912.0f));
-  float p = fmaf(0.055174145847558975f, f, 0.24261757731437683f);
-  p = fmaf(p, f, 0.6932610869407654f);
-  p = fmaf(p, f, 0.9999275803565979f);
-  return __uint_as_float(__float_as_uint(p) + (__float_as_uint(t) << 23));
-}
-
-// The same with a quintic (minimax in relative error with value 1 at f = 0;
-// max relative error 1.6e-7), for sums that are answered in f32: with the
-// cubic, a row of few keys had its lse off by up to 7e-5.
-__device__ __forceinline__ float exp2_fine(float x) {
-  x = fmaxf(x, -125.0f);
-  const float t = __fadd_rn(x, 12582912.0f);
-  const float f = __fsub_rn(x, __fsub_rn(t, 12582912.0f));
-  float p = fmaf(0.001326472731307149f, f, 0.009671512991189957f);
-  p = fmaf(p, f, 0.05550733581185341f);
-  p = fmaf(p, f, 0.24022242426872253f);
-  p = fmaf(p, f, 0.6931470036506653f);
-  p = fmaf(p, f, 1.0f);
-  return __uint_as_float(__float_as_uint(p) + (__float_as_uint(t) << 23));
-}
 
 struct AttnShape {
   int batch, seq, heads, kv_heads, group, n_tiles;
   int causal;
   float scale_log2;  // softmax scale * log2(e)
-  // SPAN: query heads a tile holds, and the positions in a 128- and a 64-row
-  // tile, floor(rows / pack) (rows behind pack * positions are left zero), with
-  // the number of such tiles in a sequence.
-  int pack, pos128, pos64, tiles128, tiles64;
 };
 
 // ------------------------------------------------------------------ forward --
@@ -130,41 +73,15 @@ struct FwdCfg {
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
-// A query row's keys [lo, hi) within [0, seq); lo = hi = 0 when it sees none.
-struct Span {
-  int lo, hi;
-};
-
-__device__ __forceinline__ Span load_span(const int* first, const int* last, int b, int i,
-                                          int seq) {
-  if (i >= seq) return {0, 0};
-  const size_t at = static_cast<size_t>(b) * seq + i;
-  const int lo = max(first[at], 0), hi = min(last[at], seq);
-  return lo < hi ? Span{lo, hi} : Span{0, 0};
-}
-
-// Zeroes rows [from, tile_rows) of `slabs` consecutive slabs (128 bytes a row),
-// which no copy fills when a packed tile has fewer rows; 384 threads, made
-// visible to the tensor cores by each thread's fence and the barrier after it.
-__device__ __forceinline__ void zero_rows(uint8_t* slab, int slabs, int tile_rows, int from) {
-  const int per = (tile_rows - from) * 8;  // 16-byte words a slab
-  for (int i = threadIdx.x; i < slabs * per; i += 384)
-    *reinterpret_cast<uint4*>(slab + (i / per * tile_rows + from) * 128 + i % per * 16) =
-        make_uint4(0, 0, 0, 0);
-  if (per > 0) fence_proxy_async_smem();
-}
-
 struct FwdParams {
   AttnShape sh;
-  const int* first;  // SPAN: [batch, seq]
-  const int* last;
   int n_pairs;
   uint16_t* out;
   float* lse;
   int* status;
 };
 
-template <int D, bool SPAN>
+template <int D>
 __global__ void __launch_bounds__(384, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
@@ -199,29 +116,18 @@ __global__ void __launch_bounds__(384, 1)
   const AttnShape& sh = p.sh;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int pack = SPAN ? sh.pack : 1;
-  const int pos_per = SPAN ? sh.pos128 : kTile;  // positions of a query tile
-  const int rows = SPAN ? pack * pos_per : kTile;
-  const int bh_count = sh.batch * (sh.heads / pack);
+  const int bh_count = sh.batch * sh.heads;
   const int bh = blockIdx.x % bh_count;
   const int pair = p.n_pairs - 1 - static_cast<int>(blockIdx.x / bh_count);
-  const int b = bh / (sh.heads / pack);
-  const int h = bh % (sh.heads / pack) * pack;  // (SPAN: the first of `pack`)
+  const int b = bh / sh.heads;
+  const int h = bh % sh.heads;
   const int hk = h / sh.group;
-  const int t0 = 2 * pair;  // first query tile
-  const bool has1 = t0 + 1 < (SPAN ? sh.tiles128 : sh.n_tiles);  // second query tile exists
-  // Key tiles [kv_lo(w), kv_hi(w)) of query tile w, all within [j0, j0 + n_kv).
-  int lo0 = 0, lo1 = 0;
-  int hi0 = sh.causal ? t0 + 1 : sh.n_tiles;
-  int hi1 = has1 ? (sh.causal ? t0 + 2 : sh.n_tiles) : 0;
-  __shared__ int range[2][2];  // SPAN: the tiles' least first and greatest last
-  if constexpr (SPAN) {
-    if (threadIdx.x < 2) {
-      range[threadIdx.x][0] = sh.seq;
-      range[threadIdx.x][1] = 0;
-    }
-    zero_rows(gbase + C::Q_OFF, 2 * C::SLABS, kTile, rows);
-  }
+  const int t0 = 2 * pair;                             // first query tile
+  const bool has1 = t0 + 1 < sh.n_tiles;               // second query tile exists
+  const int n_kv0 = sh.causal ? t0 + 1 : sh.n_tiles;  // key tiles of query tile 0
+  const int n_kv1 = has1 ? (sh.causal ? t0 + 2 : sh.n_tiles) : 0;
+  const int n_kv = n_kv0 > n_kv1 ? n_kv0 : n_kv1;
+  auto nkv_of = [&](int w) { return w == 0 ? n_kv0 : n_kv1; };
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -253,40 +159,16 @@ __global__ void __launch_bounds__(384, 1)
   griddep_launch_dependents();
   griddep_wait();
 
-  if constexpr (SPAN) {
-    if (threadIdx.x < 2 * kTile) {
-      const int w = threadIdx.x / kTile, i = threadIdx.x % kTile;
-      const Span sp = i < pos_per ? load_span(p.first, p.last, b, (t0 + w) * pos_per + i, sh.seq)
-                                  : Span{0, 0};
-      const int lo = __reduce_min_sync(0xffffffffu, sp.lo < sp.hi ? sp.lo : sh.seq);
-      const int hi = __reduce_max_sync(0xffffffffu, sp.hi);
-      if (lane == 0) {
-        atomicMin(&range[w][0], lo);
-        atomicMax(&range[w][1], hi);
-      }
-    }
-    __syncthreads();
-    hi0 = (range[0][1] + kTile - 1) / kTile;
-    hi1 = (range[1][1] + kTile - 1) / kTile;
-    lo0 = hi0 ? range[0][0] / kTile : 0;
-    lo1 = hi1 ? range[1][0] / kTile : 0;
-  }
-  const int j0 = !SPAN ? 0 : hi0 == 0 ? lo1 : hi1 == 0 ? lo0 : min(lo0, lo1);
-  const int n_kv = max(hi0, hi1) - j0;
-  auto kv_lo = [&](int w) { return w == 0 ? lo0 : lo1; };
-  auto kv_hi = [&](int w) { return w == 0 ? hi0 : hi1; };
-
   if (warp == 0) {
     // ------------------------------------------------------------- TMA
     if (elect_one_sync()) {
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      mbar_arrive_expect_tx(q_full, (has1 ? 2 : 1) * C::SLABS * rows * 128);
+      mbar_arrive_expect_tx(q_full, (has1 ? 2 : 1) * C::TILE_BYTES);
       for (int w = 0; w < (has1 ? 2 : 1); ++w)
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(q_s(w) + sl * C::SLAB_BYTES, &tm_q, q_full, sl * 64, h,
-                      (t0 + w) * pos_per, b);
+          tma_load_4d(q_s(w) + sl * C::SLAB_BYTES, &tm_q, q_full, sl * 64, h, (t0 + w) * kTile, b);
       int nk = 0, nv = 0;  // tiles issued
       // Key tile j + 1 is issued ahead of value tile j (the MMA wants K_{j+1}
       // for the next scores before it wants V_j).
@@ -295,8 +177,7 @@ __global__ void __launch_bounds__(384, 1)
         if (!mbar_wait(k_empty(s), ((j / KST) & 1) ^ 1, p.status)) return false;
         mbar_arrive_expect_tx(k_full(s), C::TILE_BYTES);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(k_s(s) + sl * C::SLAB_BYTES, &tm_k, k_full(s), sl * 64, hk,
-                      (j0 + j) * kTile, b);
+          tma_load_4d(k_s(s) + sl * C::SLAB_BYTES, &tm_k, k_full(s), sl * 64, hk, j * kTile, b);
         ++nk;
         return true;
       };
@@ -307,8 +188,7 @@ __global__ void __launch_bounds__(384, 1)
         if (!mbar_wait(v_empty(s), ((j / VST) & 1) ^ 1, p.status)) break;
         mbar_arrive_expect_tx(v_full(s), C::TILE_BYTES);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(v_s(s) + sl * C::SLAB_BYTES, &tm_v, v_full(s), sl * 64, hk,
-                      (j0 + j) * kTile, b);
+          tma_load_4d(v_s(s) + sl * C::SLAB_BYTES, &tm_v, v_full(s), sl * 64, hk, j * kTile, b);
         ++nv;
       }
       // Never leave a copy in flight.
@@ -324,13 +204,9 @@ __global__ void __launch_bounds__(384, 1)
       constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kTile, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(kTile, D, false, true);
       bool ok = mbar_wait(q_full, 0, p.status);
-      // Key tiles count from j0 here: tile t is key tile j0 + t, and query
-      // tile w takes part in t of [from(w), to(w)).
-      auto from = [&](int w) { return kv_lo(w) - j0; };
-      auto to = [&](int w) { return kv_hi(w) - j0; };
-      // S_w(t) = Q_w K_t^T into S_w.
-      auto issue_s = [&](int w, int t) {
-        const int s = t % KST;
+      // S_w(j) = Q_w K_j^T into S_w.
+      auto issue_s = [&](int w, int j) {
+        const int s = j % KST;
         const uint32_t d = tmem + C::S_COL + w * kTile;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -340,64 +216,57 @@ __global__ void __launch_bounds__(384, 1)
         }
         umma_commit(s_full(w));
       };
-      // O_w += P_w(t) V_t, P_w from the first 64 columns of S_w.
-      auto issue_pv = [&](int w, int t) {
-        const int s = t % VST;
+      // O_w += P_w(j) V_j, P_w from the first 64 columns of S_w.
+      auto issue_pv = [&](int w, int j) {
+        const int s = j % VST;
 #pragma unroll
         for (int kk = 0; kk < kTile / 16; ++kk)
           umma_bf16_ts(tmem + C::O_COL + w * D, tmem + C::S_COL + w * kTile + kk * 8,
                        make_sdesc(v_s(s) + kk * 2048, C::SLAB_BYTES, 1024, kSw128), idesc_o,
-                       (t > from(w) || kk > 0) ? 1u : 0u);
+                       (j > 0 || kk > 0) ? 1u : 0u);
         umma_commit(o_done(w));
       };
-      // The first key tile's scores, of both query tiles unless one starts later.
-      if (ok && n_kv > 0) ok = mbar_wait(k_full(0), 0, p.status);
-      if (ok && n_kv > 0) {
+      // Key tile 0: both tiles' scores.
+      if (ok) ok = mbar_wait(k_full(0), 0, p.status);
+      if (ok) {
         tc_fence_after();
-        for (int w = 0; w < 2; ++w)
-          if (from(w) == 0 && to(w) > 0) issue_s(w, 0);
+        issue_s(0, 0);
+        if (n_kv1 > 0) issue_s(1, 0);
         umma_commit(k_empty(0));
       }
-      for (int t = 0; t < n_kv && ok; ++t) {
-        const int s = t % VST;
-        const bool next = t + 1 < n_kv;
+      for (int j = 0; j < n_kv && ok; ++j) {
+        const int s = j % VST;
+        const bool next = j + 1 < n_kv;
         if (next) {
-          ok = mbar_wait(k_full((t + 1) % KST), ((t + 1) / KST) & 1, p.status);
+          ok = mbar_wait(k_full((j + 1) % KST), ((j + 1) / KST) & 1, p.status);
           if (!ok) break;
         }
-        ok = mbar_wait(v_full(s), (t / VST) & 1, p.status);
+        ok = mbar_wait(v_full(s), (j / VST) & 1, p.status);
         if (!ok) break;
         for (int w = 0; w < 2 && ok; ++w) {
-          if (t >= to(w)) continue;
-          if (t >= from(w)) {
-            ok = mbar_wait(p_ready(w), (t - from(w)) & 1, p.status);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(w, t);
-          }
-          if (t + 1 >= from(w) && t + 1 < to(w)) issue_s(w, t + 1);
+          if (j >= nkv_of(w)) continue;
+          ok = mbar_wait(p_ready(w), j & 1, p.status);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(w, j);
+          if (j + 1 < nkv_of(w)) issue_s(w, j + 1);
         }
         if (!ok) break;
         umma_commit(v_empty(s));
-        if (next) umma_commit(k_empty((t + 1) % KST));
+        if (next) umma_commit(k_empty((j + 1) % KST));
       }
       // Nothing may outlive the CTA's TMEM: wait for each tile's last PV.
       for (int w = 0; w < 2; ++w)
-        if (to(w) > from(w)) mbar_wait(o_done(w), (to(w) - from(w) - 1) & 1, p.status);
+        if (nkv_of(w) > 0) mbar_wait(o_done(w), (nkv_of(w) - 1) & 1, p.status);
     }
   } else if (warp >= 4) {
     // --------------------------------------------------------- softmax
     const int w = (warp - 4) >> 2;  // query tile of this warpgroup
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
-    const int qw0 = (t0 + w) * pos_per;
-    const int qpos = qw0 + row / pack;
-    const int head = h + row % pack;
-    const bool filled = !SPAN || row < rows;
-    const int jw = kv_lo(w), nk = kv_hi(w) - jw;
-    Span sp{0, 0};
-    // A row that no copy filled holds zeros: it is never masked, nor stored.
-    if (SPAN) sp = filled ? load_span(p.first, p.last, b, qpos, sh.seq) : Span{0, INT_MAX};
+    const int qw0 = (t0 + w) * kTile;
+    const int qpos = qw0 + row;
+    const int nk = nkv_of(w);
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t scol = lrow + C::S_COL + w * kTile;
     const uint32_t ocol = lrow + C::O_COL + w * D;
@@ -409,28 +278,15 @@ __global__ void __launch_bounds__(384, 1)
       ok = mbar_wait(s_full(w), j & 1, p.status);
       if (!ok) break;
       tc_fence_after();
-      const int kv0 = (jw + j) * kTile;
+      const int kv0 = j * kTile;
       int lim = kTile - 1;  // last column of this key tile that counts for the row
-      bool masked;
-      if constexpr (SPAN) {
-        masked = __any_sync(0xffffffffu, sp.lo > kv0 || sp.hi < kv0 + kTile);
-      } else {
-        if ((sh.causal && kv0 + kTile - 1 > qw0) || kv0 + kTile > sh.seq) {
-          lim = sh.seq - 1 - kv0;
-          if (sh.causal && qpos - kv0 < lim) lim = qpos - kv0;
-        }
-        // Only the diagonal key tile (causal) and the one past seq need a mask:
-        // both passes come in a masked and an unmasked form.
-        masked = lim < kTile - 1 || (sh.causal && kv0 + kTile - 1 > qw0);
+      if ((sh.causal && kv0 + kTile - 1 > qw0) || kv0 + kTile > sh.seq) {
+        lim = sh.seq - 1 - kv0;
+        if (sh.causal && qpos - kv0 < lim) lim = qpos - kv0;
       }
-      // Whether a column counts for the row (SPAN: lo <= key < hi in one
-      // unsigned comparison).
-      const int col0 = kv0 - sp.lo;
-      const unsigned len = sp.hi - sp.lo;
-      auto counts = [&](int col) {
-        if constexpr (SPAN) return static_cast<unsigned>(col0 + col) < len;
-        return col <= lim;
-      };
+      // Only the diagonal key tile (causal) and the one past seq need a mask:
+      // both passes come in a masked and an unmasked form.
+      const bool masked = lim < kTile - 1 || (sh.causal && kv0 + kTile - 1 > qw0);
       // Pass 1: the row maximum (eight interleaved chains, then a tree).
       float m8[8];
 #pragma unroll
@@ -444,7 +300,7 @@ __global__ void __launch_bounds__(384, 1)
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (!M || counts(c4 * 32 + i)) m8[i & 7] = fmaxf(m8[i & 7], __uint_as_float(r[i]));
+            if (!M || c4 * 32 + i <= lim) m8[i & 7] = fmaxf(m8[i & 7], __uint_as_float(r[i]));
         }
       };
       if (masked)
@@ -498,13 +354,12 @@ __global__ void __launch_bounds__(384, 1)
             float p0 = ex2_approx(fmaf(__uint_as_float(r[i]), c, -mref));
             float p1 = ex2_approx(fmaf(__uint_as_float(r[i + 1]), c, -mref));
             float p2 = ex2_approx(fmaf(__uint_as_float(r[i + 2]), c, -mref));
-            const float x3 = fmaf(__uint_as_float(r[i + 3]), c, -mref);
-            float p3 = SPAN ? exp2_fine(x3) : exp2_poly(x3);
+            float p3 = exp2_poly(fmaf(__uint_as_float(r[i + 3]), c, -mref));
             if (M) {
-              if (!counts(col)) p0 = 0.0f;
-              if (!counts(col + 1)) p1 = 0.0f;
-              if (!counts(col + 2)) p2 = 0.0f;
-              if (!counts(col + 3)) p3 = 0.0f;
+              if (col > lim) p0 = 0.0f;
+              if (col + 1 > lim) p1 = 0.0f;
+              if (col + 2 > lim) p2 = 0.0f;
+              if (col + 3 > lim) p3 = 0.0f;
             }
             a4[0] += p0;
             a4[1] += p1;
@@ -529,17 +384,10 @@ __global__ void __launch_bounds__(384, 1)
     }
     if (ok && nk > 0) ok = mbar_wait(o_done(w), (nk - 1) & 1, p.status);
     tc_fence_after();
-    if (SPAN && nk == 0 && filled && qpos < sh.seq) {  // no row of the tile sees anything
-      uint4* dst = reinterpret_cast<uint4*>(
-          p.out + ((static_cast<size_t>(b) * sh.seq + qpos) * sh.heads + head) * D);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
-      p.lse[(static_cast<size_t>(b) * sh.heads + head) * sh.seq + qpos] = -INFINITY;
-    }
     if (ok && nk > 0) {
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      const bool valid = filled && qpos < sh.seq;
-      uint16_t* orow = p.out + ((static_cast<size_t>(b) * sh.seq + qpos) * sh.heads + head) * D;
+      const bool valid = qpos < sh.seq;
+      uint16_t* orow = p.out + ((static_cast<size_t>(b) * sh.seq + qpos) * sh.heads + h) * D;
 #pragma unroll
       for (int c4 = 0; c4 < D / 32; ++c4) {
         uint32_t o[32];
@@ -558,7 +406,7 @@ __global__ void __launch_bounds__(384, 1)
         }
       }
       if (valid)
-        p.lse[(static_cast<size_t>(b) * sh.heads + head) * sh.seq + qpos] =
+        p.lse[(static_cast<size_t>(b) * sh.heads + h) * sh.seq + qpos] =
             l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
     }
   }
@@ -593,22 +441,6 @@ __global__ void __launch_bounds__(384, 1)
 // forward, every barrier used per tile t comes in two (t's parity) and a
 // parity wait is never more than one phase behind.
 
-constexpr int kHalf = 64;  // the streamed tile of the backward kernels
-
-// SPAN: what the prep launch leaves for the other two, by 64-row packed query
-// tile, 64 entries each (rows that hold nothing: no keys, lse2 = +inf, delta =
-// 0): the statistics [batch, heads / pack, tiles64, 64], each row's first key
-// and how many [batch, tiles64, 64], and over the tile the keys that any row
-// sees, [lo, hi), and those that every filled row sees, [all_lo, all_hi).
-struct SpanTile {
-  int lo, hi, all_lo, all_hi;
-};
-
-struct SpanWork {
-  int2* rows;
-  SpanTile* tiles;
-};
-
 struct PrepParams {
   const uint16_t* out;
   const uint16_t* dout;
@@ -616,71 +448,23 @@ struct PrepParams {
   float* lse2;
   float* delta;
   int batch, seq, heads, seq_pad, dim;
-  int pack, pos64, tiles64;  // SPAN
-  const int* first;
-  const int* last;
-  SpanWork span;
-  unsigned row_blocks;  // SPAN: blocks from here on do the spans, a warp a tile
 };
 
 // Eight lanes per row, dim / 8 elements each.
-template <bool SPAN>
 __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const PrepParams p) {
   griddep_wait();
   griddep_launch_dependents();
-  if (SPAN && blockIdx.x >= p.row_blocks) {
-    const long long t = static_cast<long long>(blockIdx.x - p.row_blocks) * 8 + (threadIdx.x >> 5);
-    if (t >= static_cast<long long>(p.batch) * p.tiles64) return;
-    const int b = static_cast<int>(t / p.tiles64);
-    const int i0 = static_cast<int>(t % p.tiles64) * p.pos64;
-    SpanTile s{p.seq, 0, 0, p.seq};
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = e * 32 + (threadIdx.x & 31);
-      const bool filled = r < p.pack * p.pos64;
-      const Span sp =
-          filled ? load_span(p.first, p.last, b, i0 + r / p.pack, p.seq) : Span{0, 0};
-      p.span.rows[t * kHalf + r] = make_int2(sp.lo, sp.hi - sp.lo);
-      if (!filled) continue;
-      if (sp.lo < sp.hi) s.lo = min(s.lo, sp.lo);
-      s.hi = max(s.hi, sp.hi);
-      s.all_lo = max(s.all_lo, sp.lo);
-      s.all_hi = min(s.all_hi, sp.hi);
-    }
-    s.lo = __reduce_min_sync(0xffffffffu, s.lo);
-    s.hi = __reduce_max_sync(0xffffffffu, s.hi);
-    s.all_lo = __reduce_max_sync(0xffffffffu, s.all_lo);
-    s.all_hi = __reduce_min_sync(0xffffffffu, s.all_hi);
-    if ((threadIdx.x & 31) == 0) p.span.tiles[t] = s;
-    return;
-  }
   const long long gid = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const long long row = gid >> 3;
   const int sub = threadIdx.x & 7;
-  const long long rows = SPAN ? static_cast<long long>(p.batch) * (p.heads / p.pack) *
-                                    p.tiles64 * kHalf
-                              : static_cast<long long>(p.batch) * p.heads * p.seq_pad;
+  const long long rows = static_cast<long long>(p.batch) * p.heads * p.seq_pad;
   const bool in = row < rows;
-  int b, h, s;  // the row's sequence, head and position
-  bool real = in;
-  if constexpr (SPAN) {
-    const long long t = in ? row / kHalf : 0;
-    const int r = static_cast<int>(row % kHalf);
-    const int bg = static_cast<int>(t / p.tiles64);
-    const int groups = p.heads / p.pack;
-    b = bg / groups;
-    h = bg % groups * p.pack + r % p.pack;
-    s = static_cast<int>(t % p.tiles64) * p.pos64 + r / p.pack;
-    real = in && r < p.pack * p.pos64;
-  } else {
-    const int bh = in ? static_cast<int>(row / p.seq_pad) : 0;
-    b = bh / p.heads;
-    h = bh % p.heads;
-    s = in ? static_cast<int>(row % p.seq_pad) : 0;
-  }
-  real = real && s < p.seq;
+  const int bh = in ? static_cast<int>(row / p.seq_pad) : 0;
+  const int s = in ? static_cast<int>(row % p.seq_pad) : 0;
+  const bool real = in && s < p.seq;
   float acc = 0.0f;
   if (real) {
+    const int b = bh / p.heads, h = bh % p.heads;
     const int per = p.dim / 8;
     const size_t off = ((static_cast<size_t>(b) * p.seq + s) * p.heads + h) * p.dim + sub * per;
     for (int c = 0; c < per; c += 8) {
@@ -702,7 +486,7 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const PrepParams p) 
   if (in && sub == 0) {
     float l2 = INFINITY;
     if (real) {
-      const float l = p.lse[(static_cast<size_t>(b) * p.heads + h) * p.seq + s];
+      const float l = p.lse[static_cast<size_t>(bh) * p.seq + s];
       l2 = l == -INFINITY ? INFINITY : l * kLog2e;
     }
     p.lse2[row] = l2;
@@ -712,9 +496,6 @@ __global__ void __launch_bounds__(256) attn_bwd_prep_kernel(const PrepParams p) 
 
 struct BwdParams {
   AttnShape sh;
-  const int* first;  // SPAN: [batch, seq]
-  const int* last;
-  SpanWork span;
   int seq_pad;
   float scale;
   const float* lse2;
@@ -754,7 +535,7 @@ struct DqCfg {
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
-template <int D, bool SPAN>
+template <int D>
 __global__ void __launch_bounds__(384, 1)
     attn_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q,
                        const __grid_constant__ CUtensorMap tm_do,
@@ -789,26 +570,14 @@ __global__ void __launch_bounds__(384, 1)
   const AttnShape& sh = p.sh;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int pack = SPAN ? sh.pack : 1;
-  const int pos_per = SPAN ? sh.pos128 : kTile;  // positions of the query tile
-  const int rows = SPAN ? pack * pos_per : kTile;
-  const int bh_count = sh.batch * (sh.heads / pack);
+  const int bh_count = sh.batch * sh.heads;
   const int bh = blockIdx.x % bh_count;
-  const int qt = (SPAN ? sh.tiles128 : sh.n_tiles) - 1 - static_cast<int>(blockIdx.x / bh_count);
-  const int b = bh / (sh.heads / pack);
-  const int h = bh % (sh.heads / pack) * pack;  // (SPAN: the first of `pack`)
+  const int qt = sh.n_tiles - 1 - static_cast<int>(blockIdx.x / bh_count);
+  const int b = bh / sh.heads;
+  const int h = bh % sh.heads;
   const int hk = h / sh.group;
-  const int q0 = qt * pos_per;
-  __shared__ int range[2];  // SPAN: the tile's least first and greatest last
-  if constexpr (SPAN) {
-    if (threadIdx.x == 0) {
-      range[0] = sh.seq;
-      range[1] = 0;
-    }
-    zero_rows(gbase + C::Q_OFF, 2 * C::SLABS, kTile, rows);  // Q and dO
-  }
+  const int q0 = qt * kTile;
   const int n_half = (sh.seq + kHalf - 1) / kHalf;
-  int kv_first = 0;  // first 64-key tile
   int n_kv = n_half;
   if (sh.causal && (q0 + kTile - 1) / kHalf + 1 < n_kv) n_kv = (q0 + kTile - 1) / kHalf + 1;
 
@@ -843,23 +612,6 @@ __global__ void __launch_bounds__(384, 1)
   griddep_launch_dependents();
   griddep_wait();
 
-  if constexpr (SPAN) {  // the key tiles that the tile's rows see
-    if (threadIdx.x < kTile) {
-      const int i = threadIdx.x;
-      const Span sp =
-          i < pos_per ? load_span(p.first, p.last, b, q0 + i, sh.seq) : Span{0, 0};
-      const int lo = __reduce_min_sync(0xffffffffu, sp.lo < sp.hi ? sp.lo : sh.seq);
-      const int hi = __reduce_max_sync(0xffffffffu, sp.hi);
-      if (lane == 0) {
-        atomicMin(&range[0], lo);
-        atomicMax(&range[1], hi);
-      }
-    }
-    __syncthreads();
-    kv_first = range[0] / kHalf;
-    n_kv = max((range[1] + kHalf - 1) / kHalf - kv_first, 0);
-  }
-
   if (warp == 0) {
     // ------------------------------------------------------------- TMA
     if (elect_one_sync()) {
@@ -867,7 +619,7 @@ __global__ void __launch_bounds__(384, 1)
       tma_prefetch_desc(&tm_do);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      mbar_arrive_expect_tx(q_full, 2 * C::SLABS * rows * 128);
+      mbar_arrive_expect_tx(q_full, 2 * C::QTILE);
       for (int sl = 0; sl < C::SLABS; ++sl) {
         tma_load_4d(q_s + sl * C::QSLAB, &tm_q, q_full, sl * 64, h, q0, b);
         tma_load_4d(do_s + sl * C::QSLAB, &tm_do, q_full, sl * 64, h, q0, b);
@@ -878,14 +630,12 @@ __global__ void __launch_bounds__(384, 1)
         if (!mbar_wait(k_empty(ks), ((j / KST) & 1) ^ 1, p.status)) break;
         mbar_arrive_expect_tx(k_full(ks), C::KTILE);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(k_s(ks) + sl * C::KSLAB, &tm_k, k_full(ks), sl * 64, hk,
-                      (kv_first + j) * kHalf, b);
+          tma_load_4d(k_s(ks) + sl * C::KSLAB, &tm_k, k_full(ks), sl * 64, hk, j * kHalf, b);
         ++nk;
         if (!mbar_wait(v_empty(vs), ((j / VST) & 1) ^ 1, p.status)) break;
         mbar_arrive_expect_tx(v_full(vs), C::KTILE);
         for (int sl = 0; sl < C::SLABS; ++sl)
-          tma_load_4d(v_s(vs) + sl * C::KSLAB, &tm_v, v_full(vs), sl * 64, hk,
-                      (kv_first + j) * kHalf, b);
+          tma_load_4d(v_s(vs) + sl * C::KSLAB, &tm_v, v_full(vs), sl * 64, hk, j * kHalf, b);
         ++nv;
       }
       mbar_wait(q_full, 0, p.status);
@@ -958,26 +708,11 @@ __global__ void __launch_bounds__(384, 1)
     const int half = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
-    const int qpos = q0 + row / pack;
-    const int head = h + row % pack;
-    const bool filled = !SPAN || row < rows;
+    const int qpos = q0 + row;
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    float lse2 = INFINITY, dl = 0.0f;
-    int2 sp = make_int2(0, 0);  // SPAN: first key and how many
-    if constexpr (SPAN) {
-      if (filled && qpos < sh.seq) {
-        const size_t srow = (static_cast<size_t>(bh) * sh.tiles64 + qpos / sh.pos64) * kHalf +
-                            qpos % sh.pos64 * pack + row % pack;
-        lse2 = p.lse2[srow];
-        dl = p.delta[srow];
-        const Span s = load_span(p.first, p.last, b, qpos, sh.seq);
-        sp = make_int2(s.lo, s.hi - s.lo);
-      }
-    } else {
-      const size_t srow = static_cast<size_t>(bh) * p.seq_pad + qpos;
-      lse2 = p.lse2[srow];
-      dl = p.delta[srow];
-    }
+    const size_t srow = static_cast<size_t>(bh) * p.seq_pad + qpos;
+    const float lse2 = p.lse2[srow];
+    const float dl = p.delta[srow];
     const float c = sh.scale_log2;
     bool ok = true;
     for (int j = 0; j < n_kv; ++j) {
@@ -991,25 +726,20 @@ __global__ void __launch_bounds__(384, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_free(j & 1));
-      const int kv0 = (kv_first + j) * kHalf + half * 32;
+      const int kv0 = j * kHalf + half * 32;
       int lim = 31;  // last column of this half tile that counts
-      if (!SPAN && ((sh.causal && kv0 + 31 > q0) || kv0 + 32 > sh.seq)) {
+      if ((sh.causal && kv0 + 31 > q0) || kv0 + 32 > sh.seq) {
         lim = sh.seq - 1 - kv0;
         if (sh.causal && qpos - kv0 < lim) lim = qpos - kv0;
       }
-      auto counts = [&](int col) {
-        if constexpr (SPAN)
-          return static_cast<unsigned>(kv0 + col - sp.x) < static_cast<unsigned>(sp.y);
-        return col <= lim;
-      };
       uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 32; i += 2) {
         float p0 = ex2_approx(fmaf(__uint_as_float(sv[i]), c, -lse2));
         float p1 = (i & 2) ? exp2_poly(fmaf(__uint_as_float(sv[i + 1]), c, -lse2))
                            : ex2_approx(fmaf(__uint_as_float(sv[i + 1]), c, -lse2));
-        if (!counts(i)) p0 = 0.0f;
-        if (!counts(i + 1)) p1 = 0.0f;
+        if (i > lim) p0 = 0.0f;
+        if (i + 1 > lim) p1 = 0.0f;
         pk[i / 2] = pack_bf16x2_f32(p0 * (__uint_as_float(dv[i]) - dl),
                                     p1 * (__uint_as_float(dv[i + 1]) - dl));
       }
@@ -1022,17 +752,13 @@ __global__ void __launch_bounds__(384, 1)
     if (ok) ok = mbar_wait(dq_full, 0, p.status);
     tc_fence_after();
     if (ok) {
-      const bool valid = filled && qpos < sh.seq;
-      uint16_t* orow = p.dq + ((static_cast<size_t>(b) * sh.seq + qpos) * sh.heads + head) * D;
+      const bool valid = qpos < sh.seq;
+      uint16_t* orow = p.dq + ((static_cast<size_t>(b) * sh.seq + qpos) * sh.heads + h) * D;
 #pragma unroll
       for (int c4 = half * (D / 64); c4 < (half + 1) * (D / 64); ++c4) {
         uint32_t o[32];
         tmem_ld_32x32b_x32(lrow + C::DQ_COL + c4 * 32, o);
         tmem_ld_wait();
-        if (SPAN && n_kv == 0) {  // no row of the tile sees anything
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0;
-        }
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -1089,7 +815,7 @@ struct DkvCfg {
   static_assert(SMEM > 118784, "one CTA per SM");
 };
 
-template <int D, bool SPAN>
+template <int D>
 __global__ void __launch_bounds__(384, 1)
     attn_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
                         const __grid_constant__ CUtensorMap tm_do,
@@ -1130,20 +856,10 @@ __global__ void __launch_bounds__(384, 1)
   const int b = bk / sh.kv_heads;
   const int hk = bk % sh.kv_heads;
   const int kv0 = jt * kTile;
-  const int pack = SPAN ? sh.pack : 1;
-  const int pos_per = SPAN ? sh.pos64 : kHalf;  // positions of a query tile
-  const int rows = SPAN ? pack * pos_per : kHalf;
-  const int n_half = SPAN ? sh.tiles64 : (sh.seq + kHalf - 1) / kHalf;
-  int i0 = sh.causal ? kv0 / kHalf : 0;  // first query tile that sees this key tile
-  int nq = n_half - i0;
-  __shared__ int seen[2];  // SPAN: the first and last query tile that see it
-  if constexpr (SPAN) {
-    if (threadIdx.x == 0) {
-      seen[0] = n_half;
-      seen[1] = -1;
-    }
-    zero_rows(gbase + C::Q_OFF, 2 * C::QST * C::SLABS, kHalf, rows);  // the Q and dO stages
-  }
+  const int n_half = (sh.seq + kHalf - 1) / kHalf;
+  const int i0 = sh.causal ? kv0 / kHalf : 0;  // first query tile that sees this key tile
+  const int nq = n_half - i0;
+  const int T = sh.group * nq;
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -1172,27 +888,6 @@ __global__ void __launch_bounds__(384, 1)
   griddep_launch_dependents();
   griddep_wait();
 
-  const SpanTile* const tiles =
-      SPAN ? p.span.tiles + static_cast<size_t>(b) * n_half : nullptr;
-  if constexpr (SPAN) {
-    int a = n_half, z = -1;
-    for (int i = threadIdx.x; i < n_half; i += 384)
-      if (tiles[i].lo < kv0 + kTile && tiles[i].hi > kv0) {
-        a = min(a, i);
-        z = i;
-      }
-    a = __reduce_min_sync(0xffffffffu, a);
-    z = __reduce_max_sync(0xffffffffu, z);
-    if (lane == 0) {
-      atomicMin(&seen[0], a);
-      atomicMax(&seen[1], z);
-    }
-    __syncthreads();
-    i0 = seen[0];
-    nq = max(seen[1] + 1 - i0, 0);
-  }
-  const int T = sh.group / pack * nq;
-
   if (warp == 0) {
     // ------------------------------------------------------------- TMA
     if (elect_one_sync()) {
@@ -1209,12 +904,10 @@ __global__ void __launch_bounds__(384, 1)
       for (int t = 0; t < T; ++t) {
         const int s = t % QST;
         if (!mbar_wait(q_empty(s), ((t / QST) & 1) ^ 1, p.status)) break;
-        const int h = hk * sh.group + t / nq * pack;
-        const int qq0 = (i0 + t % nq) * pos_per;
-        const size_t srow =
-            SPAN ? (static_cast<size_t>((b * sh.heads + h) / pack) * n_half + i0 + t % nq) * kHalf
-                 : static_cast<size_t>(b * sh.heads + h) * p.seq_pad + qq0;
-        mbar_arrive_expect_tx(q_full(s), 2 * C::SLABS * rows * 128 + C::STAT_BYTES);
+        const int h = hk * sh.group + t / nq;
+        const int qq0 = (i0 + t % nq) * kHalf;
+        const size_t srow = static_cast<size_t>(b * sh.heads + h) * p.seq_pad + qq0;
+        mbar_arrive_expect_tx(q_full(s), 2 * C::QTILE + C::STAT_BYTES);
         for (int sl = 0; sl < C::SLABS; ++sl) {
           tma_load_4d(q_s(s) + sl * C::QSLAB, &tm_q, q_full(s), sl * 64, h, qq0, b);
           tma_load_4d(do_s(s) + sl * C::QSLAB, &tm_do, q_full(s), sl * 64, h, qq0, b);
@@ -1313,17 +1006,7 @@ __global__ void __launch_bounds__(384, 1)
       // A key row sees query q only if q >= kvpos (causal); rows past seq
       // carry lse2 = +inf, so their probabilities are 0 already.
       int first = 0;
-      if (!SPAN && sh.causal && qq0 < kvpos) first = kvpos - qq0;
-      // SPAN: the rows' spans, unless every row of the query tile sees the
-      // whole key tile (the spans do not fit beside the tiles in shared
-      // memory; all threads read the same few words, from L1).
-      bool whole = true;
-      const int2* spans = nullptr;
-      if constexpr (SPAN) {
-        const SpanTile st4 = tiles[i0 + t % nq];
-        whole = st4.all_lo <= kv0 && st4.all_hi >= kv0 + kTile;
-        spans = p.span.rows + (static_cast<size_t>(b) * n_half + i0 + t % nq) * kHalf + half * 32;
-      }
+      if (sh.causal && qq0 < kvpos) first = kvpos - qq0;
       uint32_t pk[16], dk[16];
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
@@ -1336,14 +1019,7 @@ __global__ void __launch_bounds__(384, 1)
         for (int e = 0; e < 4; ++e) {
           const float x = fmaf(__uint_as_float(sv[i + e]), c, -la[e]);
           float pe = e == 3 ? exp2_poly(x) : ex2_approx(x);
-          if constexpr (SPAN) {
-            if (!whole) {
-              const int2 sp = spans[i + e];
-              if (static_cast<unsigned>(kvpos - sp.x) >= static_cast<unsigned>(sp.y)) pe = 0.0f;
-            }
-          } else {
-            if (i + e < first) pe = 0.0f;
-          }
+          if (i + e < first) pe = 0.0f;
           pv[e] = pe;
           dsv[e] = pe * (__uint_as_float(dv[i + e]) - da[e]);
         }
@@ -1387,10 +1063,6 @@ __global__ void __launch_bounds__(384, 1)
           uint32_t o[32];
           tmem_ld_32x32b_x32(lrow + col + c4 * 32, o);
           tmem_ld_wait();
-          if (SPAN && T == 0) {  // no query sees the key tile
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0;
-          }
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i)
@@ -1416,45 +1088,6 @@ __global__ void __launch_bounds__(384, 1)
 }
 
 
-// [batch, seq, heads, dim] bf16 as a 4D tensor map, one 64-wide dim slab x
-// `rows` positions of `pack` heads per box (128-byte swizzle).
-int map_bshd(CUtensorMap* map, const void* ptr, int64_t batch, int64_t seq, int64_t heads,
-             int64_t dim, uint32_t rows = kTile, uint32_t pack = 1) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(heads),
-                            static_cast<uint64_t>(seq), static_cast<uint64_t>(batch)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(dim) * 2,
-                               static_cast<uint64_t>(heads * dim) * 2,
-                               static_cast<uint64_t>(seq * heads * dim) * 2};
-  const uint32_t box[4] = {64, pack, rows, 1};
-  return encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, ptr, dims, strides, box,
-                     CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
-int check_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t dim) {
-  if (batch < 0 || seq < 0 || heads <= 0 || kv_heads <= 0)
-    return fail(TQ_ERR_INVALID, "attention: batch and seq must be >= 0, heads and kv_heads > 0");
-  if (heads % kv_heads != 0)
-    return fail(TQ_ERR_INVALID, "attention: heads (%lld) must be a multiple of kv_heads (%lld)",
-                (long long)heads, (long long)kv_heads);
-  if (dim != 64 && dim != 128)
-    return fail(TQ_ERR_UNSUPPORTED, "attention: head dim must be 64 or 128, got %lld",
-                (long long)dim);
-  const int64_t tiles = (seq + kTile - 1) / kTile;
-  if (seq > (1ll << 30) || batch * heads * tiles > (1ll << 31) - 1 ||
-      batch * seq * heads * dim > (1ll << 40))
-    return fail(TQ_ERR_INVALID, "attention: shape too large");
-  return TQ_OK;
-}
-
-// How many of the query heads that share a key/value head a packed tile holds:
-// the most, up to 16, that divide them and fill at least 60 of 64 rows (4, 7
-// and 8 of groups of those sizes; 7 of a group of 14; 1 of a group of 11).
-int pack_of(int group) {
-  for (int n = group < 16 ? group : 16; n > 1; --n)
-    if (group % n == 0 && kHalf / n * n >= 60) return n;
-  return 1;
-}
-
 AttnShape make_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, float scale,
                      int causal) {
   AttnShape s{};
@@ -1466,83 +1099,41 @@ AttnShape make_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads
   s.n_tiles = static_cast<int>((seq + kTile - 1) / kTile);
   s.causal = causal ? 1 : 0;
   s.scale_log2 = scale * kLog2e;
-  s.pack = pack_of(s.group);
-  s.pos128 = kTile / s.pack;
-  s.pos64 = kHalf / s.pack;
-  s.tiles128 = (s.seq + s.pos128 - 1) / s.pos128;
-  s.tiles64 = (s.seq + s.pos64 - 1) / s.pos64;
   return s;
 }
 
-template <int D, bool SPAN>
-int launch_fwd(const void* q, const void* k, const void* v, const int* first, const int* last,
-               const AttnShape& sh, void* out, float* lse, int* status, cudaStream_t stream) {
+template <int D>
+int launch_fwd(const void* q, const void* k, const void* v, const AttnShape& sh, void* out,
+               float* lse, int* status, cudaStream_t stream) {
   using C = FwdCfg<D>;
-  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_fwd_kernel<D, SPAN>), C::SMEM,
+  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_fwd_kernel<D>), C::SMEM,
                              "cudaFuncSetAttribute(attn_fwd)");
   if (rc) return rc;
   CUtensorMap tq_, tk, tv;
-  if ((rc = map_bshd(&tq_, q, sh.batch, sh.seq, sh.heads, D, SPAN ? sh.pos128 : kTile,
-                     SPAN ? sh.pack : 1)))
-    return rc;
+  if ((rc = map_bshd(&tq_, q, sh.batch, sh.seq, sh.heads, D))) return rc;
   if ((rc = map_bshd(&tk, k, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
   if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
   FwdParams p{};
   p.sh = sh;
-  p.first = first;
-  p.last = last;
-  p.n_pairs = ((SPAN ? sh.tiles128 : sh.n_tiles) + 1) / 2;
+  p.n_pairs = (sh.n_tiles + 1) / 2;
   p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.status = status;
-  const unsigned grid =
-      static_cast<unsigned>(sh.batch) * (sh.heads / (SPAN ? sh.pack : 1)) * p.n_pairs;
-  return launch_kernel(attn_fwd_kernel<D, SPAN>, dim3(grid), dim3(384), C::SMEM, stream, 1,
+  const unsigned grid = static_cast<unsigned>(sh.batch) * sh.heads * p.n_pairs;
+  return launch_kernel(attn_fwd_kernel<D>, dim3(grid), dim3(384), C::SMEM, stream, 1,
                        "attention forward launch", tq_, tk, tv, p);
 }
 
-// What the caller's workspace holds: two statistics per query row and, for
-// spans, each row's and each query tile's.
-struct BwdWork {
-  float* lse2;
-  float* delta;
-  SpanWork span;
-  int seq_pad;
-  size_t bytes;
-};
-
-BwdWork bwd_work(void* base, const AttnShape& sh, bool span) {
-  BwdWork w{};
-  w.seq_pad = sh.n_tiles * kTile;
-  const size_t tiles = static_cast<size_t>(sh.batch) * sh.tiles64;
-  const size_t rows = span ? tiles * kHalf * (sh.heads / sh.pack)
-                           : static_cast<size_t>(sh.batch) * sh.heads * w.seq_pad;
-  w.lse2 = static_cast<float*>(base);
-  w.delta = w.lse2 + rows;
-  w.bytes = 2 * rows * sizeof(float);
-  if (span) {
-    w.span.rows = reinterpret_cast<int2*>(static_cast<uint8_t*>(base) + w.bytes);
-    w.bytes += tiles * kHalf * sizeof(int2);
-    w.span.tiles = reinterpret_cast<SpanTile*>(static_cast<uint8_t*>(base) + w.bytes);
-    w.bytes += tiles * sizeof(SpanTile);
-  }
-  return w;
-}
-
-template <int D, bool SPAN>
-int launch_bwd(const void* q, const void* k, const void* v, const int* first, const int* last,
-               const void* out, const void* dout, const float* lse, const AttnShape& sh,
-               float scale, void* dq, void* dk, void* dv, const BwdWork& work, int* status,
-               cudaStream_t stream) {
-  float* const lse2 = work.lse2;
-  float* const delta = work.delta;
-  const int seq_pad = work.seq_pad;
+template <int D>
+int launch_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
+               const float* lse, const AttnShape& sh, float scale, void* dq, void* dk, void* dv,
+               float* lse2, float* delta, int seq_pad, int* status, cudaStream_t stream) {
   using Q = DqCfg<D>;
   using KV = DkvCfg<D>;
-  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dq_kernel<D, SPAN>), Q::SMEM,
+  int rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dq_kernel<D>), Q::SMEM,
                              "cudaFuncSetAttribute(attn_bwd_dq)");
   if (rc) return rc;
-  rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dkv_kernel<D, SPAN>), KV::SMEM,
+  rc = set_max_smem_once(reinterpret_cast<const void*>(attn_bwd_dkv_kernel<D>), KV::SMEM,
                          "cudaFuncSetAttribute(attn_bwd_dkv)");
   if (rc) return rc;
   PrepParams pp{};
@@ -1556,39 +1147,23 @@ int launch_bwd(const void* q, const void* k, const void* v, const int* first, co
   pp.heads = sh.heads;
   pp.seq_pad = seq_pad;
   pp.dim = D;
-  const long long rows =
-      SPAN ? static_cast<long long>(sh.batch) * (sh.heads / sh.pack) * sh.tiles64 * kHalf
-           : static_cast<long long>(sh.batch) * sh.heads * seq_pad;
-  pp.pack = sh.pack;
-  pp.pos64 = sh.pos64;
-  pp.tiles64 = sh.tiles64;
-  pp.first = first;
-  pp.last = last;
-  pp.span = work.span;
-  pp.row_blocks = static_cast<unsigned>((rows * 8 + 255) / 256);
-  const unsigned span_blocks =
-      SPAN ? static_cast<unsigned>((static_cast<long long>(sh.batch) * sh.tiles64 + 7) / 8) : 0;
-  rc = launch_kernel(attn_bwd_prep_kernel<SPAN>, dim3(pp.row_blocks + span_blocks), dim3(256), 0,
-                     stream, 1, "attention backward prep launch", pp);
+  const long long rows = static_cast<long long>(sh.batch) * sh.heads * seq_pad;
+  rc = launch_kernel(attn_bwd_prep_kernel, dim3(static_cast<unsigned>((rows * 8 + 255) / 256)),
+                     dim3(256), 0, stream, 1, "attention backward prep launch", pp);
   if (rc) return rc;
   // Query-side maps (128-row boxes for dq, 64-row boxes for dkv) and the
   // key/value maps the other way round.
   CUtensorMap q128, do128, k64, v64, q64, do64, k128, v128;
-  const uint32_t pack = SPAN ? sh.pack : 1;
-  const uint32_t rows128 = SPAN ? sh.pos128 : kTile, rows64 = SPAN ? sh.pos64 : kHalf;
-  if ((rc = map_bshd(&q128, q, sh.batch, sh.seq, sh.heads, D, rows128, pack))) return rc;
-  if ((rc = map_bshd(&do128, dout, sh.batch, sh.seq, sh.heads, D, rows128, pack))) return rc;
+  if ((rc = map_bshd(&q128, q, sh.batch, sh.seq, sh.heads, D, kTile))) return rc;
+  if ((rc = map_bshd(&do128, dout, sh.batch, sh.seq, sh.heads, D, kTile))) return rc;
   if ((rc = map_bshd(&k64, k, sh.batch, sh.seq, sh.kv_heads, D, kHalf))) return rc;
   if ((rc = map_bshd(&v64, v, sh.batch, sh.seq, sh.kv_heads, D, kHalf))) return rc;
-  if ((rc = map_bshd(&q64, q, sh.batch, sh.seq, sh.heads, D, rows64, pack))) return rc;
-  if ((rc = map_bshd(&do64, dout, sh.batch, sh.seq, sh.heads, D, rows64, pack))) return rc;
+  if ((rc = map_bshd(&q64, q, sh.batch, sh.seq, sh.heads, D, kHalf))) return rc;
+  if ((rc = map_bshd(&do64, dout, sh.batch, sh.seq, sh.heads, D, kHalf))) return rc;
   if ((rc = map_bshd(&k128, k, sh.batch, sh.seq, sh.kv_heads, D, kTile))) return rc;
   if ((rc = map_bshd(&v128, v, sh.batch, sh.seq, sh.kv_heads, D, kTile))) return rc;
   BwdParams p{};
   p.sh = sh;
-  p.first = first;
-  p.last = last;
-  p.span = work.span;
   p.seq_pad = seq_pad;
   p.scale = scale;
   p.lse2 = lse2;
@@ -1597,197 +1172,13 @@ int launch_bwd(const void* q, const void* k, const void* v, const int* first, co
   p.dk = static_cast<uint16_t*>(dk);
   p.dv = static_cast<uint16_t*>(dv);
   p.status = status;
-  const unsigned grid_q = static_cast<unsigned>(sh.batch) * (sh.heads / pack) *
-                          (SPAN ? sh.tiles128 : sh.n_tiles);
-  rc = launch_kernel(attn_bwd_dq_kernel<D, SPAN>, dim3(grid_q), dim3(384), Q::SMEM, stream, 1,
+  const unsigned grid_q = static_cast<unsigned>(sh.batch) * sh.heads * sh.n_tiles;
+  rc = launch_kernel(attn_bwd_dq_kernel<D>, dim3(grid_q), dim3(384), Q::SMEM, stream, 1,
                      "attention backward dq launch", q128, do128, k64, v64, p);
   if (rc) return rc;
   const unsigned grid_kv = static_cast<unsigned>(sh.batch) * sh.kv_heads * sh.n_tiles;
-  return launch_kernel(attn_bwd_dkv_kernel<D, SPAN>, dim3(grid_kv), dim3(384), KV::SMEM, stream, 1,
+  return launch_kernel(attn_bwd_dkv_kernel<D>, dim3(grid_kv), dim3(384), KV::SMEM, stream, 1,
                        "attention backward dkv launch", q64, do64, k128, v128, p);
-}
-
-int attention_fwd(const void* q, const void* k, const void* v, const int* first, const int* last,
-                  bool span, int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads,
-                  int64_t head_dim, float scale, int causal, void* out, float* lse,
-                  void* stream) {
-  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
-  if (rc) return rc;
-  if (!(scale > 0.0f) || !std::isfinite(scale))
-    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
-  if (batch == 0 || seq == 0) return TQ_OK;
-  if (!q || !k || !v || !out || !lse || (span && (!first || !last)))
-    return fail(TQ_ERR_INVALID, "attention: null pointer");
-  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
-      !aligned(lse, 4))
-    return fail(TQ_ERR_MISALIGNED, "attention: q, k, v and out must be 16-byte aligned");
-  if (!aligned(first, 4) || !aligned(last, 4))
-    return fail(TQ_ERR_MISALIGNED, "attention: first and last must be 4-byte aligned");
-  int* status = device_status_ptr(&rc);
-  if (!status) return rc;
-  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
-  auto launch = head_dim == 64 ? (span ? launch_fwd<64, true> : launch_fwd<64, false>)
-                               : (span ? launch_fwd<128, true> : launch_fwd<128, false>);
-  return launch(q, k, v, first, last, sh, out, lse, status, as_stream(stream));
-}
-
-int attention_bwd(const void* q, const void* k, const void* v, const int* first, const int* last,
-                  bool span, const void* out, const void* dout, const float* lse, int64_t batch,
-                  int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
-                  int causal, void* dq, void* dk, void* dv, void* workspace,
-                  size_t workspace_bytes, void* stream) {
-  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
-  if (rc) return rc;
-  if (!(scale > 0.0f) || !std::isfinite(scale))
-    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
-  if (batch == 0 || seq == 0) return TQ_OK;
-  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
-  const BwdWork work = bwd_work(workspace, sh, span);
-  const size_t need = work.bytes;
-  if (workspace_bytes < need)
-    return fail(TQ_ERR_INVALID, "attention: workspace of %zu bytes, %zu needed", workspace_bytes,
-                need);
-  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace ||
-      (span && (!first || !last)))
-    return fail(TQ_ERR_INVALID, "attention: null pointer");
-  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
-      !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
-      !aligned(workspace, 256) || !aligned(lse, 4))
-    return fail(TQ_ERR_MISALIGNED,
-                "attention: tensors must be 16-byte aligned and the workspace 256-byte aligned");
-  if (!aligned(first, 4) || !aligned(last, 4))
-    return fail(TQ_ERR_MISALIGNED, "attention: first and last must be 4-byte aligned");
-  int* status = device_status_ptr(&rc);
-  if (!status) return rc;
-  auto launch = head_dim == 64 ? (span ? launch_bwd<64, true> : launch_bwd<64, false>)
-                               : (span ? launch_bwd<128, true> : launch_bwd<128, false>);
-  return launch(q, k, v, first, last, out, dout, lse, sh, scale, dq, dk, dv, work, status,
-                as_stream(stream));
-}
-
-// --------------------------------------------------------- document spans --
-
-constexpr int kScanThreads = 1024;
-constexpr int kScanItems = 8;
-
-struct DocParams {
-  const void* documents;
-  const int* prefix;  // may be null
-  int ids64, seq, causal;
-  int* first;
-  int* last;
-};
-
-// Inclusive scan over a warp's lanes: the running maximum from the front, or
-// the running minimum from the back.
-template <bool BACK>
-__device__ __forceinline__ int scan_lanes(int v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int o = BACK ? __shfl_down_sync(0xffffffffu, v, off) : __shfl_up_sync(0xffffffffu, v, off);
-    if (BACK ? lane + off < 32 : lane >= off) v = BACK ? min(v, o) : max(v, o);
-  }
-  return v;
-}
-
-// The same over the block's threads, exclusive (rest: what the first, or
-// last, thread gets); the whole block's result goes to all.
-template <bool BACK>
-__device__ __forceinline__ int scan_threads(int v, int rest, int* sh, int& all) {
-  static_assert(kScanThreads == 1024, "one total a lane");
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto join = [](int a, int b) { return BACK ? min(a, b) : max(a, b); };
-  v = scan_lanes<BACK>(v);
-  __syncthreads();  // the last call's reads of sh
-  if (lane == (BACK ? 0 : 31)) sh[warp] = v;
-  __syncthreads();
-  const int totals = scan_lanes<BACK>(sh[lane]);
-  all = join(__shfl_sync(0xffffffffu, totals, BACK ? 0 : 31), rest);
-  const int warps = __shfl_sync(0xffffffffu, totals, BACK ? (warp + 1) & 31 : (warp + 31) & 31);
-  int in = BACK ? __shfl_down_sync(0xffffffffu, v, 1) : __shfl_up_sync(0xffffffffu, v, 1);
-  if (lane == (BACK ? 31 : 0)) in = rest;
-  if (warp != (BACK ? 31 : 0)) in = join(in, warps);
-  return join(in, rest);
-}
-
-// One CTA per row of ids.  A document is a run of equal ids: its start reaches
-// its positions by a running maximum of the runs' starts from the front, its
-// end by a running minimum from the back, stretch by stretch.
-__global__ void __launch_bounds__(kScanThreads) document_spans_kernel(const DocParams p) {
-  griddep_wait();
-  griddep_launch_dependents();
-  __shared__ int sh[kScanThreads / 32];
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * p.seq;
-  auto id = [&](int i) -> int64_t {
-    return p.ids64 ? static_cast<const int64_t*>(p.documents)[base + i]
-                   : static_cast<const int*>(p.documents)[base + i];
-  };
-  constexpr int kStretch = kScanThreads * kScanItems;
-  const int stretches = (p.seq + kStretch - 1) / kStretch;
-  const bool ends = !p.causal || p.prefix;
-  int from = 0;  // the start of the run that reaches into the stretch
-  for (int s = 0; s < stretches; ++s) {
-    const int i0 = s * kStretch + threadIdx.x * kScanItems;
-    int start[kScanItems];
-    bool padding[kScanItems];
-    int run = 0;
-    int64_t prev = i0 > 0 && i0 <= p.seq ? id(i0 - 1) : 0;
-#pragma unroll
-    for (int e = 0; e < kScanItems; ++e) {
-      const int i = i0 + e;
-      padding[e] = true;
-      if (i < p.seq) {
-        const int64_t now = id(i);
-        padding[e] = now < 0;
-        if (i == 0 || now != prev) run = i;
-        prev = now;
-      }
-      start[e] = run;
-    }
-    const int in = scan_threads<false>(run, from, sh, from);
-#pragma unroll
-    for (int e = 0; e < kScanItems; ++e) {
-      const int i = i0 + e;
-      if (i >= p.seq) continue;
-      p.first[base + i] = max(start[e], in);
-      if (!ends || padding[e]) p.last[base + i] = padding[e] ? max(start[e], in) : i + 1;
-    }
-  }
-  if (!ends) return;
-  int next = p.seq;  // the start of the run after the stretch's last
-  for (int s = stretches - 1; s >= 0; --s) {
-    const int i0 = s * kStretch + threadIdx.x * kScanItems;
-    int end[kScanItems];
-    bool padding[kScanItems];
-    int run = p.seq;
-    int64_t after = i0 + kScanItems < p.seq ? id(i0 + kScanItems) : 0;
-#pragma unroll
-    for (int e = kScanItems - 1; e >= 0; --e) {
-      const int i = i0 + e;
-      padding[e] = true;
-      if (i < p.seq) {
-        const int64_t now = id(i);
-        padding[e] = now < 0;
-        if (i + 1 < p.seq && now != after) run = i + 1;
-        after = now;
-      }
-      end[e] = run;
-    }
-    const int in = scan_threads<true>(run, next, sh, next);
-#pragma unroll
-    for (int e = 0; e < kScanItems; ++e) {
-      const int i = i0 + e;
-      if (i >= p.seq || padding[e]) continue;
-      const int stop = min(end[e], in);
-      int last = stop;
-      if (p.causal) {
-        const int64_t seen = static_cast<int64_t>(p.first[base + i]) + max(p.prefix[base + i], 0);
-        last = max(i + 1, seen < stop ? static_cast<int>(seen) : stop);
-      }
-      p.last[base + i] = last;
-    }
-  }
 }
 
 }  // namespace
@@ -1796,8 +1187,21 @@ __global__ void __launch_bounds__(kScanThreads) document_spans_kernel(const DocP
 extern "C" int tq_attention_fwd(const void* q, const void* k, const void* v, int64_t batch,
                                 int64_t seq, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                 float scale, int causal, void* out, float* lse, void* stream) {
-  return tq::attention_fwd(q, k, v, nullptr, nullptr, false, batch, seq, heads, kv_heads, head_dim,
-                           scale, causal, out, lse, stream);
+  using namespace tq;
+  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
+  if (rc) return rc;
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
+  if (batch == 0 || seq == 0) return TQ_OK;
+  if (!q || !k || !v || !out || !lse) return fail(TQ_ERR_INVALID, "attention: null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      !aligned(lse, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: q, k, v and out must be 16-byte aligned");
+  int* status = device_status_ptr(&rc);
+  if (!status) return rc;
+  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
+  if (head_dim == 64) return launch_fwd<64>(q, k, v, sh, out, lse, status, as_stream(stream));
+  return launch_fwd<128>(q, k, v, sh, out, lse, status, as_stream(stream));
 }
 
 extern "C" int tq_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
@@ -1816,61 +1220,34 @@ extern "C" int tq_attention_bwd(const void* q, const void* k, const void* v, con
                                 int64_t heads, int64_t kv_heads, int64_t head_dim, float scale,
                                 int causal, void* dq, void* dk, void* dv, void* workspace,
                                 size_t workspace_bytes, void* stream) {
-  return tq::attention_bwd(q, k, v, nullptr, nullptr, false, out, dout, lse, batch, seq, heads,
-                           kv_heads, head_dim, scale, causal, dq, dk, dv, workspace,
-                           workspace_bytes, stream);
-}
-
-extern "C" int tq_span_attention_fwd(const void* q, const void* k, const void* v,
-                                     const int32_t* first, const int32_t* last, int64_t batch,
-                                     int64_t seq, int64_t heads, int64_t kv_heads,
-                                     int64_t head_dim, float scale, void* out, float* lse,
-                                     void* stream) {
-  return tq::attention_fwd(q, k, v, first, last, true, batch, seq, heads, kv_heads, head_dim,
-                           scale, 0, out, lse, stream);
-}
-
-extern "C" int tq_span_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
-                                                     int64_t kv_heads, size_t* bytes) {
   using namespace tq;
-  if (!bytes) return fail(TQ_ERR_INVALID, "attention: null bytes pointer");
-  const int rc = check_shape(batch, seq, heads, kv_heads, 128);
+  int rc = check_shape(batch, seq, heads, kv_heads, head_dim);
   if (rc) return rc;
-  *bytes = bwd_work(nullptr, make_shape(batch, seq, heads, kv_heads, 1.0f, 0), true).bytes;
-  return TQ_OK;
-}
-
-extern "C" int tq_span_attention_bwd(const void* q, const void* k, const void* v,
-                                     const int32_t* first, const int32_t* last, const void* out,
-                                     const void* dout, const float* lse, int64_t batch,
-                                     int64_t seq, int64_t heads, int64_t kv_heads,
-                                     int64_t head_dim, float scale, void* dq, void* dk, void* dv,
-                                     void* workspace, size_t workspace_bytes, void* stream) {
-  return tq::attention_bwd(q, k, v, first, last, true, out, dout, lse, batch, seq, heads, kv_heads,
-                           head_dim, scale, 0, dq, dk, dv, workspace, workspace_bytes, stream);
-}
-
-extern "C" int tq_document_spans(const void* documents, int ids_bits, const int32_t* prefix,
-                                 int64_t batch, int64_t seq, int causal, int32_t* first,
-                                 int32_t* last, void* stream) {
-  using namespace tq;
-  if (ids_bits != 32 && ids_bits != 64)
-    return fail(TQ_ERR_UNSUPPORTED, "document_spans: document ids must be 32- or 64-bit integers");
-  if (batch < 0 || seq < 0 || batch > (1ll << 31) - 1 || seq > (1ll << 30))
-    return fail(TQ_ERR_INVALID, "document_spans: batch and seq must be >= 0, seq at most 2^30");
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
   if (batch == 0 || seq == 0) return TQ_OK;
-  if (!documents || !first || !last) return fail(TQ_ERR_INVALID, "document_spans: null pointer");
-  if (!aligned(documents, ids_bits / 8) || !aligned(prefix, 4) || !aligned(first, 4) ||
-      !aligned(last, 4))
-    return fail(TQ_ERR_MISALIGNED, "document_spans: a pointer is not aligned to its type");
-  DocParams p{};
-  p.documents = documents;
-  p.prefix = causal ? prefix : nullptr;
-  p.ids64 = ids_bits == 64;
-  p.seq = static_cast<int>(seq);
-  p.causal = causal ? 1 : 0;
-  p.first = first;
-  p.last = last;
-  return launch_kernel(document_spans_kernel, dim3(static_cast<unsigned>(batch)),
-                       dim3(kScanThreads), 0, as_stream(stream), 1, "document_spans launch", p);
+  size_t need = 0;
+  rc = tq_attention_bwd_workspace_bytes(batch, seq, heads, &need);
+  if (rc) return rc;
+  if (workspace_bytes < need)
+    return fail(TQ_ERR_INVALID, "attention: workspace of %zu bytes, %zu needed", workspace_bytes,
+                need);
+  if (!q || !k || !v || !out || !dout || !lse || !dq || !dk || !dv || !workspace)
+    return fail(TQ_ERR_INVALID, "attention: null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
+      !aligned(workspace, 256) || !aligned(lse, 4))
+    return fail(TQ_ERR_MISALIGNED,
+                "attention: tensors must be 16-byte aligned and the workspace 256-byte aligned");
+  int* status = device_status_ptr(&rc);
+  if (!status) return rc;
+  const AttnShape sh = make_shape(batch, seq, heads, kv_heads, scale, causal);
+  const int seq_pad = sh.n_tiles * kTile;
+  float* lse2 = static_cast<float*>(workspace);
+  float* delta = lse2 + static_cast<size_t>(batch * heads) * seq_pad;
+  if (head_dim == 64)
+    return launch_bwd<64>(q, k, v, out, dout, lse, sh, scale, dq, dk, dv, lse2, delta, seq_pad,
+                          status, as_stream(stream));
+  return launch_bwd<128>(q, k, v, out, dout, lse, sh, scale, dq, dk, dv, lse2, delta, seq_pad,
+                         status, as_stream(stream));
 }

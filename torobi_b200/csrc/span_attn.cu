@@ -1,0 +1,1958 @@
+// Attention in which every query sees a span of keys: query i of sequence b
+// sees first[b, i] <= j < last[b, i] (two ints a position) in place of the
+// causal rule of attn.cu -- rows that pack several documents, prompts seen in
+// both directions, sliding windows, padding -- forward and backward, and the
+// spans of packed documents.  The reference has no such mode (its node takes a
+// causal mode or a mask tensor: engine/src/interp.rs:405-432).
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i) for j in the span
+//   dP = dO V^T,  delta_i = sum_d dO_id O_id,  dS = P * (dP - delta)
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO
+// Layouts as in attn.cu: q, o [batch, seq, heads, dim], k, v [batch, seq,
+// kv_heads, dim] bf16, lse [batch, heads, seq] f32 (natural logarithm).  A query
+// that sees nothing gets o = 0, lse = -inf and no gradient.  P, dS and the
+// results are rounded to bf16, every sum is f32.
+//
+// What short documents ask for, and how the kernels differ from attn.cu's:
+// * A query tile's rows are the `pack` heads that share a key/value head at a
+//   few positions (row = position * pack + head, the order in which a box {64
+//   dims, pack heads, positions} lands), not one head's at 128: its rows see
+//   nearly the same keys, so little of a key tile is masked at a document's
+//   borders, and the heads share the key tile.  Key tiles that no row sees are
+//   neither loaded nor multiplied; 32-column chunks that no row of a warp sees
+//   are not read, those that all see take the unmasked code.
+// * A query tile of a short document has two to six key tiles.  With one CTA
+//   a tile, its start (barriers, tensor memory, the first copies: some 6000
+//   cycles) and end (4000) were half of its life.  The CTAs stay (one an SM)
+//   and take one tile after another: a scheduler warp reads the next tile's
+//   spans, its copies and first product run while the last one's results are
+//   stored.
+#include <cuda_bf16.h>
+
+#include <climits>
+#include <cmath>
+
+#include "attn.cuh"
+
+namespace tq {
+namespace {
+
+constexpr int kAttnThreads = 384;
+constexpr int kReaders = 10;  // who reads a tile's description: TMA, MMA, eight compute warps
+// Registers a thread: the four warps that copy, multiply and schedule need
+// fewer, the eight compute warps hold a row of 128 scores.
+// 128 * 96 + 256 * 200 = 63,488 of the launch's 384 * 168 = 64,512.
+constexpr int kFewRegs = 96;
+constexpr int kManyRegs = 200;
+
+struct SpanShape {
+  int batch, seq, heads, kv_heads, group;
+  float scale_log2;  // softmax scale * log2(e)
+  // Query heads a tile holds, the positions in a 128- and a 64-row tile,
+  // floor(rows / pack) (rows behind pack * positions hold zeros), and the
+  // number of such tiles and of 128-key tiles in a sequence.
+  int pack, pos128, pos64, tiles128, tiles64, key_tiles;
+};
+
+// A query's keys [lo, hi) within [0, seq); 0, 0 when it sees none.
+struct Span {
+  int lo, hi;
+};
+
+__device__ __forceinline__ Span load_span(const int* first, const int* last, int b, int i,
+                                          int seq) {
+  if (i >= seq) return {0, 0};
+  const size_t at = static_cast<size_t>(b) * seq + i;
+  const int lo = max(__ldg(first + at), 0), hi = min(__ldg(last + at), seq);
+  return lo < hi ? Span{lo, hi} : Span{0, 0};
+}
+
+// The keys that any of the positions [i0, i0 + n) sees, [lo, hi) (0, 0 for
+// none), for every lane of the calling warp.
+__device__ __forceinline__ Span span_of_positions(const int* first, const int* last, int b, int i0,
+                                                  int n, int seq) {
+  int lo = INT_MAX, hi = 0;
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
+    const Span s = load_span(first, last, b, i0 + i, seq);
+    if (s.lo < s.hi) {
+      lo = min(lo, s.lo);
+      hi = max(hi, s.hi);
+    }
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  return hi > 0 ? Span{lo, hi} : Span{0, 0};
+}
+
+// Zeroes rows [from, tile_rows) of `slabs` consecutive slabs (128 bytes a row),
+// which no copy fills when a packed tile has fewer rows; made visible to the
+// tensor cores by each thread's fence and the barrier after it.
+__device__ __forceinline__ void zero_rows(uint8_t* slab, int slabs, int tile_rows, int from) {
+  const int per = (tile_rows - from) * 8;  // 16-byte words a slab
+  for (int i = threadIdx.x; i < slabs * per; i += kAttnThreads)
+    *reinterpret_cast<uint4*>(slab + (i / per * tile_rows + from) * 128 + i % per * 16) =
+        make_uint4(0, 0, 0, 0);
+  if (per > 0) fence_proxy_async_smem();
+}
+
+// 2^x of two values on the FMA pipe: attn.cuh's method with a quintic (minimax
+// in relative error with value 1 at f = 0; max relative error 1.6e-7), since
+// the row's sum is answered in f32.
+__device__ __forceinline__ F2 exp2_fine(F2 x) {
+  const float2 v = split(x);
+  const F2 c = f2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
+  const F2 t = c + f2(12582912.0f, 12582912.0f);
+  const F2 f = fma2(t + f2(-12582912.0f, -12582912.0f), f2(-1.0f, -1.0f), c);
+  F2 p = fma2(f2(0.001326472731307149f, 0.001326472731307149f), f,
+              f2(0.009671512991189957f, 0.009671512991189957f));
+  p = fma2(p, f, f2(0.05550733581185341f, 0.05550733581185341f));
+  p = fma2(p, f, f2(0.24022242426872253f, 0.24022242426872253f));
+  p = fma2(p, f, f2(0.6931470036506653f, 0.6931470036506653f));
+  p = fma2(p, f, f2(1.0f, 1.0f));
+  const float2 pv = split(p), tv = split(t);
+  return f2(__uint_as_float(__float_as_uint(pv.x) + (__float_as_uint(tv.x) << 23)),
+            __uint_as_float(__float_as_uint(pv.y) + (__float_as_uint(tv.y) << 23)));
+}
+
+__device__ __forceinline__ F2 exp2_mufu(F2 x) {
+  const float2 v = split(x);
+  return f2(ex2_approx(v.x), ex2_approx(v.y));
+}
+
+__device__ __forceinline__ F2 pair_of(uint32_t a, uint32_t b) {
+  return f2(__uint_as_float(a), __uint_as_float(b));
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(F2 x) {
+  const float2 v = split(x);
+  return pack_bf16x2_f32(v.x, v.y);
+}
+
+// Rows of results: 32 values a lane, in the widest stores the address allows.
+__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&w)[16], bool wide) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i),
+                   "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
+                   "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+}
+
+__device__ __forceinline__ bool wide_rows(const void* p) {
+  return (reinterpret_cast<uintptr_t>(p) & 31u) == 0;
+}
+
+// ------------------------------------------------------------------ forward --
+//
+// A tile of work is a pair of adjacent packed query tiles of one sequence and
+// key/value head; both share every key/value tile the pair needs.
+//   warp 0       TMA: the query tiles, key and value tiles through a ring
+//   warp 1       one thread issues every tcgen05 MMA
+//   warp 2       allocates / frees the 512 TMEM columns
+//   warp 3       scheduler: the next pairs' descriptions, two in shared memory
+//   warps 4-7    softmax of query tile 0 (thread i owns row i, TMEM lane i)
+//   warps 8-11   softmax of query tile 1
+// TMEM: S_0 | S_1 (128 f32 columns each) | O_0 | O_1 (dim columns each).  A
+// softmax thread reads its row of S once into registers and writes P (bf16
+// pairs, 64 columns) over its first half.  MMA issue order per key tile t:
+//   O_0 += P_0(t) V_t,  S_0 = Q_0 K_{t+1}^T,  O_1 += P_1(t) V_t,  S_1 = Q_1 K_{t+1}^T
+// and tcgen05.mma operations issued by one thread execute in that order, so
+// S_w(t+1) overwrites P_w(t) right after its product has read it.  Every
+// barrier that completes once per key tile (or once per pair) counts through
+// all pairs; no waiter is two phases behind.
+// Three in eight exponentials of an unmasked chunk run on the FMA pipe: the
+// MUFU unit alone (16 a cycle) would take 1024 cycles a 128 x 128 tile, as long
+// as its MMAs.
+
+struct FwdItem {
+  int b, h, t0;              // b < 0: no more; first of `pack` heads, first query tile
+  int lo0, hi0, lo1, hi1;    // key tiles of the two query tiles
+  int pad;
+};
+
+template <int D>
+struct FwdCfg {
+  static_assert(D == 64 || D == 128, "head dim");
+  static constexpr int SLABS = D / 64;            // 128-byte swizzle atoms along dim
+  static constexpr int SLAB_BYTES = kTile * 128;  // 128 rows x 64 bf16
+  static constexpr int TILE_BYTES = SLABS * SLAB_BYTES;
+  static constexpr int KST = D == 128 ? 3 : 4;
+  static constexpr int VST = D == 128 ? 2 : 4;
+  static constexpr int Q_OFF = 0;  // two query tiles
+  static constexpr int K_OFF = 2 * TILE_BYTES;
+  static constexpr int V_OFF = K_OFF + KST * TILE_BYTES;
+  static constexpr int ITEM_OFF = V_OFF + VST * TILE_BYTES;
+  static constexpr int BAR_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(FwdItem));
+  // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
+  // p_ready[2], o_done[2], o_free[2], item_full[2], item_empty[2]; then the TMEM slot
+  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 12;
+  static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
+  static constexpr int S_COL = 0;    // S_w (and P_w) at 128 w
+  static constexpr int O_COL = 256;  // O_w at 256 + D w
+  static constexpr int TMEM_COLS = 512;
+  static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory map");
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+  static_assert(SMEM > 118784, "one CTA per SM");
+};
+
+struct FwdParams {
+  SpanShape sh;
+  const int* first;  // [batch, seq]
+  const int* last;
+  int n_pairs, n_items;
+  uint16_t* out;
+  float* lse;
+  int* status;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    span_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
+                    const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
+  using C = FwdCfg<D>;
+  constexpr int KST = C::KST;
+  constexpr int VST = C::VST;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const gbase = smem_raw + (base - raw);
+  auto q_s = [&](int w) { return base + C::Q_OFF + w * C::TILE_BYTES; };
+  auto k_s = [&](int s) { return base + C::K_OFF + s * C::TILE_BYTES; };
+  auto v_s = [&](int s) { return base + C::V_OFF + s * C::TILE_BYTES; };
+  const uint32_t bars = base + C::BAR_OFF;
+  const uint32_t q_full = bars, q_empty = bars + 8u;
+  auto k_full = [&](int s) { return bars + 8u * (2 + s); };
+  auto k_empty = [&](int s) { return bars + 8u * (2 + KST + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 + 2 * KST + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (2 + 2 * KST + VST + s); };
+  constexpr int X = 2 + 2 * KST + 2 * VST;
+  auto s_full = [&](int w) { return bars + 8u * (X + w); };
+  auto p_ready = [&](int w) { return bars + 8u * (X + 2 + w); };
+  auto o_done = [&](int w) { return bars + 8u * (X + 4 + w); };
+  auto o_free = [&](int w) { return bars + 8u * (X + 6 + w); };
+  auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
+  auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
+  const uint32_t tmem_slot = bars + 8u * C::NBAR;
+  volatile uint32_t* tmem_slot_ptr =
+      reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
+  FwdItem* const items = reinterpret_cast<FwdItem*>(gbase + C::ITEM_OFF);
+
+  const SpanShape& sh = p.sh;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rows = sh.pack * sh.pos128;  // filled rows of a query tile
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < KST; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+    }
+    for (int s = 0; s < VST; ++s) {
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full(w), 1);
+      mbar_init(p_ready(w), 4);
+      mbar_init(o_done(w), 1);
+      mbar_init(o_free(w), 4);
+      mbar_init(item_full(w), 1);
+      mbar_init(item_empty(w), kReaders);
+    }
+    fence_mbar_init();
+  }
+  zero_rows(gbase + C::Q_OFF, 2 * C::SLABS, kTile, rows);
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot_ptr;
+  // Signalled only once this CTA holds its tensor memory: a dependent
+  // kernel's CTA placed on this SM may then wait for it, never hold it.
+  griddep_launch_dependents();
+  griddep_wait();
+
+  // The i-th item's description; one arrival a reader.
+  auto wait_item = [&](int i, bool& ok) {
+    FwdItem it{-1, 0, 0, 0, 0, 0, 0, 0};
+    ok = mbar_wait(item_full(i & 1), (i >> 1) & 1, p.status);
+    if (ok) it = items[i & 1];
+    return it;
+  };
+
+  if (warp < 4) {
+    registers_down<kFewRegs>();
+    if (warp == 0 && elect_one_sync()) {
+      // ----------------------------------------------------------- TMA
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      int nk = 0, nv = 0, nq = 0;  // tiles issued, of all items
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const FwdItem it = wait_item(i, ok);
+        if (it.b < 0) break;
+        mbar_arrive(item_empty(i & 1));
+        const int hk = it.h / sh.group;
+        const int j0 = it.hi0 == 0 ? it.lo1 : it.hi1 == 0 ? it.lo0 : min(it.lo0, it.lo1);
+        const int n_kv = max(it.hi0, it.hi1) - j0;
+        if (n_kv <= 0) continue;
+        auto load_k = [&](int t) -> bool {
+          const int s = nk % KST;
+          if (!mbar_wait(k_empty(s), ((nk / KST) & 1) ^ 1, p.status)) return false;
+          mbar_arrive_expect_tx(k_full(s), C::TILE_BYTES);
+          for (int sl = 0; sl < C::SLABS; ++sl)
+            tma_load_4d(k_s(s) + sl * C::SLAB_BYTES, &tm_k, k_full(s), sl * 64, hk,
+                        (j0 + t) * kTile, it.b);
+          ++nk;
+          return true;
+        };
+        // The first key tile needs no room of the last item's query tiles.
+        ok = load_k(0) && mbar_wait(q_empty, (nq & 1) ^ 1, p.status);
+        if (!ok) break;
+        const int tiles = it.t0 + 1 < sh.tiles128 ? 2 : 1;
+        mbar_arrive_expect_tx(q_full, tiles * C::SLABS * rows * 128);
+        for (int w = 0; w < tiles; ++w)
+          for (int sl = 0; sl < C::SLABS; ++sl)
+            tma_load_4d(q_s(w) + sl * C::SLAB_BYTES, &tm_q, q_full, sl * 64, it.h,
+                        (it.t0 + w) * sh.pos128, it.b);
+        ++nq;
+        for (int t = 0; t < n_kv && ok; ++t) {
+          // Key tile t + 1 is issued ahead of value tile t (the MMA wants
+          // K_{t+1} for the next scores before it wants V_t).
+          if (t + 1 < n_kv && !load_k(t + 1)) {
+            ok = false;
+            break;
+          }
+          const int s = nv % VST;
+          ok = mbar_wait(v_empty(s), ((nv / VST) & 1) ^ 1, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(v_full(s), C::TILE_BYTES);
+          for (int sl = 0; sl < C::SLABS; ++sl)
+            tma_load_4d(v_s(s) + sl * C::SLAB_BYTES, &tm_v, v_full(s), sl * 64, hk,
+                        (j0 + t) * kTile, it.b);
+          ++nv;
+        }
+      }
+      // Never leave a copy in flight.
+      if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, p.status);
+      for (int j = nk - KST < 0 ? 0 : nk - KST; j < nk; ++j)
+        mbar_wait(k_full(j % KST), (j / KST) & 1, p.status);
+      for (int j = nv - VST < 0 ? 0 : nv - VST; j < nv; ++j)
+        mbar_wait(v_full(j % VST), (j / VST) & 1, p.status);
+    } else if (warp == 1 && elect_one_sync()) {
+      // ----------------------------------------------------------- MMA
+      constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kTile, false, false);
+      constexpr uint32_t idesc_o = make_idesc_bf16(kTile, D, false, true);
+      int kc = 0, vc = 0, qc = 0;           // key, value and query tiles used
+      int steps[2] = {0, 0};                // products P V issued for tile w
+      int outs[2] = {0, 0};                 // O_w begun
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const FwdItem it = wait_item(i, ok);
+        if (it.b < 0) break;
+        mbar_arrive(item_empty(i & 1));
+        const int j0 = it.hi0 == 0 ? it.lo1 : it.hi1 == 0 ? it.lo0 : min(it.lo0, it.lo1);
+        const int n_kv = max(it.hi0, it.hi1) - j0;
+        if (n_kv <= 0) continue;
+        // Key tile t is j0 + t; query tile w takes part in t of [from, to).
+        const int from[2] = {it.lo0 - j0, it.lo1 - j0}, to[2] = {it.hi0 - j0, it.hi1 - j0};
+        int left = max(to[0] - from[0], 0) + max(to[1] - from[1], 0);  // scores to issue
+        auto issue_s = [&](int w, int kt) {  // S_w = Q_w K^T
+          const int s = kt % KST;
+          const uint32_t d = tmem + C::S_COL + w * kTile;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * C::SLAB_BYTES + (kk & 3) * 32;
+            umma_bf16(d, make_sdesc(q_s(w) + off, 16, 1024, kSw128),
+                      make_sdesc(k_s(s) + off, 16, 1024, kSw128), idesc_s, kk > 0);
+          }
+          umma_commit(s_full(w));
+          if (--left == 0) umma_commit(q_empty);
+        };
+        auto issue_pv = [&](int w, int s, bool begin) {  // O_w += P_w V
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            umma_bf16_ts(tmem + C::O_COL + w * D, tmem + C::S_COL + w * kTile + kk * 8,
+                         make_sdesc(v_s(s) + kk * 2048, C::SLAB_BYTES, 1024, kSw128), idesc_o,
+                         (!begin || kk > 0) ? 1u : 0u);
+          umma_commit(o_done(w));
+        };
+        ok = mbar_wait(q_full, qc & 1, p.status) &&
+             mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
+        if (!ok) break;
+        ++qc;
+        tc_fence_after();
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          if (from[w] == 0 && to[w] > 0) issue_s(w, kc);
+        umma_commit(k_empty(kc % KST));
+        ++kc;
+        for (int t = 0; t < n_kv && ok; ++t) {
+          const int s = vc % VST;
+          const bool next = t + 1 < n_kv;
+          if (next) {
+            ok = mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
+            if (!ok) break;
+          }
+          ok = mbar_wait(v_full(s), (vc / VST) & 1, p.status);
+          if (!ok) break;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (!ok || t >= to[w]) continue;
+            if (t >= from[w]) {
+              ok = mbar_wait(p_ready(w), steps[w] & 1, p.status);
+              // O_w's last item has been read before it is begun again.
+              if (ok && t == from[w] && outs[w] > 0)
+                ok = mbar_wait(o_free(w), (outs[w] - 1) & 1, p.status);
+              if (!ok) continue;
+              tc_fence_after();
+              issue_pv(w, s, t == from[w]);
+              ++steps[w];
+              outs[w] += t == from[w];
+            }
+            if (t + 1 >= from[w] && t + 1 < to[w]) issue_s(w, kc);
+          }
+          if (!ok) break;
+          umma_commit(v_empty(s));
+          ++vc;
+          if (next) {
+            umma_commit(k_empty(kc % KST));
+            ++kc;
+          }
+        }
+      }
+      // Nothing may outlive the CTA's TMEM: wait for each tile's last PV.
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (steps[w] > 0) mbar_wait(o_done(w), (steps[w] - 1) & 1, p.status);
+    } else if (warp == 3) {
+      // ------------------------------------------------------ scheduler
+      const int groups = sh.heads / sh.pack;
+      const int bh_count = sh.batch * groups;
+      for (int i = 0;; ++i) {
+        const int n = blockIdx.x + i * gridDim.x;
+        if (!mbar_wait(item_empty(i & 1), ((i >> 1) & 1) ^ 1, p.status)) break;
+        FwdItem it{-1, 0, 0, 0, 0, 0, 0, 0};
+        if (n < p.n_items) {
+          // Late positions (the heaviest, causally) first.
+          const int bh = n % bh_count;
+          it.b = bh / groups;
+          it.h = bh % groups * sh.pack;
+          it.t0 = 2 * (p.n_pairs - 1 - n / bh_count);
+          const int i0 = it.t0 * sh.pos128;
+          const Span a = span_of_positions(p.first, p.last, it.b, i0, sh.pos128, sh.seq);
+          const Span c =
+              span_of_positions(p.first, p.last, it.b, i0 + sh.pos128, sh.pos128, sh.seq);
+          it.lo0 = a.lo / kTile;
+          it.hi0 = (a.hi + kTile - 1) / kTile;
+          it.lo1 = c.lo / kTile;
+          it.hi1 = (c.hi + kTile - 1) / kTile;
+        }
+        if (lane == 0) {
+          items[i & 1] = it;
+          mbar_arrive(item_full(i & 1));
+        }
+        __syncwarp();
+        if (it.b < 0) break;
+      }
+    }
+  } else {
+    registers_up<kManyRegs>();
+    // --------------------------------------------------------- softmax
+    const int w = (warp - 4) >> 2;  // query tile of this warpgroup
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const bool filled = row < rows;
+    const int at = row / sh.pack, head = row % sh.pack;  // position and head within the tile
+    const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t scol = lrow + C::S_COL + w * kTile;
+    const uint32_t ocol = lrow + C::O_COL + w * D;
+    const float c = sh.scale_log2;
+    const F2 c2 = f2(c, c);
+    const bool wide = wide_rows(p.out);
+    bool ok = true;
+    int steps = 0;  // key tiles of query tile w, of all items
+    FwdItem it = wait_item(0, ok);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_empty(0));
+    auto span_of_row = [&](const FwdItem& item) {
+      return filled && item.b >= 0
+                 ? load_span(p.first, p.last, item.b, (item.t0 + w) * sh.pos128 + at, sh.seq)
+                 : Span{0, 0};
+    };
+    Span sp = span_of_row(it);
+    for (int i = 0; ok && it.b >= 0; ++i) {
+      const int jw = w == 0 ? it.lo0 : it.lo1;
+      const int nk = (w == 0 ? it.hi0 : it.hi1) - jw;
+      const int qpos = (it.t0 + w) * sh.pos128 + at;
+      const unsigned len = sp.hi - sp.lo;
+      // What any row of the warp sees, and what every filled row sees.
+      const int any_lo = __reduce_min_sync(0xffffffffu, sp.lo < sp.hi ? sp.lo : INT_MAX);
+      const int any_hi = __reduce_max_sync(0xffffffffu, sp.hi);
+      const int all_lo = __reduce_max_sync(0xffffffffu, filled ? sp.lo : 0);
+      const int all_hi = __reduce_min_sync(0xffffffffu, filled ? sp.hi : INT_MAX);
+      float m = -INFINITY;
+      float l = 0.0f;
+      for (int j = 0; j < nk; ++j, ++steps) {
+        ok = mbar_wait(s_full(w), steps & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        const int kv0 = (jw + j) * kTile;
+        auto none = [&](int c4) {
+          return kv0 + 32 * c4 + 32 <= any_lo || kv0 + 32 * c4 >= any_hi;
+        };
+        auto full = [&](int c4) {
+          return kv0 + 32 * c4 >= all_lo && kv0 + 32 * c4 + 32 <= all_hi;
+        };
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4)
+          if (!none(c4)) tmem_ld_32x32b_x32(scol + c4 * 32, r[c4]);
+        tmem_ld_wait();
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          if (none(c4)) continue;
+          if (!full(c4)) {
+            const int col0 = kv0 + 32 * c4 - sp.lo;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (static_cast<unsigned>(col0 + e) >= len) r[c4][e] = 0xFF800000u;  // -inf
+          }
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(r[c4][e]));
+        }
+        const float m_new =
+            fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c);
+        // A row that has summed nothing yet just takes its maximum.
+        const bool fresh = m == -INFINITY;
+        if (__any_sync(0xffffffffu, !fresh && filled && m_new > m + kRescaleLog2)) {
+          // Move m and rescale this row of O_w, once its last product is done.
+          const float f = fresh ? 1.0f : ex2_approx(m - m_new);
+          ok = mbar_wait(o_done(w), (steps - 1) & 1, p.status);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c4 = 0; c4 < D / 16; ++c4) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(ocol + c4 * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st_32x32b_x16(ocol + c4 * 16, o);
+          }
+          tmem_st_wait();
+          l *= f;
+          m = m_new;
+        } else if (fresh) {
+          m = m_new;
+        }
+        const float mref = m == -INFINITY ? 0.0f : m;
+        const F2 shift = f2(-mref, -mref);
+        F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          uint32_t pk[16];
+          if (none(c4)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = 0;
+          } else if (full(c4)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const F2 x = fma2(pair_of(r[c4][2 * e], r[c4][2 * e + 1]), c2, shift);
+              const F2 q = (e & 7) == 2 || (e & 7) == 5 || (e & 7) == 7 ? exp2_fine(x)
+                                                                      : exp2_mufu(x);
+              sum[e & 1] = sum[e & 1] + q;
+              pk[e] = pack_bf16(q);
+            }
+          } else {  // 2^-inf is 0 on the MUFU unit
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const F2 q = exp2_mufu(fma2(pair_of(r[c4][2 * e], r[c4][2 * e + 1]), c2, shift));
+              sum[e & 1] = sum[e & 1] + q;
+              pk[e] = pack_bf16(q);
+            }
+          }
+          tmem_st_32x32b_x16(scol + c4 * 16, pk);
+        }
+        const float2 s = split(sum[0] + sum[1]);
+        l += s.x + s.y;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready(w));
+      }
+      if (!ok) break;
+      // The next item's description and span, read while this one ends.
+      const FwdItem nx = wait_item(i + 1, ok);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty((i + 1) & 1));
+      const Span nsp = span_of_row(nx);
+      const bool valid = filled && qpos < sh.seq;
+      uint16_t* orow =
+          p.out + ((static_cast<size_t>(it.b) * sh.seq + qpos) * sh.heads + it.h + head) * D;
+      float* const lse =
+          p.lse + (static_cast<size_t>(it.b) * sh.heads + it.h + head) * sh.seq + qpos;
+      if (nk > 0) {
+        ok = ok && mbar_wait(o_done(w), (steps - 1) & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const F2 inv2 = f2(inv, inv);
+#pragma unroll
+        for (int c4 = 0; c4 < D / 32; ++c4) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(ocol + c4 * 32, o);
+          tmem_ld_wait();
+          if (c4 == D / 32 - 1) {  // O_w may be begun again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_free(w));
+          }
+          uint32_t wd[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            wd[e] = pack_bf16(pair_of(o[2 * e], o[2 * e + 1]) * inv2);
+          if (valid) store_row32(orow + c4 * 32, wd, wide);
+        }
+        if (valid) *lse = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      } else if (valid) {  // no row of the tile sees anything
+        const uint32_t zero[16] = {};
+#pragma unroll
+        for (int c4 = 0; c4 < D / 32; ++c4) store_row32(orow + c4 * 32, zero, wide);
+        *lse = -INFINITY;
+      }
+      it = nx;
+      sp = nsp;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// ----------------------------------------------------------------- backward --
+//
+// Three launches, no atomics on results (the gradients are deterministic):
+//   prep   per packed query row -lse log2(e) and -delta (f32), in 64-row packed
+//          tiles (rows that hold nothing: -inf and 0, so their probabilities
+//          are 0), each row's span in the same order, each tile's spans, and
+//          the two counters that the others take their tiles from;
+//   dq     a tile of work is a packed 128-row query tile, key tiles of 64 (two
+//          compute warpgroups, each half of every tile's columns):
+//            S = Q K_j^T, dP = dO V_j^T (tensor memory, double-buffered),
+//            dS = P * (dP - delta), P = exp2(S c - lse2)  (compute warps),
+//            dQ += dS K_j  (dS written back to tensor memory, A from TMEM);
+//   dkv    a tile of work is a 128-key tile of one key/value head, with the
+//          packed 64-row query tiles that see it (two compute warpgroups,
+//          each half of every tile's columns):
+//            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, into
+//            shared memory as K-major operands), dV += P^T dO_i, dK += dS^T Q_i.
+// Both take their tiles from a counter in the workspace (how long one lasts
+// depends on the spans; which CTA does it changes no result).
+
+// Over a 64-row packed query tile: the keys that any row sees, [lo, hi), and
+// those that every filled row sees, [all_lo, all_hi).
+struct SpanTile {
+  int lo, hi, all_lo, all_hi;
+};
+
+// The workspace: statistics [batch, heads / pack, tiles64, 64], spans (first
+// key, how many) [batch, tiles64, 64], tiles [batch, tiles64], two counters.
+struct BwdWork {
+  float* nlse2;
+  float* ndelta;
+  int2* rows;
+  SpanTile* tiles;
+  int* next;
+  size_t bytes;
+};
+
+struct PrepParams {
+  SpanShape sh;
+  const uint16_t* out;
+  const uint16_t* dout;
+  const float* lse;
+  const int* first;
+  const int* last;
+  BwdWork work;
+  int dim;
+  unsigned row_blocks;  // blocks from here on do the spans, a warp a tile
+};
+
+// Eight lanes per row, dim / 8 elements each.
+__global__ void __launch_bounds__(256) span_prep_kernel(const PrepParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const SpanShape& sh = p.sh;
+  const int filled_rows = sh.pack * sh.pos64;
+  if (blockIdx.x >= p.row_blocks) {
+    const long long t = static_cast<long long>(blockIdx.x - p.row_blocks) * 8 + (threadIdx.x >> 5);
+    if (t == 0 && threadIdx.x < 2) p.work.next[threadIdx.x] = 0;
+    if (t >= static_cast<long long>(sh.batch) * sh.tiles64) return;
+    const int b = static_cast<int>(t / sh.tiles64);
+    const int i0 = static_cast<int>(t % sh.tiles64) * sh.pos64;
+    SpanTile s{sh.seq, 0, 0, sh.seq};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = e * 32 + (threadIdx.x & 31);
+      const bool filled = r < filled_rows;
+      const Span sp =
+          filled ? load_span(p.first, p.last, b, i0 + r / sh.pack, sh.seq) : Span{0, 0};
+      p.work.rows[t * kHalf + r] = make_int2(sp.lo, sp.hi - sp.lo);
+      if (!filled) continue;
+      if (sp.lo < sp.hi) s.lo = min(s.lo, sp.lo);
+      s.hi = max(s.hi, sp.hi);
+      s.all_lo = max(s.all_lo, sp.lo);
+      s.all_hi = min(s.all_hi, sp.hi);
+    }
+    s.lo = __reduce_min_sync(0xffffffffu, s.lo);
+    s.hi = __reduce_max_sync(0xffffffffu, s.hi);
+    s.all_lo = __reduce_max_sync(0xffffffffu, s.all_lo);
+    s.all_hi = __reduce_min_sync(0xffffffffu, s.all_hi);
+    if ((threadIdx.x & 31) == 0) p.work.tiles[t] = s;
+    return;
+  }
+  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 3;
+  const int sub = threadIdx.x & 7;
+  const int groups = sh.heads / sh.pack;
+  const bool in = row < static_cast<long long>(sh.batch) * groups * sh.tiles64 * kHalf;
+  const long long t = in ? row / kHalf : 0;
+  const int r = static_cast<int>(row % kHalf);
+  const int bg = static_cast<int>(t / sh.tiles64);
+  const int b = bg / groups;
+  const int h = bg % groups * sh.pack + r % sh.pack;
+  const int i = static_cast<int>(t % sh.tiles64) * sh.pos64 + r / sh.pack;
+  const bool real = in && r < filled_rows && i < sh.seq;
+  float acc = 0.0f;
+  if (real) {
+    const int per = p.dim / 8;
+    const size_t off = ((static_cast<size_t>(b) * sh.seq + i) * sh.heads + h) * p.dim + sub * per;
+    for (int c = 0; c < per; c += 8) {
+      const uint4 o = *reinterpret_cast<const uint4*>(p.out + off + c);
+      const uint4 d = *reinterpret_cast<const uint4*>(p.dout + off + c);
+      const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+      const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc = fmaf(__uint_as_float(ow[e] << 16), __uint_as_float(dw[e] << 16), acc);
+        acc = fmaf(__uint_as_float(ow[e] & 0xFFFF0000u), __uint_as_float(dw[e] & 0xFFFF0000u),
+                   acc);
+      }
+    }
+  }
+  acc += __shfl_xor_sync(0xffffffffu, acc, 1);
+  acc += __shfl_xor_sync(0xffffffffu, acc, 2);
+  acc += __shfl_xor_sync(0xffffffffu, acc, 4);
+  if (in && sub == 0) {
+    float nl = -INFINITY;
+    if (real) {
+      const float l = p.lse[(static_cast<size_t>(b) * sh.heads + h) * sh.seq + i];
+      if (l != -INFINITY) nl = -l * kLog2e;
+    }
+    p.work.nlse2[row] = nl;
+    p.work.ndelta[row] = real ? -acc : 0.0f;
+  }
+}
+
+struct BwdParams {
+  SpanShape sh;
+  const int* first;  // [batch, seq]
+  const int* last;
+  BwdWork work;
+  float scale;
+  int n_items;
+  uint16_t* dq;
+  uint16_t* dk;
+  uint16_t* dv;
+  int* status;
+};
+
+struct DqItem {
+  int b, h, q0;       // b < 0: no more; first of `pack` heads, first position
+  int kv0, n_kv;      // 64-key tiles
+  int pad[3];
+};
+
+template <int D>
+struct DqCfg {
+  static constexpr int SLABS = D / 64;
+  static constexpr int QSLAB = kTile * 128;  // 128 rows x 64 bf16
+  static constexpr int QTILE = SLABS * QSLAB;
+  static constexpr int KSLAB = kHalf * 128;  // 64 rows x 64 bf16
+  static constexpr int KTILE = SLABS * KSLAB;
+  static constexpr int KST = D == 128 ? 5 : 8;
+  static constexpr int VST = KST;
+  static constexpr int Q_OFF = 0;
+  static constexpr int DO_OFF = QTILE;
+  static constexpr int K_OFF = 2 * QTILE;
+  static constexpr int V_OFF = K_OFF + KST * KTILE;
+  static constexpr int ITEM_OFF = V_OFF + VST * KTILE;
+  static constexpr int BAR_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DqItem));
+  // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
+  // s_free[2], ds_ready[2], dq_full, dq_free, item_full[2], item_empty[2]; TMEM slot
+  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 12;
+  static constexpr int SMEM_USED = 1024 + BAR_OFF + 8 * (NBAR + 1);
+  // At least ~116 KB, so that one CTA (and its 512 TMEM columns) fits an SM.
+  static constexpr int SMEM = SMEM_USED > 118784 ? SMEM_USED : 118784;
+  static constexpr int S_COL = 0;     // S_b at 64 b
+  static constexpr int DP_COL = 128;  // dP_b at 128 + 64 b
+  static constexpr int DQ_COL = 256;
+  static constexpr int DS_COL = 256 + D;  // dS_b (bf16 pairs) at DS_COL + 32 b
+  static constexpr int TMEM_COLS = 512;
+  static_assert(DS_COL + 64 <= TMEM_COLS, "tensor memory map");
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+};
+
+template <int D>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    span_dq_kernel(const __grid_constant__ CUtensorMap tm_q,
+                   const __grid_constant__ CUtensorMap tm_do,
+                   const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const BwdParams p) {
+  using C = DqCfg<D>;
+  constexpr int KST = C::KST;
+  constexpr int VST = C::VST;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const gbase = smem_raw + (base - raw);
+  const uint32_t q_s = base + C::Q_OFF;
+  const uint32_t do_s = base + C::DO_OFF;
+  auto k_s = [&](int s) { return base + C::K_OFF + s * C::KTILE; };
+  auto v_s = [&](int s) { return base + C::V_OFF + s * C::KTILE; };
+  const uint32_t bars = base + C::BAR_OFF;
+  const uint32_t q_full = bars, q_empty = bars + 8u;
+  auto k_full = [&](int s) { return bars + 8u * (2 + s); };
+  auto k_empty = [&](int s) { return bars + 8u * (2 + KST + s); };
+  auto v_full = [&](int s) { return bars + 8u * (2 + 2 * KST + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (2 + 2 * KST + VST + s); };
+  constexpr int X = 2 + 2 * KST + 2 * VST;
+  auto s_full = [&](int b) { return bars + 8u * (X + b); };
+  auto s_free = [&](int b) { return bars + 8u * (X + 2 + b); };
+  auto ds_ready = [&](int b) { return bars + 8u * (X + 4 + b); };
+  const uint32_t dq_full = bars + 8u * (X + 6), dq_free = bars + 8u * (X + 7);
+  auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
+  auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
+  const uint32_t tmem_slot = bars + 8u * C::NBAR;
+  volatile uint32_t* tmem_slot_ptr =
+      reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
+  DqItem* const items = reinterpret_cast<DqItem*>(gbase + C::ITEM_OFF);
+
+  const SpanShape& sh = p.sh;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rows = sh.pack * sh.pos128;  // filled rows of the query tile
+  const int groups = sh.heads / sh.pack;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < KST; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+    }
+    for (int s = 0; s < VST; ++s) {
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full(i), 1);
+      mbar_init(s_free(i), 8);
+      mbar_init(ds_ready(i), 8);
+      mbar_init(item_full(i), 1);
+      mbar_init(item_empty(i), kReaders);
+    }
+    mbar_init(dq_full, 1);
+    mbar_init(dq_free, 8);
+    fence_mbar_init();
+  }
+  zero_rows(gbase + C::Q_OFF, 2 * C::SLABS, kTile, rows);  // Q and dO
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot_ptr;
+  griddep_launch_dependents();  // this CTA holds its tensor memory
+  griddep_wait();
+
+  auto wait_item = [&](int i, bool& ok) {
+    DqItem it{-1, 0, 0, 0, 0, {0, 0, 0}};
+    ok = mbar_wait(item_full(i & 1), (i >> 1) & 1, p.status);
+    if (ok) it = items[i & 1];
+    return it;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- TMA
+    if (elect_one_sync()) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_do);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      int nk = 0, nv = 0, nq = 0;  // tiles issued, of all items
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const DqItem it = wait_item(i, ok);
+        if (it.b < 0) break;
+        mbar_arrive(item_empty(i & 1));
+        const int hk = it.h / sh.group;
+        for (int j = 0; j < it.n_kv && ok; ++j) {
+          const int ks = nk % KST, vs = nv % VST;
+          ok = mbar_wait(k_empty(ks), ((nk / KST) & 1) ^ 1, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(k_full(ks), C::KTILE);
+          for (int sl = 0; sl < C::SLABS; ++sl)
+            tma_load_4d(k_s(ks) + sl * C::KSLAB, &tm_k, k_full(ks), sl * 64, hk,
+                        (it.kv0 + j) * kHalf, it.b);
+          ++nk;
+          if (j == 0) {
+            ok = mbar_wait(q_empty, (nq & 1) ^ 1, p.status);
+            if (!ok) break;
+            mbar_arrive_expect_tx(q_full, 2 * C::SLABS * rows * 128);
+            for (int sl = 0; sl < C::SLABS; ++sl) {
+              tma_load_4d(q_s + sl * C::QSLAB, &tm_q, q_full, sl * 64, it.h, it.q0, it.b);
+              tma_load_4d(do_s + sl * C::QSLAB, &tm_do, q_full, sl * 64, it.h, it.q0, it.b);
+            }
+            ++nq;
+          }
+          ok = mbar_wait(v_empty(vs), ((nv / VST) & 1) ^ 1, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(v_full(vs), C::KTILE);
+          for (int sl = 0; sl < C::SLABS; ++sl)
+            tma_load_4d(v_s(vs) + sl * C::KSLAB, &tm_v, v_full(vs), sl * 64, hk,
+                        (it.kv0 + j) * kHalf, it.b);
+          ++nv;
+        }
+      }
+      // Never leave a copy in flight.
+      if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, p.status);
+      for (int j = nk - KST < 0 ? 0 : nk - KST; j < nk; ++j)
+        mbar_wait(k_full(j % KST), (j / KST) & 1, p.status);
+      for (int j = nv - VST < 0 ? 0 : nv - VST; j < nv; ++j)
+        mbar_wait(v_full(j % VST), (j / VST) & 1, p.status);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA
+    if (elect_one_sync()) {
+      constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
+      constexpr uint32_t idesc_dq = make_idesc_bf16(kTile, D, false, true);
+      int g = 0;   // key tiles, of all items: buffer g & 1, stage g % KST
+      int n = 0;   // items with any
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const DqItem it = wait_item(i, ok);
+        if (it.b < 0) break;
+        mbar_arrive(item_empty(i & 1));
+        if (it.n_kv == 0) continue;
+        // dQ += dS K: A = dS from tensor memory, B = K MN-major (N = dim).
+        auto issue_dq = [&](int t, bool begin) -> bool {
+          if (!mbar_wait(ds_ready(t & 1), (t >> 1) & 1, p.status)) return false;
+          // The last item's dQ has been read before it is begun again.
+          if (begin && n > 0 && !mbar_wait(dq_free, (n - 1) & 1, p.status)) return false;
+          tc_fence_after();
+          const int ks = t % KST;
+#pragma unroll
+          for (int kk = 0; kk < kHalf / 16; ++kk)
+            umma_bf16_ts(tmem + C::DQ_COL, tmem + C::DS_COL + (t & 1) * 32 + kk * 8,
+                         make_sdesc(k_s(ks) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_dq,
+                         (!begin || kk > 0) ? 1u : 0u);
+          umma_commit(k_empty(ks));
+          return true;
+        };
+        ok = mbar_wait(q_full, n & 1, p.status);
+        for (int j = 0; j < it.n_kv && ok; ++j, ++g) {
+          const int ks = g % KST, vs = g % VST;
+          ok = mbar_wait(k_full(ks), (g / KST) & 1, p.status) &&
+               mbar_wait(v_full(vs), (g / VST) & 1, p.status) &&
+               (g < 2 || mbar_wait(s_free(g & 1), ((g - 2) >> 1) & 1, p.status));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sd = tmem + C::S_COL + (g & 1) * kHalf;
+          const uint32_t pd = tmem + C::DP_COL + (g & 1) * kHalf;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
+            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
+            umma_bf16(sd, make_sdesc(q_s + qoff, 16, 1024, kSw128),
+                      make_sdesc(k_s(ks) + koff, 16, 1024, kSw128), idesc_s, kk > 0);
+          }
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
+            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
+            umma_bf16(pd, make_sdesc(do_s + qoff, 16, 1024, kSw128),
+                      make_sdesc(v_s(vs) + koff, 16, 1024, kSw128), idesc_s, kk > 0);
+          }
+          umma_commit(s_full(g & 1));
+          umma_commit(v_empty(vs));
+          if (j + 1 == it.n_kv) umma_commit(q_empty);
+          if (j >= 1) ok = issue_dq(g - 1, j == 1);
+        }
+        if (!ok) break;
+        ok = issue_dq(g - 1, it.n_kv == 1);
+        umma_commit(dq_full);
+        ++n;
+      }
+      // Nothing may outlive the CTA's TMEM: the last commit covers every MMA.
+      if (n > 0) mbar_wait(dq_full, (n - 1) & 1, p.status);
+    }
+  } else if (warp == 3) {
+    // -------------------------------------------------------- scheduler
+    const int bh_count = sh.batch * groups;
+    for (int i = 0;; ++i) {
+      if (!mbar_wait(item_empty(i & 1), ((i >> 1) & 1) ^ 1, p.status)) break;
+      int n = 0;
+      if (lane == 0) n = atomicAdd(p.work.next, 1);
+      n = __shfl_sync(0xffffffffu, n, 0);
+      DqItem it{-1, 0, 0, 0, 0, {0, 0, 0}};
+      if (n < p.n_items) {
+        const int bh = n % bh_count;
+        it.b = bh / groups;
+        it.h = bh % groups * sh.pack;
+        it.q0 = (sh.tiles128 - 1 - n / bh_count) * sh.pos128;
+        const Span s = span_of_positions(p.first, p.last, it.b, it.q0, sh.pos128, sh.seq);
+        it.kv0 = s.lo / kHalf;
+        it.n_kv = (s.hi + kHalf - 1) / kHalf - it.kv0;
+      }
+      if (lane == 0) {
+        items[i & 1] = it;
+        mbar_arrive(item_full(i & 1));
+      }
+      __syncwarp();
+      if (it.b < 0) break;
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------ compute warps
+    // Two warpgroups on the same 128 rows: warps 4-7 take key columns 0-31
+    // of each 64-key tile, warps 8-11 columns 32-63 (the gradient is
+    // elementwise given the row's lse and delta); likewise halves of dQ.
+    const int half = (warp - 4) >> 2;
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const bool filled = row < rows;
+    const int at = row / sh.pack, head = row % sh.pack;  // position and head within the tile
+    const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const float c = sh.scale_log2;
+    const F2 c2 = f2(c, c), scale2 = f2(p.scale, p.scale);
+    const bool wide = wide_rows(p.dq);
+    bool ok = true;
+    int g = 0, n = 0;
+    struct RowState {
+      float nlse2, ndelta;
+      Span sp;
+    };
+    auto row_state = [&](const DqItem& it) {
+      RowState s{-INFINITY, 0.0f, {0, 0}};
+      const int qpos = it.q0 + at;
+      if (it.b >= 0 && filled && qpos < sh.seq) {
+        const size_t srow =
+            (static_cast<size_t>(it.b * groups + it.h / sh.pack) * sh.tiles64 + qpos / sh.pos64) *
+                kHalf +
+            qpos % sh.pos64 * sh.pack + head;
+        s.nlse2 = p.work.nlse2[srow];
+        s.ndelta = p.work.ndelta[srow];
+        s.sp = load_span(p.first, p.last, it.b, qpos, sh.seq);
+      }
+      return s;
+    };
+    DqItem it = wait_item(0, ok);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_empty(0));
+    RowState st = row_state(it);
+    for (int i = 0; ok && it.b >= 0; ++i) {
+      const Span sp = st.sp;
+      const unsigned len = sp.hi - sp.lo;
+      const int any_lo = __reduce_min_sync(0xffffffffu, sp.lo < sp.hi ? sp.lo : INT_MAX);
+      const int any_hi = __reduce_max_sync(0xffffffffu, sp.hi);
+      const int all_lo = __reduce_max_sync(0xffffffffu, filled ? sp.lo : 0);
+      const int all_hi = __reduce_min_sync(0xffffffffu, filled ? sp.hi : INT_MAX);
+      const F2 shift = f2(st.nlse2, st.nlse2), nd = f2(st.ndelta, st.ndelta);
+      for (int j = 0; j < it.n_kv; ++j, ++g) {
+        ok = mbar_wait(s_full(g & 1), (g >> 1) & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        const int k0 = (it.kv0 + j) * kHalf + half * 32;
+        const bool none = k0 + 32 <= any_lo || k0 >= any_hi;
+        uint32_t sv[32], dv[32];
+        if (!none) {
+          tmem_ld_32x32b_x32(lrow + C::S_COL + (g & 1) * kHalf + half * 32, sv);
+          tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + half * 32, dv);
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free(g & 1));
+        uint32_t pk[16];
+        if (none) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = 0;
+        } else {
+          if (k0 < all_lo || k0 + 32 > all_hi) {
+            const int col0 = k0 - sp.lo;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (static_cast<unsigned>(col0 + e) >= len) sv[e] = 0xFF800000u;  // P = 0
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const F2 q =
+                exp2_mufu(fma2(pair_of(sv[2 * e], sv[2 * e + 1]), c2, shift));
+            pk[e] = pack_bf16(q * (pair_of(dv[2 * e], dv[2 * e + 1]) + nd));
+          }
+        }
+        tmem_st_32x32b_x16(lrow + C::DS_COL + (g & 1) * 32 + half * 16, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_ready(g & 1));
+      }
+      if (!ok) break;
+      const DqItem nx = wait_item(i + 1, ok);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty((i + 1) & 1));
+      const RowState nst = row_state(nx);
+      const int qpos = it.q0 + at;
+      const bool valid = filled && qpos < sh.seq;
+      uint16_t* orow =
+          p.dq + ((static_cast<size_t>(it.b) * sh.seq + qpos) * sh.heads + it.h + head) * D;
+      if (it.n_kv > 0) {
+        ok = ok && mbar_wait(dq_full, n & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        ++n;
+      }
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) {
+        const int c4 = half * (D / 64) + e;
+        uint32_t o[32];
+        uint32_t w[16] = {};
+        if (it.n_kv > 0) {
+          tmem_ld_32x32b_x32(lrow + C::DQ_COL + c4 * 32, o);
+          tmem_ld_wait();
+          if (e == D / 64 - 1) {  // dQ may be begun again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dq_free);
+          }
+#pragma unroll
+          for (int q = 0; q < 16; ++q) w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * scale2);
+        }
+        if (valid) store_row32(orow + c4 * 32, w, wide);
+      }
+      it = nx;
+      st = nst;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+struct DkvItem {
+  int b, hk, kv0;  // b < 0: no more; key/value head, first key
+  int i0, nq;      // 64-row query tiles that see it
+  int pad[3];
+};
+
+template <int D>
+struct DkvCfg {
+  static constexpr int SLABS = D / 64;
+  static constexpr int KSLAB = kTile * 128;  // K_j, V_j: 128 rows x 64 bf16
+  static constexpr int KTILE = SLABS * KSLAB;
+  static constexpr int QSLAB = kHalf * 128;  // Q_i, dO_i: 64 rows x 64 bf16
+  static constexpr int QTILE = SLABS * QSLAB;
+  static constexpr int PTILE = kTile * 128;  // P^T or dS^T: 128 key rows x 64 queries bf16
+  static constexpr int QST = D == 128 ? 3 : 6;
+  static constexpr int STAT_BYTES = 2 * kHalf * 4;  // the statistics of one query tile
+  static constexpr int K_OFF = 0;
+  static constexpr int V_OFF = KTILE;
+  static constexpr int Q_OFF = 2 * KTILE;
+  static constexpr int DO_OFF = Q_OFF + QST * QTILE;
+  static constexpr int P_OFF = DO_OFF + QST * QTILE;
+  static constexpr int DS_OFF = P_OFF + 2 * PTILE;
+  static constexpr int STAT_OFF = DS_OFF + 2 * PTILE;
+  static constexpr int ITEM_OFF = STAT_OFF + QST * STAT_BYTES;
+  static constexpr int BAR_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DkvItem));
+  // kv_full, kv_empty, q_full[QST], q_empty[QST], s_full[2], s_free[2], pds_ready[2],
+  // acc_full, acc_free, item_full[2], item_empty[2]; then the TMEM slot
+  static constexpr int NBAR = 2 + 2 * QST + 12;
+  static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
+  static constexpr int S_COL = 0;     // S^T_b at 64 b
+  static constexpr int DP_COL = 128;  // dP^T_b at 128 + 64 b
+  static constexpr int DV_COL = 256;
+  static constexpr int DK_COL = 256 + D;
+  static constexpr int TMEM_COLS = 512;
+  static_assert(DK_COL + D <= TMEM_COLS, "tensor memory map");
+  static_assert(SMEM <= 232448, "shared memory per CTA");
+  static_assert(SMEM > 118784, "one CTA per SM");
+};
+
+// Lane i holds row i of a 32 x 32 bit matrix (column j in bit j); returns its
+// column i (row j in bit j): halves of halves change places, by the lane.
+__device__ __forceinline__ uint32_t transpose_bits(uint32_t x) {
+  const int lane = threadIdx.x & 31;
+  uint32_t m = 0x0000FFFFu;
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, j);
+    x = lane & j ? (x & ~m) | ((y & ~m) >> j) : (x & m) | ((y & m) << j);
+    m ^= m << (j >> 1);
+  }
+  return x;
+}
+
+// Bits [a, z) of a word, 0 <= a, z <= 32.
+__device__ __forceinline__ uint32_t bit_range(int a, int z) {
+  if (a >= z) return 0;
+  return (z == 32 ? 0xFFFFFFFFu : (1u << z) - 1u) & ~((1u << a) - 1u);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kAttnThreads, 1)
+    span_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
+                    const __grid_constant__ CUtensorMap tm_do,
+                    const __grid_constant__ CUtensorMap tm_k,
+                    const __grid_constant__ CUtensorMap tm_v, const BwdParams p) {
+  using C = DkvCfg<D>;
+  constexpr int QST = C::QST;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* const gbase = smem_raw + (base - raw);
+  const uint32_t k_s = base + C::K_OFF;
+  const uint32_t v_s = base + C::V_OFF;
+  auto q_s = [&](int s) { return base + C::Q_OFF + s * C::QTILE; };
+  auto do_s = [&](int s) { return base + C::DO_OFF + s * C::QTILE; };
+  auto p_s = [&](int b) { return base + C::P_OFF + b * C::PTILE; };
+  auto ds_s = [&](int b) { return base + C::DS_OFF + b * C::PTILE; };
+  auto stat_s = [&](int s) { return base + C::STAT_OFF + s * C::STAT_BYTES; };
+  const uint32_t bars = base + C::BAR_OFF;
+  const uint32_t kv_full = bars, kv_empty = bars + 8u;
+  auto q_full = [&](int s) { return bars + 8u * (2 + s); };
+  auto q_empty = [&](int s) { return bars + 8u * (2 + QST + s); };
+  constexpr int X = 2 + 2 * QST;
+  auto s_full = [&](int b) { return bars + 8u * (X + b); };
+  auto s_free = [&](int b) { return bars + 8u * (X + 2 + b); };
+  auto pds_ready = [&](int b) { return bars + 8u * (X + 4 + b); };
+  const uint32_t acc_full = bars + 8u * (X + 6), acc_free = bars + 8u * (X + 7);
+  auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
+  auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
+  const uint32_t tmem_slot = bars + 8u * C::NBAR;
+  volatile uint32_t* tmem_slot_ptr =
+      reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
+  DkvItem* const items = reinterpret_cast<DkvItem*>(gbase + C::ITEM_OFF);
+
+  const SpanShape& sh = p.sh;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rows = sh.pack * sh.pos64;       // filled rows of a query tile
+  const int subs = sh.group / sh.pack;       // packs that share the key/value head
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(kv_empty, 1);
+    for (int s = 0; s < QST; ++s) {
+      mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1 + 8);  // the MMAs' commit and the compute warps' stat reads
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full(i), 1);
+      mbar_init(s_free(i), 8);
+      mbar_init(pds_ready(i), 8);
+      mbar_init(item_full(i), 1);
+      mbar_init(item_empty(i), kReaders);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 8);
+    fence_mbar_init();
+  }
+  zero_rows(gbase + C::Q_OFF, 2 * QST * C::SLABS, kHalf, rows);  // the Q and dO stages
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot_ptr;
+  griddep_launch_dependents();  // this CTA holds its tensor memory
+  griddep_wait();
+
+  auto wait_item = [&](int i, bool& ok) {
+    DkvItem it{-1, 0, 0, 0, 0, {0, 0, 0}};
+    ok = mbar_wait(item_full(i & 1), (i >> 1) & 1, p.status);
+    if (ok) it = items[i & 1];
+    return it;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- TMA
+    if (elect_one_sync()) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_do);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+      int issued = 0, n = 0;  // query tiles, key tiles
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const DkvItem it = wait_item(i, ok);
+        if (it.b < 0) break;
+        mbar_arrive(item_empty(i & 1));
+        if (it.nq == 0) continue;
+        ok = mbar_wait(kv_empty, (n & 1) ^ 1, p.status);
+        if (!ok) break;
+        mbar_arrive_expect_tx(kv_full, 2 * C::KTILE);
+        for (int sl = 0; sl < C::SLABS; ++sl) {
+          tma_load_4d(k_s + sl * C::KSLAB, &tm_k, kv_full, sl * 64, it.hk, it.kv0, it.b);
+          tma_load_4d(v_s + sl * C::KSLAB, &tm_v, kv_full, sl * 64, it.hk, it.kv0, it.b);
+        }
+        ++n;
+        for (int t = 0; t < subs * it.nq && ok; ++t) {
+          const int s = issued % QST;
+          ok = mbar_wait(q_empty(s), ((issued / QST) & 1) ^ 1, p.status);
+          if (!ok) break;
+          const int h = it.hk * sh.group + t / it.nq * sh.pack;
+          const int tile = it.i0 + t % it.nq;
+          const size_t srow =
+              (static_cast<size_t>((it.b * sh.heads + h) / sh.pack) * sh.tiles64 + tile) * kHalf;
+          mbar_arrive_expect_tx(q_full(s), 2 * C::SLABS * rows * 128 + C::STAT_BYTES);
+          for (int sl = 0; sl < C::SLABS; ++sl) {
+            tma_load_4d(q_s(s) + sl * C::QSLAB, &tm_q, q_full(s), sl * 64, h, tile * sh.pos64,
+                        it.b);
+            tma_load_4d(do_s(s) + sl * C::QSLAB, &tm_do, q_full(s), sl * 64, h, tile * sh.pos64,
+                        it.b);
+          }
+          bulk_load(stat_s(s), p.work.nlse2 + srow, kHalf * 4, q_full(s));
+          bulk_load(stat_s(s) + kHalf * 4, p.work.ndelta + srow, kHalf * 4, q_full(s));
+          ++issued;
+        }
+      }
+      // Never leave a copy in flight.
+      if (n > 0) mbar_wait(kv_full, (n - 1) & 1, p.status);
+      for (int t = issued - QST < 0 ? 0 : issued - QST; t < issued; ++t)
+        mbar_wait(q_full(t % QST), (t / QST) & 1, p.status);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA
+    if (elect_one_sync()) {
+      constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
+      constexpr uint32_t idesc_acc = make_idesc_bf16(kTile, D, false, true);
+      int g = 0;  // query tiles, of all items: buffer g & 1, stage g % QST
+      int n = 0;  // items with any
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        const DkvItem it = wait_item(i, ok);
+        if (it.b < 0) break;
+        mbar_arrive(item_empty(i & 1));
+        const int T = subs * it.nq;
+        if (T == 0) continue;
+        // dV += P^T_t dO_t and dK += dS^T_t Q_t: A K-major from shared memory,
+        // B MN-major (N = dim, K = the tile's 64 queries).
+        auto issue_acc = [&](int t, bool begin) -> bool {
+          if (!mbar_wait(pds_ready(t & 1), (t >> 1) & 1, p.status)) return false;
+          // The last item's dV and dK have been read before they begin again.
+          if (begin && n > 0 && !mbar_wait(acc_free, (n - 1) & 1, p.status)) return false;
+          tc_fence_after();
+          const int s = t % QST;
+#pragma unroll
+          for (int kk = 0; kk < kHalf / 16; ++kk)
+            umma_bf16(tmem + C::DV_COL, make_sdesc(p_s(t & 1) + kk * 32, 16, 1024, kSw128),
+                      make_sdesc(do_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
+                      (!begin || kk > 0) ? 1u : 0u);
+#pragma unroll
+          for (int kk = 0; kk < kHalf / 16; ++kk)
+            umma_bf16(tmem + C::DK_COL, make_sdesc(ds_s(t & 1) + kk * 32, 16, 1024, kSw128),
+                      make_sdesc(q_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
+                      (!begin || kk > 0) ? 1u : 0u);
+          umma_commit(q_empty(s));
+          return true;
+        };
+        ok = mbar_wait(kv_full, n & 1, p.status);
+        for (int t = 0; t < T && ok; ++t, ++g) {
+          const int s = g % QST;
+          ok = mbar_wait(q_full(s), (g / QST) & 1, p.status) &&
+               (g < 2 || mbar_wait(s_free(g & 1), ((g - 2) >> 1) & 1, p.status));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sd = tmem + C::S_COL + (g & 1) * kHalf;
+          const uint32_t pd = tmem + C::DP_COL + (g & 1) * kHalf;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
+            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
+            umma_bf16(sd, make_sdesc(k_s + koff, 16, 1024, kSw128),
+                      make_sdesc(q_s(s) + qoff, 16, 1024, kSw128), idesc_s, kk > 0);
+          }
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
+            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
+            umma_bf16(pd, make_sdesc(v_s + koff, 16, 1024, kSw128),
+                      make_sdesc(do_s(s) + qoff, 16, 1024, kSw128), idesc_s, kk > 0);
+          }
+          umma_commit(s_full(g & 1));
+          if (t + 1 == T) umma_commit(kv_empty);
+          if (t >= 1) ok = issue_acc(g - 1, t == 1);
+        }
+        if (!ok) break;
+        ok = issue_acc(g - 1, T == 1);
+        umma_commit(acc_full);
+        ++n;
+      }
+      // Nothing may outlive the CTA's TMEM: the last commit covers every MMA.
+      if (n > 0) mbar_wait(acc_full, (n - 1) & 1, p.status);
+    }
+  } else if (warp == 3) {
+    // -------------------------------------------------------- scheduler
+    const int bk_count = sh.batch * sh.kv_heads;
+    for (int i = 0;; ++i) {
+      if (!mbar_wait(item_empty(i & 1), ((i >> 1) & 1) ^ 1, p.status)) break;
+      int n = 0;
+      if (lane == 0) n = atomicAdd(p.work.next + 1, 1);
+      n = __shfl_sync(0xffffffffu, n, 0);
+      DkvItem it{-1, 0, 0, 0, 0, {0, 0, 0}};
+      if (n < p.n_items) {
+        const int bk = n % bk_count;
+        it.b = bk / sh.kv_heads;
+        it.hk = bk % sh.kv_heads;
+        it.kv0 = n / bk_count * kTile;
+        const SpanTile* tiles = p.work.tiles + static_cast<size_t>(it.b) * sh.tiles64;
+        int a = INT_MAX, z = -1;  // the first and last query tile that see it
+        for (int q = lane; q < sh.tiles64; q += 32)
+          if (tiles[q].lo < it.kv0 + kTile && tiles[q].hi > it.kv0) {
+            a = min(a, q);
+            z = q;
+          }
+        a = __reduce_min_sync(0xffffffffu, a);
+        z = __reduce_max_sync(0xffffffffu, z);
+        it.i0 = z >= 0 ? a : 0;
+        it.nq = z >= 0 ? z + 1 - a : 0;
+      }
+      if (lane == 0) {
+        items[i & 1] = it;
+        mbar_arrive(item_full(i & 1));
+      }
+      __syncwarp();
+      if (it.b < 0) break;
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------ compute warps
+    // Two warpgroups on the same 128 key rows: warps 4-7 take query columns
+    // 0-31 of each 64-query tile, warps 8-11 columns 32-63; likewise halves
+    // of the dV and dK rows at the end.
+    const int half = (warp - 4) >> 2;
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;
+    const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const float c = sh.scale_log2;
+    const F2 c2 = f2(c, c);
+    const bool wide = wide_rows(p.dk) && wide_rows(p.dv);
+    bool ok = true;
+    int g = 0, n = 0;
+    for (int i = 0; ok; ++i) {
+      const DkvItem it = wait_item(i, ok);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_empty(i & 1));
+      if (it.b < 0) break;
+      const int T = subs * it.nq;
+      const size_t tile0 = static_cast<size_t>(it.b) * sh.tiles64 + it.i0;
+      const int key0 = it.kv0 + quad * 32;  // the warp's 32 keys
+      for (int t = 0; t < T; ++t, ++g) {
+        const int s = g % QST;
+        // Which of the tile's queries see which of the warp's keys, a bit each:
+        // lane i turns its query's span into bits of the keys, the transpose
+        // gives each key's queries.
+        const size_t tile = tile0 + t % it.nq;
+        const int2 sp = p.work.rows[tile * kHalf + half * 32 + lane];
+        const int from = min(max(sp.x - key0, 0), 32);
+        const uint32_t seen =
+            transpose_bits(bit_range(from, min(max(sp.x + sp.y - key0, 0), 32)));
+        const bool none = !__any_sync(0xffffffffu, seen != 0);
+        ok = mbar_wait(s_full(g & 1), (g >> 1) & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sv[32], dv[32];
+        if (!none) {
+          tmem_ld_32x32b_x32(lrow + C::S_COL + (g & 1) * kHalf + half * 32, sv);
+          tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + half * 32, dv);
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free(g & 1));
+        uint32_t pk[16], dk[16];
+        if (none) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = dk[e] = 0;
+        } else {
+          if (!__all_sync(0xffffffffu, seen == 0xFFFFFFFFu)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!(seen >> e & 1)) sv[e] = 0xFF800000u;  // P = 0
+          }
+          // The query tile's statistics (landed with its Q and dO).
+          ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
+          if (!ok) break;
+          const float* st = reinterpret_cast<const float*>(gbase + (stat_s(s) - base)) + half * 32;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 l4 = *reinterpret_cast<const float4*>(st + e);
+            const float4 d4 = *reinterpret_cast<const float4*>(st + kHalf + e);
+            const F2 pa = exp2_mufu(fma2(pair_of(sv[e], sv[e + 1]), c2, f2(l4.x, l4.y)));
+            const F2 pb = exp2_mufu(fma2(pair_of(sv[e + 2], sv[e + 3]), c2, f2(l4.z, l4.w)));
+            pk[e / 2] = pack_bf16(pa);
+            pk[e / 2 + 1] = pack_bf16(pb);
+            dk[e / 2] = pack_bf16(pa * (pair_of(dv[e], dv[e + 1]) + f2(d4.x, d4.y)));
+            dk[e / 2 + 1] = pack_bf16(pb * (pair_of(dv[e + 2], dv[e + 3]) + f2(d4.z, d4.w)));
+          }
+          // The stat reads above are ordered before the copies that refill
+          // the stage (generic-proxy reads, async-proxy writes).
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_empty(s));
+        // Row `row` of the K-major operand: 64 bf16 = eight 16-byte chunks,
+        // chunk ch stored at ch ^ (row & 7) (the 128-byte swizzle); this half
+        // writes chunks 4 half .. 4 half + 3.
+        const uint32_t prow = p_s(g & 1) + row * 128;
+        const uint32_t drow = ds_s(g & 1) + row * 128;
+#pragma unroll
+        for (int q4 = 0; q4 < 4; ++q4) {
+          const uint32_t off = static_cast<uint32_t>(((4 * half + q4) ^ (row & 7)) * 16);
+          sts128(prow + off, pk[4 * q4], pk[4 * q4 + 1], pk[4 * q4 + 2], pk[4 * q4 + 3]);
+          sts128(drow + off, dk[4 * q4], dk[4 * q4 + 1], dk[4 * q4 + 2], dk[4 * q4 + 3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pds_ready(g & 1));
+      }
+      if (!ok) break;
+      if (T > 0) {
+        ok = mbar_wait(acc_full, n & 1, p.status);
+        if (!ok) break;
+        tc_fence_after();
+        ++n;
+      }
+      const int key = it.kv0 + row;
+      const bool valid = key < sh.seq;
+      const size_t roff = ((static_cast<size_t>(it.b) * sh.seq + key) * sh.kv_heads + it.hk) * D;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const uint32_t col = which == 0 ? C::DV_COL : C::DK_COL;
+        const float f = which == 0 ? 1.0f : p.scale;
+        const F2 ff = f2(f, f);
+        uint16_t* orow = (which == 0 ? p.dv : p.dk) + roff;
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) {
+          const int c4 = half * (D / 64) + e;
+          uint32_t o[32];
+          uint32_t w[16] = {};
+          if (T > 0) {
+            tmem_ld_32x32b_x32(lrow + col + c4 * 32, o);
+            tmem_ld_wait();
+            if (which == 1 && e == D / 64 - 1) {  // dV and dK may begin again
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(acc_free);
+            }
+#pragma unroll
+            for (int q = 0; q < 16; ++q) w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * ff);
+          }
+          if (valid) store_row32(orow + c4 * 32, w, wide);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+// --------------------------------------------------------- document spans --
+
+constexpr int kScanThreads = 1024;
+constexpr int kScanItems = 8;
+
+struct DocParams {
+  const void* documents;
+  const int* prefix;  // may be null
+  int ids64, seq, causal;
+  int* first;
+  int* last;
+};
+
+// Inclusive scan over a warp's lanes: the running maximum from the front, or
+// the running minimum from the back.
+template <bool BACK>
+__device__ __forceinline__ int scan_lanes(int v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = BACK ? __shfl_down_sync(0xffffffffu, v, off) : __shfl_up_sync(0xffffffffu, v, off);
+    if (BACK ? lane + off < 32 : lane >= off) v = BACK ? min(v, o) : max(v, o);
+  }
+  return v;
+}
+
+// The same over the block's threads, exclusive (rest: what the first, or
+// last, thread gets); the whole block's result goes to all.
+template <bool BACK>
+__device__ __forceinline__ int scan_threads(int v, int rest, int* sh, int& all) {
+  static_assert(kScanThreads == 1024, "one total a lane");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto join = [](int a, int b) { return BACK ? min(a, b) : max(a, b); };
+  v = scan_lanes<BACK>(v);
+  __syncthreads();  // the last call's reads of sh
+  if (lane == (BACK ? 0 : 31)) sh[warp] = v;
+  __syncthreads();
+  const int totals = scan_lanes<BACK>(sh[lane]);
+  all = join(__shfl_sync(0xffffffffu, totals, BACK ? 0 : 31), rest);
+  const int warps = __shfl_sync(0xffffffffu, totals, BACK ? (warp + 1) & 31 : (warp + 31) & 31);
+  int in = BACK ? __shfl_down_sync(0xffffffffu, v, 1) : __shfl_up_sync(0xffffffffu, v, 1);
+  if (lane == (BACK ? 31 : 0)) in = rest;
+  if (warp != (BACK ? 31 : 0)) in = join(in, warps);
+  return join(in, rest);
+}
+
+// One CTA per row of ids.  A document is a run of equal ids: its start reaches
+// its positions by a running maximum of the runs' starts from the front, its
+// end by a running minimum from the back, stretch by stretch.
+__global__ void __launch_bounds__(kScanThreads) document_spans_kernel(const DocParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  __shared__ int sh[kScanThreads / 32];
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * p.seq;
+  auto id = [&](int i) -> int64_t {
+    return p.ids64 ? static_cast<const int64_t*>(p.documents)[base + i]
+                   : static_cast<const int*>(p.documents)[base + i];
+  };
+  constexpr int kStretch = kScanThreads * kScanItems;
+  const int stretches = (p.seq + kStretch - 1) / kStretch;
+  const bool ends = !p.causal || p.prefix;
+  int from = 0;  // the start of the run that reaches into the stretch
+  for (int s = 0; s < stretches; ++s) {
+    const int i0 = s * kStretch + threadIdx.x * kScanItems;
+    int start[kScanItems];
+    bool padding[kScanItems];
+    int run = 0;
+    int64_t prev = i0 > 0 && i0 <= p.seq ? id(i0 - 1) : 0;
+#pragma unroll
+    for (int e = 0; e < kScanItems; ++e) {
+      const int i = i0 + e;
+      padding[e] = true;
+      if (i < p.seq) {
+        const int64_t now = id(i);
+        padding[e] = now < 0;
+        if (i == 0 || now != prev) run = i;
+        prev = now;
+      }
+      start[e] = run;
+    }
+    const int in = scan_threads<false>(run, from, sh, from);
+#pragma unroll
+    for (int e = 0; e < kScanItems; ++e) {
+      const int i = i0 + e;
+      if (i >= p.seq) continue;
+      p.first[base + i] = max(start[e], in);
+      if (!ends || padding[e]) p.last[base + i] = padding[e] ? max(start[e], in) : i + 1;
+    }
+  }
+  if (!ends) return;
+  int next = p.seq;  // the start of the run after the stretch's last
+  for (int s = stretches - 1; s >= 0; --s) {
+    const int i0 = s * kStretch + threadIdx.x * kScanItems;
+    int end[kScanItems];
+    bool padding[kScanItems];
+    int run = p.seq;
+    int64_t after = i0 + kScanItems < p.seq ? id(i0 + kScanItems) : 0;
+#pragma unroll
+    for (int e = kScanItems - 1; e >= 0; --e) {
+      const int i = i0 + e;
+      padding[e] = true;
+      if (i < p.seq) {
+        const int64_t now = id(i);
+        padding[e] = now < 0;
+        if (i + 1 < p.seq && now != after) run = i + 1;
+        after = now;
+      }
+      end[e] = run;
+    }
+    const int in = scan_threads<true>(run, next, sh, next);
+#pragma unroll
+    for (int e = 0; e < kScanItems; ++e) {
+      const int i = i0 + e;
+      if (i >= p.seq || padding[e]) continue;
+      const int stop = min(end[e], in);
+      int last = stop;
+      if (p.causal) {
+        const int64_t seen = static_cast<int64_t>(p.first[base + i]) + max(p.prefix[base + i], 0);
+        last = max(i + 1, seen < stop ? static_cast<int>(seen) : stop);
+      }
+      p.last[base + i] = last;
+    }
+  }
+}
+
+// -------------------------------------------------------------------- host --
+
+// How many of the query heads that share a key/value head a packed tile holds:
+// the most, up to 16, that divide them and fill at least 60 of 64 rows (4, 7
+// and 8 of groups of those sizes; 7 of a group of 14; 1 of a group of 11).
+int pack_of(int group) {
+  for (int n = group < 16 ? group : 16; n > 1; --n)
+    if (group % n == 0 && kHalf / n * n >= 60) return n;
+  return 1;
+}
+
+SpanShape make_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, float scale) {
+  SpanShape s{};
+  s.batch = static_cast<int>(batch);
+  s.seq = static_cast<int>(seq);
+  s.heads = static_cast<int>(heads);
+  s.kv_heads = static_cast<int>(kv_heads);
+  s.group = static_cast<int>(heads / kv_heads);
+  s.scale_log2 = scale * kLog2e;
+  s.pack = pack_of(s.group);
+  s.pos128 = kTile / s.pack;
+  s.pos64 = kHalf / s.pack;
+  s.tiles128 = (s.seq + s.pos128 - 1) / s.pos128;
+  s.tiles64 = (s.seq + s.pos64 - 1) / s.pos64;
+  s.key_tiles = (s.seq + kTile - 1) / kTile;
+  return s;
+}
+
+BwdWork bwd_work(void* base, const SpanShape& sh) {
+  const size_t tiles = static_cast<size_t>(sh.batch) * sh.tiles64;
+  const size_t rows = tiles * kHalf * (sh.heads / sh.pack);
+  uint8_t* at = static_cast<uint8_t*>(base);
+  BwdWork w{};
+  w.nlse2 = reinterpret_cast<float*>(at);
+  w.ndelta = w.nlse2 + rows;
+  w.bytes = 2 * rows * sizeof(float);
+  w.rows = reinterpret_cast<int2*>(at + w.bytes);
+  w.bytes += tiles * kHalf * sizeof(int2);
+  w.tiles = reinterpret_cast<SpanTile*>(at + w.bytes);
+  w.bytes += tiles * sizeof(SpanTile);
+  w.next = reinterpret_cast<int*>(at + w.bytes);
+  w.bytes += 16;
+  return w;
+}
+
+int check_span_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads, int64_t dim,
+                     float scale) {
+  const int rc = check_shape(batch, seq, heads, kv_heads, dim);
+  if (rc) return rc;
+  // Packed tiles number at most 64 / 60 of the plain ones and one more.
+  if (batch * heads * (seq / kHalf + 2) > (1ll << 30))
+    return fail(TQ_ERR_INVALID, "attention: shape too large");
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(TQ_ERR_INVALID, "attention: scale must be positive and finite");
+  return TQ_OK;
+}
+
+unsigned grid_of(int items) {
+  const int sms = sm_count();
+  return static_cast<unsigned>(items < sms ? items : sms);
+}
+
+template <int D>
+int launch_fwd(const void* q, const void* k, const void* v, FwdParams p, cudaStream_t stream) {
+  using C = FwdCfg<D>;
+  const SpanShape& sh = p.sh;
+  int rc = set_max_smem_once(reinterpret_cast<const void*>(span_fwd_kernel<D>), C::SMEM,
+                             "cudaFuncSetAttribute(span_fwd)");
+  if (rc) return rc;
+  CUtensorMap tq_, tk, tv;
+  if ((rc = map_bshd(&tq_, q, sh.batch, sh.seq, sh.heads, D, sh.pos128, sh.pack))) return rc;
+  if ((rc = map_bshd(&tk, k, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
+  if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
+  p.n_pairs = (sh.tiles128 + 1) / 2;
+  p.n_items = sh.batch * (sh.heads / sh.pack) * p.n_pairs;
+  return launch_kernel(span_fwd_kernel<D>, dim3(grid_of(p.n_items)), dim3(kAttnThreads), C::SMEM,
+                       stream, 1, "span attention forward launch", tq_, tk, tv, p);
+}
+
+template <int D>
+int launch_bwd(const void* q, const void* k, const void* v, const void* out, const void* dout,
+               const float* lse, BwdParams p, cudaStream_t stream) {
+  using Q = DqCfg<D>;
+  using KV = DkvCfg<D>;
+  const SpanShape& sh = p.sh;
+  int rc = set_max_smem_once(reinterpret_cast<const void*>(span_dq_kernel<D>), Q::SMEM,
+                             "cudaFuncSetAttribute(span_dq)");
+  if (rc) return rc;
+  rc = set_max_smem_once(reinterpret_cast<const void*>(span_dkv_kernel<D>), KV::SMEM,
+                         "cudaFuncSetAttribute(span_dkv)");
+  if (rc) return rc;
+  // Query-side maps (128-row tiles for dq, 64-row tiles for dkv) and the
+  // key/value maps the other way round.
+  const uint32_t pack = sh.pack;
+  CUtensorMap q128, do128, k64, v64, q64, do64, k128, v128;
+  if ((rc = map_bshd(&q128, q, sh.batch, sh.seq, sh.heads, D, sh.pos128, pack))) return rc;
+  if ((rc = map_bshd(&do128, dout, sh.batch, sh.seq, sh.heads, D, sh.pos128, pack))) return rc;
+  if ((rc = map_bshd(&k64, k, sh.batch, sh.seq, sh.kv_heads, D, kHalf))) return rc;
+  if ((rc = map_bshd(&v64, v, sh.batch, sh.seq, sh.kv_heads, D, kHalf))) return rc;
+  if ((rc = map_bshd(&q64, q, sh.batch, sh.seq, sh.heads, D, sh.pos64, pack))) return rc;
+  if ((rc = map_bshd(&do64, dout, sh.batch, sh.seq, sh.heads, D, sh.pos64, pack))) return rc;
+  if ((rc = map_bshd(&k128, k, sh.batch, sh.seq, sh.kv_heads, D, kTile))) return rc;
+  if ((rc = map_bshd(&v128, v, sh.batch, sh.seq, sh.kv_heads, D, kTile))) return rc;
+  PrepParams pp{};
+  pp.sh = sh;
+  pp.out = static_cast<const uint16_t*>(out);
+  pp.dout = static_cast<const uint16_t*>(dout);
+  pp.lse = lse;
+  pp.first = p.first;
+  pp.last = p.last;
+  pp.work = p.work;
+  pp.dim = D;
+  const long long tiles = static_cast<long long>(sh.batch) * sh.tiles64;
+  const long long rows = tiles * (sh.heads / sh.pack) * kHalf;
+  pp.row_blocks = static_cast<unsigned>((rows * 8 + 255) / 256);
+  const unsigned span_blocks = static_cast<unsigned>((tiles + 7) / 8);
+  rc = launch_kernel(span_prep_kernel, dim3(pp.row_blocks + span_blocks), dim3(256), 0, stream, 1,
+                     "span attention backward prep launch", pp);
+  if (rc) return rc;
+  p.n_items = sh.batch * (sh.heads / sh.pack) * sh.tiles128;
+  rc = launch_kernel(span_dq_kernel<D>, dim3(grid_of(p.n_items)), dim3(kAttnThreads), Q::SMEM,
+                     stream, 1, "span attention backward dq launch", q128, do128, k64, v64, p);
+  if (rc) return rc;
+  p.n_items = sh.batch * sh.kv_heads * sh.key_tiles;
+  return launch_kernel(span_dkv_kernel<D>, dim3(grid_of(p.n_items)), dim3(kAttnThreads), KV::SMEM,
+                       stream, 1, "span attention backward dkv launch", q64, do64, k128, v128, p);
+}
+
+}  // namespace
+}  // namespace tq
+
+extern "C" int tq_span_attention_fwd(const void* q, const void* k, const void* v,
+                                     const int32_t* first, const int32_t* last, int64_t batch,
+                                     int64_t seq, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, float scale, void* out, float* lse,
+                                     void* stream) {
+  using namespace tq;
+  int rc = check_span_shape(batch, seq, heads, kv_heads, head_dim, scale);
+  if (rc) return rc;
+  if (batch == 0 || seq == 0) return TQ_OK;
+  if (!q || !k || !v || !first || !last || !out || !lse)
+    return fail(TQ_ERR_INVALID, "attention: null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      !aligned(lse, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: q, k, v and out must be 16-byte aligned");
+  if (!aligned(first, 4) || !aligned(last, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: first and last must be 4-byte aligned");
+  FwdParams p{};
+  p.status = device_status_ptr(&rc);
+  if (!p.status) return rc;
+  p.sh = make_shape(batch, seq, heads, kv_heads, scale);
+  p.first = first;
+  p.last = last;
+  p.out = static_cast<uint16_t*>(out);
+  p.lse = lse;
+  return head_dim == 64 ? launch_fwd<64>(q, k, v, p, as_stream(stream))
+                        : launch_fwd<128>(q, k, v, p, as_stream(stream));
+}
+
+extern "C" int tq_span_attention_bwd_workspace_bytes(int64_t batch, int64_t seq, int64_t heads,
+                                                     int64_t kv_heads, size_t* bytes) {
+  using namespace tq;
+  if (!bytes) return fail(TQ_ERR_INVALID, "attention: null bytes pointer");
+  const int rc = check_span_shape(batch, seq, heads, kv_heads, 128, 1.0f);
+  if (rc) return rc;
+  *bytes = bwd_work(nullptr, make_shape(batch, seq, heads, kv_heads, 1.0f)).bytes;
+  return TQ_OK;
+}
+
+extern "C" int tq_span_attention_bwd(const void* q, const void* k, const void* v,
+                                     const int32_t* first, const int32_t* last, const void* out,
+                                     const void* dout, const float* lse, int64_t batch,
+                                     int64_t seq, int64_t heads, int64_t kv_heads,
+                                     int64_t head_dim, float scale, void* dq, void* dk, void* dv,
+                                     void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace tq;
+  int rc = check_span_shape(batch, seq, heads, kv_heads, head_dim, scale);
+  if (rc) return rc;
+  if (batch == 0 || seq == 0) return TQ_OK;
+  BwdParams p{};
+  p.sh = make_shape(batch, seq, heads, kv_heads, scale);
+  p.work = bwd_work(workspace, p.sh);
+  if (workspace_bytes < p.work.bytes)
+    return fail(TQ_ERR_INVALID, "attention: workspace of %zu bytes, %zu needed", workspace_bytes,
+                p.work.bytes);
+  if (!q || !k || !v || !first || !last || !out || !dout || !lse || !dq || !dk || !dv ||
+      !workspace)
+    return fail(TQ_ERR_INVALID, "attention: null pointer");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
+      !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 16) || !aligned(dv, 16) ||
+      !aligned(workspace, 256) || !aligned(lse, 4))
+    return fail(TQ_ERR_MISALIGNED,
+                "attention: tensors must be 16-byte aligned and the workspace 256-byte aligned");
+  if (!aligned(first, 4) || !aligned(last, 4))
+    return fail(TQ_ERR_MISALIGNED, "attention: first and last must be 4-byte aligned");
+  p.status = device_status_ptr(&rc);
+  if (!p.status) return rc;
+  p.first = first;
+  p.last = last;
+  p.scale = scale;
+  p.dq = static_cast<uint16_t*>(dq);
+  p.dk = static_cast<uint16_t*>(dk);
+  p.dv = static_cast<uint16_t*>(dv);
+  return head_dim == 64 ? launch_bwd<64>(q, k, v, out, dout, lse, p, as_stream(stream))
+                        : launch_bwd<128>(q, k, v, out, dout, lse, p, as_stream(stream));
+}
+
+extern "C" int tq_document_spans(const void* documents, int ids_bits, const int32_t* prefix,
+                                 int64_t batch, int64_t seq, int causal, int32_t* first,
+                                 int32_t* last, void* stream) {
+  using namespace tq;
+  if (ids_bits != 32 && ids_bits != 64)
+    return fail(TQ_ERR_UNSUPPORTED, "document_spans: document ids must be 32- or 64-bit integers");
+  if (batch < 0 || seq < 0 || batch > (1ll << 31) - 1 || seq > (1ll << 30))
+    return fail(TQ_ERR_INVALID, "document_spans: batch and seq must be >= 0, seq at most 2^30");
+  if (batch == 0 || seq == 0) return TQ_OK;
+  if (!documents || !first || !last) return fail(TQ_ERR_INVALID, "document_spans: null pointer");
+  if (!aligned(documents, ids_bits / 8) || !aligned(prefix, 4) || !aligned(first, 4) ||
+      !aligned(last, 4))
+    return fail(TQ_ERR_MISALIGNED, "document_spans: a pointer is not aligned to its type");
+  DocParams p{};
+  p.documents = documents;
+  p.prefix = causal ? prefix : nullptr;
+  p.ids64 = ids_bits == 64;
+  p.seq = static_cast<int>(seq);
+  p.causal = causal ? 1 : 0;
+  p.first = first;
+  p.last = last;
+  return launch_kernel(document_spans_kernel, dim3(static_cast<unsigned>(batch)),
+                       dim3(kScanThreads), 0, as_stream(stream), 1, "document_spans launch", p);
+}
