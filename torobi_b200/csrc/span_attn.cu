@@ -24,9 +24,11 @@
 // * A query tile of a short document has two to six key tiles.  With one CTA
 //   a tile, its start (barriers, tensor memory, the first copies: some 6000
 //   cycles) and end (4000) were half of its life.  The CTAs stay (one an SM)
-//   and take one tile after another: a scheduler warp reads the next tile's
-//   spans, its copies and first product run while the last one's results are
-//   stored.
+//   and take the work of CTAs that have not started (cluster launch control:
+//   how long a tile lasts depends on the spans, and a fixed share each left
+//   SMs idle for a quarter to a third of the time), a little before their own
+//   ends: a scheduler warp reads the next tile's spans, its copies and first
+//   product run while the last one's results are stored.
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -128,6 +130,40 @@ __device__ __forceinline__ uint32_t pack_bf16(F2 x) {
   return pack_bf16x2_f32(v.x, v.y);
 }
 
+// The index of a CTA of this grid that has not started and now never will (its
+// work is the caller's), or -1 if all have.  One warp; slot: 16 bytes of
+// shared memory, bar: an mbarrier of one arrival, both for this alone; n: how
+// many calls came before.  Not called again after a -1.
+__device__ __forceinline__ int take_cta(uint32_t slot, uint32_t bar, int n, int* status) {
+  if ((threadIdx.x & 31) == 0) {
+    fence_proxy_async_smem();  // the last answer has been read
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 "
+        "[%0], [%1];" ::"r"(slot),
+        "r"(bar)
+        : "memory");
+  }
+  __syncwarp();
+  if (!mbar_wait(bar, n & 1, status)) return -1;
+  uint32_t x, ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      ".reg .b128 r;\n"
+      "ld.shared.b128 r, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      "selp.u32 %1, 1, 0, p;\n"
+      "mov.u32 %0, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n"
+      "}\n"
+      : "=r"(x), "=r"(ok)
+      : "r"(slot)
+      : "memory");
+  __syncwarp();
+  return ok ? static_cast<int>(x) : -1;
+}
+
 // Rows of results: 32 values a lane, in the widest stores the address allows.
 __device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&w)[16], bool wide) {
   if (wide) {
@@ -188,10 +224,11 @@ struct FwdCfg {
   static constexpr int K_OFF = 2 * TILE_BYTES;
   static constexpr int V_OFF = K_OFF + KST * TILE_BYTES;
   static constexpr int ITEM_OFF = V_OFF + VST * TILE_BYTES;
-  static constexpr int BAR_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(FwdItem));
+  static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(FwdItem));
+  static constexpr int BAR_OFF = TAKE_OFF + 16;
   // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
-  // p_ready[2], o_done[2], o_free[2], item_full[2], item_empty[2]; then the TMEM slot
-  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 12;
+  // p_ready[2], o_done[2], o_free[2], item_full[2], item_empty[2], taken; TMEM slot
+  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 13;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
   static constexpr int S_COL = 0;    // S_w (and P_w) at 128 w
   static constexpr int O_COL = 256;  // O_w at 256 + D w
@@ -205,7 +242,7 @@ struct FwdParams {
   SpanShape sh;
   const int* first;  // [batch, seq]
   const int* last;
-  int n_pairs, n_items;
+  int n_pairs;
   uint16_t* out;
   float* lse;
   int* status;
@@ -239,6 +276,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   auto o_free = [&](int w) { return bars + 8u * (X + 6 + w); };
   auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
   auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
+  const uint32_t taken = bars + 8u * (X + 12);
   const uint32_t tmem_slot = bars + 8u * C::NBAR;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
@@ -268,6 +306,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(item_full(w), 1);
       mbar_init(item_empty(w), kReaders);
     }
+    mbar_init(taken, 1);
     fence_mbar_init();
   }
   zero_rows(gbase + C::Q_OFF, 2 * C::SLABS, kTile, rows);
@@ -363,10 +402,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int i = 0; ok; ++i) {
         const FwdItem it = wait_item(i, ok);
         if (it.b < 0) break;
-        mbar_arrive(item_empty(i & 1));
         const int j0 = it.hi0 == 0 ? it.lo1 : it.hi1 == 0 ? it.lo0 : min(it.lo0, it.lo1);
         const int n_kv = max(it.hi0, it.hi1) - j0;
-        if (n_kv <= 0) continue;
+        if (n_kv <= 0) {
+          mbar_arrive(item_empty(i & 1));
+          continue;
+        }
         // Key tile t is j0 + t; query tile w takes part in t of [from, to).
         const int from[2] = {it.lo0 - j0, it.lo1 - j0}, to[2] = {it.hi0 - j0, it.hi1 - j0};
         int left = max(to[0] - from[0], 0) + max(to[1] - from[1], 0);  // scores to issue
@@ -403,6 +444,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         for (int t = 0; t < n_kv && ok; ++t) {
           const int s = vc % VST;
           const bool next = t + 1 < n_kv;
+          // Two key tiles before the end it is time to look for the next item.
+          if (t == max(n_kv - 2, 0)) mbar_arrive(item_empty(i & 1));
           if (next) {
             ok = mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
             if (!ok) break;
@@ -443,10 +486,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int groups = sh.heads / sh.pack;
       const int bh_count = sh.batch * groups;
       for (int i = 0;; ++i) {
-        const int n = blockIdx.x + i * gridDim.x;
-        if (!mbar_wait(item_empty(i & 1), ((i >> 1) & 1) ^ 1, p.status)) break;
+        // Not before the item before it nears its end.
+        if (i > 0 && !mbar_wait(item_empty((i - 1) & 1), ((i - 1) >> 1) & 1, p.status)) break;
+        const int n = i == 0 ? static_cast<int>(blockIdx.x)
+                             : take_cta(base + C::TAKE_OFF, taken, i - 1, p.status);
         FwdItem it{-1, 0, 0, 0, 0, 0, 0, 0};
-        if (n < p.n_items) {
+        if (n >= 0) {
           // Late positions (the heaviest, causally) first.
           const int bh = n % bh_count;
           it.b = bh / groups;
@@ -654,8 +699,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 // Three launches, no atomics on results (the gradients are deterministic):
 //   prep   per packed query row -lse log2(e) and -delta (f32), in 64-row packed
 //          tiles (rows that hold nothing: -inf and 0, so their probabilities
-//          are 0), each row's span in the same order, each tile's spans, and
-//          the two counters that the others take their tiles from;
+//          are 0), each row's span in the same order, and each tile's spans;
 //   dq     a tile of work is a packed 128-row query tile, key tiles of 64 (two
 //          compute warpgroups, each half of every tile's columns):
 //            S = Q K_j^T, dP = dO V_j^T (tensor memory, double-buffered),
@@ -666,8 +710,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 //          each half of every tile's columns):
 //            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, into
 //            shared memory as K-major operands), dV += P^T dO_i, dK += dS^T Q_i.
-// Both take their tiles from a counter in the workspace (how long one lasts
-// depends on the spans; which CTA does it changes no result).
+// Which CTA does a tile changes no result.
 
 // Over a 64-row packed query tile: the keys that any row sees, [lo, hi), and
 // those that every filled row sees, [all_lo, all_hi).
@@ -676,13 +719,12 @@ struct SpanTile {
 };
 
 // The workspace: statistics [batch, heads / pack, tiles64, 64], spans (first
-// key, how many) [batch, tiles64, 64], tiles [batch, tiles64], two counters.
+// key, how many) [batch, tiles64, 64], tiles [batch, tiles64].
 struct BwdWork {
   float* nlse2;
   float* ndelta;
   int2* rows;
   SpanTile* tiles;
-  int* next;
   size_t bytes;
 };
 
@@ -706,7 +748,6 @@ __global__ void __launch_bounds__(256) span_prep_kernel(const PrepParams p) {
   const int filled_rows = sh.pack * sh.pos64;
   if (blockIdx.x >= p.row_blocks) {
     const long long t = static_cast<long long>(blockIdx.x - p.row_blocks) * 8 + (threadIdx.x >> 5);
-    if (t == 0 && threadIdx.x < 2) p.work.next[threadIdx.x] = 0;
     if (t >= static_cast<long long>(sh.batch) * sh.tiles64) return;
     const int b = static_cast<int>(t / sh.tiles64);
     const int i0 = static_cast<int>(t % sh.tiles64) * sh.pos64;
@@ -779,7 +820,6 @@ struct BwdParams {
   const int* last;
   BwdWork work;
   float scale;
-  int n_items;
   uint16_t* dq;
   uint16_t* dk;
   uint16_t* dv;
@@ -806,10 +846,11 @@ struct DqCfg {
   static constexpr int K_OFF = 2 * QTILE;
   static constexpr int V_OFF = K_OFF + KST * KTILE;
   static constexpr int ITEM_OFF = V_OFF + VST * KTILE;
-  static constexpr int BAR_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DqItem));
+  static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DqItem));
+  static constexpr int BAR_OFF = TAKE_OFF + 16;
   // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
-  // s_free[2], ds_ready[2], dq_full, dq_free, item_full[2], item_empty[2]; TMEM slot
-  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 12;
+  // s_free[2], ds_ready[2], dq_full, dq_free, item_full[2], item_empty[2], taken; TMEM slot
+  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 13;
   static constexpr int SMEM_USED = 1024 + BAR_OFF + 8 * (NBAR + 1);
   // At least ~116 KB, so that one CTA (and its 512 TMEM columns) fits an SM.
   static constexpr int SMEM = SMEM_USED > 118784 ? SMEM_USED : 118784;
@@ -852,6 +893,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t dq_full = bars + 8u * (X + 6), dq_free = bars + 8u * (X + 7);
   auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
   auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
+  const uint32_t taken = bars + 8u * (X + 12);
   const uint32_t tmem_slot = bars + 8u * C::NBAR;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
@@ -883,6 +925,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     mbar_init(dq_full, 1);
     mbar_init(dq_free, 8);
+    mbar_init(taken, 1);
     fence_mbar_init();
   }
   zero_rows(gbase + C::Q_OFF, 2 * C::SLABS, kTile, rows);  // Q and dO
@@ -964,8 +1007,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int i = 0; ok; ++i) {
         const DqItem it = wait_item(i, ok);
         if (it.b < 0) break;
-        mbar_arrive(item_empty(i & 1));
-        if (it.n_kv == 0) continue;
+        if (it.n_kv == 0) {
+          mbar_arrive(item_empty(i & 1));
+          continue;
+        }
         // dQ += dS K: A = dS from tensor memory, B = K MN-major (N = dim).
         auto issue_dq = [&](int t, bool begin) -> bool {
           if (!mbar_wait(ds_ready(t & 1), (t >> 1) & 1, p.status)) return false;
@@ -984,6 +1029,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ok = mbar_wait(q_full, n & 1, p.status);
         for (int j = 0; j < it.n_kv && ok; ++j, ++g) {
           const int ks = g % KST, vs = g % VST;
+          // Four key tiles before the end it is time to look for the next item.
+          if (j == max(it.n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
           ok = mbar_wait(k_full(ks), (g / KST) & 1, p.status) &&
                mbar_wait(v_full(vs), (g / VST) & 1, p.status) &&
                (g < 2 || mbar_wait(s_free(g & 1), ((g - 2) >> 1) & 1, p.status));
@@ -1022,12 +1069,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     // -------------------------------------------------------- scheduler
     const int bh_count = sh.batch * groups;
     for (int i = 0;; ++i) {
-      if (!mbar_wait(item_empty(i & 1), ((i >> 1) & 1) ^ 1, p.status)) break;
-      int n = 0;
-      if (lane == 0) n = atomicAdd(p.work.next, 1);
-      n = __shfl_sync(0xffffffffu, n, 0);
+      // Not before the item before it nears its end.
+      if (i > 0 && !mbar_wait(item_empty((i - 1) & 1), ((i - 1) >> 1) & 1, p.status)) break;
+      const int n = i == 0 ? static_cast<int>(blockIdx.x)
+                           : take_cta(base + C::TAKE_OFF, taken, i - 1, p.status);
       DqItem it{-1, 0, 0, 0, 0, {0, 0, 0}};
-      if (n < p.n_items) {
+      if (n >= 0) {
         const int bh = n % bh_count;
         it.b = bh / groups;
         it.h = bh % groups * sh.pack;
@@ -1199,10 +1246,11 @@ struct DkvCfg {
   static constexpr int DS_OFF = P_OFF + 2 * PTILE;
   static constexpr int STAT_OFF = DS_OFF + 2 * PTILE;
   static constexpr int ITEM_OFF = STAT_OFF + QST * STAT_BYTES;
-  static constexpr int BAR_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DkvItem));
+  static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DkvItem));
+  static constexpr int BAR_OFF = TAKE_OFF + 16;
   // kv_full, kv_empty, q_full[QST], q_empty[QST], s_full[2], s_free[2], pds_ready[2],
-  // acc_full, acc_free, item_full[2], item_empty[2]; then the TMEM slot
-  static constexpr int NBAR = 2 + 2 * QST + 12;
+  // acc_full, acc_free, item_full[2], item_empty[2], taken; then the TMEM slot
+  static constexpr int NBAR = 2 + 2 * QST + 13;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
   static constexpr int S_COL = 0;     // S^T_b at 64 b
   static constexpr int DP_COL = 128;  // dP^T_b at 128 + 64 b
@@ -1264,6 +1312,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   const uint32_t acc_full = bars + 8u * (X + 6), acc_free = bars + 8u * (X + 7);
   auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
   auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
+  const uint32_t taken = bars + 8u * (X + 12);
   const uint32_t tmem_slot = bars + 8u * C::NBAR;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
@@ -1291,6 +1340,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 8);
+    mbar_init(taken, 1);
     fence_mbar_init();
   }
   zero_rows(gbase + C::Q_OFF, 2 * QST * C::SLABS, kHalf, rows);  // the Q and dO stages
@@ -1370,9 +1420,11 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       for (int i = 0; ok; ++i) {
         const DkvItem it = wait_item(i, ok);
         if (it.b < 0) break;
-        mbar_arrive(item_empty(i & 1));
         const int T = subs * it.nq;
-        if (T == 0) continue;
+        if (T == 0) {
+          mbar_arrive(item_empty(i & 1));
+          continue;
+        }
         // dV += P^T_t dO_t and dK += dS^T_t Q_t: A K-major from shared memory,
         // B MN-major (N = dim, K = the tile's 64 queries).
         auto issue_acc = [&](int t, bool begin) -> bool {
@@ -1397,6 +1449,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ok = mbar_wait(kv_full, n & 1, p.status);
         for (int t = 0; t < T && ok; ++t, ++g) {
           const int s = g % QST;
+          // Four query tiles before the end it is time to look for the next item.
+          if (t == max(T - 4, 0)) mbar_arrive(item_empty(i & 1));
           ok = mbar_wait(q_full(s), (g / QST) & 1, p.status) &&
                (g < 2 || mbar_wait(s_free(g & 1), ((g - 2) >> 1) & 1, p.status));
           if (!ok) break;
@@ -1433,12 +1487,12 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     // -------------------------------------------------------- scheduler
     const int bk_count = sh.batch * sh.kv_heads;
     for (int i = 0;; ++i) {
-      if (!mbar_wait(item_empty(i & 1), ((i >> 1) & 1) ^ 1, p.status)) break;
-      int n = 0;
-      if (lane == 0) n = atomicAdd(p.work.next + 1, 1);
-      n = __shfl_sync(0xffffffffu, n, 0);
+      // Not before the item before it nears its end.
+      if (i > 0 && !mbar_wait(item_empty((i - 1) & 1), ((i - 1) >> 1) & 1, p.status)) break;
+      const int n = i == 0 ? static_cast<int>(blockIdx.x)
+                           : take_cta(base + C::TAKE_OFF, taken, i - 1, p.status);
       DkvItem it{-1, 0, 0, 0, 0, {0, 0, 0}};
-      if (n < p.n_items) {
+      if (n >= 0) {
         const int bk = n % bk_count;
         it.b = bk / sh.kv_heads;
         it.hk = bk % sh.kv_heads;
@@ -1484,13 +1538,18 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int T = subs * it.nq;
       const size_t tile0 = static_cast<size_t>(it.b) * sh.tiles64 + it.i0;
       const int key0 = it.kv0 + quad * 32;  // the warp's 32 keys
+      // A query tile's spans, a lane each, loaded a tile ahead (tile t % nq).
+      const int2* const spans = p.work.rows + tile0 * kHalf + half * 32 + lane;
+      int ahead = 0;
+      int2 nsp = T > 0 ? spans[0] : make_int2(0, 0);
       for (int t = 0; t < T; ++t, ++g) {
         const int s = g % QST;
         // Which of the tile's queries see which of the warp's keys, a bit each:
         // lane i turns its query's span into bits of the keys, the transpose
         // gives each key's queries.
-        const size_t tile = tile0 + t % it.nq;
-        const int2 sp = p.work.rows[tile * kHalf + half * 32 + lane];
+        const int2 sp = nsp;
+        if (++ahead == it.nq) ahead = 0;
+        nsp = spans[static_cast<size_t>(ahead) * kHalf];
         const int from = min(max(sp.x - key0, 0), 32);
         const uint32_t seen =
             transpose_bits(bit_range(from, min(max(sp.x + sp.y - key0, 0), 32)));
@@ -1765,8 +1824,6 @@ BwdWork bwd_work(void* base, const SpanShape& sh) {
   w.bytes += tiles * kHalf * sizeof(int2);
   w.tiles = reinterpret_cast<SpanTile*>(at + w.bytes);
   w.bytes += tiles * sizeof(SpanTile);
-  w.next = reinterpret_cast<int*>(at + w.bytes);
-  w.bytes += 16;
   return w;
 }
 
@@ -1782,11 +1839,6 @@ int check_span_shape(int64_t batch, int64_t seq, int64_t heads, int64_t kv_heads
   return TQ_OK;
 }
 
-unsigned grid_of(int items) {
-  const int sms = sm_count();
-  return static_cast<unsigned>(items < sms ? items : sms);
-}
-
 template <int D>
 int launch_fwd(const void* q, const void* k, const void* v, FwdParams p, cudaStream_t stream) {
   using C = FwdCfg<D>;
@@ -1799,8 +1851,8 @@ int launch_fwd(const void* q, const void* k, const void* v, FwdParams p, cudaStr
   if ((rc = map_bshd(&tk, k, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
   if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
   p.n_pairs = (sh.tiles128 + 1) / 2;
-  p.n_items = sh.batch * (sh.heads / sh.pack) * p.n_pairs;
-  return launch_kernel(span_fwd_kernel<D>, dim3(grid_of(p.n_items)), dim3(kAttnThreads), C::SMEM,
+  const unsigned grid = static_cast<unsigned>(sh.batch) * (sh.heads / sh.pack) * p.n_pairs;
+  return launch_kernel(span_fwd_kernel<D>, dim3(grid), dim3(kAttnThreads), C::SMEM,
                        stream, 1, "span attention forward launch", tq_, tk, tv, p);
 }
 
@@ -1844,12 +1896,12 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
   rc = launch_kernel(span_prep_kernel, dim3(pp.row_blocks + span_blocks), dim3(256), 0, stream, 1,
                      "span attention backward prep launch", pp);
   if (rc) return rc;
-  p.n_items = sh.batch * (sh.heads / sh.pack) * sh.tiles128;
-  rc = launch_kernel(span_dq_kernel<D>, dim3(grid_of(p.n_items)), dim3(kAttnThreads), Q::SMEM,
+  const unsigned grid_q = static_cast<unsigned>(sh.batch) * (sh.heads / sh.pack) * sh.tiles128;
+  rc = launch_kernel(span_dq_kernel<D>, dim3(grid_q), dim3(kAttnThreads), Q::SMEM,
                      stream, 1, "span attention backward dq launch", q128, do128, k64, v64, p);
   if (rc) return rc;
-  p.n_items = sh.batch * sh.kv_heads * sh.key_tiles;
-  return launch_kernel(span_dkv_kernel<D>, dim3(grid_of(p.n_items)), dim3(kAttnThreads), KV::SMEM,
+  const unsigned grid_kv = static_cast<unsigned>(sh.batch) * sh.kv_heads * sh.key_tiles;
+  return launch_kernel(span_dkv_kernel<D>, dim3(grid_kv), dim3(kAttnThreads), KV::SMEM,
                        stream, 1, "span attention backward dkv launch", q64, do64, k128, v128, p);
 }
 
