@@ -259,6 +259,34 @@ def _span_operands(op: str, q, k, v, first, last):
     return q, k, v, first.contiguous(), last.contiguous()
 
 
+def _scale(scale: float | None, dim: int) -> float:
+    return float(scale) if scale is not None else dim ** -0.5
+
+
+def _span_forward(q, k, v, first, last, sc):
+    b, s, h, d = q.shape
+    o = torch.empty_like(q)
+    lse = torch.empty(b, h, s, dtype=torch.float32, device=q.device)
+    _on(q.device, "attention", lambda stream: lib().tq_span_attention_fwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), first.data_ptr(), last.data_ptr(), b, s, h,
+        k.shape[2], d, sc, o.data_ptr(), lse.data_ptr(), stream))
+    return o, lse
+
+
+def _span_backward(q, k, v, first, last, o, do, lse, sc):
+    b, s, h, d = q.shape
+    hk = k.shape[2]
+    nbytes = ctypes.c_size_t()
+    check(lib().tq_span_attention_bwd_workspace_bytes(b, s, h, hk, ctypes.byref(nbytes)))
+    ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=q.device)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    _on(q.device, "attention", lambda stream: lib().tq_span_attention_bwd(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), first.data_ptr(), last.data_ptr(),
+        o.data_ptr(), do.data_ptr(), lse.data_ptr(), b, s, h, hk, d, sc, dq.data_ptr(),
+        dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes.value, stream))
+    return dq, dk, dv
+
+
 def span_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                            first: torch.Tensor, last: torch.Tensor,
                            scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -269,14 +297,7 @@ def span_attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     op = "span_attention"
     _one_device(op, q=q, k=k, v=v, first=first, last=last)
     q, k, v, first, last = _span_operands(op, q, k, v, first, last)
-    b, s, h, d = q.shape
-    sc = float(scale) if scale is not None else d ** -0.5
-    o = torch.empty_like(q)
-    lse = torch.empty(b, h, s, dtype=torch.float32, device=q.device)
-    _on(q.device, "attention", lambda stream: lib().tq_span_attention_fwd(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), b, s, h, k.shape[2], d, sc,
-        _ptr(o), _ptr(lse), stream))
-    return o, lse
+    return _span_forward(q, k, v, first, last, _scale(scale, q.shape[3]))
 
 
 def span_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -293,33 +314,23 @@ def span_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     b, s, h, d = q.shape
     if lse.dtype != torch.float32 or tuple(lse.shape) != (b, h, s):
         raise ValueError(f"[{op}] lse must be f32 [{b}, {h}, {s}]")
-    lse = lse.contiguous()
-    sc = float(scale) if scale is not None else d ** -0.5
-    nbytes = ctypes.c_size_t()
-    check(lib().tq_span_attention_bwd_workspace_bytes(b, s, h, k.shape[2],
-                                                       ctypes.byref(nbytes)))
-    ws = torch.empty(max(1, nbytes.value), dtype=torch.uint8, device=q.device)
-    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    _on(q.device, "attention", lambda stream: lib().tq_span_attention_bwd(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(first), _ptr(last), _ptr(o), _ptr(do), _ptr(lse), b,
-        s, h, k.shape[2], d, sc, _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), nbytes.value, stream))
-    return dq, dk, dv
+    return _span_backward(q, k, v, first, last, o, do, lse.contiguous(), _scale(scale, d))
 
 
 class _SpanAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, first, last, scale):
-        o, lse = span_attention_forward(q, k, v, first, last, scale)
+    def forward(ctx, q, k, v, first, last, sc):
+        o, lse = _span_forward(q, k, v, first, last, sc)
         ctx.save_for_backward(q, k, v, first, last, o, lse)
-        ctx.scale = scale
+        ctx.scale = sc
         return o
 
     @staticmethod
     def backward(ctx, do):
         _once("span_attention")
         q, k, v, first, last, o, lse = ctx.saved_tensors
-        dq, dk, dv = span_attention_backward(q, k, v, first, last, o, do, lse, ctx.scale)
-        return dq, dk, dv, None, None, None
+        do = _bf16_contig("do", do)
+        return *_span_backward(q, k, v, first, last, o, do, lse, ctx.scale), None, None, None
 
 
 def span_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: torch.Tensor,
@@ -332,7 +343,10 @@ def span_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: tor
     layout; the scale defaults to dim^-1/2.  A query that sees nothing gets 0
     and passes no gradient.  What a query does not see still enters products
     with 0, so k and v, and q of queries that see nothing, must be finite."""
-    return _SpanAttention.apply(q, k, v, first, last, scale)
+    op = "span_attention"
+    _one_device(op, q=q, k=k, v=v, first=first, last=last)
+    q, k, v, first, last = _span_operands(op, q, k, v, first, last)
+    return _SpanAttention.apply(q, k, v, first, last, _scale(scale, q.shape[3]))
 
 
 class _SwiGLU(torch.autograd.Function):
