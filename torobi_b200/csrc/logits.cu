@@ -38,6 +38,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+// Forward: 32-byte chunks a thread has in flight, and CTAs an SM.  Four and
+// four (64 registers) read 2046 x 128256 logits with the entropy in 88 us;
+// two and six 92, two and eight 91, four and five 92, one and eight 93, and
+// with the registers left to the compiler (two chunks: 92 registers) 115.
+constexpr int kInFlight = 4;
+constexpr int kPerSm = 4;
 constexpr int kMaxTop = 128;     // alternatives a call may ask for or give
 constexpr int kMaxSplit = 8;     // CTAs (one cluster) that may share a row
 constexpr int kSpare = 32;       // chunks above the threshold taken beyond top
@@ -194,8 +200,10 @@ __device__ __forceinline__ void st_chunk(void* p, const uint32_t (&w)[8]) {
 // ------------------------------------------------------------ running sums --
 
 // What a row's sums are of, beside s = sum 2^x: nothing, a = sum x 2^x (the
-// entropy's), or a = sum 2^y, y = (z - m) log2(e) (a second temperature, 1).
-enum Mode { kPlain, kEntropy, kTwo };
+// entropy's), or a = sum 2^y, y = (z - m) log2(e) (a second temperature, 1);
+// at temperature 2, 2^y is the square of 2^x, which spares the MUFU unit the
+// second exponential (2046 x 128256: 141 -> 96 us forward).
+enum Mode { kPlain, kEntropy, kTwo, kSquare };
 
 struct Sums {
   float m = -INFINITY, s = 0.0f, a = 0.0f;
@@ -211,6 +219,7 @@ __device__ __forceinline__ void move_to(Sums& v, float m, float c) {
   const float f = ex2_approx(-d);
   if (M == kEntropy) v.a = f * fmaf(-d, v.s, v.a);
   if (M == kTwo) v.a *= ex2_approx(-up * kLog2e);
+  if (M == kSquare) v.a *= f * f;
   v.s *= f;
   v.m = m;
 }
@@ -250,6 +259,7 @@ __device__ __forceinline__ void add_chunks(Sums& v, const uint32_t (&w)[U][8], f
         const float2 y = split(d * c1);
         a = a + f2(ex2_approx(y.x), ex2_approx(y.y));
       }
+      if (M == kSquare) a = fma2(p, p, a);
     }
   }
   const float2 ss = split(s), aa = split(a);
@@ -500,8 +510,8 @@ struct LogprobParams {
 // One CTA per row, or a cluster of `split` CTAs when rows are few, each a
 // contiguous slice of the row's chunks; rank 0 joins them in rank order.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_fwd_kernel(const LogprobParams p) {
-  constexpr int U = 2;
+__global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const LogprobParams p) {
+  constexpr int U = kInFlight;
   extern __shared__ uint64_t pool[];
   __shared__ Sums sums[kWarps];
   __shared__ float2 total;
@@ -797,11 +807,12 @@ struct DistillParams {
   float4* stats;  // m, log2 s at the temperature, log2 s at 1
 };
 
-// TWO: the targets' cross-entropy needs the row's sum at temperature 1 too.
-template <typename T, bool TWO>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const DistillParams p) {
-  constexpr Mode M = TWO ? kTwo : kPlain;
-  constexpr int U = 2;
+// kTwo, kSquare: the targets' cross-entropy needs the row's sum at temperature
+// 1 too.
+template <typename T, Mode M>
+__global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const DistillParams p) {
+  constexpr bool TWO = M != kPlain;
+  constexpr int U = kInFlight;
   __shared__ Sums sums[kWarps];
   griddep_wait();
   griddep_launch_dependents();
@@ -894,7 +905,7 @@ struct DistillGradParams {
 // Every element first as if nothing were given (the two softmaxes alone); the
 // few given ones are then written again by the CTA that wrote them, with what
 // all their entries in the row take off (the same id may be given twice).
-template <typename T, bool SAME, bool TWO>
+template <typename T, bool SAME, Mode M>
 __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGradParams p) {
   __shared__ int ids[kMaxTop + 1];
   __shared__ float off[kMaxTop + 1];
@@ -940,13 +951,14 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGrad
   const bool zero = us == 0.0f && v == 0.0f;
   float ca = dead ? 0.0f : us * exp2f(-st.y);
   float cb = dead ? 0.0f : v * exp2f(-st.z);
-  if (!TWO) ca += cb;
+  if (M == kPlain) ca += cb;
   auto soft = [&](float f) {
     if (zero || dead) return 0.0f;
     const float d = f - st.x;
-    float g = ca * ex2_approx(d * p.c);
-    if (TWO) g = fmaf(cb, ex2_approx(d * kLog2e), g);
-    return g;
+    const float e = ex2_approx(d * p.c);
+    if (M == kSquare) return e * fmaf(cb, e, ca);
+    if (M == kTwo) return fmaf(cb, ex2_approx(d * kLog2e), ca * e);
+    return ca * e;
   };
   // The given elements' logits, before anything is written over them.
   const int mine = static_cast<int>(threadIdx.x) <= k ? ids[threadIdx.x] : -1;
@@ -1112,6 +1124,12 @@ extern "C" int tq_token_logprobs_bwd(const void* logits, int dtype, const int64_
 namespace tq {
 namespace {
 
+// Which sums a call needs: the temperature's alone (0), those at temperature 1
+// beside them (1), or as their squares (2).
+int which_sums(bool targets, float temperature) {
+  return !targets || temperature == 1.0f ? 0 : temperature == 2.0f ? 2 : 1;
+}
+
 int check_teacher(const char* who, const void* ids, int ids_bits, const void* logits,
                   int logits_dtype, int64_t k, int64_t rows, Teacher* t) {
   if (k < 1 || k > kMaxTop)
@@ -1165,11 +1183,14 @@ extern "C" int tq_distill_fwd(const void* logits, int dtype, const void* teacher
   p.kl = kl;
   p.ce = ce;
   p.stats = reinterpret_cast<float4*>(stats);
-  const bool two = targets && temperature != 1.0f;
-  auto kernel = dtype == TQ_DTYPE_F32
-                    ? (two ? distill_fwd_kernel<float, true> : distill_fwd_kernel<float, false>)
-                    : (two ? distill_fwd_kernel<uint16_t, true>
-                           : distill_fwd_kernel<uint16_t, false>);
+  using Kernel = void (*)(const DistillParams);
+  const Kernel f32[3] = {distill_fwd_kernel<float, kPlain>, distill_fwd_kernel<float, kTwo>,
+                         distill_fwd_kernel<float, kSquare>};
+  const Kernel bf16[3] = {distill_fwd_kernel<uint16_t, kPlain>,
+                          distill_fwd_kernel<uint16_t, kTwo>,
+                          distill_fwd_kernel<uint16_t, kSquare>};
+  const Kernel kernel =
+      (dtype == TQ_DTYPE_F32 ? f32 : bf16)[which_sums(targets != nullptr, temperature)];
   return launch_kernel(kernel, dim3(static_cast<unsigned>(rows * p.split)), dim3(kThreads), 0,
                        as_stream(stream), dim3(p.split), "distillation forward launch", p);
 }
@@ -1209,18 +1230,20 @@ extern "C" int tq_distill_bwd(const void* logits, int dtype, const void* teacher
   p.parts = split_for(rows, vocab, 32 / elem_bytes(dtype), 16);
   p.c = kLog2e / temperature;
   p.inv_t = 1.0f / temperature;
-  const bool two = dce && temperature != 1.0f;
   const bool same = same_offset(logits, dlogits, rows, ld, ld_out, elem_bytes(dtype));
   using Kernel = void (*)(const DistillGradParams);
-  const Kernel f32[2][2] = {{distill_bwd_kernel<float, false, false>,
-                             distill_bwd_kernel<float, false, true>},
-                            {distill_bwd_kernel<float, true, false>,
-                             distill_bwd_kernel<float, true, true>}};
-  const Kernel bf16[2][2] = {{distill_bwd_kernel<uint16_t, false, false>,
-                              distill_bwd_kernel<uint16_t, false, true>},
-                             {distill_bwd_kernel<uint16_t, true, false>,
-                              distill_bwd_kernel<uint16_t, true, true>}};
-  const Kernel kernel = (dtype == TQ_DTYPE_F32 ? f32 : bf16)[same][two];
+  const Kernel f32[2][3] = {
+      {distill_bwd_kernel<float, false, kPlain>, distill_bwd_kernel<float, false, kTwo>,
+       distill_bwd_kernel<float, false, kSquare>},
+      {distill_bwd_kernel<float, true, kPlain>, distill_bwd_kernel<float, true, kTwo>,
+       distill_bwd_kernel<float, true, kSquare>}};
+  const Kernel bf16[2][3] = {
+      {distill_bwd_kernel<uint16_t, false, kPlain>, distill_bwd_kernel<uint16_t, false, kTwo>,
+       distill_bwd_kernel<uint16_t, false, kSquare>},
+      {distill_bwd_kernel<uint16_t, true, kPlain>, distill_bwd_kernel<uint16_t, true, kTwo>,
+       distill_bwd_kernel<uint16_t, true, kSquare>}};
+  const Kernel kernel =
+      (dtype == TQ_DTYPE_F32 ? f32 : bf16)[same][which_sums(dce != nullptr, temperature)];
   return launch_kernel(kernel, dim3(static_cast<unsigned>(rows * p.parts)), dim3(kThreads), 0,
                        as_stream(stream), 1, "distillation backward launch", p);
 }
