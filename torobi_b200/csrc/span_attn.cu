@@ -39,13 +39,16 @@
 namespace tq {
 namespace {
 
-constexpr int kAttnThreads = 384;
-constexpr int kReaders = 10;  // who reads a tile's description: TMA, MMA, eight compute warps
-// Registers a thread: the four warps that copy, multiply and schedule need
-// fewer, the eight compute warps hold a row of 128 scores.
-// 128 * 96 + 256 * 200 = 63,488 of the launch's 384 * 168 = 64,512.
-constexpr int kFewRegs = 96;
-constexpr int kManyRegs = 200;
+constexpr int kFwdThreads = 384;  // four warps of roles, eight of softmax
+constexpr int kBwdWarps = 16;     // that compute, beside the four of roles
+constexpr int kBwdThreads = 128 + 32 * kBwdWarps;
+// Who reads a tile's description: TMA, MMA and every computing warp.
+constexpr int kFwdReaders = 2 + 8;
+constexpr int kBwdReaders = 2 + kBwdWarps;
+// How far (log2) a row's scores may grow past its reference before its sums
+// are scaled down to a new one.  P, l and O keep their relative precision at
+// any exponent, so only their range counts.
+constexpr float kGrowLog2 = 60.0f;
 
 struct SpanShape {
   int batch, seq, heads, kv_heads, group;
@@ -91,29 +94,10 @@ __device__ __forceinline__ Span span_of_positions(const int* first, const int* l
 // tensor cores by each thread's fence and the barrier after it.
 __device__ __forceinline__ void zero_rows(uint8_t* slab, int slabs, int tile_rows, int from) {
   const int per = (tile_rows - from) * 8;  // 16-byte words a slab
-  for (int i = threadIdx.x; i < slabs * per; i += kAttnThreads)
+  for (int i = threadIdx.x; i < slabs * per; i += blockDim.x)
     *reinterpret_cast<uint4*>(slab + (i / per * tile_rows + from) * 128 + i % per * 16) =
         make_uint4(0, 0, 0, 0);
   if (per > 0) fence_proxy_async_smem();
-}
-
-// 2^x of two values on the FMA pipe: attn.cuh's method with a quintic (minimax
-// in relative error with value 1 at f = 0; max relative error 1.6e-7), since
-// the row's sum is answered in f32.
-__device__ __forceinline__ F2 exp2_fine(F2 x) {
-  const float2 v = split(x);
-  const F2 c = f2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
-  const F2 t = c + f2(12582912.0f, 12582912.0f);
-  const F2 f = fma2(t + f2(-12582912.0f, -12582912.0f), f2(-1.0f, -1.0f), c);
-  F2 p = fma2(f2(0.001326472731307149f, 0.001326472731307149f), f,
-              f2(0.009671512991189957f, 0.009671512991189957f));
-  p = fma2(p, f, f2(0.05550733581185341f, 0.05550733581185341f));
-  p = fma2(p, f, f2(0.24022242426872253f, 0.24022242426872253f));
-  p = fma2(p, f, f2(0.6931470036506653f, 0.6931470036506653f));
-  p = fma2(p, f, f2(1.0f, 1.0f));
-  const float2 pv = split(p), tv = split(t);
-  return f2(__uint_as_float(__float_as_uint(pv.x) + (__float_as_uint(tv.x) << 23)),
-            __uint_as_float(__float_as_uint(pv.y) + (__float_as_uint(tv.y) << 23)));
 }
 
 __device__ __forceinline__ F2 exp2_mufu(F2 x) {
@@ -164,20 +148,29 @@ __device__ __forceinline__ int take_cta(uint32_t slot, uint32_t bar, int n, int*
   return ok ? static_cast<int>(x) : -1;
 }
 
-// Rows of results: 32 values a lane, in the widest stores the address allows.
-__device__ __forceinline__ void store_row32(uint16_t* dst, const uint32_t (&w)[16], bool wide) {
+// Rows of results: 2 N values a lane, in the widest stores the address allows.
+template <int N>
+__device__ __forceinline__ void store_row(uint16_t* dst, const uint32_t (&w)[N], bool wide) {
+  static_assert(N % 8 == 0, "whole wide stores");
   if (wide) {
 #pragma unroll
-    for (int i = 0; i < 16; i += 8)
+    for (int i = 0; i < N; i += 8)
       asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i),
                    "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
                    "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
                    : "memory");
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
+    for (int i = 0; i < N; i += 4)
       *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   }
+}
+
+__device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[32]) {
+  tmem_ld_32x32b_x32(at, r);
+}
+__device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[16]) {
+  tmem_ld_32x32b_x16(at, r);
 }
 
 __device__ __forceinline__ bool wide_rows(const void* p) {
@@ -195,16 +188,18 @@ __device__ __forceinline__ bool wide_rows(const void* p) {
 //   warps 4-7    softmax of query tile 0 (thread i owns row i, TMEM lane i)
 //   warps 8-11   softmax of query tile 1
 // TMEM: S_0 | S_1 (128 f32 columns each) | O_0 | O_1 (dim columns each).  A
-// softmax thread reads its row of S once into registers and writes P (bf16
-// pairs, 64 columns) over its first half.  MMA issue order per key tile t:
+// softmax thread reads its row of S once, 32 columns at a time, and writes P
+// (bf16 pairs) over columns already read.  It needs no maximum of the row
+// first: the reference m is the maximum of the first chunk that the row sees,
+// and stays until a chunk exceeds it by 2^60 (then l, O and the tile's earlier
+// P are scaled).  With all 128 scores held for the maximum, the registers left
+// no room to overlap one chunk's exponentials with the next one's load.  MMA
+// issue order per key tile t:
 //   O_0 += P_0(t) V_t,  S_0 = Q_0 K_{t+1}^T,  O_1 += P_1(t) V_t,  S_1 = Q_1 K_{t+1}^T
 // and tcgen05.mma operations issued by one thread execute in that order, so
 // S_w(t+1) overwrites P_w(t) right after its product has read it.  Every
 // barrier that completes once per key tile (or once per pair) counts through
 // all pairs; no waiter is two phases behind.
-// Three in eight exponentials of an unmasked chunk run on the FMA pipe: the
-// MUFU unit alone (16 a cycle) would take 1024 cycles a 128 x 128 tile, as long
-// as its MMAs.
 
 struct FwdItem {
   int b, h, t0;              // b < 0: no more; first of `pack` heads, first query tile
@@ -249,7 +244,7 @@ struct FwdParams {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kFwdThreads, 1)
     span_fwd_kernel(const __grid_constant__ CUtensorMap tm_q,
                     const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
@@ -304,7 +299,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       mbar_init(o_done(w), 1);
       mbar_init(o_free(w), 4);
       mbar_init(item_full(w), 1);
-      mbar_init(item_empty(w), kReaders);
+      mbar_init(item_empty(w), kFwdReaders);
     }
     mbar_init(taken, 1);
     fence_mbar_init();
@@ -332,7 +327,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
   };
 
   if (warp < 4) {
-    registers_down<kFewRegs>();
     if (warp == 0 && elect_one_sync()) {
       // ----------------------------------------------------------- TMA
       tma_prefetch_desc(&tm_q);
@@ -515,7 +509,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       }
     }
   } else {
-    registers_up<kManyRegs>();
     // --------------------------------------------------------- softmax
     const int w = (warp - 4) >> 2;  // query tile of this warpgroup
     const int quad = warp & 3;
@@ -562,77 +555,85 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         auto full = [&](int c4) {
           return kv0 + 32 * c4 >= all_lo && kv0 + 32 * c4 + 32 <= all_hi;
         };
-        uint32_t r[4][32];
-#pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4)
-          if (!none(c4)) tmem_ld_32x32b_x32(scol + c4 * 32, r[c4]);
-        tmem_ld_wait();
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4) {
-          if (none(c4)) continue;
-          if (!full(c4)) {
-            const int col0 = kv0 + 32 * c4 - sp.lo;
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (static_cast<unsigned>(col0 + e) >= len) r[c4][e] = 0xFF800000u;  // -inf
-          }
-#pragma unroll
-          for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(r[c4][e]));
-        }
-        const float m_new =
-            fmaxf(m, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c);
-        // A row that has summed nothing yet just takes its maximum.
-        const bool fresh = m == -INFINITY;
-        if (__any_sync(0xffffffffu, !fresh && filled && m_new > m + kRescaleLog2)) {
-          // Move m and rescale this row of O_w, once its last product is done.
-          const float f = fresh ? 1.0f : ex2_approx(m - m_new);
-          ok = mbar_wait(o_done(w), (steps - 1) & 1, p.status);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll 1
-          for (int c4 = 0; c4 < D / 16; ++c4) {
-            uint32_t o[16];
-            tmem_ld_32x32b_x16(ocol + c4 * 16, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st_32x32b_x16(ocol + c4 * 16, o);
-          }
-          tmem_st_wait();
-          l *= f;
-          m = m_new;
-        } else if (fresh) {
-          m = m_new;
-        }
-        const float mref = m == -INFINITY ? 0.0f : m;
-        const F2 shift = f2(-mref, -mref);
         F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+        uint32_t rb[2][32];
+        if (!none(0)) tmem_ld_32x32b_x32(scol, rb[0]);
 #pragma unroll
         for (int c4 = 0; c4 < 4; ++c4) {
+          tmem_ld_wait();
+          if (c4 + 1 < 4 && !none(c4 + 1))
+            tmem_ld_32x32b_x32(scol + (c4 + 1) * 32, rb[(c4 + 1) & 1]);
+          uint32_t(&r)[32] = rb[c4 & 1];
           uint32_t pk[16];
           if (none(c4)) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) pk[e] = 0;
-          } else if (full(c4)) {
+          } else {
+            if (!full(c4)) {
+              const int col0 = kv0 + 32 * c4 - sp.lo;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const F2 x = fma2(pair_of(r[c4][2 * e], r[c4][2 * e + 1]), c2, shift);
-              const F2 q = (e & 7) == 2 || (e & 7) == 5 || (e & 7) == 7 ? exp2_fine(x)
-                                                                      : exp2_mufu(x);
-              sum[e & 1] = sum[e & 1] + q;
-              pk[e] = pack_bf16(q);
+              for (int e = 0; e < 32; ++e)
+                if (static_cast<unsigned>(col0 + e) >= len) r[e] = 0xFF800000u;  // -inf
             }
-          } else {  // 2^-inf is 0 on the MUFU unit
+            float m4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m4[e] = __uint_as_float(r[e]);
+#pragma unroll
+            for (int e = 4; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(r[e]));
+            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
+            if (m == -INFINITY) m = mx;  // nothing summed yet
+            if (__any_sync(0xffffffffu, mx > m + kGrowLog2)) {
+              // The rows that outgrew their reference take a new one; the
+              // others go through with a factor of 1.
+              const bool grow = mx > m + kGrowLog2;
+              const float f = grow ? ex2_approx(m - mx) : 1.0f;
+              const F2 ff = f2(f, f);
+              if (grow) m = mx;
+              l *= f;
+              sum[0] = sum[0] * ff;
+              sum[1] = sum[1] * ff;
+              tmem_ld_wait();  // the next chunk's scores, ahead of P's here
+              tmem_st_wait();
+#pragma unroll 1
+              for (int cc = 0; cc < c4; ++cc) {
+                uint32_t o[16];
+                tmem_ld_32x32b_x16(scol + cc * 16, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  o[e] = pack_bf16x2_f32(__uint_as_float(o[e] << 16) * f,
+                                         __uint_as_float(o[e] & 0xFFFF0000u) * f);
+                tmem_st_32x32b_x16(scol + cc * 16, o);
+              }
+              if (j > 0) {  // O_w, once its last product is done
+                ok = mbar_wait(o_done(w), (steps - 1) & 1, p.status);
+                tc_fence_after();
+#pragma unroll 1
+                for (int cc = 0; cc < D / 16; ++cc) {
+                  uint32_t o[16];
+                  tmem_ld_32x32b_x16(ocol + cc * 16, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e)
+                    o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  tmem_st_32x32b_x16(ocol + cc * 16, o);
+                }
+              }
+              tmem_st_wait();
+            }
+            // A row that sees nothing yet has only -inf here: 2^-inf = 0.
+            const float mref = m == -INFINITY ? 0.0f : m;
+            const F2 shift = f2(-mref, -mref);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const F2 q = exp2_mufu(fma2(pair_of(r[c4][2 * e], r[c4][2 * e + 1]), c2, shift));
+              const F2 q = exp2_mufu(fma2(pair_of(r[2 * e], r[2 * e + 1]), c2, shift));
               sum[e & 1] = sum[e & 1] + q;
               pk[e] = pack_bf16(q);
             }
           }
           tmem_st_32x32b_x16(scol + c4 * 16, pk);
         }
+        if (!ok) break;
         const float2 s = split(sum[0] + sum[1]);
         l += s.x + s.y;
         tmem_st_wait();
@@ -671,13 +672,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             wd[e] = pack_bf16(pair_of(o[2 * e], o[2 * e + 1]) * inv2);
-          if (valid) store_row32(orow + c4 * 32, wd, wide);
+          if (valid) store_row(orow + c4 * 32, wd, wide);
         }
         if (valid) *lse = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
       } else if (valid) {  // no row of the tile sees anything
         const uint32_t zero[16] = {};
 #pragma unroll
-        for (int c4 = 0; c4 < D / 32; ++c4) store_row32(orow + c4 * 32, zero, wide);
+        for (int c4 = 0; c4 < D / 32; ++c4) store_row(orow + c4 * 32, zero, wide);
         *lse = -INFINITY;
       }
       it = nx;
@@ -700,14 +701,14 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
 //   prep   per packed query row -lse log2(e) and -delta (f32), in 64-row packed
 //          tiles (rows that hold nothing: -inf and 0, so their probabilities
 //          are 0), each row's span in the same order, and each tile's spans;
-//   dq     a tile of work is a packed 128-row query tile, key tiles of 64 (two
-//          compute warpgroups, each half of every tile's columns):
+//   dq     a tile of work is a packed 128-row query tile, key tiles of 64 (four
+//          compute warpgroups, each 16 of every tile's columns):
 //            S = Q K_j^T, dP = dO V_j^T (tensor memory, double-buffered),
 //            dS = P * (dP - delta), P = exp2(S c - lse2)  (compute warps),
 //            dQ += dS K_j  (dS written back to tensor memory, A from TMEM);
 //   dkv    a tile of work is a 128-key tile of one key/value head, with the
-//          packed 64-row query tiles that see it (two compute warpgroups,
-//          each half of every tile's columns):
+//          packed 64-row query tiles that see it (four compute warpgroups,
+//          each 16 of every tile's columns):
 //            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, into
 //            shared memory as K-major operands), dV += P^T dO_i, dK += dS^T Q_i.
 // Which CTA does a tile changes no result.
@@ -758,7 +759,10 @@ __global__ void __launch_bounds__(256) span_prep_kernel(const PrepParams p) {
       const bool filled = r < filled_rows;
       const Span sp =
           filled ? load_span(p.first, p.last, b, i0 + r / sh.pack, sh.seq) : Span{0, 0};
-      p.work.rows[t * kHalf + r] = make_int2(sp.lo, sp.hi - sp.lo);
+      // A row that holds nothing (its lse2 is +inf) must not make the tile a
+      // masked one.
+      p.work.rows[t * kHalf + r] = filled ? make_int2(sp.lo, sp.hi - sp.lo)
+                                          : make_int2(0, sh.seq);
       if (!filled) continue;
       if (sp.lo < sp.hi) s.lo = min(s.lo, sp.lo);
       s.hi = max(s.hi, sp.hi);
@@ -864,7 +868,7 @@ struct DqCfg {
 };
 
 template <int D>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
     span_dq_kernel(const __grid_constant__ CUtensorMap tm_q,
                    const __grid_constant__ CUtensorMap tm_do,
                    const __grid_constant__ CUtensorMap tm_k,
@@ -918,13 +922,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full(i), 1);
-      mbar_init(s_free(i), 8);
-      mbar_init(ds_ready(i), 8);
+      mbar_init(s_free(i), kBwdWarps);
+      mbar_init(ds_ready(i), kBwdWarps);
       mbar_init(item_full(i), 1);
-      mbar_init(item_empty(i), kReaders);
+      mbar_init(item_empty(i), kBwdReaders);
     }
     mbar_init(dq_full, 1);
-    mbar_init(dq_free, 8);
+    mbar_init(dq_free, kBwdWarps);
     mbar_init(taken, 1);
     fence_mbar_init();
   }
@@ -1092,10 +1096,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------ compute warps
-    // Two warpgroups on the same 128 rows: warps 4-7 take key columns 0-31
-    // of each 64-key tile, warps 8-11 columns 32-63 (the gradient is
-    // elementwise given the row's lse and delta); likewise halves of dQ.
-    const int half = (warp - 4) >> 2;
+    // Four warpgroups on the same 128 rows, 16 of each tile's 64 key columns
+    // each (the gradient is elementwise given the row's lse and delta);
+    // likewise quarters of dQ.
+    const int part = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const bool filled = row < rows;
@@ -1140,36 +1144,35 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         ok = mbar_wait(s_full(g & 1), (g >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        const int k0 = (it.kv0 + j) * kHalf + half * 32;
-        const bool none = k0 + 32 <= any_lo || k0 >= any_hi;
-        uint32_t sv[32], dv[32];
+        const int k0 = (it.kv0 + j) * kHalf + part * 16;
+        const bool none = k0 + 16 <= any_lo || k0 >= any_hi;
+        uint32_t sv[16], dv[16];
         if (!none) {
-          tmem_ld_32x32b_x32(lrow + C::S_COL + (g & 1) * kHalf + half * 32, sv);
-          tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + half * 32, dv);
+          tmem_ld_32x32b_x16(lrow + C::S_COL + (g & 1) * kHalf + part * 16, sv);
+          tmem_ld_32x32b_x16(lrow + C::DP_COL + (g & 1) * kHalf + part * 16, dv);
           tmem_ld_wait();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free(g & 1));
-        uint32_t pk[16];
+        uint32_t pk[8];
         if (none) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = 0;
+          for (int e = 0; e < 8; ++e) pk[e] = 0;
         } else {
-          if (k0 < all_lo || k0 + 32 > all_hi) {
+          if (k0 < all_lo || k0 + 16 > all_hi) {
             const int col0 = k0 - sp.lo;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 16; ++e)
               if (static_cast<unsigned>(col0 + e) >= len) sv[e] = 0xFF800000u;  // P = 0
           }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const F2 q =
-                exp2_mufu(fma2(pair_of(sv[2 * e], sv[2 * e + 1]), c2, shift));
+          for (int e = 0; e < 8; ++e) {
+            const F2 q = exp2_mufu(fma2(pair_of(sv[2 * e], sv[2 * e + 1]), c2, shift));
             pk[e] = pack_bf16(q * (pair_of(dv[2 * e], dv[2 * e + 1]) + nd));
           }
         }
-        tmem_st_32x32b_x16(lrow + C::DS_COL + (g & 1) * 32 + half * 16, pk);
+        tmem_st_32x32b_x8(lrow + C::DS_COL + (g & 1) * 32 + part * 8, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -1190,24 +1193,20 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         tc_fence_after();
         ++n;
       }
+      constexpr int COLS = D / 4;
+      uint32_t o[COLS];
+      uint32_t w[COLS / 2] = {};
+      if (it.n_kv > 0) {
+        tmem_ld_cols(lrow + C::DQ_COL + part * COLS, o);
+        tmem_ld_wait();
+        tc_fence_before();  // dQ may be begun again
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dq_free);
 #pragma unroll
-      for (int e = 0; e < D / 64; ++e) {
-        const int c4 = half * (D / 64) + e;
-        uint32_t o[32];
-        uint32_t w[16] = {};
-        if (it.n_kv > 0) {
-          tmem_ld_32x32b_x32(lrow + C::DQ_COL + c4 * 32, o);
-          tmem_ld_wait();
-          if (e == D / 64 - 1) {  // dQ may be begun again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(dq_free);
-          }
-#pragma unroll
-          for (int q = 0; q < 16; ++q) w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * scale2);
-        }
-        if (valid) store_row32(orow + c4 * 32, w, wide);
+        for (int q = 0; q < COLS / 2; ++q)
+          w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * scale2);
       }
+      if (valid) store_row(orow + part * COLS, w, wide);
       it = nx;
       st = nst;
     }
@@ -1283,7 +1282,7 @@ __device__ __forceinline__ uint32_t bit_range(int a, int z) {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kAttnThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
     span_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
                     const __grid_constant__ CUtensorMap tm_do,
                     const __grid_constant__ CUtensorMap tm_k,
@@ -1329,17 +1328,17 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     mbar_init(kv_empty, 1);
     for (int s = 0; s < QST; ++s) {
       mbar_init(q_full(s), 1);
-      mbar_init(q_empty(s), 1 + 8);  // the MMAs' commit and the compute warps' stat reads
+      mbar_init(q_empty(s), 1 + kBwdWarps);  // the MMAs' commit, the warps' stat reads
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full(i), 1);
-      mbar_init(s_free(i), 8);
-      mbar_init(pds_ready(i), 8);
+      mbar_init(s_free(i), kBwdWarps);
+      mbar_init(pds_ready(i), kBwdWarps);
       mbar_init(item_full(i), 1);
-      mbar_init(item_empty(i), kReaders);
+      mbar_init(item_empty(i), kBwdReaders);
     }
     mbar_init(acc_full, 1);
-    mbar_init(acc_free, 8);
+    mbar_init(acc_free, kBwdWarps);
     mbar_init(taken, 1);
     fence_mbar_init();
   }
@@ -1518,10 +1517,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------ compute warps
-    // Two warpgroups on the same 128 key rows: warps 4-7 take query columns
-    // 0-31 of each 64-query tile, warps 8-11 columns 32-63; likewise halves
-    // of the dV and dK rows at the end.
-    const int half = (warp - 4) >> 2;
+    // Four warpgroups on the same 128 key rows, 16 of each tile's 64 query
+    // columns each; likewise quarters of the dV and dK rows at the end.
+    const int part = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
@@ -1538,50 +1536,51 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
       const int T = subs * it.nq;
       const size_t tile0 = static_cast<size_t>(it.b) * sh.tiles64 + it.i0;
       const int key0 = it.kv0 + quad * 32;  // the warp's 32 keys
-      // A query tile's spans, a lane each, loaded a tile ahead (tile t % nq).
-      const int2* const spans = p.work.rows + tile0 * kHalf + half * 32 + lane;
+      // The part's 16 spans, two lanes each, loaded a tile ahead (tile t % nq).
+      const int2* const spans = p.work.rows + tile0 * kHalf + part * 16 + (lane & 15);
       int ahead = 0;
       int2 nsp = T > 0 ? spans[0] : make_int2(0, 0);
       for (int t = 0; t < T; ++t, ++g) {
         const int s = g % QST;
-        // Which of the tile's queries see which of the warp's keys, a bit each:
-        // lane i turns its query's span into bits of the keys, the transpose
-        // gives each key's queries.
+        // Which of the tile's queries see which of the warp's keys: all, none,
+        // or a bit each (lane i turns its query's span into bits of the keys,
+        // the transpose gives each key's queries).
         const int2 sp = nsp;
         if (++ahead == it.nq) ahead = 0;
         nsp = spans[static_cast<size_t>(ahead) * kHalf];
         const int from = min(max(sp.x - key0, 0), 32);
-        const uint32_t seen =
-            transpose_bits(bit_range(from, min(max(sp.x + sp.y - key0, 0), 32)));
-        const bool none = !__any_sync(0xffffffffu, seen != 0);
+        const int to = min(max(sp.x + sp.y - key0, 0), 32);
+        const bool none = !__any_sync(0xffffffffu, from < to);
+        const bool some = !__all_sync(0xffffffffu, from == 0 && to == 32);
+        const uint32_t seen = !none && some ? transpose_bits(bit_range(from, to)) : 0;
         ok = mbar_wait(s_full(g & 1), (g >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        uint32_t sv[32], dv[32];
+        uint32_t sv[16], dv[16];
         if (!none) {
-          tmem_ld_32x32b_x32(lrow + C::S_COL + (g & 1) * kHalf + half * 32, sv);
-          tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + half * 32, dv);
+          tmem_ld_32x32b_x16(lrow + C::S_COL + (g & 1) * kHalf + part * 16, sv);
+          tmem_ld_32x32b_x16(lrow + C::DP_COL + (g & 1) * kHalf + part * 16, dv);
           tmem_ld_wait();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free(g & 1));
-        uint32_t pk[16], dk[16];
+        uint32_t pk[8], dk[8];
         if (none) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = dk[e] = 0;
+          for (int e = 0; e < 8; ++e) pk[e] = dk[e] = 0;
         } else {
-          if (!__all_sync(0xffffffffu, seen == 0xFFFFFFFFu)) {
+          if (some) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 16; ++e)
               if (!(seen >> e & 1)) sv[e] = 0xFF800000u;  // P = 0
           }
           // The query tile's statistics (landed with its Q and dO).
           ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
           if (!ok) break;
-          const float* st = reinterpret_cast<const float*>(gbase + (stat_s(s) - base)) + half * 32;
+          const float* st = reinterpret_cast<const float*>(gbase + (stat_s(s) - base)) + part * 16;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
+          for (int e = 0; e < 16; e += 4) {
             const float4 l4 = *reinterpret_cast<const float4*>(st + e);
             const float4 d4 = *reinterpret_cast<const float4*>(st + kHalf + e);
             const F2 pa = exp2_mufu(fma2(pair_of(sv[e], sv[e + 1]), c2, f2(l4.x, l4.y)));
@@ -1598,13 +1597,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty(s));
         // Row `row` of the K-major operand: 64 bf16 = eight 16-byte chunks,
-        // chunk ch stored at ch ^ (row & 7) (the 128-byte swizzle); this half
-        // writes chunks 4 half .. 4 half + 3.
+        // chunk ch stored at ch ^ (row & 7) (the 128-byte swizzle); this part
+        // writes chunks 2 part and 2 part + 1.
         const uint32_t prow = p_s(g & 1) + row * 128;
         const uint32_t drow = ds_s(g & 1) + row * 128;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-          const uint32_t off = static_cast<uint32_t>(((4 * half + q4) ^ (row & 7)) * 16);
+        for (int q4 = 0; q4 < 2; ++q4) {
+          const uint32_t off = static_cast<uint32_t>(((2 * part + q4) ^ (row & 7)) * 16);
           sts128(prow + off, pk[4 * q4], pk[4 * q4 + 1], pk[4 * q4 + 2], pk[4 * q4 + 3]);
           sts128(drow + off, dk[4 * q4], dk[4 * q4 + 1], dk[4 * q4 + 2], dk[4 * q4 + 3]);
         }
@@ -1628,24 +1627,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1)
         const float f = which == 0 ? 1.0f : p.scale;
         const F2 ff = f2(f, f);
         uint16_t* orow = (which == 0 ? p.dv : p.dk) + roff;
-#pragma unroll
-        for (int e = 0; e < D / 64; ++e) {
-          const int c4 = half * (D / 64) + e;
-          uint32_t o[32];
-          uint32_t w[16] = {};
-          if (T > 0) {
-            tmem_ld_32x32b_x32(lrow + col + c4 * 32, o);
-            tmem_ld_wait();
-            if (which == 1 && e == D / 64 - 1) {  // dV and dK may begin again
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(acc_free);
-            }
-#pragma unroll
-            for (int q = 0; q < 16; ++q) w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * ff);
+        constexpr int COLS = D / 4;
+        uint32_t o[COLS];
+        uint32_t w[COLS / 2] = {};
+        if (T > 0) {
+          tmem_ld_cols(lrow + col + part * COLS, o);
+          tmem_ld_wait();
+          if (which == 1) {  // dV and dK may begin again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_free);
           }
-          if (valid) store_row32(orow + c4 * 32, w, wide);
+#pragma unroll
+          for (int q = 0; q < COLS / 2; ++q) w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * ff);
         }
+        if (valid) store_row(orow + part * COLS, w, wide);
       }
     }
   }
@@ -1852,7 +1848,7 @@ int launch_fwd(const void* q, const void* k, const void* v, FwdParams p, cudaStr
   if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
   p.n_pairs = (sh.tiles128 + 1) / 2;
   const unsigned grid = static_cast<unsigned>(sh.batch) * (sh.heads / sh.pack) * p.n_pairs;
-  return launch_kernel(span_fwd_kernel<D>, dim3(grid), dim3(kAttnThreads), C::SMEM,
+  return launch_kernel(span_fwd_kernel<D>, dim3(grid), dim3(kFwdThreads), C::SMEM,
                        stream, 1, "span attention forward launch", tq_, tk, tv, p);
 }
 
@@ -1897,11 +1893,11 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
                      "span attention backward prep launch", pp);
   if (rc) return rc;
   const unsigned grid_q = static_cast<unsigned>(sh.batch) * (sh.heads / sh.pack) * sh.tiles128;
-  rc = launch_kernel(span_dq_kernel<D>, dim3(grid_q), dim3(kAttnThreads), Q::SMEM,
+  rc = launch_kernel(span_dq_kernel<D>, dim3(grid_q), dim3(kBwdThreads), Q::SMEM,
                      stream, 1, "span attention backward dq launch", q128, do128, k64, v64, p);
   if (rc) return rc;
   const unsigned grid_kv = static_cast<unsigned>(sh.batch) * sh.kv_heads * sh.key_tiles;
-  return launch_kernel(span_dkv_kernel<D>, dim3(grid_kv), dim3(kAttnThreads), KV::SMEM,
+  return launch_kernel(span_dkv_kernel<D>, dim3(grid_kv), dim3(kBwdThreads), KV::SMEM,
                        stream, 1, "span attention backward dkv launch", q64, do64, k128, v128, p);
 }
 
