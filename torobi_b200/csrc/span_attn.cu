@@ -40,8 +40,10 @@ namespace tq {
 namespace {
 
 constexpr int kFwdThreads = 384;  // four warps of roles, eight of softmax
-constexpr int kBwdWarps = 16;     // that compute, beside the four of roles
+constexpr int kBwdWarps = 8;      // that compute, beside the four of roles
 constexpr int kBwdThreads = 128 + 32 * kBwdWarps;
+constexpr int kParts = kBwdWarps / 4;     // of a streamed 64-wide tile's columns
+constexpr int kPartCols = kHalf / kParts;
 // Who reads a tile's description: TMA, MMA and every computing warp.
 constexpr int kFwdReaders = 2 + 8;
 constexpr int kBwdReaders = 2 + kBwdWarps;
@@ -164,13 +166,6 @@ __device__ __forceinline__ void store_row(uint16_t* dst, const uint32_t (&w)[N],
     for (int i = 0; i < N; i += 4)
       *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   }
-}
-
-__device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[32]) {
-  tmem_ld_32x32b_x32(at, r);
-}
-__device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[16]) {
-  tmem_ld_32x32b_x16(at, r);
 }
 
 __device__ __forceinline__ bool wide_rows(const void* p) {
@@ -701,16 +696,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //   prep   per packed query row -lse log2(e) and -delta (f32), in 64-row packed
 //          tiles (rows that hold nothing: -inf and 0, so their probabilities
 //          are 0), each row's span in the same order, and each tile's spans;
-//   dq     a tile of work is a packed 128-row query tile, key tiles of 64 (four
-//          compute warpgroups, each 16 of every tile's columns):
+//   dq     a tile of work is a packed 128-row query tile, key tiles of 64:
 //            S = Q K_j^T, dP = dO V_j^T (tensor memory, double-buffered),
 //            dS = P * (dP - delta), P = exp2(S c - lse2)  (compute warps),
 //            dQ += dS K_j  (dS written back to tensor memory, A from TMEM);
 //   dkv    a tile of work is a 128-key tile of one key/value head, with the
-//          packed 64-row query tiles that see it (four compute warpgroups,
-//          each 16 of every tile's columns):
-//            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, into
-//            shared memory as K-major operands), dV += P^T dO_i, dK += dS^T Q_i.
+//          packed 64-row query tiles that see it:
+//            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, back
+//            into tensor memory), dV += P^T dO_i, dK += dS^T Q_i.
+//          What bounds it is shared memory's 128 bytes a cycle, which feed the
+//          tensor cores: K and Q, V and dO, dO and Q again, 128 KB a tile
+//          and 32 KB of copies -- 1280 cycles; with P^T and dS^T as operands
+//          there too it was 1800.
 // Which CTA does a tile changes no result.
 
 // Over a 64-row packed query tile: the keys that any row sees, [lo, hi), and
@@ -1096,9 +1093,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------ compute warps
-    // Four warpgroups on the same 128 rows, 16 of each tile's 64 key columns
-    // each (the gradient is elementwise given the row's lse and delta);
-    // likewise quarters of dQ.
+    // The warpgroups share the 128 rows and split each tile's 64 key columns
+    // (the gradient is elementwise given the row's lse and delta), and dQ's
+    // columns at the end.  Two of them: four (96 registers a thread) took 97 us
+    // where two take 94.
     const int part = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
@@ -1144,35 +1142,35 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = mbar_wait(s_full(g & 1), (g >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        const int k0 = (it.kv0 + j) * kHalf + part * 16;
-        const bool none = k0 + 16 <= any_lo || k0 >= any_hi;
-        uint32_t sv[16], dv[16];
+        const int k0 = (it.kv0 + j) * kHalf + part * kPartCols;
+        const bool none = k0 + kPartCols <= any_lo || k0 >= any_hi;
+        uint32_t sv[kPartCols], dv[kPartCols];
         if (!none) {
-          tmem_ld_32x32b_x16(lrow + C::S_COL + (g & 1) * kHalf + part * 16, sv);
-          tmem_ld_32x32b_x16(lrow + C::DP_COL + (g & 1) * kHalf + part * 16, dv);
+          tmem_ld_32x32b_x32(lrow + C::S_COL + (g & 1) * kHalf + part * kPartCols, sv);
+          tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + part * kPartCols, dv);
           tmem_ld_wait();
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free(g & 1));
-        uint32_t pk[8];
+        uint32_t pk[kPartCols / 2];
         if (none) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) pk[e] = 0;
+          for (int e = 0; e < kPartCols / 2; ++e) pk[e] = 0;
         } else {
-          if (k0 < all_lo || k0 + 16 > all_hi) {
+          if (k0 < all_lo || k0 + kPartCols > all_hi) {
             const int col0 = k0 - sp.lo;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
+            for (int e = 0; e < kPartCols; ++e)
               if (static_cast<unsigned>(col0 + e) >= len) sv[e] = 0xFF800000u;  // P = 0
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
+          for (int e = 0; e < kPartCols / 2; ++e) {
             const F2 q = exp2_mufu(fma2(pair_of(sv[2 * e], sv[2 * e + 1]), c2, shift));
             pk[e] = pack_bf16(q * (pair_of(dv[2 * e], dv[2 * e + 1]) + nd));
           }
         }
-        tmem_st_32x32b_x8(lrow + C::DS_COL + (g & 1) * 32 + part * 8, pk);
+        tmem_st_32x32b_x16(lrow + C::DS_COL + (g & 1) * 32 + part * (kPartCols / 2), pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -1193,20 +1191,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         ++n;
       }
-      constexpr int COLS = D / 4;
-      uint32_t o[COLS];
-      uint32_t w[COLS / 2] = {};
-      if (it.n_kv > 0) {
-        tmem_ld_cols(lrow + C::DQ_COL + part * COLS, o);
-        tmem_ld_wait();
-        tc_fence_before();  // dQ may be begun again
-        __syncwarp();
-        if (lane == 0) mbar_arrive(dq_free);
+      constexpr int COLS = D / kParts < 32 ? D / kParts : 32;
 #pragma unroll
-        for (int q = 0; q < COLS / 2; ++q)
-          w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * scale2);
+      for (int e = 0; e < D / kParts / COLS; ++e) {
+        const int c0 = part * (D / kParts) + e * COLS;
+        uint32_t o[COLS];
+        uint32_t w[COLS / 2] = {};
+        if (it.n_kv > 0) {
+          tmem_ld_32x32b_x32(lrow + C::DQ_COL + c0, o);
+          tmem_ld_wait();
+          if (e == D / kParts / COLS - 1) {  // dQ may be begun again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(dq_free);
+          }
+#pragma unroll
+          for (int q = 0; q < COLS / 2; ++q)
+            w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * scale2);
+        }
+        if (valid) store_row(orow + c0, w, wide);
       }
-      if (valid) store_row(orow + part * COLS, w, wide);
       it = nx;
       st = nst;
     }
@@ -1234,25 +1238,25 @@ struct DkvCfg {
   static constexpr int KTILE = SLABS * KSLAB;
   static constexpr int QSLAB = kHalf * 128;  // Q_i, dO_i: 64 rows x 64 bf16
   static constexpr int QTILE = SLABS * QSLAB;
-  static constexpr int PTILE = kTile * 128;  // P^T or dS^T: 128 key rows x 64 queries bf16
-  static constexpr int QST = D == 128 ? 3 : 6;
+  static constexpr int QST = D == 128 ? 4 : 8;
   static constexpr int STAT_BYTES = 2 * kHalf * 4;  // the statistics of one query tile
   static constexpr int K_OFF = 0;
   static constexpr int V_OFF = KTILE;
   static constexpr int Q_OFF = 2 * KTILE;
   static constexpr int DO_OFF = Q_OFF + QST * QTILE;
-  static constexpr int P_OFF = DO_OFF + QST * QTILE;
-  static constexpr int DS_OFF = P_OFF + 2 * PTILE;
-  static constexpr int STAT_OFF = DS_OFF + 2 * PTILE;
+  static constexpr int STAT_OFF = DO_OFF + QST * QTILE;
   static constexpr int ITEM_OFF = STAT_OFF + QST * STAT_BYTES;
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DkvItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
-  // kv_full, kv_empty, q_full[QST], q_empty[QST], s_full[2], s_free[2], pds_ready[2],
-  // acc_full, acc_free, item_full[2], item_empty[2], taken; then the TMEM slot
-  static constexpr int NBAR = 2 + 2 * QST + 13;
+  // kv_full, kv_empty, q_full[QST], q_empty[QST], s_full[2], pds_ready[2], acc_full,
+  // acc_free, item_full[2], item_empty[2], taken; then the TMEM slot
+  static constexpr int NBAR = 2 + 2 * QST + 11;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
-  static constexpr int S_COL = 0;     // S^T_b at 64 b
-  static constexpr int DP_COL = 128;  // dP^T_b at 128 + 64 b
+  // S^T_b at 64 b and dP^T_b at 128 + 64 b; P^T_b and dS^T_b (bf16 pairs) over
+  // them, each 16 queries in the first 8 of those queries' 16 columns, so that
+  // a warp writes only over what it has read.
+  static constexpr int S_COL = 0;
+  static constexpr int DP_COL = 128;
   static constexpr int DV_COL = 256;
   static constexpr int DK_COL = 256 + D;
   static constexpr int TMEM_COLS = 512;
@@ -1297,8 +1301,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   const uint32_t v_s = base + C::V_OFF;
   auto q_s = [&](int s) { return base + C::Q_OFF + s * C::QTILE; };
   auto do_s = [&](int s) { return base + C::DO_OFF + s * C::QTILE; };
-  auto p_s = [&](int b) { return base + C::P_OFF + b * C::PTILE; };
-  auto ds_s = [&](int b) { return base + C::DS_OFF + b * C::PTILE; };
   auto stat_s = [&](int s) { return base + C::STAT_OFF + s * C::STAT_BYTES; };
   const uint32_t bars = base + C::BAR_OFF;
   const uint32_t kv_full = bars, kv_empty = bars + 8u;
@@ -1306,12 +1308,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   auto q_empty = [&](int s) { return bars + 8u * (2 + QST + s); };
   constexpr int X = 2 + 2 * QST;
   auto s_full = [&](int b) { return bars + 8u * (X + b); };
-  auto s_free = [&](int b) { return bars + 8u * (X + 2 + b); };
-  auto pds_ready = [&](int b) { return bars + 8u * (X + 4 + b); };
-  const uint32_t acc_full = bars + 8u * (X + 6), acc_free = bars + 8u * (X + 7);
-  auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
-  auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
-  const uint32_t taken = bars + 8u * (X + 12);
+  auto pds_ready = [&](int b) { return bars + 8u * (X + 2 + b); };
+  const uint32_t acc_full = bars + 8u * (X + 4), acc_free = bars + 8u * (X + 5);
+  auto item_full = [&](int i) { return bars + 8u * (X + 6 + i); };
+  auto item_empty = [&](int i) { return bars + 8u * (X + 8 + i); };
+  const uint32_t taken = bars + 8u * (X + 10);
   const uint32_t tmem_slot = bars + 8u * C::NBAR;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
@@ -1332,7 +1333,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full(i), 1);
-      mbar_init(s_free(i), kBwdWarps);
       mbar_init(pds_ready(i), kBwdWarps);
       mbar_init(item_full(i), 1);
       mbar_init(item_empty(i), kBwdReaders);
@@ -1424,8 +1424,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mbar_arrive(item_empty(i & 1));
           continue;
         }
-        // dV += P^T_t dO_t and dK += dS^T_t Q_t: A K-major from shared memory,
-        // B MN-major (N = dim, K = the tile's 64 queries).
+        // dV += P^T_t dO_t and dK += dS^T_t Q_t: A from tensor memory, B
+        // MN-major (N = dim, K = the tile's 64 queries).
         auto issue_acc = [&](int t, bool begin) -> bool {
           if (!mbar_wait(pds_ready(t & 1), (t >> 1) & 1, p.status)) return false;
           // The last item's dV and dK have been read before they begin again.
@@ -1434,14 +1434,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int s = t % QST;
 #pragma unroll
           for (int kk = 0; kk < kHalf / 16; ++kk)
-            umma_bf16(tmem + C::DV_COL, make_sdesc(p_s(t & 1) + kk * 32, 16, 1024, kSw128),
-                      make_sdesc(do_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
-                      (!begin || kk > 0) ? 1u : 0u);
+            umma_bf16_ts(tmem + C::DV_COL, tmem + C::S_COL + (t & 1) * kHalf + kk * 16,
+                         make_sdesc(do_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
+                         (!begin || kk > 0) ? 1u : 0u);
 #pragma unroll
           for (int kk = 0; kk < kHalf / 16; ++kk)
-            umma_bf16(tmem + C::DK_COL, make_sdesc(ds_s(t & 1) + kk * 32, 16, 1024, kSw128),
-                      make_sdesc(q_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
-                      (!begin || kk > 0) ? 1u : 0u);
+            umma_bf16_ts(tmem + C::DK_COL, tmem + C::DP_COL + (t & 1) * kHalf + kk * 16,
+                         make_sdesc(q_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
+                         (!begin || kk > 0) ? 1u : 0u);
           umma_commit(q_empty(s));
           return true;
         };
@@ -1450,8 +1450,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int s = g % QST;
           // Four query tiles before the end it is time to look for the next item.
           if (t == max(T - 4, 0)) mbar_arrive(item_empty(i & 1));
-          ok = mbar_wait(q_full(s), (g / QST) & 1, p.status) &&
-               (g < 2 || mbar_wait(s_free(g & 1), ((g - 2) >> 1) & 1, p.status));
+          // S^T_g and dP^T_g go over P^T and dS^T of two tiles ago, whose
+          // products were issued before.
+          ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sd = tmem + C::S_COL + (g & 1) * kHalf;
@@ -1517,8 +1518,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------ compute warps
-    // Four warpgroups on the same 128 key rows, 16 of each tile's 64 query
-    // columns each; likewise quarters of the dV and dK rows at the end.
+    // The warpgroups share the 128 key rows and split each tile's 64 query
+    // columns, and dV's and dK's columns at the end.
     const int part = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
@@ -1536,8 +1537,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int T = subs * it.nq;
       const size_t tile0 = static_cast<size_t>(it.b) * sh.tiles64 + it.i0;
       const int key0 = it.kv0 + quad * 32;  // the warp's 32 keys
-      // The part's 16 spans, two lanes each, loaded a tile ahead (tile t % nq).
-      const int2* const spans = p.work.rows + tile0 * kHalf + part * 16 + (lane & 15);
+      // The part's spans, a lane each, loaded a tile ahead (tile t % nq).
+      const int2* const spans =
+          p.work.rows + tile0 * kHalf + part * kPartCols + (lane & (kPartCols - 1));
       int ahead = 0;
       int2 nsp = T > 0 ? spans[0] : make_int2(0, 0);
       for (int t = 0; t < T; ++t, ++g) {
@@ -1556,39 +1558,40 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = mbar_wait(s_full(g & 1), (g >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        uint32_t sv[16], dv[16];
+        const uint32_t scol = lrow + C::S_COL + (g & 1) * kHalf + part * kPartCols;
+        const uint32_t dcol = lrow + C::DP_COL + (g & 1) * kHalf + part * kPartCols;
+        uint32_t sv[kPartCols], dv[kPartCols];
         if (!none) {
-          tmem_ld_32x32b_x16(lrow + C::S_COL + (g & 1) * kHalf + part * 16, sv);
-          tmem_ld_32x32b_x16(lrow + C::DP_COL + (g & 1) * kHalf + part * 16, dv);
+          tmem_ld_32x32b_x32(scol, sv);
+          tmem_ld_32x32b_x32(dcol, dv);
           tmem_ld_wait();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free(g & 1));
-        uint32_t pk[8], dk[8];
+        uint32_t pk[kPartCols / 16][8], dk[kPartCols / 16][8];  // by 16 queries
         if (none) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) pk[e] = dk[e] = 0;
+          for (int e = 0; e < kPartCols / 2; ++e) pk[e / 8][e % 8] = dk[e / 8][e % 8] = 0;
         } else {
           if (some) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
+            for (int e = 0; e < kPartCols; ++e)
               if (!(seen >> e & 1)) sv[e] = 0xFF800000u;  // P = 0
           }
           // The query tile's statistics (landed with its Q and dO).
           ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
           if (!ok) break;
-          const float* st = reinterpret_cast<const float*>(gbase + (stat_s(s) - base)) + part * 16;
+          const float* st = reinterpret_cast<const float*>(gbase + (stat_s(s) - base)) + part * kPartCols;
 #pragma unroll
-          for (int e = 0; e < 16; e += 4) {
+          for (int e = 0; e < kPartCols; e += 4) {
             const float4 l4 = *reinterpret_cast<const float4*>(st + e);
             const float4 d4 = *reinterpret_cast<const float4*>(st + kHalf + e);
             const F2 pa = exp2_mufu(fma2(pair_of(sv[e], sv[e + 1]), c2, f2(l4.x, l4.y)));
             const F2 pb = exp2_mufu(fma2(pair_of(sv[e + 2], sv[e + 3]), c2, f2(l4.z, l4.w)));
-            pk[e / 2] = pack_bf16(pa);
-            pk[e / 2 + 1] = pack_bf16(pb);
-            dk[e / 2] = pack_bf16(pa * (pair_of(dv[e], dv[e + 1]) + f2(d4.x, d4.y)));
-            dk[e / 2 + 1] = pack_bf16(pb * (pair_of(dv[e + 2], dv[e + 3]) + f2(d4.z, d4.w)));
+            uint32_t(&pq)[8] = pk[e / 16];
+            uint32_t(&dq)[8] = dk[e / 16];
+            pq[e % 16 / 2] = pack_bf16(pa);
+            pq[e % 16 / 2 + 1] = pack_bf16(pb);
+            dq[e % 16 / 2] = pack_bf16(pa * (pair_of(dv[e], dv[e + 1]) + f2(d4.x, d4.y)));
+            dq[e % 16 / 2 + 1] = pack_bf16(pb * (pair_of(dv[e + 2], dv[e + 3]) + f2(d4.z, d4.w)));
           }
           // The stat reads above are ordered before the copies that refill
           // the stage (generic-proxy reads, async-proxy writes).
@@ -1596,18 +1599,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(q_empty(s));
-        // Row `row` of the K-major operand: 64 bf16 = eight 16-byte chunks,
-        // chunk ch stored at ch ^ (row & 7) (the 128-byte swizzle); this part
-        // writes chunks 2 part and 2 part + 1.
-        const uint32_t prow = p_s(g & 1) + row * 128;
-        const uint32_t drow = ds_s(g & 1) + row * 128;
 #pragma unroll
-        for (int q4 = 0; q4 < 2; ++q4) {
-          const uint32_t off = static_cast<uint32_t>(((2 * part + q4) ^ (row & 7)) * 16);
-          sts128(prow + off, pk[4 * q4], pk[4 * q4 + 1], pk[4 * q4 + 2], pk[4 * q4 + 3]);
-          sts128(drow + off, dk[4 * q4], dk[4 * q4 + 1], dk[4 * q4 + 2], dk[4 * q4 + 3]);
+        for (int e = 0; e < kPartCols / 16; ++e) {
+          tmem_st_32x32b_x8(scol + 16 * e, pk[e]);
+          tmem_st_32x32b_x8(dcol + 16 * e, dk[e]);
         }
-        fence_proxy_async_smem();
+        tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(pds_ready(g & 1));
       }
@@ -1627,21 +1625,26 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const float f = which == 0 ? 1.0f : p.scale;
         const F2 ff = f2(f, f);
         uint16_t* orow = (which == 0 ? p.dv : p.dk) + roff;
-        constexpr int COLS = D / 4;
-        uint32_t o[COLS];
-        uint32_t w[COLS / 2] = {};
-        if (T > 0) {
-          tmem_ld_cols(lrow + col + part * COLS, o);
-          tmem_ld_wait();
-          if (which == 1) {  // dV and dK may begin again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_free);
-          }
+        constexpr int COLS = D / kParts < 32 ? D / kParts : 32;
 #pragma unroll
-          for (int q = 0; q < COLS / 2; ++q) w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * ff);
+        for (int e = 0; e < D / kParts / COLS; ++e) {
+          const int c0 = part * (D / kParts) + e * COLS;
+          uint32_t o[COLS];
+          uint32_t w[COLS / 2] = {};
+          if (T > 0) {
+            tmem_ld_32x32b_x32(lrow + col + c0, o);
+            tmem_ld_wait();
+            if (which == 1 && e == D / kParts / COLS - 1) {  // dV and dK may begin again
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(acc_free);
+            }
+#pragma unroll
+            for (int q = 0; q < COLS / 2; ++q)
+              w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * ff);
+          }
+          if (valid) store_row(orow + c0, w, wide);
         }
-        if (valid) store_row(orow + part * COLS, w, wide);
       }
     }
   }
