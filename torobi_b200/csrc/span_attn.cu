@@ -1659,9 +1659,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 }
 
 // --------------------------------------------------------- document spans --
+//
+// One CTA per row of ids.  A document is a run of equal ids: a position's run
+// starts at the last start at or before it and ends before the first one
+// behind it.  A warp holds 256 positions in eight coalesced words a lane; a
+// vote a word gives where runs start, bit operations the nearest start of a
+// lane, and one value a warp in shared memory joins the warps.  A row longer
+// than a stretch of 8192 goes stretch by stretch, from the front for the
+// starts and from the back for the ends.
 
-constexpr int kScanThreads = 1024;
-constexpr int kScanItems = 8;
+constexpr int kDocWarps = 32;
+constexpr int kDocWords = 8;
+constexpr int kStretch = kDocWarps * kDocWords * 32;
 
 struct DocParams {
   const void* documents;
@@ -1671,116 +1680,108 @@ struct DocParams {
   int* last;
 };
 
-// Inclusive scan over a warp's lanes: the running maximum from the front, or
-// the running minimum from the back.
-template <bool BACK>
-__device__ __forceinline__ int scan_lanes(int v) {
+// A warp's positions [i0, i0 + 256) of a row: bit l of starts[e] says whether a
+// run starts at i0 + 32 e + l, bit l of pads[e] whether padding is there.
+struct DocWords {
+  uint32_t starts[kDocWords], pads[kDocWords];
+};
+
+template <typename I>
+__device__ __forceinline__ DocWords read_words(const I* ids, int i0, int seq) {
   const int lane = threadIdx.x & 31;
+  I v[kDocWords];
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const int o = BACK ? __shfl_down_sync(0xffffffffu, v, off) : __shfl_up_sync(0xffffffffu, v, off);
-    if (BACK ? lane + off < 32 : lane >= off) v = BACK ? min(v, o) : max(v, o);
+  for (int e = 0; e < kDocWords; ++e) v[e] = i0 + 32 * e + lane < seq ? ids[i0 + 32 * e + lane] : 0;
+  I before = i0 > 0 && i0 <= seq ? ids[i0 - 1] : 0;  // the position ahead of the warp's
+  DocWords w;
+#pragma unroll
+  for (int e = 0; e < kDocWords; ++e) {
+    const int i = i0 + 32 * e + lane;
+    I prev = __shfl_up_sync(0xffffffffu, v[e], 1);
+    if (lane == 0) prev = before;
+    before = __shfl_sync(0xffffffffu, v[e], 31);
+    w.starts[e] = __ballot_sync(0xffffffffu, i < seq && (i == 0 || v[e] != prev));
+    w.pads[e] = __ballot_sync(0xffffffffu, v[e] < 0);
   }
-  return v;
+  return w;
 }
 
-// The same over the block's threads, exclusive (rest: what the first, or
-// last, thread gets); the whole block's result goes to all.
-template <bool BACK>
-__device__ __forceinline__ int scan_threads(int v, int rest, int* sh, int& all) {
-  static_assert(kScanThreads == 1024, "one total a lane");
+template <typename I>
+__device__ void document_spans(const DocParams& p) {
+  __shared__ int sh[kDocWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto join = [](int a, int b) { return BACK ? min(a, b) : max(a, b); };
-  v = scan_lanes<BACK>(v);
-  __syncthreads();  // the last call's reads of sh
-  if (lane == (BACK ? 0 : 31)) sh[warp] = v;
-  __syncthreads();
-  const int totals = scan_lanes<BACK>(sh[lane]);
-  all = join(__shfl_sync(0xffffffffu, totals, BACK ? 0 : 31), rest);
-  const int warps = __shfl_sync(0xffffffffu, totals, BACK ? (warp + 1) & 31 : (warp + 31) & 31);
-  int in = BACK ? __shfl_down_sync(0xffffffffu, v, 1) : __shfl_up_sync(0xffffffffu, v, 1);
-  if (lane == (BACK ? 31 : 0)) in = rest;
-  if (warp != (BACK ? 31 : 0)) in = join(in, warps);
-  return join(in, rest);
-}
-
-// One CTA per row of ids.  A document is a run of equal ids: its start reaches
-// its positions by a running maximum of the runs' starts from the front, its
-// end by a running minimum from the back, stretch by stretch.
-__global__ void __launch_bounds__(kScanThreads) document_spans_kernel(const DocParams p) {
-  griddep_wait();
-  griddep_launch_dependents();
-  __shared__ int sh[kScanThreads / 32];
   const int64_t base = static_cast<int64_t>(blockIdx.x) * p.seq;
-  auto id = [&](int i) -> int64_t {
-    return p.ids64 ? static_cast<const int64_t*>(p.documents)[base + i]
-                   : static_cast<const int*>(p.documents)[base + i];
-  };
-  constexpr int kStretch = kScanThreads * kScanItems;
+  const I* const ids = static_cast<const I*>(p.documents) + base;
+  const uint32_t upto = 0xFFFFFFFFu >> (31 - lane);  // this lane and those below
   const int stretches = (p.seq + kStretch - 1) / kStretch;
   const bool ends = !p.causal || p.prefix;
   int from = 0;  // the start of the run that reaches into the stretch
   for (int s = 0; s < stretches; ++s) {
-    const int i0 = s * kStretch + threadIdx.x * kScanItems;
-    int start[kScanItems];
-    bool padding[kScanItems];
-    int run = 0;
-    int64_t prev = i0 > 0 && i0 <= p.seq ? id(i0 - 1) : 0;
+    const int i0 = s * kStretch + warp * (kDocWords * 32);
+    const DocWords w = read_words(ids, i0, p.seq);
+    int latest = -1;
 #pragma unroll
-    for (int e = 0; e < kScanItems; ++e) {
-      const int i = i0 + e;
-      padding[e] = true;
-      if (i < p.seq) {
-        const int64_t now = id(i);
-        padding[e] = now < 0;
-        if (i == 0 || now != prev) run = i;
-        prev = now;
-      }
-      start[e] = run;
-    }
-    const int in = scan_threads<false>(run, from, sh, from);
+    for (int e = 0; e < kDocWords; ++e)
+      if (w.starts[e]) latest = i0 + 32 * e + 31 - __clz(w.starts[e]);
+    __syncthreads();  // the last stretch's reads
+    if (lane == 0) sh[warp] = latest;
+    __syncthreads();
+    int in = max(__reduce_max_sync(0xffffffffu, lane < warp ? sh[lane] : -1), from);
+    from = max(__reduce_max_sync(0xffffffffu, sh[lane]), from);
 #pragma unroll
-    for (int e = 0; e < kScanItems; ++e) {
-      const int i = i0 + e;
+    for (int e = 0; e < kDocWords; ++e) {
+      const int i = i0 + 32 * e + lane;
+      const uint32_t mine = w.starts[e] & upto;
+      const int start = mine ? i0 + 32 * e + 31 - __clz(mine) : in;
+      if (w.starts[e]) in = i0 + 32 * e + 31 - __clz(w.starts[e]);
       if (i >= p.seq) continue;
-      p.first[base + i] = max(start[e], in);
-      if (!ends || padding[e]) p.last[base + i] = padding[e] ? max(start[e], in) : i + 1;
+      const bool pad = w.pads[e] >> lane & 1;
+      p.first[base + i] = start;
+      if (!ends || pad) p.last[base + i] = pad ? start : i + 1;
     }
   }
   if (!ends) return;
   int next = p.seq;  // the start of the run after the stretch's last
   for (int s = stretches - 1; s >= 0; --s) {
-    const int i0 = s * kStretch + threadIdx.x * kScanItems;
-    int end[kScanItems];
-    bool padding[kScanItems];
-    int run = p.seq;
-    int64_t after = i0 + kScanItems < p.seq ? id(i0 + kScanItems) : 0;
+    const int i0 = s * kStretch + warp * (kDocWords * 32);
+    const DocWords w = read_words(ids, i0, p.seq);
+    int prefix[kDocWords], first[kDocWords];
 #pragma unroll
-    for (int e = kScanItems - 1; e >= 0; --e) {
-      const int i = i0 + e;
-      padding[e] = true;
-      if (i < p.seq) {
-        const int64_t now = id(i);
-        padding[e] = now < 0;
-        if (i + 1 < p.seq && now != after) run = i + 1;
-        after = now;
-      }
-      end[e] = run;
+    for (int e = 0; e < kDocWords; ++e) {
+      const int i = i0 + 32 * e + lane;
+      first[e] = i < p.seq ? p.first[base + i] : 0;  // this thread wrote it
+      prefix[e] = p.prefix && i < p.seq ? max(p.prefix[base + i], 0) : 0;
     }
-    const int in = scan_threads<true>(run, next, sh, next);
+    int earliest = INT_MAX;
 #pragma unroll
-    for (int e = 0; e < kScanItems; ++e) {
-      const int i = i0 + e;
-      if (i >= p.seq || padding[e]) continue;
-      const int stop = min(end[e], in);
-      int last = stop;
-      if (p.causal) {
-        const int64_t seen = static_cast<int64_t>(p.first[base + i]) + max(p.prefix[base + i], 0);
-        last = max(i + 1, seen < stop ? static_cast<int>(seen) : stop);
-      }
-      p.last[base + i] = last;
+    for (int e = kDocWords - 1; e >= 0; --e)
+      if (w.starts[e]) earliest = i0 + 32 * e + __ffs(w.starts[e]) - 1;
+    __syncthreads();
+    if (lane == 0) sh[warp] = earliest;
+    __syncthreads();
+    int in = min(__reduce_min_sync(0xffffffffu, lane > warp ? sh[lane] : INT_MAX), next);
+    next = min(__reduce_min_sync(0xffffffffu, sh[lane]), next);
+#pragma unroll
+    for (int e = kDocWords - 1; e >= 0; --e) {
+      const int i = i0 + 32 * e + lane;
+      const uint32_t behind = w.starts[e] & ~upto;
+      const int stop = behind ? i0 + 32 * e + __ffs(behind) - 1 : in;
+      if (w.starts[e]) in = i0 + 32 * e + __ffs(w.starts[e]) - 1;
+      if (i >= p.seq || (w.pads[e] >> lane & 1)) continue;
+      // Causally up to itself, and its prompt (which ends with the document).
+      const int seen = prefix[e] < stop - first[e] ? first[e] + prefix[e] : stop;
+      p.last[base + i] = p.causal ? max(i + 1, seen) : stop;
     }
   }
+}
+
+__global__ void __launch_bounds__(kDocWarps * 32) document_spans_kernel(const DocParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  if (p.ids64)
+    document_spans<int64_t>(p);
+  else
+    document_spans<int>(p);
 }
 
 // -------------------------------------------------------------------- host --
@@ -2005,5 +2006,5 @@ extern "C" int tq_document_spans(const void* documents, int ids_bits, const int3
   p.first = first;
   p.last = last;
   return launch_kernel(document_spans_kernel, dim3(static_cast<unsigned>(batch)),
-                       dim3(kScanThreads), 0, as_stream(stream), 1, "document_spans launch", p);
+                       dim3(kDocWarps * 32), 0, as_stream(stream), 1, "document_spans launch", p);
 }
