@@ -89,7 +89,7 @@ def _same_specials(got, want):
     return want.isfinite()
 
 
-def _check_forward(z, tokens, top, temperature):
+def _check_forward(z, tokens, top, temperature, scale_err=False):
     import torch
 
     from torobi_b200 import glue
@@ -98,6 +98,8 @@ def _check_forward(z, tokens, top, temperature):
     r = glue.token_logprobs(z, tokens, top=top, temperature=temperature)
     lp, ent, tlp, ids, *_ = _reference(z, tokens, top, temperature)
     lnv = math.log(vocab) + 1
+    if scale_err:  # 1/T is rounded: every ln q errs by as much of the spread it came from
+        lnv += float((lp.abs() + tlp.abs().amax(1)).nan_to_num(0, 0, 0).clamp(max=1e30).max())
     for name, got, want, tol in (
             ("logprobs", r.logprobs, lp, lambda w: _sum_err(vocab) + 4 * E * (w.abs() + lnv)),
             ("entropy", r.entropy, ent, lambda w: 3 * _sum_err(vocab) * lnv + 4 * E * w.abs()),
@@ -111,6 +113,22 @@ def _check_forward(z, tokens, top, temperature):
     if top:
         assert r.top_ids.dtype == torch.int64 and torch.equal(r.top_ids, ids)
     return r
+
+
+@pytest.mark.parametrize("temperature", [1e-4, 1e-2, 50.0, 1e6, 1e30])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_token_logprobs_far_temperatures(cuda, dtype, temperature):
+    """Temperatures at which the scaled logits leave every usual range, with
+    ruled-out tokens: the distribution goes from one-hot to uniform."""
+    import torch
+
+    z = _logits(cuda, 7, 2003, dtype, 21).contiguous()
+    z[:, ::5] = NINF
+    z[3] = torch.finfo(z.dtype).min
+    z[4, 1] = 200.0
+    t = torch.tensor([1, 2, 3, 4, 1, 6, 7], device=cuda)
+    r = _check_forward(z, t, 6, temperature, scale_err=True)
+    assert (r.entropy >= 0).all() and torch.isfinite(r.entropy).all()
 
 
 FORWARD = [
@@ -174,9 +192,17 @@ def test_token_logprobs_odd_rows(cuda, dtype, vocab, rows):
     z[11] += 300.0
     z[12] = -1000.0
     z[12, 3] = 0.0                                   # one certain token
+    if rows > 13:
+        z[13] = lowest                               # the finite way, and ruled out
+        z[13, 1::2] = NINF
+        z[14] = -1e35                                # far below any logit, and uneven
+        z[14, vocab // 2] = -9e34
+        z[15, ::2] = -1e34                           # such entries beside ordinary ones
     t = torch.randint(0, vocab, (rows,), device=cuda)
     t[4] = vocab // 2 + 1
     t[12] = 3
+    if rows > 13:
+        t[13] = 2 * (vocab // 4)
     for top in (1, 7, min(128, vocab)):
         r = _check_forward(z, t, top, 1.0)
         assert torch.isfinite(r.entropy).all() and (r.entropy >= 0).all()

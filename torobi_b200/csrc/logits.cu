@@ -28,6 +28,7 @@
 #include <cuda_bf16.h>
 
 #include <cmath>
+#include <cstddef>
 #include <type_traits>
 
 #include "tq_ptx.cuh"
@@ -47,6 +48,7 @@ constexpr int kPerSm = 4;
 constexpr int kMaxTop = 128;     // alternatives a call may ask for or give
 constexpr int kMaxSplit = 8;     // CTAs (one cluster) that may share a row
 constexpr int kSpare = 32;       // chunks above the threshold taken beyond top
+constexpr int kPool = 1024;      // candidates one CTA holds at a time
 constexpr int kMaxChunks = 16384;  // chunk maxima one CTA keeps (top > 0)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -350,21 +352,28 @@ __device__ void sort_descending(uint64_t* v, int n) {
   __syncthreads();
 }
 
-// The k greatest of n distinct numbers in `in` (room for the next power of
-// two), in order, to out[0, k); places past n get 0.  in may be reordered.
-__device__ void greatest(uint64_t* in, int n, int k, uint64_t* out) {
-  __syncthreads();
-  if (n <= 384) {
-    // Each number's rank is how many are greater.
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint64_t x = in[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += in[j] > x;
-      if (rank < k) out[rank] = x;
-    }
-    for (int i = n + threadIdx.x; i < k; i += kThreads) out[i] = 0;
+// The k greatest of n <= kPool distinct numbers in `in` (room for kPool), in
+// order, to out[0, k), which may be in itself; places past n get 0.  in may be
+// reordered; rank: kThreads ints.
+__device__ void greatest(uint64_t* in, int n, int k, uint64_t* out, int* rank) {
+  if (n <= kThreads) {
+    // Each number's rank is how many are greater: `parts` threads count for
+    // one number.
+    rank[threadIdx.x] = 0;
+    __syncthreads();
+    int p = 16;
+    while (p < n) p <<= 1;
+    const int i = threadIdx.x & (p - 1), parts = kThreads / p;
+    const uint64_t x = i < n ? in[i] : 0;
+    int greater = 0;
+    if (i < n)
+      for (int j = threadIdx.x / p; j < n; j += parts) greater += in[j] > x;
+    if (greater) atomicAdd(rank + i, greater);
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < n && rank[i] < k) out[rank[i]] = x;
+    for (int j = n + threadIdx.x; j < k; j += kThreads) out[j] = 0;
   } else {
-    int p = 512;
+    int p = 2 * kThreads;
     while (p < n) p <<= 1;
     for (int i = n + threadIdx.x; i < p; i += kThreads) in[i] = 0;
     sort_descending(in, p);
@@ -381,65 +390,135 @@ __device__ __forceinline__ ChunkKey<T> chunk_key(float m) {
   return static_cast<ChunkKey<T>>(order_key(m) >> (sizeof(T) == 2 ? 16 : 0));
 }
 
-struct TopShared {
+struct alignas(16) TopShared {  // mine is read in 16-byte words
   uint64_t best[kMaxTop];
+  union {
+    uint32_t mine[kThreads];  // the threads' maxima
+    int rank[kThreads];
+  };
   int chunks[2 * kMaxTop + kSpare];
   int scan[kWarps];
   int above, equal, listed, found;
 };
+static_assert(offsetof(TopShared, mine) % 16 == 0, "16-byte words");
 
-// Elements that `greatest` may be handed: every element of the chunks taken,
-// up to the next power of two.
-__host__ __device__ constexpr int candidate_room(int top, int ch) {
-  int p = 512;
-  while (p < (2 * top + kSpare) * ch) p <<= 1;
-  return p;
+// The largest t that at least `top` of the 256 keys in sh.mine reach, for
+// every thread: each warp searches for itself, bit by bit below the highest
+// bit in which the greatest and the least key differ.
+__device__ __forceinline__ uint32_t threshold(const TopShared& sh, int top) {
+  const uint4* k = reinterpret_cast<const uint4*>(sh.mine) + 2 * (threadIdx.x & 31);
+  const uint4 a = k[0], b = k[1];
+  const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t lo = v[0], hi = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) {
+    lo = min(lo, v[i]);
+    hi = max(hi, v[i]);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lo == hi) return hi;
+  uint32_t bit = 0x80000000u >> __clz(lo ^ hi);
+  uint32_t t = hi & ~(2 * bit - 1);
+#pragma unroll 1
+  for (; bit; bit >>= 1) {
+    const uint32_t probe = t | bit;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) n += v[i] >= probe;
+    if (__reduce_add_sync(0xffffffffu, n) >= top) t = probe;
+  }
+  return t;
+}
+
+// Every element of the chunks listed in [l0, l1) that reaches the threshold,
+// behind the sh.found that are in the pool already; a thread a chunk.  Counts
+// what does not fit, too.
+template <typename T>
+__device__ __forceinline__ void gather(const Row<T>& row, int l0, int l1, uint32_t floor_key,
+                                       uint64_t* pool, TopShared& sh) {
+  constexpr int CH = Elem<T>::CH;
+  for (int i = l0 + threadIdx.x; i < l1; i += kThreads) {
+    const int c = sh.chunks[i];
+    uint32_t w[8];
+    if (c >= row.lo && c < row.hi)
+      ldg_chunk(row.chunk(c), w);
+    else
+      row.load_edge(c, w);
+    float f[CH];
+    Elem<T>::unpack(w, f);
+    const int64_t j0 = row.first(c);
+#pragma unroll
+    for (int e = 0; e < CH; ++e) {
+      const uint32_t k = order_key(f[e]);
+      if (k < floor_key || j0 + e < 0 || j0 + e >= row.vocab) continue;
+      const int at = atomicAdd(&sh.found, 1);
+      if (at < kPool) pool[at] = candidate(k, static_cast<uint32_t>(j0 + e));
+    }
+  }
+  __syncthreads();
 }
 
 // The slice's `top` greatest logits, in order, to sh.best (0 past its end).
 //   keys[0, n)  the largest logit of each chunk c0 + i
 //   mine        the largest of this thread's chunks (the chunks are disjoint)
 // The threshold t is the top-th greatest of the threads' maxima: at least
-// `top` chunks reach it, and few more do unless the row is built against it;
-// then t becomes the top-th greatest of all chunk maxima.  Every chunk above t
-// is read again and, of the chunks that only equal it, the first `top` (ties
-// go to the lowest index, and each holds one): 2 top + 32 chunks at the most.
-// pool holds the keys and, once the chunks are listed, the candidates.
+// `top` chunks reach it, and few more do.  Those are read again, and every
+// element that reaches t is a candidate.  A row built against this (equal
+// logits, large ones side by side) may have more chunks at or above t than
+// the list holds: t then becomes the top-th greatest of all chunk maxima,
+// fewer than `top` chunks are above it, and of those that equal it the first
+// `top` are enough (ties go to the lowest index, and each holds one).  More
+// candidates than the pool holds are gone through in parts.  What this costs
+// behind the pass over the row (4092 x 151936, 184 us without alternatives):
+// see the launch for the times; it is latency -- one barrier to share the
+// maxima, one scan of the keys, one reading of the chunks, one ranking --
+// which the SM's other CTAs cover.
 template <typename T>
 __device__ void slice_top(const Row<T>& row, int c0, int n, int top, ChunkKey<T>* keys, float mine,
                           bool any, uint64_t* pool, TopShared& sh) {
-  constexpr int CH = Elem<T>::CH;
   constexpr int BITS = 8 * sizeof(ChunkKey<T>);
+  constexpr int PER = 16 / sizeof(ChunkKey<T>);  // keys in 16 bytes
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t own = any ? chunk_key<T>(mine) : 0;
-  uint32_t t = 0;
-#pragma unroll 1
-  for (int b = BITS - 1; b >= 0; --b) {
-    const uint32_t probe = t | (1u << b);
-    if (__syncthreads_count(own >= probe) >= top) t = probe;
+  const int room = 2 * top + kSpare;
+  sh.mine[threadIdx.x] = any ? chunk_key<T>(mine) : 0;
+  if (threadIdx.x == 0) sh.listed = sh.found = 0;
+  __syncthreads();
+  uint32_t t = threshold(sh, top);
+  for (int i = PER * threadIdx.x; i < n; i += PER * kThreads) {
+    // The keys' room is whole 16-byte words; what is behind the last is not
+    // looked at.
+    const uint4 q = *reinterpret_cast<const uint4*>(keys + i);
+    const ChunkKey<T>* k = reinterpret_cast<const ChunkKey<T>*>(&q);
+#pragma unroll
+    for (int e = 0; e < PER; ++e)
+      if (k[e] >= t && i + e < n) {
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < room) sh.chunks[at] = c0 + i + e;
+      }
   }
-  auto count = [&](uint32_t at, int& above, int& equal) {
-    if (threadIdx.x == 0) sh.above = sh.equal = 0;
-    __syncthreads();
-    int a = 0, q = 0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      a += keys[i] > at;
-      q += keys[i] == at;
-    }
-    a = __reduce_add_sync(0xffffffffu, a);
-    q = __reduce_add_sync(0xffffffffu, q);
-    if (lane == 0) {
-      atomicAdd(&sh.above, a);
-      atomicAdd(&sh.equal, q);
-    }
-    __syncthreads();
-    above = sh.above;
-    equal = sh.equal;
-    __syncthreads();
-  };
-  int above, equal;
-  count(t, above, equal);
-  if (above > top + kSpare) {
+  __syncthreads();
+  if (sh.listed > room) {
+    auto count = [&](uint32_t at, int& above, int& equal) {
+      if (threadIdx.x == 0) sh.above = sh.equal = 0;
+      __syncthreads();
+      int a = 0, q = 0;
+      for (int i = threadIdx.x; i < n; i += kThreads) {
+        a += keys[i] > at;
+        q += keys[i] == at;
+      }
+      a = __reduce_add_sync(0xffffffffu, a);
+      q = __reduce_add_sync(0xffffffffu, q);
+      if (lane == 0) {
+        atomicAdd(&sh.above, a);
+        atomicAdd(&sh.equal, q);
+      }
+      __syncthreads();
+      above = sh.above;
+      equal = sh.equal;
+      __syncthreads();
+    };
+    int above, equal;
     t = 0;
 #pragma unroll 1
     for (int b = BITS - 1; b >= 0; --b) {
@@ -447,14 +526,7 @@ __device__ void slice_top(const Row<T>& row, int c0, int n, int top, ChunkKey<T>
       count(probe, above, equal);
       if (above + equal >= top) t = probe;
     }
-    count(t, above, equal);
-  }
-  if (threadIdx.x == 0) sh.listed = sh.found = 0;
-  __syncthreads();
-  if (equal <= top) {
-    for (int i = threadIdx.x; i < n; i += kThreads)
-      if (keys[i] >= t) sh.chunks[atomicAdd(&sh.listed, 1)] = c0 + i;
-  } else {
+    if (threadIdx.x == 0) sh.listed = 0;
     // The first `top` of the equal ones in index order: each thread counts
     // its own stretch, a prefix sum gives its places.
     const int per = (n + kThreads - 1) / kThreads;
@@ -476,20 +548,31 @@ __device__ void slice_top(const Row<T>& row, int c0, int n, int top, ChunkKey<T>
       if (keys[i] > t || (eq && before < top)) sh.chunks[atomicAdd(&sh.listed, 1)] = c0 + i;
       before += eq;
     }
+    __syncthreads();
   }
-  __syncthreads();  // the keys' room is the candidates' from here
+  // The keys' room is the candidates' from here.
   const int listed = sh.listed;
-  const uint32_t floor_key = static_cast<uint32_t>(t) << (32 - BITS);
-  for (int i = threadIdx.x / CH; i < listed; i += kThreads / CH) {
-    const int c = sh.chunks[i], e = threadIdx.x % CH;
-    const int64_t j = row.first(c) + e;
-    if (j >= 0 && j < row.vocab) {
-      const uint32_t k = order_key(Elem<T>::load(row.chunk(c) + e));
-      if (k >= floor_key) pool[atomicAdd(&sh.found, 1)] = candidate(k, static_cast<uint32_t>(j));
-    }
+  const uint32_t floor_key = t << (32 - BITS);
+  gather<T>(row, 0, listed, floor_key, pool, sh);
+  if (sh.found <= kPool) {
+    greatest(pool, sh.found, top, sh.best, sh.rank);
+    return;
   }
-  __syncthreads();
-  greatest(pool, sh.found, top, sh.best);
+  // As many chunks at a time as surely fit beside the best so far.
+  constexpr int STEP = (kPool - kMaxTop) / Elem<T>::CH;
+  for (int l0 = 0; l0 < listed; l0 += STEP) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = l0 ? top : 0;
+    if (l0)
+      for (int i = threadIdx.x; i < top; i += kThreads) {
+        const uint64_t x = sh.best[i];
+        // Places not yet taken: distinct, below every logit.
+        pool[i] = x ? x : static_cast<uint64_t>(i) + 1;
+      }
+    __syncthreads();
+    gather<T>(row, l0, min(listed, l0 + STEP), floor_key, pool, sh);
+    greatest(pool, sh.found, top, sh.best, sh.rank);
+  }
 }
 
 // ----------------------------------------------------------- token_logprobs --
@@ -512,7 +595,7 @@ struct LogprobParams {
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const LogprobParams p) {
   constexpr int U = kInFlight;
-  extern __shared__ uint64_t pool[];
+  extern __shared__ __align__(16) uint64_t pool[];
   __shared__ Sums sums[kWarps];
   __shared__ float2 total;
   griddep_wait();
@@ -573,10 +656,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
   }
   block_sums<kEntropy>(v, sums, c);
   uint64_t* best = nullptr;
+  int* rank_of = nullptr;
   if constexpr (TOP) {
     __shared__ TopShared sh;
     slice_top<T>(row, c0, c1 - c0, p.top, keys, mine, any, pool, sh);
     best = sh.best;
+    rank_of = sh.rank;
   }
   if (p.split > 1) {
     cluster_sync();
@@ -585,13 +670,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
         for (int i = threadIdx.x; i < p.split * p.top; i += kThreads) {
           const uint64_t x = ld_cluster_u64(mapa_shared(smem_u32(best + i % p.top), i / p.top));
           // Places past a short slice's end: distinct, below every logit.
-          pool[i] = x ? x : static_cast<uint64_t>(i);
+          pool[i] = x ? x : static_cast<uint64_t>(i) + 1;
         }
       if (threadIdx.x == 0) v = cluster_sums<kEntropy>(sums, p.split, c);
     }
     cluster_sync();  // the leader has read every CTA's shared memory
     if (rank != 0) return;
-    if constexpr (TOP) greatest(pool, p.split * p.top, p.top, best);
+    if constexpr (TOP) greatest(pool, p.split * p.top, p.top, best, rank_of);
   } else if (threadIdx.x == 0) {
     v = sums[0];
   }
@@ -1064,8 +1149,8 @@ extern "C" int tq_token_logprobs_fwd(const void* logits, int dtype, const int64_
     while ((vocab / ch + 2 + p.split - 1) / p.split > kMaxChunks) p.split *= 2;
     const size_t key = dtype == TQ_DTYPE_F32 ? 4 : 2;
     const size_t keys = static_cast<size_t>((vocab / ch + 2 + p.split - 1) / p.split) * key;
-    const size_t room = static_cast<size_t>(candidate_room(p.top, ch)) * 8;
-    smem = (keys > room ? keys : room) + 16;
+    const size_t room = static_cast<size_t>(kPool) * 8;
+    smem = ((keys > room ? keys : room) + 15) / 16 * 16;
   }
   auto kernel = dtype == TQ_DTYPE_F32
                     ? (top > 0 ? logprobs_fwd_kernel<float, true> : logprobs_fwd_kernel<float, false>)
