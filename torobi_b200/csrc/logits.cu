@@ -83,6 +83,14 @@ __device__ __forceinline__ float warp_add(float v) {
   return v;
 }
 
+// Order-preserving image of a float: greater float, greater key; -0 is +0 and
+// every NaN is above +inf.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (f != f) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(f + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
 // ------------------------------------------------------------------- rows --
 
 template <typename T>
@@ -108,11 +116,30 @@ struct Elem<uint16_t> {  // bf16
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2_f32(f[2 * i], f[2 * i + 1]);
   }
-  __device__ static float chunk_max(const uint32_t (&w)[8]) {
+  // The largest of a chunk, or of several: in a pair's two halves until value().
+  using Max = uint32_t;
+  using Bits = uint16_t;
+  __device__ static Max chunk_max(const uint32_t (&w)[8]) {
     const uint32_t a = max_nan_bf2(max_nan_bf2(w[0], w[1]), max_nan_bf2(w[2], w[3]));
     const uint32_t b = max_nan_bf2(max_nan_bf2(w[4], w[5]), max_nan_bf2(w[6], w[7]));
-    const uint32_t m = max_nan_bf2(a, b);
+    return max_nan_bf2(a, b);
+  }
+  __device__ static Max join(Max a, Max b) { return max_nan_bf2(a, b); }
+  __device__ static Bits bits(Max m) {
+    return static_cast<Bits>(max_nan_bf2(m, prmt(m, m, 0x1032)));
+  }
+  __device__ static float value(Max m) {
     return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+  }
+  // order_key's upper half of the two values of a word: -0 becomes +0, then
+  // negative ones are turned over and the others get the top bit.
+  __device__ static uint32_t order_word(uint32_t w) {
+    w = bf2_fma(w, 0x3F803F80u, 0);
+    return w ^ (((w >> 15) & 0x00010001u) * 0x7FFFu | 0x80008000u);
+  }
+  __device__ static uint32_t max_words(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+  __device__ static bool reaches(uint32_t w, uint32_t t) {
+    return (w >> 16) >= t || (w & 0xFFFFu) >= t;
   }
 };
 template <>
@@ -129,12 +156,20 @@ struct Elem<float> {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
   }
-  __device__ static float chunk_max(const uint32_t (&w)[8]) {
+  using Max = float;
+  using Bits = uint32_t;
+  __device__ static Max chunk_max(const uint32_t (&w)[8]) {
     float f[8];
     unpack(w, f);
     return max_nan(max_nan(max_nan(f[0], f[1]), max_nan(f[2], f[3])),
                    max_nan(max_nan(f[4], f[5]), max_nan(f[6], f[7])));
   }
+  __device__ static Max join(Max a, Max b) { return max_nan(a, b); }
+  __device__ static Bits bits(Max m) { return __float_as_uint(m); }
+  __device__ static float value(Max m) { return m; }
+  __device__ static uint32_t order_word(uint32_t w) { return order_key(__uint_as_float(w)); }
+  __device__ static uint32_t max_words(uint32_t a, uint32_t b) { return max(a, b); }
+  __device__ static bool reaches(uint32_t w, uint32_t t) { return w >= t; }
 };
 
 // A row as the 32-byte chunks of memory that it touches.  Chunks in [lo, hi)
@@ -279,11 +314,15 @@ __device__ __forceinline__ void block_sums(Sums v, Sums* sh, float c) {
   v.a = warp_add(v.a);
   if (lane == 0) sh[warp] = v;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    Sums t = sh[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) merge<M>(t, sh[i], c);
-    sh[0] = t;
+  if (warp == 0) {
+    Sums t;
+    if (lane < kWarps) t = sh[lane];
+    const float top = warp_max(t.m);
+    if (top != -INFINITY) move_to<M>(t, top, c);
+    t.s = warp_add(t.s);
+    t.a = warp_add(t.a);
+    __syncwarp();
+    if (lane == 0) sh[0] = t;
   }
   __syncthreads();
 }
@@ -317,14 +356,6 @@ __device__ __forceinline__ Sums cluster_sums(Sums* sh, int split, float c) {
 }
 
 // ------------------------------------------------------------ alternatives --
-
-// Order-preserving image of a float: greater float, greater key; -0 is +0 and
-// every NaN is above +inf.
-__device__ __forceinline__ uint32_t order_key(float f) {
-  if (f != f) return 0xFFFFFFFFu;
-  const uint32_t b = __float_as_uint(f + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
 
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
@@ -383,7 +414,7 @@ __device__ void greatest(uint64_t* in, int n, int k, uint64_t* out, int* rank) {
 }
 
 template <typename T>
-using ChunkKey = typename std::conditional<sizeof(T) == 2, uint16_t, uint32_t>::type;
+using ChunkKey = typename Elem<T>::Bits;
 
 template <typename T>
 __device__ __forceinline__ ChunkKey<T> chunk_key(float m) {
@@ -399,12 +430,13 @@ struct alignas(16) TopShared {  // mine is read in 16-byte words
   int chunks[2 * kMaxTop + kSpare];
   int scan[kWarps];
   int above, equal, listed, found;
+  uint32_t threshold;
 };
 static_assert(offsetof(TopShared, mine) % 16 == 0, "16-byte words");
 
-// The largest t that at least `top` of the 256 keys in sh.mine reach, for
-// every thread: each warp searches for itself, bit by bit below the highest
-// bit in which the greatest and the least key differ.
+// The largest t that at least `top` of the 256 keys in sh.mine reach; one warp
+// searches bit by bit below the highest bit in which the greatest and the
+// least key differ.
 __device__ __forceinline__ uint32_t threshold(const TopShared& sh, int top) {
   const uint4* k = reinterpret_cast<const uint4*>(sh.mine) + 2 * (threadIdx.x & 31);
   const uint4 a = k[0], b = k[1];
@@ -438,6 +470,8 @@ template <typename T>
 __device__ __forceinline__ void gather(const Row<T>& row, int l0, int l1, uint32_t floor_key,
                                        uint64_t* pool, TopShared& sh) {
   constexpr int CH = Elem<T>::CH;
+  const float least = key_value(floor_key);
+  const bool nan = floor_key > order_key(INFINITY);
   for (int i = l0 + threadIdx.x; i < l1; i += kThreads) {
     const int c = sh.chunks[i];
     uint32_t w[8];
@@ -448,19 +482,27 @@ __device__ __forceinline__ void gather(const Row<T>& row, int l0, int l1, uint32
     float f[CH];
     Elem<T>::unpack(w, f);
     const int64_t j0 = row.first(c);
+    // A bit an element, then one place in the pool a thread.  (A NaN is not
+    // below any number; where the threshold is NaN itself, only NaN reaches it.)
+    uint32_t hits = 0;
 #pragma unroll
     for (int e = 0; e < CH; ++e) {
-      const uint32_t k = order_key(f[e]);
-      if (k < floor_key || j0 + e < 0 || j0 + e >= row.vocab) continue;
-      const int at = atomicAdd(&sh.found, 1);
-      if (at < kPool) pool[at] = candidate(k, static_cast<uint32_t>(j0 + e));
+      const bool in = c >= row.lo && c < row.hi ? true : j0 + e >= 0 && j0 + e < row.vocab;
+      if (in && (nan ? f[e] != f[e] : !(f[e] < least))) hits |= 1u << e;
     }
+    int at = hits ? atomicAdd(&sh.found, __popc(hits)) : 0;
+#pragma unroll
+    for (int e = 0; e < CH; ++e)
+      if (hits >> e & 1) {
+        if (at < kPool) pool[at] = candidate(order_key(f[e]), static_cast<uint32_t>(j0 + e));
+        ++at;
+      }
   }
   __syncthreads();
 }
 
 // The slice's `top` greatest logits, in order, to sh.best (0 past its end).
-//   keys[0, n)  the largest logit of each chunk c0 + i
+//   keys[0, n)  the largest logit of each chunk c0 + i, its bits
 //   mine        the largest of this thread's chunks (the chunks are disjoint)
 // The threshold t is the top-th greatest of the threads' maxima: at least
 // `top` chunks reach it, and few more do.  Those are read again, and every
@@ -469,11 +511,11 @@ __device__ __forceinline__ void gather(const Row<T>& row, int l0, int l1, uint32
 // the list holds: t then becomes the top-th greatest of all chunk maxima,
 // fewer than `top` chunks are above it, and of those that equal it the first
 // `top` are enough (ties go to the lowest index, and each holds one).  More
-// candidates than the pool holds are gone through in parts.  What this costs
-// behind the pass over the row (4092 x 151936, 184 us without alternatives):
-// see the launch for the times; it is latency -- one barrier to share the
-// maxima, one scan of the keys, one reading of the chunks, one ranking --
-// which the SM's other CTAs cover.
+// candidates than the pool holds are gone through in parts.  It is latency
+// behind the pass over the row -- one barrier to share the maxima, one scan of
+// the keys, one reading of the chunks, one ranking -- and the SM's other three
+// CTAs cover only part of it: 4092 x 151936 takes 185 us without alternatives,
+// 219 with one, 247 with 64, 293 with 128.
 template <typename T>
 __device__ void slice_top(const Row<T>& row, int c0, int n, int top, ChunkKey<T>* keys, float mine,
                           bool any, uint64_t* pool, TopShared& sh) {
@@ -484,18 +526,36 @@ __device__ void slice_top(const Row<T>& row, int c0, int n, int top, ChunkKey<T>
   sh.mine[threadIdx.x] = any ? chunk_key<T>(mine) : 0;
   if (threadIdx.x == 0) sh.listed = sh.found = 0;
   __syncthreads();
-  uint32_t t = threshold(sh, top);
+  if (warp == 0) {
+    const uint32_t found = threshold(sh, top);
+    if (lane == 0) sh.threshold = found;
+  }
+  __syncthreads();
+  uint32_t t = sh.threshold;
   for (int i = PER * threadIdx.x; i < n; i += PER * kThreads) {
-    // The keys' room is whole 16-byte words; what is behind the last is not
-    // looked at.
-    const uint4 q = *reinterpret_cast<const uint4*>(keys + i);
-    const ChunkKey<T>* k = reinterpret_cast<const ChunkKey<T>*>(&q);
+    // In order from here.  The keys' room is whole 16-byte words; what is
+    // behind the last key is not looked at.
+    uint4* const at4 = reinterpret_cast<uint4*>(keys + i);
+    uint4 q = *at4;
+    q.x = Elem<T>::order_word(q.x);
+    q.y = Elem<T>::order_word(q.y);
+    q.z = Elem<T>::order_word(q.z);
+    q.w = Elem<T>::order_word(q.w);
+    *at4 = q;
+    const uint32_t m =
+        Elem<T>::max_words(Elem<T>::max_words(q.x, q.y), Elem<T>::max_words(q.z, q.w));
+    if (!Elem<T>::reaches(m, t)) continue;
+    const uint32_t words[4] = {q.x, q.y, q.z, q.w};
+    uint32_t hits = 0;
 #pragma unroll
-    for (int e = 0; e < PER; ++e)
-      if (k[e] >= t && i + e < n) {
-        const int at = atomicAdd(&sh.listed, 1);
-        if (at < room) sh.chunks[at] = c0 + i + e;
-      }
+    for (int e = 0; e < PER; ++e) {
+      const uint32_t k = PER == 4 ? words[e % 4] : words[e / 2] >> (e & 1) * 16 & 0xFFFFu;
+      if (k >= t && i + e < n) hits |= 1u << e;
+    }
+    if (!hits) continue;
+    int at = atomicAdd(&sh.listed, __popc(hits));
+    for (; hits; hits &= hits - 1, ++at)
+      if (at < room) sh.chunks[at] = c0 + i + __ffs(hits) - 1;
   }
   __syncthreads();
   if (sh.listed > room) {
@@ -607,13 +667,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
   const int c0 = min(row.n, rank * per), c1 = min(row.n, c0 + per);
   ChunkKey<T>* keys = reinterpret_cast<ChunkKey<T>*>(pool);
   const float c = p.c;
+  // The given token's logit, ahead of the row (two loads one behind the other
+  // at the row's end would cost as much as the selection).
+  bool given = false;
+  float picked = 0.0f;
+  if (threadIdx.x == 0 && rank == 0) {
+    const int64_t tok = p.tokens[r];
+    given = tok >= 0 && tok < p.vocab;
+    if (given) picked = Elem<T>::load(static_cast<const T*>(p.z) + r * p.ld + tok);
+  }
   Sums v;
   float mine = -INFINITY;
   bool any = false;
   auto one = [&](int ch, const uint32_t (&w)[1][8]) {
-    const float mx = Elem<T>::chunk_max(w[0]);
+    const typename Elem<T>::Max cm = Elem<T>::chunk_max(w[0]);
+    const float mx = Elem<T>::value(cm);
     if constexpr (TOP) {
-      keys[ch - c0] = chunk_key<T>(mx);
+      keys[ch - c0] = Elem<T>::bits(cm);
       mine = max_nan(mine, mx);
       any = true;
     }
@@ -636,13 +706,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
     uint32_t w[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) ldg_chunk(row.chunk(ch + u * kThreads), w[u]);
-    float mx = -INFINITY;
+    typename Elem<T>::Max all;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float m = Elem<T>::chunk_max(w[u]);
-      if constexpr (TOP) keys[ch + u * kThreads - c0] = chunk_key<T>(m);
-      mx = max_nan(mx, m);
+      const typename Elem<T>::Max cm = Elem<T>::chunk_max(w[u]);
+      if constexpr (TOP) keys[ch + u * kThreads - c0] = Elem<T>::bits(cm);
+      all = u ? Elem<T>::join(all, cm) : cm;
     }
+    const float mx = Elem<T>::value(all);
     if constexpr (TOP) {
       mine = max_nan(mine, mx);
       any = true;
@@ -685,12 +756,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
     const float m = none ? 0.0f : v.m;
     const float l2 = log2f(v.s);  // -inf for a row of nothing but -inf
     const float h = none ? 0.0f : (l2 - v.a / v.s) * kLn2;
-    const int64_t tok = p.tokens[r];
     float lp = 0.0f;
-    if (tok >= 0 && tok < p.vocab) {
-      const float z = Elem<T>::load(static_cast<const T*>(p.z) + r * p.ld + tok);
-      lp = none ? -INFINITY : fmaf(z - m, p.inv_t, -l2 * kLn2);
-    }
+    if (given) lp = none ? -INFINITY : fmaf(picked - m, p.inv_t, -l2 * kLn2);
     p.logprobs[r] = lp;
     p.entropy[r] = h;
     if (p.stats) p.stats[r] = make_float4(m, l2, h, 0.0f);
@@ -840,8 +907,10 @@ struct Alternatives {
   float lp[kPerLane], p[kPerLane];
 };
 
-__device__ __forceinline__ Alternatives load_teacher(const Teacher& t, int64_t r, int vocab,
-                                                     float c) {
+// id(e) and logit(e) answer for entry e < k.
+template <typename Id, typename Logit>
+__device__ __forceinline__ Alternatives weigh(int k, int vocab, float c, Id&& id_of,
+                                              Logit&& logit_of) {
   const int lane = threadIdx.x & 31;
   Alternatives a;
   float mx = -INFINITY;
@@ -850,11 +919,11 @@ __device__ __forceinline__ Alternatives load_teacher(const Teacher& t, int64_t r
     const int e = lane + 32 * i;
     a.id[i] = -1;
     a.lp[i] = -INFINITY;
-    if (e < t.k) {
-      const int64_t id = t.id(r * t.k + e);
+    if (e < k) {
+      const int64_t id = id_of(e);
       if (id >= 0 && id < vocab) {
         a.id[i] = static_cast<int>(id);
-        a.lp[i] = t.logit(r * t.k + e);
+        a.lp[i] = logit_of(e);
       }
     }
     mx = max_nan(mx, a.lp[i]);
@@ -908,9 +977,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const Dis
   const int per = (row.n + p.split - 1) / p.split;
   const int c0 = min(row.n, rank * per), c1 = min(row.n, c0 + per);
   const float c = p.c;
+  // What is given, and the student's logits there, ahead of the row: loads one
+  // behind the other at its end would hold up the CTA's last warp.
+  __shared__ int ids[kMaxTop + 1];
+  __shared__ float given[kMaxTop], picked[kMaxTop + 1];
+  if (rank == 0 && threadIdx.x <= kMaxTop) {
+    const int e = threadIdx.x, k = p.teacher.k;
+    int64_t id = -1;
+    if (e < k) id = p.teacher.id(r * k + e);
+    if (e == kMaxTop && p.targets) id = p.targets[r];
+    if (id < 0 || id >= p.vocab) id = -1;
+    ids[e] = static_cast<int>(id);
+    picked[e] = id >= 0 ? Elem<T>::load(z + id) : 0.0f;
+    if (e < k) given[e] = p.teacher.logit(r * k + e);
+  }
   Sums v;
   auto one = [&](const uint32_t (&w)[1][8]) {
-    add_chunks<T, M, 1>(v, w, Elem<T>::chunk_max(w[0]), c);
+    add_chunks<T, M, 1>(v, w, Elem<T>::value(Elem<T>::chunk_max(w[0])), c);
   };
   const int lo = max(c0, row.lo), hi = min(c1, row.hi);
   if (threadIdx.x == 0 && c0 == 0 && c1 > 0 && row.lo == 1) {
@@ -929,10 +1012,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const Dis
     uint32_t w[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u) ldg_chunk(row.chunk(ch + u * kThreads), w[u]);
-    float mx = -INFINITY;
+    typename Elem<T>::Max all = Elem<T>::chunk_max(w[0]);
 #pragma unroll
-    for (int u = 0; u < U; ++u) mx = max_nan(mx, Elem<T>::chunk_max(w[u]));
-    add_chunks<T, M, U>(v, w, mx, c);
+    for (int u = 1; u < U; ++u) all = Elem<T>::join(all, Elem<T>::chunk_max(w[u]));
+    add_chunks<T, M, U>(v, w, Elem<T>::value(all), c);
   }
   for (; ch < hi; ch += kThreads) {
     uint32_t w[1][8];
@@ -952,23 +1035,23 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const Dis
   v = sums[0];
   const bool none = v.m == -INFINITY;
   const float m = none ? 0.0f : v.m, l2 = log2f(v.s), l21 = TWO ? log2f(v.a) : l2;
-  const Alternatives a = load_teacher(p.teacher, r, p.vocab, c);
+  const Alternatives a = weigh(
+      p.teacher.k, p.vocab, c, [&](int e) { return ids[e]; }, [&](int e) { return given[e]; });
   float kl = 0.0f;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
     if (a.id[i] < 0 || a.p[i] == 0.0f) continue;
     const float lq =
-        none ? -INFINITY : fmaf(Elem<T>::load(z + a.id[i]) - m, p.inv_t, -l2 * kLn2);
+        none ? -INFINITY
+             : fmaf(picked[(threadIdx.x & 31) + 32 * i] - m, p.inv_t, -l2 * kLn2);
     kl = fmaf(a.p[i], fmaf(a.lp[i], kLn2, -lq), kl);
   }
   kl = warp_add(kl);
   if (threadIdx.x != 0) return;
   p.kl[r] = kl;
   if (p.ce) {
-    const int64_t t = p.targets[r];
     float ce = 0.0f;
-    if (t >= 0 && t < p.vocab)
-      ce = none ? INFINITY : fmaf(l21, kLn2, m - Elem<T>::load(z + t));
+    if (ids[kMaxTop] >= 0) ce = none ? INFINITY : fmaf(l21, kLn2, m - picked[kMaxTop]);
     p.ce[r] = ce;
   }
   if (p.stats) p.stats[r] = make_float4(m, l2, l21, 0.0f);
@@ -1008,7 +1091,9 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGrad
   const float u = p.dkl ? p.dkl[r] * p.inv_t : 0.0f;
   const float v = picked && p.dce ? p.dce[r] : 0.0f;
   if (threadIdx.x < 32) {
-    const Alternatives a = load_teacher(p.teacher, r, p.vocab, p.c);
+    const Alternatives a =
+        weigh(k, p.vocab, p.c, [&](int e) { return p.teacher.id(r * k + e); },
+              [&](int e) { return p.teacher.logit(r * k + e); });
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int e = threadIdx.x + 32 * i;
