@@ -464,7 +464,8 @@ int tq_cross_entropy_bwd(const void* logits, const int64_t* targets, const float
  *   top_logprobs, top_ids [rows, top]: the top largest logits' ln q and
  *                 indices, largest first, ties to the lowest index (NaN above
  *                 everything); top 0 to 128 and at most vocab (and vocab at
- *                 most 2^20 with f32 or 2^21 with bf16 logits when top > 0);
+ *                 most 2^20 - 16 with f32, 2^21 - 32 with bf16 logits when
+ *                 top > 0);
  *                 both may be NULL when top is 0
  *   stats       [rows, 4] f32, 16-byte aligned, what the backward reads; may
  *               be NULL

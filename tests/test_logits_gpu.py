@@ -356,6 +356,45 @@ def test_token_logprobs_gradient_against_differences(cuda):
         assert ((dz[:, j].double() - diff).abs() <= 50 * step ** 2 + 1e-9 + 200 * E).all()
 
 
+def test_rows_past_32_bit_offsets(cuda):
+    """14200 x 151936 logits, over 2^31: the last rows, forward and (in place)
+    backward, give what they give alone (where clusters share a row, so that
+    its f32 sums come in another order)."""
+    import torch
+
+    from torobi_b200 import glue
+
+    rows, vocab, n = 14200, 151936, 3
+    g = torch.Generator(device=cuda).manual_seed(8)
+    z = torch.randn(rows, vocab, device=cuda, dtype=torch.bfloat16, generator=g)
+    tokens = torch.randint(0, vocab, (rows,), device=cuda, generator=g)
+    tail = z[-n:].clone()
+    _check_forward(tail, tokens[-n:], 8, 1.0)
+    with torch.no_grad():
+        top = glue.token_logprobs(z, tokens, top=8)
+    ids, given = top.top_ids, top.top_logprobs * 0.5
+
+    def run(z, t, ids, given):
+        leaf = z.requires_grad_()
+        r = glue.token_logprobs(leaf, t, top=8)
+        kl, ce = glue.distillation(leaf, ids, given, targets=t, temperature=2.0, inplace=True)
+        dz, = torch.autograd.grad(kl.sum() + ce.sum(), leaf)
+        return [x.detach()[-n:] for x in (r.top_ids, r.logprobs, r.entropy, kl, ce, dz)]
+
+    many = run(z, tokens, ids, given)
+    few = run(tail, tokens[-n:], ids[-n:], given[-n:])
+    assert torch.equal(many[0], few[0])
+    lnv = math.log(vocab) + 1
+    for a, b in zip(many[1:5], few[1:5]):
+        assert ((a - b).abs() <= 6 * _sum_err(vocab) * lnv + 8 * E * (b.abs() + lnv)).all()
+    # The gradient: two roundings to bf16, and where something is given a
+    # difference of shares of 1.
+    a, b = many[5].double(), few[5].double()
+    room = torch.zeros_like(b)
+    room.scatter_(1, torch.cat([ids[-n:], tokens[-n:, None]], 1), 8 * _sum_err(vocab))
+    assert ((a - b).abs() <= 2 * HALF["bf16"] * 1.1 * b.abs() + room).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_gradient_with_another_pitch(cuda, dtype):
     """dlogits in rows of another pitch than the logits': elements go one by

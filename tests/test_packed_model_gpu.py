@@ -94,6 +94,21 @@ def test_prompts_are_seen_in_both_directions(cuda):
     assert zero[59] and zero[60:64].all() and not zero[64:].any()
 
 
+@pytest.mark.parametrize("longest", [2 ** 31 - 1, 2 ** 40])
+def test_prompts_longer_than_their_documents(cuda, longest):
+    """A prompt length past the document's end, however large: the whole
+    document is a prompt, and nothing in it a target."""
+    import torch
+
+    model = _model(1)
+    ids, docs, _ = _rows(cuda, [[60, 40]], 100)
+    prefix = torch.zeros_like(docs, dtype=torch.int32 if longest < 2 ** 31 else torch.int64)
+    prefix[:, 60:] = longest
+    with torch.no_grad():
+        lp = model.token_logprobs(ids, documents=docs, prefix=prefix).logprobs[0]
+    assert (lp[:59] != 0).all() and (lp[59:] == 0).all()
+
+
 def _plain_distill(model, ids, tids, tlogits, docs, prefix_mask, temperature, alpha):
     import torch
 

@@ -1,17 +1,17 @@
-"""span_attention and document_spans (csrc/attn.cu) against their definitions
+"""span_attention and document_spans (csrc/span_attn.cu) against their definitions
 in 64 bits.
 
 Tolerances.  The operands are bf16 and the products are summed in f32; what is
 rounded on the way is P (and dS) to bf16 before a product and the result: each
 half a step, 2^-8 of the value at most.  |o| errs by at most
-2^-8 (sum_j p_j |v_j| + |o|), plus the exponentials' 8e-5 and f32 sums, for
+2^-8 (sum_j p_j |v_j| + |o|), plus the exponentials' errors and f32 sums, for
 which a tenth of that bound is ample.  For the gradients the same holds with
 the products' magnitudes: dv by 2^-8 (sum_i p_ij |do_i| + |dv|), dq and dk by
 2^-8 times sums of |dS| |k| (or |q|), where dS's own error comes from its
 rounding and from delta = sum do o, whose o is rounded to bf16:
-p_ij 2^-8 sum_d |do o|.  lse: f32, within 1e-4 (a quarter of the
-exponentials are a polynomial of relative error 7.5e-5; log is 1-Lipschitz
-here) plus 4 steps of f32 of its own size and of the scores'.
+p_ij 2^-8 sum_d |do o|.  lse: f32, within 1e-4 (room for exponentials of
+relative error 7.5e-5, the polynomial of attn.cu; log is 1-Lipschitz here)
+plus 4 steps of f32 of its own size and of the scores'.
 """
 from __future__ import annotations
 
@@ -80,6 +80,10 @@ def test_document_spans(cuda, seq, mean, ids):
         first, last = glue.document_spans(d, use, causal=causal)
         f, l = _spans_reference(rows, None if use is None else prefix, causal)
         assert first.tolist() == f and last.tolist() == l
+    # Prompt lengths past 32 bits are lengths still, as are those below zero.
+    wide = torch.where(pre == 10 ** 9, 2 ** 32 + 1, torch.where(pre < 0, -2 ** 33 + 7, pre.long()))
+    for a, b in zip(glue.document_spans(d, wide), glue.document_spans(d, pre)):
+        assert torch.equal(a, b)
 
 
 def _reference(q, k, v, first, last, scale, do=None):
@@ -270,6 +274,62 @@ def test_one_causal_document_is_causal_attention(cuda, dim):
     x, y = glue.span_attention(*a, first, last), glue.attention(*c, True)
     for s, t in zip((x, *torch.autograd.grad(x, a, do)), (y, *torch.autograd.grad(y, c, do))):
         assert ((s - t).abs().max() / t.abs().max()).item() <= 1e-2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_nan_query_is_nan_alone(cuda, dim):
+    """A NaN in one query: its output and log-sum-exp are NaN, no other's are."""
+    import torch
+
+    from torobi_b200 import glue
+
+    b, s, h, hk = 2, 300, 4, 2
+    first, last = _spans(cuda, [[0] * 130 + [1] * 170] * b)
+    q, k, v, _ = _inputs(cuda, 77, b, s, h, hk, dim)
+    want, wlse = glue.span_attention_forward(q, k, v, first, last)
+    q[1, 200, 3, 7] = float("nan")
+    o, lse = glue.span_attention_forward(q, k, v, first, last)
+    assert o[1, 200, 3].isnan().all() and lse[1, 3, 200].isnan()
+    o[1, 200, 3], lse[1, 3, 200] = want[1, 200, 3], wlse[1, 3, 200]
+    assert torch.equal(o, want) and torch.equal(lse, wlse)
+
+
+@pytest.mark.gpu
+def test_span_attention_past_32_bit_offsets(cuda):
+    """Three rows of 262144 positions, 32 heads of 128: the last row's queries,
+    outputs and gradients lie past 2^31 elements.  It gives what it gives alone."""
+    import torch
+
+    from torobi_b200 import glue
+
+    b, s, h, hk, d = 3, 262144, 32, 8, 128
+    g = torch.Generator(device=cuda).manual_seed(3)
+
+    def mk(n):
+        return torch.randn(b, s, n, d, device=cuda, dtype=torch.bfloat16, generator=g)
+
+    q, k, v, do = mk(h), mk(hk), mk(hk), mk(h)
+    i = torch.arange(s, device=cuda, dtype=torch.int32)
+    docs = torch.stack([i // 190, i // 77, i // 301])
+    docs[2, -50:] = -1
+    first, last = glue.document_spans(docs)
+    o, lse = glue.span_attention_forward(q, k, v, first, last)
+    grads = glue.span_attention_backward(q, k, v, first, last, o, do, lse)
+    alone = [t[2:].clone() for t in (q, k, v, first, last)]
+    o1, lse1 = glue.span_attention_forward(*alone)
+    assert torch.equal(o[2:], o1) and torch.equal(lse[2:], lse1)
+    grads1 = glue.span_attention_backward(*alone, o1, do[2:].clone(), lse1)
+    for a, c in zip(grads, grads1):
+        assert torch.equal(a[2:], c)
+    assert (o[2, -50:] == 0).all() and (grads[0][2, -50:] == 0).all()
+    # And its last document, in a row of its own: |o| errs by R (sum p |v| + |o|).
+    at = (s - 51) // 301 * 301
+    part = [t[2:, at:s - 50].contiguous() for t in (q, k, v)]
+    one = torch.zeros(1, s - 50 - at, dtype=torch.int32, device=cuda)
+    o2, _ = _check(*part, do[2:, at:s - 50].contiguous(), *glue.document_spans(one))
+    off = (o2.double() - o[2:, at:s - 50].double()).abs().max().item()
+    assert off <= 2 * R * 2 * part[2].abs().max().item()
 
 
 @pytest.mark.gpu

@@ -21,6 +21,25 @@
 namespace tq {
 namespace {
 
+constexpr float kRescaleLog2 = 8.0f;  // move m only when the row max grows by > 2^8
+
+// 2^x on the FMA pipe, for a share of the softmax's exponentials (the MUFU
+// unit alone would take as long as the tile's MMAs).  Range reduction by the
+// round-to-nearest of x + 1.5 * 2^23 (n = nearest integer, f = x - n in
+// [-0.5, 0.5]), 2^f by a cubic least-squares fit in relative error (fitted for
+// this kernel; max relative error 7.5e-5 in f32, below bf16's 2^-9), and n
+// added to the exponent field.  x is clamped at -125 so that the result stays
+// a normal number.
+__device__ __forceinline__ float exp2_poly(float x) {
+  x = fmaxf(x, -125.0f);
+  const float t = __fadd_rn(x, 12582912.0f);
+  const float f = __fsub_rn(x, __fsub_rn(t, 12582912.0f));
+  float p = fmaf(0.055174145847558975f, f, 0.24261757731437683f);
+  p = fmaf(p, f, 0.6932610869407654f);
+  p = fmaf(p, f, 0.9999275803565979f);
+  return __uint_as_float(__float_as_uint(p) + (__float_as_uint(t) << 23));
+}
+
 struct AttnShape {
   int batch, seq, heads, kv_heads, group, n_tiles;
   int causal;

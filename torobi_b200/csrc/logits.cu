@@ -29,7 +29,6 @@
 
 #include <cmath>
 #include <cstddef>
-#include <type_traits>
 
 #include "tq_ptx.cuh"
 #include "tq_runtime.h"
@@ -212,14 +211,16 @@ struct Row {
   }
 };
 
-__device__ __forceinline__ void ldg_chunk(const void* p, uint32_t (&w)[8]) {
-  asm("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+// A chunk that is read once.  (Not the read-only path: the kernel that writes
+// the row may still run when this one is started.)
+__device__ __forceinline__ void ld_chunk_once(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
                  "=r"(w[6]), "=r"(w[7])
-               : "l"(p));
+               : "l"(p)
+               : "memory");
 }
 
-// Coherent form, for rows that the kernel's own stores overwrite.
 __device__ __forceinline__ void ld_chunk(const void* p, uint32_t (&w)[8]) {
   asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
@@ -476,7 +477,7 @@ __device__ __forceinline__ void gather(const Row<T>& row, int l0, int l1, uint32
     const int c = sh.chunks[i];
     uint32_t w[8];
     if (c >= row.lo && c < row.hi)
-      ldg_chunk(row.chunk(c), w);
+      ld_chunk_once(row.chunk(c), w);
     else
       row.load_edge(c, w);
     float f[CH];
@@ -705,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
   for (; ch + (U - 1) * kThreads < hi; ch += U * kThreads) {
     uint32_t w[U][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) ldg_chunk(row.chunk(ch + u * kThreads), w[u]);
+    for (int u = 0; u < U; ++u) ld_chunk_once(row.chunk(ch + u * kThreads), w[u]);
     typename Elem<T>::Max all;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -722,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
   }
   for (; ch < hi; ch += kThreads) {
     uint32_t w[1][8];
-    ldg_chunk(row.chunk(ch), w[0]);
+    ld_chunk_once(row.chunk(ch), w[0]);
     one(ch, w);
   }
   block_sums<kEntropy>(v, sums, c);
@@ -1011,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const Dis
   for (; ch + (U - 1) * kThreads < hi; ch += U * kThreads) {
     uint32_t w[U][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) ldg_chunk(row.chunk(ch + u * kThreads), w[u]);
+    for (int u = 0; u < U; ++u) ld_chunk_once(row.chunk(ch + u * kThreads), w[u]);
     typename Elem<T>::Max all = Elem<T>::chunk_max(w[0]);
 #pragma unroll
     for (int u = 1; u < U; ++u) all = Elem<T>::join(all, Elem<T>::chunk_max(w[u]));
@@ -1019,7 +1020,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const Dis
   }
   for (; ch < hi; ch += kThreads) {
     uint32_t w[1][8];
-    ldg_chunk(row.chunk(ch), w[0]);
+    ld_chunk_once(row.chunk(ch), w[0]);
     one(w);
   }
   block_sums<M>(v, sums, c);

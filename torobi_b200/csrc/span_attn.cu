@@ -70,7 +70,9 @@ __device__ __forceinline__ Span load_span(const int* first, const int* last, int
                                           int seq) {
   if (i >= seq) return {0, 0};
   const size_t at = static_cast<size_t>(b) * seq + i;
-  const int lo = max(__ldg(first + at), 0), hi = min(__ldg(last + at), seq);
+  // Plain loads: the spans may be the last kernel's, which still ran when this
+  // one was started.
+  const int lo = max(first[at], 0), hi = min(last[at], seq);
   return lo < hi ? Span{lo, hi} : Span{0, 0};
 }
 
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         ok = ok && mbar_wait(o_done(w), (steps - 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: sees nothing
         const F2 inv2 = f2(inv, inv);
 #pragma unroll
         for (int c4 = 0; c4 < D / 32; ++c4) {
@@ -669,7 +671,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             wd[e] = pack_bf16(pair_of(o[2 * e], o[2 * e + 1]) * inv2);
           if (valid) store_row(orow + c4 * 32, wd, wide);
         }
-        if (valid) *lse = l > 0.0f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        if (valid) *lse = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
       } else if (valid) {  // no row of the tile sees anything
         const uint32_t zero[16] = {};
 #pragma unroll

@@ -233,6 +233,8 @@ def document_spans(documents: torch.Tensor, prefix: torch.Tensor | None = None,
         if prefix.shape != documents.shape or prefix.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"[{op}] prefix must be int32 or int64 {tuple(documents.shape)}, got "
                              f"{prefix.dtype} {tuple(prefix.shape)}")
+        if prefix.dtype == torch.int64:
+            prefix = prefix.clamp(max=2 ** 31 - 1).clamp_(min=0)
         prefix = prefix.to(torch.int32).contiguous()
     documents = documents.contiguous()
     b, s = documents.shape

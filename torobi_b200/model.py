@@ -159,7 +159,7 @@ def _counted(documents: torch.Tensor, prefix: torch.Tensor | None) -> torch.Tens
     if prefix is not None:
         first, _ = glue.document_spans(documents)
         index = torch.arange(documents.shape[1], device=documents.device)
-        counted &= (index >= first + prefix)[:, 1:]
+        counted &= (index - first >= prefix)[:, 1:]
     return counted
 
 
@@ -348,10 +348,10 @@ class QLoRACausalLM:
         probability (0 where the target does not count), the entropy and the
         ``top`` most likely alternatives (``glue.token_logprobs``);
         differentiable through the first two."""
+        z = self.logits(self.hidden(ids, documents, prefix)[:, :-1])
         tgt = ids[:, 1:]
         if documents is not None:
             tgt = torch.where(_counted(documents, prefix), tgt, -1)
-        z = self.logits(self.hidden(ids, documents, prefix)[:, :-1])
         return glue.token_logprobs(z, tgt, top=top, temperature=temperature, inplace=True)
 
     def distill_loss(self, ids: torch.Tensor, teacher_ids: torch.Tensor,
