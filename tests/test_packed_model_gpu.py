@@ -157,6 +157,27 @@ def test_a_student_distilled_from_a_teachers_alternatives(cuda, graph):
         trainer.step(ids, docs[:1])
 
 
+def test_a_captured_step_beside_a_score_that_keeps_its_graph(cuda):
+    """The teacher's answer is held with its graph while the student's step is
+    captured and replayed; the teacher's own backward still runs after."""
+    import torch
+
+    from torobi_b200.train import AdamWConfig, Trainer
+
+    teacher, student = _model(3), _model(4)
+    ids, docs, _ = _rows(cuda, [[100], [64, 64]], 128)
+    held = teacher.token_logprobs(ids, top=8, documents=docs)
+    assert held.logprobs.requires_grad
+    trainers = [Trainer(m, AdamWConfig(lr=1e-3), micro_batch=2, graph=g, objective=m.distill_loss)
+                for m, g in ((student, True), (_model(4), False))]
+    for far in (1e-5, 1e-2):  # the second after a step of 1e-3 by gradients' signs
+        a, b = (t.step(ids, held.top_ids, held.top_logprobs, docs).item() for t in trainers)
+        assert abs(a - b) <= far * abs(a)
+    teacher.store.zero_grad()
+    held.logprobs.sum().backward()
+    assert torch.isfinite(teacher.store.grads).all() and (teacher.store.grads != 0).any()
+
+
 def test_distill_gradient_reaches_the_adapters_by_the_formula(cuda):
     """The adapters' gradients of distill_loss against those of the same loss
     written in torch operations on the model's logits."""

@@ -320,6 +320,14 @@ def _trigger(device: torch.device) -> torch.Tensor:
     return t
 
 
+def renew_trigger(device: torch.device) -> None:
+    """Another trigger from here on.  Autograd keeps one accumulation node per
+    leaf while any graph over it lives, bound to the stream it was made on: a
+    backward pass that is captured must not meet the node of an eager graph
+    that is still held (a score kept with its graph)."""
+    _TRIGGERS.pop(device, None)
+
+
 def qlora_linear(x: torch.Tensor, w: QuantizedWeight, adapter: Adapter | None = None):
     """y = x W^T (+ bias) (+ LoRA), differentiable wrt x (and the adapter)."""
     trig = _trigger(x.device) if (adapter is not None and torch.is_grad_enabled()) else None

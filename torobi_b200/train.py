@@ -26,6 +26,7 @@ import torch
 
 from . import ops
 from ._lib import TQ_DTYPE_F32, check, lib
+from .qlora import renew_trigger
 
 
 # ------------------------------------------------------------ batch plan ---
@@ -270,6 +271,7 @@ class Trainer:
                 for _ in range(2):
                     self._gradients(*static)
             torch.cuda.current_stream().wait_stream(side)
+            renew_trigger(rows[0].device)
             g = torch.cuda.CUDAGraph()
             with torch.cuda.graph(g, capture_error_mode="thread_local"):
                 self._gradients(*static)
