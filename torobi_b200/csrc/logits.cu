@@ -29,6 +29,7 @@
 
 #include <cmath>
 #include <cstddef>
+#include <type_traits>
 
 #include "tq_ptx.cuh"
 #include "tq_runtime.h"
@@ -227,6 +228,22 @@ __device__ __forceinline__ void ld_chunk(const void* p, uint32_t (&w)[8]) {
                  "=r"(w[6]), "=r"(w[7])
                : "l"(p)
                : "memory");
+}
+
+// The chunks c + u * kThreads, all in flight at once.  PART: those below `end`,
+// -inf for the others (a thread's last round: one by one they would cost as
+// many latencies).
+template <bool PART, typename T, int U>
+__device__ __forceinline__ void ld_chunks(const Row<T>& row, int c, int end, uint32_t (&w)[U][8]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!PART || c + u * kThreads < end) {
+      ld_chunk_once(row.chunk(c + u * kThreads), w[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[u][i] = Elem<T>::NEG_INF2;
+    }
+  }
 }
 
 __device__ __forceinline__ void st_chunk(void* p, const uint32_t (&w)[8]) {
@@ -702,16 +719,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
     row.load_edge(row.n - 1, w[0]);
     one(row.n - 1, w);
   }
-  int ch = lo + threadIdx.x;
-  for (; ch + (U - 1) * kThreads < hi; ch += U * kThreads) {
+  auto many = [&](int ch, auto part) {
+    constexpr bool PART = decltype(part)::value;
     uint32_t w[U][8];
-#pragma unroll
-    for (int u = 0; u < U; ++u) ld_chunk_once(row.chunk(ch + u * kThreads), w[u]);
+    ld_chunks<PART>(row, ch, hi, w);
     typename Elem<T>::Max all;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const typename Elem<T>::Max cm = Elem<T>::chunk_max(w[u]);
-      if constexpr (TOP) keys[ch + u * kThreads - c0] = Elem<T>::bits(cm);
+      if constexpr (TOP)
+        if (!PART || ch + u * kThreads < hi) keys[ch + u * kThreads - c0] = Elem<T>::bits(cm);
       all = u ? Elem<T>::join(all, cm) : cm;
     }
     const float mx = Elem<T>::value(all);
@@ -720,7 +737,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
       any = true;
     }
     add_chunks<T, kEntropy, U>(v, w, mx, c);
-  }
+  };
+  int ch = lo + threadIdx.x;
+  for (; ch + (U - 1) * kThreads < hi; ch += U * kThreads) many(ch, std::false_type());
+  if constexpr (!TOP)  // (with the selection it would spill registers)
+    if (ch + kThreads < hi) {
+      many(ch, std::true_type());
+      ch = hi;
+    }
   for (; ch < hi; ch += kThreads) {
     uint32_t w[1][8];
     ld_chunk_once(row.chunk(ch), w[0]);
@@ -778,12 +802,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const Lo
 // --------------------------------------------------------------- gradients --
 
 // Hands grad(j0, f) the logits f[0, N) of this CTA's share of a row, j0 the
-// index of the first, and stores what it leaves in f.  SAME: z's and dz's rows start at the same
-// offset in their 32-byte chunks, so a chunk is loaded and stored whole;
-// otherwise elements go one by one.
-template <typename T, bool SAME, typename Grad>
+// index of the first, and stores what it leaves in f.  ready() is called once
+// by every thread before grad, with the first loads under way.  SAME: z's and
+// dz's rows start at the same offset in their 32-byte chunks, so a chunk is
+// loaded and stored whole; otherwise elements go one by one.
+template <typename T, bool SAME, typename Ready, typename Grad>
 __device__ __forceinline__ void row_gradient(const T* z, T* dz, int vocab, int part, int parts,
-                                             Grad&& grad) {
+                                             Ready&& ready, Grad&& grad) {
   constexpr int CH = Elem<T>::CH;
   const Row<T> row(z, vocab);
   const int per = (row.n + parts - 1) / parts;
@@ -799,18 +824,19 @@ __device__ __forceinline__ void row_gradient(const T* z, T* dz, int vocab, int p
       st_chunk(out + static_cast<int64_t>(c) * CH, w);
     };
     // Two chunks' loads in flight a thread before either is finished.
+    uint32_t w0[8], w1[8];
     int c = lo + threadIdx.x;
-    for (; c + kThreads < hi; c += 2 * kThreads) {
-      uint32_t w0[8], w1[8];
-      ld_chunk(row.chunk(c), w0);
-      ld_chunk(row.chunk(c + kThreads), w1);
+    auto load = [&] {
+      if (c < hi) ld_chunk(row.chunk(c), w0);
+      if (c + kThreads < hi) ld_chunk(row.chunk(c + kThreads), w1);
+    };
+    load();
+    ready();
+    while (c < hi) {
       finish(c, w0);
-      finish(c + kThreads, w1);
-    }
-    if (c < hi) {
-      uint32_t w0[8];
-      ld_chunk(row.chunk(c), w0);
-      finish(c, w0);
+      if (c + kThreads < hi) finish(c + kThreads, w1);
+      c += 2 * kThreads;
+      load();
     }
     // The first and last chunk, where they reach out of the row.
     const int64_t head = c0 == 0 && row.lo == 1 ? min(CH - row.off, vocab) : 0;
@@ -825,6 +851,7 @@ __device__ __forceinline__ void row_gradient(const T* z, T* dz, int vocab, int p
       Elem<T>::store(dz + j, f[0]);
     }
   } else {
+    ready();
     const int64_t j0 = max(row.first(c0), static_cast<int64_t>(0));
     const int64_t j1 = min(row.first(c1), static_cast<int64_t>(vocab));
     for (int64_t j = j0 + threadIdx.x; j < j1; j += kThreads) {
@@ -854,22 +881,30 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const LogprobGra
   // Last row first: the forward's last rows may still be in L2.
   const int64_t r = gridDim.x / p.parts - 1 - blockIdx.x / p.parts;
   const int part = static_cast<int>(blockIdx.x % p.parts);
-  const float4 st = p.stats[r];  // m, log2 s, entropy
-  const int64_t tok = p.tokens[r];
-  const bool picked = tok >= 0 && tok < p.vocab;
-  const float g = picked && p.dlogprobs ? p.dlogprobs[r] : 0.0f;
-  const float h = p.dentropy ? p.dentropy[r] : 0.0f;
-  const float c = p.c, m = st.x;
-  // q_j (g + h (ln q_j + H)) / T = 2^x (ca + cb x); a row that no gradient
-  // reaches, or without a distribution, gets zeros whatever it holds.
-  const bool zero = (g == 0.0f && h == 0.0f) || st.y == -INFINITY;
-  const float inv_s = exp2f(-st.y) * p.inv_t;
-  const float ca = inv_s * (g + h * (st.z - st.y * kLn2));
-  const float cb = inv_s * h * kLn2;
-  const float hot = zero ? 0.0f : g * p.inv_t;
+  const float c = p.c;
+  int64_t tok;
+  float m, ca, cb, hot;
+  bool zero;
   row_gradient<T, SAME>(
       static_cast<const T*>(p.z) + r * p.ld, static_cast<T*>(p.dz) + r * p.ld_out, p.vocab, part,
-      p.parts, [&](int64_t j0, auto& f) {
+      p.parts,
+      [&] {
+        const float4 st = p.stats[r];  // m, log2 s, entropy
+        tok = p.tokens[r];
+        const bool picked = tok >= 0 && tok < p.vocab;
+        float g = p.dlogprobs ? p.dlogprobs[r] : 0.0f;
+        const float h = p.dentropy ? p.dentropy[r] : 0.0f;
+        if (!picked) g = 0.0f;
+        m = st.x;
+        // q_j (g + h (ln q_j + H)) / T = 2^x (ca + cb x); a row that no gradient
+        // reaches, or without a distribution, gets zeros whatever it holds.
+        zero = (g == 0.0f && h == 0.0f) || st.y == -INFINITY;
+        const float inv_s = exp2f(-st.y) * p.inv_t;
+        ca = inv_s * (g + h * (st.z - st.y * kLn2));
+        cb = inv_s * h * kLn2;
+        hot = zero ? 0.0f : g * p.inv_t;
+      },
+      [&](int64_t j0, auto& f) {
         constexpr int N = sizeof(f) / sizeof(float);
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -1008,17 +1043,19 @@ __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const Dis
     row.load_edge(row.n - 1, w[0]);
     one(w);
   }
-  int ch = lo + threadIdx.x;
-  for (; ch + (U - 1) * kThreads < hi; ch += U * kThreads) {
+  auto many = [&](int ch, auto part) {
     uint32_t w[U][8];
-#pragma unroll
-    for (int u = 0; u < U; ++u) ld_chunk_once(row.chunk(ch + u * kThreads), w[u]);
+    ld_chunks<decltype(part)::value>(row, ch, hi, w);
     typename Elem<T>::Max all = Elem<T>::chunk_max(w[0]);
 #pragma unroll
     for (int u = 1; u < U; ++u) all = Elem<T>::join(all, Elem<T>::chunk_max(w[u]));
     add_chunks<T, M, U>(v, w, Elem<T>::value(all), c);
-  }
-  for (; ch < hi; ch += kThreads) {
+  };
+  int ch = lo + threadIdx.x;
+  for (; ch + (U - 1) * kThreads < hi; ch += U * kThreads) many(ch, std::false_type());
+  if (ch + kThreads < hi) {
+    many(ch, std::true_type());
+  } else if (ch < hi) {
     uint32_t w[1][8];
     ld_chunk_once(row.chunk(ch), w[0]);
     one(w);
@@ -1086,56 +1123,59 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGrad
   const T* const z = static_cast<const T*>(p.z) + r * p.ld;
   T* const dz = static_cast<T*>(p.dz) + r * p.ld_out;
   const int k = p.teacher.k;
-  const float4 st = p.stats[r];
-  const int64_t target = p.targets ? p.targets[r] : -1;
-  const bool picked = target >= 0 && target < p.vocab;
-  const float u = p.dkl ? p.dkl[r] * p.inv_t : 0.0f;
-  const float v = picked && p.dce ? p.dce[r] : 0.0f;
-  if (threadIdx.x < 32) {
-    const Alternatives a =
-        weigh(k, p.vocab, p.c, [&](int e) { return p.teacher.id(r * k + e); },
-              [&](int e) { return p.teacher.logit(r * k + e); });
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int e = threadIdx.x + 32 * i;
-      if (e < k) {
-        ids[e] = a.id[i];
-        off[e] = a.id[i] < 0 ? 0.0f : u * a.p[i];
-      }
-    }
-    if (threadIdx.x == 0) {
-      ids[k] = picked ? static_cast<int>(target) : -1;
-      off[k] = v;
-    }
-  }
-  // Whether anything of the teacher's is given; also orders ids and off.
-  const bool given =
-      __syncthreads_or(threadIdx.x < 32 ? [&] {
-        bool g = false;
-        for (int e = threadIdx.x; e < k; e += 32) g |= ids[e] >= 0;
-        return g;
-      }() : false);
-  const float us = given ? u : 0.0f;
-  // A row that no gradient reaches gets zeros whatever it holds; one without
-  // a distribution has q = 0.
-  const bool dead = st.y == -INFINITY;
-  const bool zero = us == 0.0f && v == 0.0f;
-  float ca = dead ? 0.0f : us * exp2f(-st.y);
-  float cb = dead ? 0.0f : v * exp2f(-st.z);
-  if (M == kPlain) ca += cb;
+  float m, ca, cb;
+  bool zero, dead;
   auto soft = [&](float f) {
     if (zero || dead) return 0.0f;
-    const float d = f - st.x;
+    const float d = f - m;
     const float e = ex2_approx(d * p.c);
     if (M == kSquare) return e * fmaf(cb, e, ca);
     if (M == kTwo) return fmaf(cb, ex2_approx(d * kLog2e), ca * e);
     return ca * e;
   };
-  // The given elements' logits, before anything is written over them.
-  const int mine = static_cast<int>(threadIdx.x) <= k ? ids[threadIdx.x] : -1;
-  const float zi = mine >= 0 ? Elem<T>::load(z + mine) : 0.0f;
-  __syncthreads();
-  row_gradient<T, SAME>(z, dz, p.vocab, part, p.parts, [&](int64_t, auto& f) {
+  int mine;
+  float zi;
+  auto ready = [&] {
+    const float4 st = p.stats[r];
+    const int64_t target = p.targets ? p.targets[r] : -1;
+    const bool picked = target >= 0 && target < p.vocab;
+    const float u = p.dkl ? p.dkl[r] * p.inv_t : 0.0f;
+    const float v = picked && p.dce ? p.dce[r] : 0.0f;
+    bool any = false;
+    if (threadIdx.x < 32) {
+      const Alternatives a =
+          weigh(k, p.vocab, p.c, [&](int e) { return p.teacher.id(r * k + e); },
+                [&](int e) { return p.teacher.logit(r * k + e); });
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        const int e = threadIdx.x + 32 * i;
+        if (e < k) {
+          ids[e] = a.id[i];
+          off[e] = a.id[i] < 0 ? 0.0f : u * a.p[i];
+          any |= a.id[i] >= 0;
+        }
+      }
+      if (threadIdx.x == 0) {
+        ids[k] = picked ? static_cast<int>(target) : -1;
+        off[k] = v;
+      }
+    }
+    // Whether anything of the teacher's is given; also orders ids and off.
+    const float us = __syncthreads_or(any) ? u : 0.0f;
+    // A row that no gradient reaches gets zeros whatever it holds; one without
+    // a distribution has q = 0.
+    m = st.x;
+    dead = st.y == -INFINITY;
+    zero = us == 0.0f && v == 0.0f;
+    ca = dead ? 0.0f : us * exp2f(-st.y);
+    cb = dead ? 0.0f : v * exp2f(-st.z);
+    if (M == kPlain) ca += cb;
+    // The given elements' logits, before anything is written over them.
+    mine = static_cast<int>(threadIdx.x) <= k ? ids[threadIdx.x] : -1;
+    zi = mine >= 0 ? Elem<T>::load(z + mine) : 0.0f;
+    __syncthreads();
+  };
+  row_gradient<T, SAME>(z, dz, p.vocab, part, p.parts, ready, [&](int64_t, auto& f) {
     constexpr int N = sizeof(f) / sizeof(float);
 #pragma unroll
     for (int e = 0; e < N; ++e) f[e] = soft(f[e]);
@@ -1175,14 +1215,35 @@ int check_rows(const char* who, const void* z, int dtype, int64_t rows, int64_t 
   return TQ_OK;
 }
 
-// How many CTAs share a row: enough that the grid offers every SM several
-// (forward: in clusters of a power of two), none with less than 512 chunks.
-int split_for(int64_t rows, int64_t vocab, int ch, int most) {
-  const int64_t want = 4ll * sm_count();
+// Forward: how many CTAs (a cluster of a power of two) share a row: enough that
+// the grid has one for each of 1.5 SMs, none with less than 512 chunks.  What a
+// CTA costs beside its chunks (the joins, the selection) is not split: 148 x
+// 151936 takes 20.5 us with one CTA a row, 16.5 with two, 22.5 with four; 257 x
+// 96259 f32 22.6, 24.4 and 26.6; 511 x 151936 with 20 alternatives 43, 51 and
+// 70; 67 x 128256 with 5 22.6, 20.5 and 18.5.
+int split_for(int64_t rows, int64_t vocab, int ch) {
+  const int64_t want = 3ll * sm_count() / 2;
   int s = 1;
-  while (s < most && rows * s < want && vocab / (2 * s) >= 512ll * ch) s *= 2;
+  while (s < kMaxSplit && rows * s < want && vocab / (2 * s) >= 512ll * ch) s *= 2;
   return s;
 }
+
+// Backward: how many CTAs write a row.  As many as leave each `least` chunks
+// (short CTAs close together in memory, and a short last wave: 2046 x 128256 by
+// one CTA a row 177 us, two 168, four 164, eight 160), and down to 512 where
+// the grid would not offer every SM several.
+int parts_for(int64_t rows, int64_t vocab, int ch, int least) {
+  const int64_t chunks = vocab / ch, want = 4ll * sm_count();
+  int s = 1;
+  while (s < 16 && chunks >= 2ll * s * (rows * s < want ? 512 : least)) s *= 2;
+  return s;
+}
+
+// What a CTA of a backward kernel reads before its chunks can be finished is
+// hidden behind about so many of them: a few numbers, or the alternatives and
+// their softmax (four CTAs a row of 2046 x 128256 170 us, one 188, eight 189).
+constexpr int kLeastLogprobs = 900;
+constexpr int kLeastDistill = 1800;
 
 // Whether z's and dz's rows all start at the same offset in a 32-byte chunk.
 bool same_offset(const void* z, const void* dz, int64_t rows, int64_t ld, int64_t ld_out,
@@ -1221,7 +1282,7 @@ extern "C" int tq_token_logprobs_fwd(const void* logits, int dtype, const int64_
   p.tokens = tokens;
   p.ld = ld;
   p.vocab = static_cast<int>(vocab);
-  p.split = split_for(rows, vocab, ch, kMaxSplit);
+  p.split = split_for(rows, vocab, ch);
   p.top = static_cast<int>(top);
   p.c = kLog2e / temperature;
   p.inv_t = 1.0f / temperature;
@@ -1280,7 +1341,7 @@ extern "C" int tq_token_logprobs_bwd(const void* logits, int dtype, const int64_
   p.ld = ld;
   p.ld_out = ld_out;
   p.vocab = static_cast<int>(vocab);
-  p.parts = split_for(rows, vocab, 32 / elem_bytes(dtype), 16);
+  p.parts = parts_for(rows, vocab, 32 / elem_bytes(dtype), kLeastLogprobs);
   p.c = kLog2e / temperature;
   p.inv_t = 1.0f / temperature;
   const bool same = same_offset(logits, dlogits, rows, ld, ld_out, elem_bytes(dtype));
@@ -1348,7 +1409,7 @@ extern "C" int tq_distill_fwd(const void* logits, int dtype, const void* teacher
   p.targets = targets;
   p.ld = ld;
   p.vocab = static_cast<int>(vocab);
-  p.split = split_for(rows, vocab, 32 / elem_bytes(dtype), kMaxSplit);
+  p.split = split_for(rows, vocab, 32 / elem_bytes(dtype));
   p.c = kLog2e / temperature;
   p.inv_t = 1.0f / temperature;
   p.kl = kl;
@@ -1398,7 +1459,7 @@ extern "C" int tq_distill_bwd(const void* logits, int dtype, const void* teacher
   p.ld = ld;
   p.ld_out = ld_out;
   p.vocab = static_cast<int>(vocab);
-  p.parts = split_for(rows, vocab, 32 / elem_bytes(dtype), 16);
+  p.parts = parts_for(rows, vocab, 32 / elem_bytes(dtype), kLeastDistill);
   p.c = kLog2e / temperature;
   p.inv_t = 1.0f / temperature;
   const bool same = same_offset(logits, dlogits, rows, ld, ld_out, elem_bytes(dtype));
