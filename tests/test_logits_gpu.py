@@ -519,6 +519,8 @@ DISTILL = [
     (2, 151936, 64, "bf16", 2.0, True, 0, 0, "int32", "bf16"),
     (4, 32003, 50, "f32", 1.0, True, 61, 0, "int64", "f32"),
     (650, 4099, 5, "bf16", 3.0, False, 0, 0, "int64", "f32"),
+    (3, 128256, 64, "bf16", 3.0, True, 0, 0, "int64", "f32"),   # sums at two temperatures
+    (33, 5003, 8, "f32", 1.7, True, 0, 0, "int64", "f32"),
 ]
 
 
@@ -626,6 +628,26 @@ def test_given_at_minus_infinity_and_dead_rows(cuda):
 
 
 # ------------------------------------------------------------- how it is called --
+
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0])
+def test_distillation_nan_and_inf_rows(cuda, temperature):
+    """A NaN or +inf anywhere makes its row's answers NaN, at any temperature;
+    the rows beside it are as they were."""
+    import torch
+
+    from torobi_b200 import glue
+
+    z = _logits(cuda, 9, 4099, "bf16", 31).contiguous()
+    ids = torch.arange(9 * 6, device=cuda).view(9, 6) * 70
+    given, targets = torch.randn(9, 6, device=cuda), torch.full((9,), 7, device=cuda)
+    want = glue.distillation(z, ids, given, targets=targets, temperature=temperature)
+    for r, (at, value) in enumerate([(0, "nan"), (4098, "nan"), (2000, "inf"), (2002, "inf"),
+                                     (17, "-nan"), (33, "inf")]):
+        z[r, at] = float(value)
+    got = glue.distillation(z, ids, given, targets=targets, temperature=temperature)
+    for a, b in zip(got, want):
+        assert a[:6].isnan().all() and torch.equal(a[6:], b[6:])
+
 
 def test_calls_in_a_graph_and_on_another_stream(cuda):
     """Forward and backward on a side stream, then captured with static
