@@ -712,19 +712,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //          there too it was 1800.
 // Which CTA does a tile changes no result.
 
-// Over a 64-row packed query tile: the keys that any row sees, [lo, hi), and
-// those that every filled row sees, [all_lo, all_hi).
-struct SpanTile {
-  int lo, hi, all_lo, all_hi;
-};
-
 // The workspace: statistics [batch, heads / pack, tiles64, 64], spans (first
-// key, how many) [batch, tiles64, 64], tiles [batch, tiles64].
+// key, how many) [batch, tiles64, 64], tiles: what any row of a 64-row packed
+// query tile sees [batch, tiles64].
 struct BwdWork {
   float* nlse2;
   float* ndelta;
   int2* rows;
-  SpanTile* tiles;
+  Span* tiles;
   size_t bytes;
 };
 
@@ -736,84 +731,101 @@ struct PrepParams {
   const int* first;
   const int* last;
   BwdWork work;
-  int dim;
   unsigned row_blocks;  // blocks from here on do the spans, a warp a tile
 };
 
-// Eight lanes per row, dim / 8 elements each.
-__global__ void __launch_bounds__(256) span_prep_kernel(const PrepParams p) {
+__device__ __forceinline__ void load_16(const uint16_t* p, bool wide, uint32_t (&w)[8]) {
+  if (wide) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]),
+                   "=r"(w[6]), "=r"(w[7])
+                 : "l"(p)
+                 : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+  }
+}
+
+// A CTA a 64-row tile: two rows a thread, 16 elements of each.  Bound by
+// reading out and dout (packed rows of 2048: 134 MB).
+template <int D>
+__global__ void __launch_bounds__(2 * D) span_prep_kernel(const PrepParams p) {
+  constexpr int LANES = D / 16;
   griddep_wait();
   griddep_launch_dependents();
   const SpanShape& sh = p.sh;
   const int filled_rows = sh.pack * sh.pos64;
   if (blockIdx.x >= p.row_blocks) {
-    const long long t = static_cast<long long>(blockIdx.x - p.row_blocks) * 8 + (threadIdx.x >> 5);
-    if (t >= static_cast<long long>(sh.batch) * sh.tiles64) return;
-    const int b = static_cast<int>(t / sh.tiles64);
-    const int i0 = static_cast<int>(t % sh.tiles64) * sh.pos64;
-    SpanTile s{sh.seq, 0, 0, sh.seq};
+    const int t = (blockIdx.x - p.row_blocks) * (2 * D / 32) + (threadIdx.x >> 5);
+    if (t >= sh.batch * sh.tiles64) return;
+    const int b = t / sh.tiles64;
+    const int i0 = t % sh.tiles64 * sh.pos64;
+    Span s{sh.seq, 0};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int r = e * 32 + (threadIdx.x & 31);
       const bool filled = r < filled_rows;
       const Span sp =
           filled ? load_span(p.first, p.last, b, i0 + r / sh.pack, sh.seq) : Span{0, 0};
-      // A row that holds nothing (its lse2 is +inf) must not make the tile a
-      // masked one.
-      p.work.rows[t * kHalf + r] = filled ? make_int2(sp.lo, sp.hi - sp.lo)
-                                          : make_int2(0, sh.seq);
+      // A row that holds nothing (P = 0 by its statistics) must not make the
+      // tile a masked one.
+      p.work.rows[static_cast<size_t>(t) * kHalf + r] =
+          filled ? make_int2(sp.lo, sp.hi - sp.lo) : make_int2(0, sh.seq);
       if (!filled) continue;
       if (sp.lo < sp.hi) s.lo = min(s.lo, sp.lo);
       s.hi = max(s.hi, sp.hi);
-      s.all_lo = max(s.all_lo, sp.lo);
-      s.all_hi = min(s.all_hi, sp.hi);
     }
     s.lo = __reduce_min_sync(0xffffffffu, s.lo);
     s.hi = __reduce_max_sync(0xffffffffu, s.hi);
-    s.all_lo = __reduce_max_sync(0xffffffffu, s.all_lo);
-    s.all_hi = __reduce_min_sync(0xffffffffu, s.all_hi);
     if ((threadIdx.x & 31) == 0) p.work.tiles[t] = s;
     return;
   }
-  const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 3;
-  const int sub = threadIdx.x & 7;
+  const int t = blockIdx.x;
   const int groups = sh.heads / sh.pack;
-  const bool in = row < static_cast<long long>(sh.batch) * groups * sh.tiles64 * kHalf;
-  const long long t = in ? row / kHalf : 0;
-  const int r = static_cast<int>(row % kHalf);
-  const int bg = static_cast<int>(t / sh.tiles64);
-  const int b = bg / groups;
-  const int h = bg % groups * sh.pack + r % sh.pack;
-  const int i = static_cast<int>(t % sh.tiles64) * sh.pos64 + r / sh.pack;
-  const bool real = in && r < filled_rows && i < sh.seq;
-  float acc = 0.0f;
-  if (real) {
-    const int per = p.dim / 8;
-    const size_t off = ((static_cast<size_t>(b) * sh.seq + i) * sh.heads + h) * p.dim + sub * per;
-    for (int c = 0; c < per; c += 8) {
-      const uint4 o = *reinterpret_cast<const uint4*>(p.out + off + c);
-      const uint4 d = *reinterpret_cast<const uint4*>(p.dout + off + c);
-      const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-      const uint32_t dw[4] = {d.x, d.y, d.z, d.w};
+  const int bg = t / sh.tiles64;
+  const int b = bg / groups, h0 = bg % groups * sh.pack;
+  const int i0 = t % sh.tiles64 * sh.pos64;
+  const int sub = threadIdx.x % LANES;
+  const bool wide = wide_rows(p.out) && wide_rows(p.dout);
+  uint32_t o[2][8], d[2][8];
+  float l[2];
+  bool real[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc = fmaf(__uint_as_float(ow[e] << 16), __uint_as_float(dw[e] << 16), acc);
-        acc = fmaf(__uint_as_float(ow[e] & 0xFFFF0000u), __uint_as_float(dw[e] & 0xFFFF0000u),
-                   acc);
+  for (int e = 0; e < 2; ++e) {
+    const int r = e * 32 + threadIdx.x / LANES;
+    const int i = i0 + r / sh.pack, h = h0 + r % sh.pack;
+    real[e] = r < filled_rows && i < sh.seq;
+    if (!real[e]) continue;
+    const size_t off = ((static_cast<size_t>(b) * sh.seq + i) * sh.heads + h) * D + sub * 16;
+    load_16(p.out + off, wide, o[e]);
+    load_16(p.dout + off, wide, d[e]);
+    if (sub == 0) l[e] = p.lse[(static_cast<size_t>(b) * sh.heads + h) * sh.seq + i];
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float acc = 0.0f;
+    if (real[e]) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        acc = fmaf(__uint_as_float(o[e][k] << 16), __uint_as_float(d[e][k] << 16), acc);
+        acc = fmaf(__uint_as_float(o[e][k] & 0xFFFF0000u),
+                   __uint_as_float(d[e][k] & 0xFFFF0000u), acc);
       }
     }
-  }
-  acc += __shfl_xor_sync(0xffffffffu, acc, 1);
-  acc += __shfl_xor_sync(0xffffffffu, acc, 2);
-  acc += __shfl_xor_sync(0xffffffffu, acc, 4);
-  if (in && sub == 0) {
-    float nl = -INFINITY;
-    if (real) {
-      const float l = p.lse[(static_cast<size_t>(b) * sh.heads + h) * sh.seq + i];
-      if (l != -INFINITY) nl = -l * kLog2e;
+#pragma unroll
+    for (int off = 1; off < LANES; off <<= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (sub == 0) {
+      const size_t row = static_cast<size_t>(t) * kHalf + e * 32 + threadIdx.x / LANES;
+      p.work.nlse2[row] = real[e] && l[e] != -INFINITY ? -l[e] * kLog2e : -INFINITY;
+      p.work.ndelta[row] = real[e] ? -acc : 0.0f;
     }
-    p.work.nlse2[row] = nl;
-    p.work.ndelta[row] = real ? -acc : 0.0f;
   }
 }
 
@@ -1499,7 +1511,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         it.b = bk / sh.kv_heads;
         it.hk = bk % sh.kv_heads;
         it.kv0 = n / bk_count * kTile;
-        const SpanTile* tiles = p.work.tiles + static_cast<size_t>(it.b) * sh.tiles64;
+        const Span* tiles = p.work.tiles + static_cast<size_t>(it.b) * sh.tiles64;
         int a = INT_MAX, z = -1;  // the first and last query tile that see it
         for (int q = lane; q < sh.tiles64; q += 32)
           if (tiles[q].lo < it.kv0 + kTile && tiles[q].hi > it.kv0) {
@@ -1824,8 +1836,8 @@ BwdWork bwd_work(void* base, const SpanShape& sh) {
   w.bytes = 2 * rows * sizeof(float);
   w.rows = reinterpret_cast<int2*>(at + w.bytes);
   w.bytes += tiles * kHalf * sizeof(int2);
-  w.tiles = reinterpret_cast<SpanTile*>(at + w.bytes);
-  w.bytes += tiles * sizeof(SpanTile);
+  w.tiles = reinterpret_cast<Span*>(at + w.bytes);
+  w.bytes += tiles * sizeof(Span);
   return w;
 }
 
@@ -1890,13 +1902,12 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* out, con
   pp.first = p.first;
   pp.last = p.last;
   pp.work = p.work;
-  pp.dim = D;
-  const long long tiles = static_cast<long long>(sh.batch) * sh.tiles64;
-  const long long rows = tiles * (sh.heads / sh.pack) * kHalf;
-  pp.row_blocks = static_cast<unsigned>((rows * 8 + 255) / 256);
-  const unsigned span_blocks = static_cast<unsigned>((tiles + 7) / 8);
-  rc = launch_kernel(span_prep_kernel, dim3(pp.row_blocks + span_blocks), dim3(256), 0, stream, 1,
-                     "span attention backward prep launch", pp);
+  const int64_t tiles = static_cast<int64_t>(sh.batch) * sh.tiles64;
+  constexpr int THREADS = 2 * D, WARPS = THREADS / 32;
+  pp.row_blocks = static_cast<unsigned>(tiles * (sh.heads / sh.pack));
+  const unsigned span_blocks = static_cast<unsigned>((tiles + WARPS - 1) / WARPS);
+  rc = launch_kernel(span_prep_kernel<D>, dim3(pp.row_blocks + span_blocks), dim3(THREADS), 0,
+                     stream, 1, "span attention backward prep launch", pp);
   if (rc) return rc;
   const unsigned grid_q = static_cast<unsigned>(sh.batch) * (sh.heads / sh.pack) * sh.tiles128;
   rc = launch_kernel(span_dq_kernel<D>, dim3(grid_q), dim3(kBwdThreads), Q::SMEM,
