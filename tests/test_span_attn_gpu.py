@@ -490,9 +490,9 @@ def test_span_entry_points_refuse_on_the_host():
 
     need, plain = ctypes.c_size_t(), ctypes.c_size_t()
     # 4 heads over 2: 64-row tiles of 32 positions, five of them; per tile and
-    # two heads 64 rows of two statistics, per tile 64 spans and four bounds.
+    # two heads 64 rows of two statistics, per tile 64 spans and two bounds.
     assert L.tq_span_attention_bwd_workspace_bytes(2, 129, 4, 2, ctypes.byref(need)) == 0
-    assert need.value == 2 * 5 * (2 * 64 * 8 + 64 * 8 + 16)
+    assert need.value == 2 * 5 * (2 * 64 * 8 + 64 * 8 + 8)
     # 11 heads over one: too few rows would be filled, a tile holds one head.
     assert L.tq_span_attention_bwd_workspace_bytes(1, 65, 11, 1, ctypes.byref(plain)) == 0
     assert plain.value == 2 * (11 * 64 * 8 + 64 * 8 + 16)
