@@ -495,7 +495,7 @@ def test_span_entry_points_refuse_on_the_host():
     assert need.value == 2 * 5 * (2 * 64 * 8 + 64 * 8 + 8)
     # 11 heads over one: too few rows would be filled, a tile holds one head.
     assert L.tq_span_attention_bwd_workspace_bytes(1, 65, 11, 1, ctypes.byref(plain)) == 0
-    assert plain.value == 2 * (11 * 64 * 8 + 64 * 8 + 16)
+    assert plain.value == 2 * (11 * 64 * 8 + 64 * 8 + 8)
     assert L.tq_span_attention_bwd_workspace_bytes(2, 129, 4, 3, ctypes.byref(plain)) == 1
 
     def bwd(ws_bytes=need.value, ws=P, first=P):
