@@ -864,17 +864,20 @@ struct DqCfg {
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DqItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
   // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
-  // s_free[2], ds_ready[2], dq_full, dq_free, item_full[2], item_empty[2], taken; TMEM slot
-  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 13;
+  // ds_ready[2], a_ready, dq_full, dq_free, item_full[2], item_empty[2], taken; TMEM slot
+  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 12;
   static constexpr int SMEM_USED = 1024 + BAR_OFF + 8 * (NBAR + 1);
   // At least ~116 KB, so that one CTA (and its 512 TMEM columns) fits an SM.
   static constexpr int SMEM = SMEM_USED > 118784 ? SMEM_USED : 118784;
-  static constexpr int S_COL = 0;     // S_b at 64 b
+  // S_b at 64 b, dS_b (bf16 pairs) over it, each half of the keys in the first
+  // 16 of its 32 columns, so that a warp writes only over what it has read.
+  static constexpr int S_COL = 0;
   static constexpr int DP_COL = 128;  // dP_b at 128 + 64 b
   static constexpr int DQ_COL = 256;
-  static constexpr int DS_COL = 256 + D;  // dS_b (bf16 pairs) at DS_COL + 32 b
+  static constexpr int Q_COL = 256 + D;  // Q, then dO (bf16 pairs)
+  static constexpr int DO_COL = Q_COL + D / 2;
   static constexpr int TMEM_COLS = 512;
-  static_assert(DS_COL + 64 <= TMEM_COLS, "tensor memory map");
+  static_assert(DO_COL + D / 2 <= TMEM_COLS, "tensor memory map");
   static_assert(SMEM <= 232448, "shared memory per CTA");
 };
 
@@ -903,12 +906,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   auto v_empty = [&](int s) { return bars + 8u * (2 + 2 * KST + VST + s); };
   constexpr int X = 2 + 2 * KST + 2 * VST;
   auto s_full = [&](int b) { return bars + 8u * (X + b); };
-  auto s_free = [&](int b) { return bars + 8u * (X + 2 + b); };
-  auto ds_ready = [&](int b) { return bars + 8u * (X + 4 + b); };
-  const uint32_t dq_full = bars + 8u * (X + 6), dq_free = bars + 8u * (X + 7);
-  auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
-  auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
-  const uint32_t taken = bars + 8u * (X + 12);
+  auto ds_ready = [&](int b) { return bars + 8u * (X + 2 + b); };
+  const uint32_t a_ready = bars + 8u * (X + 4);
+  const uint32_t dq_full = bars + 8u * (X + 5), dq_free = bars + 8u * (X + 6);
+  auto item_full = [&](int i) { return bars + 8u * (X + 7 + i); };
+  auto item_empty = [&](int i) { return bars + 8u * (X + 9 + i); };
+  const uint32_t taken = bars + 8u * (X + 11);
   const uint32_t tmem_slot = bars + 8u * C::NBAR;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
@@ -922,7 +925,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, kBwdWarps);
     for (int s = 0; s < KST; ++s) {
       mbar_init(k_full(s), 1);
       mbar_init(k_empty(s), 1);
@@ -933,11 +936,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(s_full(i), 1);
-      mbar_init(s_free(i), kBwdWarps);
       mbar_init(ds_ready(i), kBwdWarps);
       mbar_init(item_full(i), 1);
       mbar_init(item_empty(i), kBwdReaders);
     }
+    mbar_init(a_ready, kBwdWarps);
     mbar_init(dq_full, 1);
     mbar_init(dq_free, kBwdWarps);
     mbar_init(taken, 1);
@@ -1035,41 +1038,40 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int ks = t % KST;
 #pragma unroll
           for (int kk = 0; kk < kHalf / 16; ++kk)
-            umma_bf16_ts(tmem + C::DQ_COL, tmem + C::DS_COL + (t & 1) * 32 + kk * 8,
+            umma_bf16_ts(tmem + C::DQ_COL,
+                         tmem + C::S_COL + (t & 1) * kHalf + (kk >> 1) * 32 + (kk & 1) * 8,
                          make_sdesc(k_s(ks) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_dq,
                          (!begin || kk > 0) ? 1u : 0u);
           umma_commit(k_empty(ks));
           return true;
         };
-        ok = mbar_wait(q_full, n & 1, p.status);
+        ok = mbar_wait(a_ready, n & 1, p.status);
         for (int j = 0; j < it.n_kv && ok; ++j, ++g) {
           const int ks = g % KST, vs = g % VST;
           // Four key tiles before the end it is time to look for the next item.
           if (j == max(it.n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
+          // S_g and dP_g go over dS and dP of two tiles ago: read, and their
+          // product issued before.
           ok = mbar_wait(k_full(ks), (g / KST) & 1, p.status) &&
-               mbar_wait(v_full(vs), (g / VST) & 1, p.status) &&
-               (g < 2 || mbar_wait(s_free(g & 1), ((g - 2) >> 1) & 1, p.status));
+               mbar_wait(v_full(vs), (g / VST) & 1, p.status);
           if (!ok) break;
           tc_fence_after();
           const uint32_t sd = tmem + C::S_COL + (g & 1) * kHalf;
           const uint32_t pd = tmem + C::DP_COL + (g & 1) * kHalf;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
-            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
-            umma_bf16(sd, make_sdesc(q_s + qoff, 16, 1024, kSw128),
-                      make_sdesc(k_s(ks) + koff, 16, 1024, kSw128), idesc_s, kk > 0);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16_ts(sd, tmem + C::Q_COL + kk * 8,
+                         make_sdesc(k_s(ks) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
+                                    kSw128),
+                         idesc_s, kk > 0);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
-            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
-            umma_bf16(pd, make_sdesc(do_s + qoff, 16, 1024, kSw128),
-                      make_sdesc(v_s(vs) + koff, 16, 1024, kSw128), idesc_s, kk > 0);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16_ts(pd, tmem + C::DO_COL + kk * 8,
+                         make_sdesc(v_s(vs) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
+                                    kSw128),
+                         idesc_s, kk > 0);
           umma_commit(s_full(g & 1));
           umma_commit(v_empty(vs));
-          if (j + 1 == it.n_kv) umma_commit(q_empty);
           if (j >= 1) ok = issue_dq(g - 1, j == 1);
         }
         if (!ok) break;
@@ -1121,7 +1123,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const F2 c2 = f2(c, c), scale2 = f2(p.scale, p.scale);
     const bool wide = wide_rows(p.dq);
     bool ok = true;
-    int g = 0, n = 0;
+    int g = 0, n = 0, nq = 0;
     struct RowState {
       float nlse2, ndelta;
       Span sp;
@@ -1140,9 +1142,43 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       return s;
     };
+    // The item's Q (warpgroup 0) and dO (1) from shared to tensor memory, a row a
+    // thread, once the products of the item before have read theirs there (the
+    // last tile's scores are complete).
+    auto stage = [&](const DqItem& item) {
+      if (item.b < 0 || item.n_kv == 0) return;
+      ok = ok && mbar_wait(q_full, nq & 1, p.status);
+      if (!ok) return;
+      ++nq;
+      const uint8_t* src = gbase + (part == 0 ? C::Q_OFF : C::DO_OFF) + row * 128;
+      const uint32_t dst = lrow + (part == 0 ? C::Q_COL : C::DO_COL);
+#pragma unroll
+      for (int sl = 0; sl < C::SLABS; ++sl) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint4 x =
+              *reinterpret_cast<const uint4*>(src + sl * C::QSLAB + ((e ^ (row & 7)) << 4));
+          w[4 * e] = x.x;
+          w[4 * e + 1] = x.y;
+          w[4 * e + 2] = x.z;
+          w[4 * e + 3] = x.w;
+        }
+        tmem_st_32x32b_x32(dst + sl * 32, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      fence_proxy_async_smem();  // the reads above come before the next copies
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(q_empty);
+        mbar_arrive(a_ready);
+      }
+    };
     DqItem it = wait_item(0, ok);
     __syncwarp();
     if (lane == 0) mbar_arrive(item_empty(0));
+    stage(it);
     RowState st = row_state(it);
     for (int i = 0; ok && it.b >= 0; ++i) {
       const Span sp = st.sp;
@@ -1164,9 +1200,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + part * kPartCols, dv);
           tmem_ld_wait();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free(g & 1));
         uint32_t pk[kPartCols / 2];
         if (none) {
 #pragma unroll
@@ -1184,7 +1217,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             pk[e] = pack_bf16(q * (pair_of(dv[2 * e], dv[2 * e + 1]) + nd));
           }
         }
-        tmem_st_32x32b_x16(lrow + C::DS_COL + (g & 1) * 32 + part * (kPartCols / 2), pk);
+        tmem_st_32x32b_x16(lrow + C::S_COL + (g & 1) * kHalf + part * kPartCols, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -1194,6 +1227,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const DqItem nx = wait_item(i + 1, ok);
       __syncwarp();
       if (lane == 0) mbar_arrive(item_empty((i + 1) & 1));
+      stage(nx);
       const RowState nst = row_state(nx);
       const int qpos = it.q0 + at;
       const bool valid = filled && qpos < sh.seq;
