@@ -47,10 +47,12 @@ constexpr int kPartCols = kHalf / kParts;
 // Who reads a tile's description: TMA, MMA and every computing warp.
 constexpr int kFwdReaders = 2 + 8;
 constexpr int kBwdReaders = 2 + kBwdWarps;
-// How far (log2) a row's scores may grow past its reference before its sums
-// are scaled down to a new one.  P, l and O keep their relative precision at
-// any exponent, so only their range counts.
-constexpr float kGrowLog2 = 60.0f;
+// A row's exponentials are taken against the maximum of the first tile that it
+// sees until their sum over a tile passes kMost; then against that tile's
+// maximum.  P, l and O keep their relative precision at any exponent, so only
+// their range counts.
+constexpr float kMost = 1.152921504606846976e18f;  // 2^60
+constexpr float kGrowLog2 = 50.0f;  // below 60 by more than the log of a tile's keys
 
 struct SpanShape {
   int batch, seq, heads, kv_heads, group;
@@ -116,6 +118,25 @@ __device__ __forceinline__ F2 pair_of(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t pack_bf16(F2 x) {
   const float2 v = split(x);
   return pack_bf16x2_f32(v.x, v.y);
+}
+
+// Bits [a, z) of a word, 0 <= a, z <= 32.
+__device__ __forceinline__ uint32_t bit_range(int a, int z) {
+  if (a >= z) return 0;
+  return (z == 32 ? 0xFFFFFFFFu : (1u << z) - 1u) & ~((1u << a) - 1u);
+}
+
+// 2^(r c - m) of 32 scores as bf16 pairs to pk[0, 16); their sum, in two parts.
+__device__ __forceinline__ F2 exp_chunk(const uint32_t (&r)[32], F2 c, float m, uint32_t* pk) {
+  const F2 shift = f2(-m, -m);
+  F2 sum[2];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const F2 q = exp2_mufu(fma2(pair_of(r[2 * e], r[2 * e + 1]), c, shift));
+    sum[e & 1] = e < 2 ? q : sum[e & 1] + q;
+    pk[e] = pack_bf16(q);
+  }
+  return sum[0] + sum[1];
 }
 
 // The index of a CTA of this grid that has not started and now never will (its
@@ -184,45 +205,48 @@ __device__ __forceinline__ bool wide_rows(const void* p) {
 //   warp 3       scheduler: the next pairs' descriptions, two in shared memory
 //   warps 4-7    softmax of query tile 0 (thread i owns row i, TMEM lane i)
 //   warps 8-11   softmax of query tile 1
-// TMEM: S_0 | S_1 (128 f32 columns each) | O_0 | O_1 (dim columns each).  A
-// softmax thread reads its row of S once, 32 columns at a time, and writes P
-// (bf16 pairs) over columns already read.  It needs no maximum of the row
-// first: the reference m is the maximum of the first chunk that the row sees,
-// and stays until a chunk exceeds it by 2^60 (then l, O and the tile's earlier
-// P are scaled).  With all 128 scores held for the maximum, the registers left
-// no room to overlap one chunk's exponentials with the next one's load.  MMA
-// issue order per key tile t:
-//   O_0 += P_0(t) V_t,  S_0 = Q_0 K_{t+1}^T,  O_1 += P_1(t) V_t,  S_1 = Q_1 K_{t+1}^T
+// TMEM: S_w,b (64 f32 columns each: key tiles of 64, two of each query tile) |
+// O_0 | O_1 (dim columns each); P_w,b (bf16 pairs) over S_w,b.  MMA issue order
+// per key tile t, with S of tiles 0 and 1 ahead of the first:
+//   O_0 += P_0(t) V_t,  S_0(t+2) = Q_0 K_{t+2}^T,  O_1 += P_1(t) V_t,  S_1(t+2) ...
 // and tcgen05.mma operations issued by one thread execute in that order, so
-// S_w(t+1) overwrites P_w(t) right after its product has read it.  Every
-// barrier that completes once per key tile (or once per pair) counts through
-// all pairs; no waiter is two phases behind.
+// S_w(t+2) overwrites P_w(t) right after its product has read it, and a softmax
+// warp has its next scores while it works on these.  (With key tiles of 128 and
+// one S a query tile it waited 1300 of 4000 cycles for its next scores.)
+// A softmax thread needs no maximum before the exponentials: it keeps a
+// reference (kMost) and looks at its sum.  Barriers count through all pairs, and
+// no waiter is two phases behind: s_full, p_ready and o_done come in two, by the
+// tile's parity, and S_w(t) complete says that O_w's product t-2 is, too.
 
 struct FwdItem {
   int b, h, t0;              // b < 0: no more; first of `pack` heads, first query tile
-  int lo0, hi0, lo1, hi1;    // key tiles of the two query tiles
+  int lo0, hi0, lo1, hi1;    // 64-key tiles of the two query tiles
   int pad;
 };
 
 template <int D>
 struct FwdCfg {
   static_assert(D == 64 || D == 128, "head dim");
-  static constexpr int SLABS = D / 64;            // 128-byte swizzle atoms along dim
-  static constexpr int SLAB_BYTES = kTile * 128;  // 128 rows x 64 bf16
-  static constexpr int TILE_BYTES = SLABS * SLAB_BYTES;
-  static constexpr int KST = D == 128 ? 3 : 4;
-  static constexpr int VST = D == 128 ? 2 : 4;
+  static constexpr int SLABS = D / 64;        // 128-byte swizzle atoms along dim
+  static constexpr int QSLAB = kTile * 128;   // 128 rows x 64 bf16
+  static constexpr int QTILE = SLABS * QSLAB;
+  static constexpr int KSLAB = kHalf * 128;   // 64 rows x 64 bf16
+  static constexpr int KTILE = SLABS * KSLAB;
+  // The scores want K two tiles before the product wants V.
+  static constexpr int KST = D == 128 ? 6 : 8;
+  static constexpr int VST = D == 128 ? 4 : 8;
   static constexpr int Q_OFF = 0;  // two query tiles
-  static constexpr int K_OFF = 2 * TILE_BYTES;
-  static constexpr int V_OFF = K_OFF + KST * TILE_BYTES;
-  static constexpr int ITEM_OFF = V_OFF + VST * TILE_BYTES;
+  static constexpr int K_OFF = 2 * QTILE;
+  static constexpr int V_OFF = K_OFF + KST * KTILE;
+  static constexpr int ITEM_OFF = V_OFF + VST * KTILE;
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(FwdItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
-  // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
-  // p_ready[2], o_done[2], o_free[2], item_full[2], item_empty[2], taken; TMEM slot
-  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 13;
+  // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST],
+  // s_full[2][2], p_ready[2][2], o_done[2][2], o_free[2], item_full[2],
+  // item_empty[2], taken; TMEM slot
+  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 19;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
-  static constexpr int S_COL = 0;    // S_w (and P_w) at 128 w
+  static constexpr int S_COL = 0;    // S_w,b (and P_w,b) at 128 w + 64 b
   static constexpr int O_COL = 256;  // O_w at 256 + D w
   static constexpr int TMEM_COLS = 512;
   static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory map");
@@ -252,9 +276,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const gbase = smem_raw + (base - raw);
-  auto q_s = [&](int w) { return base + C::Q_OFF + w * C::TILE_BYTES; };
-  auto k_s = [&](int s) { return base + C::K_OFF + s * C::TILE_BYTES; };
-  auto v_s = [&](int s) { return base + C::V_OFF + s * C::TILE_BYTES; };
+  auto q_s = [&](int w) { return base + C::Q_OFF + w * C::QTILE; };
+  auto k_s = [&](int s) { return base + C::K_OFF + s * C::KTILE; };
+  auto v_s = [&](int s) { return base + C::V_OFF + s * C::KTILE; };
   const uint32_t bars = base + C::BAR_OFF;
   const uint32_t q_full = bars, q_empty = bars + 8u;
   auto k_full = [&](int s) { return bars + 8u * (2 + s); };
@@ -262,13 +286,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   auto v_full = [&](int s) { return bars + 8u * (2 + 2 * KST + s); };
   auto v_empty = [&](int s) { return bars + 8u * (2 + 2 * KST + VST + s); };
   constexpr int X = 2 + 2 * KST + 2 * VST;
-  auto s_full = [&](int w) { return bars + 8u * (X + w); };
-  auto p_ready = [&](int w) { return bars + 8u * (X + 2 + w); };
-  auto o_done = [&](int w) { return bars + 8u * (X + 4 + w); };
-  auto o_free = [&](int w) { return bars + 8u * (X + 6 + w); };
-  auto item_full = [&](int i) { return bars + 8u * (X + 8 + i); };
-  auto item_empty = [&](int i) { return bars + 8u * (X + 10 + i); };
-  const uint32_t taken = bars + 8u * (X + 12);
+  // n: which of tile w's key tiles it is, counted through all items.
+  auto s_full = [&](int w, int n) { return bars + 8u * (X + 2 * w + (n & 1)); };
+  auto p_ready = [&](int w, int n) { return bars + 8u * (X + 4 + 2 * w + (n & 1)); };
+  auto o_done = [&](int w, int n) { return bars + 8u * (X + 8 + 2 * w + (n & 1)); };
+  auto o_free = [&](int w) { return bars + 8u * (X + 12 + w); };
+  auto item_full = [&](int i) { return bars + 8u * (X + 14 + i); };
+  auto item_empty = [&](int i) { return bars + 8u * (X + 16 + i); };
+  const uint32_t taken = bars + 8u * (X + 18);
   const uint32_t tmem_slot = bars + 8u * C::NBAR;
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(gbase + (tmem_slot - base));
@@ -291,9 +316,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       mbar_init(v_empty(s), 1);
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(s_full(w), 1);
-      mbar_init(p_ready(w), 4);
-      mbar_init(o_done(w), 1);
+      for (int n = 0; n < 2; ++n) {
+        mbar_init(s_full(w, n), 1);
+        mbar_init(p_ready(w, n), 4);
+        mbar_init(o_done(w, n), 1);
+      }
       mbar_init(o_free(w), 4);
       mbar_init(item_full(w), 1);
       mbar_init(item_empty(w), kFwdReaders);
@@ -342,10 +369,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         auto load_k = [&](int t) -> bool {
           const int s = nk % KST;
           if (!mbar_wait(k_empty(s), ((nk / KST) & 1) ^ 1, p.status)) return false;
-          mbar_arrive_expect_tx(k_full(s), C::TILE_BYTES);
+          mbar_arrive_expect_tx(k_full(s), C::KTILE);
           for (int sl = 0; sl < C::SLABS; ++sl)
-            tma_load_4d(k_s(s) + sl * C::SLAB_BYTES, &tm_k, k_full(s), sl * 64, hk,
-                        (j0 + t) * kTile, it.b);
+            tma_load_4d(k_s(s) + sl * C::KSLAB, &tm_k, k_full(s), sl * 64, hk,
+                        (j0 + t) * kHalf, it.b);
           ++nk;
           return true;
         };
@@ -356,23 +383,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         mbar_arrive_expect_tx(q_full, tiles * C::SLABS * rows * 128);
         for (int w = 0; w < tiles; ++w)
           for (int sl = 0; sl < C::SLABS; ++sl)
-            tma_load_4d(q_s(w) + sl * C::SLAB_BYTES, &tm_q, q_full, sl * 64, it.h,
+            tma_load_4d(q_s(w) + sl * C::QSLAB, &tm_q, q_full, sl * 64, it.h,
                         (it.t0 + w) * sh.pos128, it.b);
         ++nq;
+        ok = n_kv < 2 || load_k(1);
         for (int t = 0; t < n_kv && ok; ++t) {
-          // Key tile t + 1 is issued ahead of value tile t (the MMA wants
-          // K_{t+1} for the next scores before it wants V_t).
-          if (t + 1 < n_kv && !load_k(t + 1)) {
+          if (t + 2 < n_kv && !load_k(t + 2)) {
             ok = false;
             break;
           }
           const int s = nv % VST;
           ok = mbar_wait(v_empty(s), ((nv / VST) & 1) ^ 1, p.status);
           if (!ok) break;
-          mbar_arrive_expect_tx(v_full(s), C::TILE_BYTES);
+          mbar_arrive_expect_tx(v_full(s), C::KTILE);
           for (int sl = 0; sl < C::SLABS; ++sl)
-            tma_load_4d(v_s(s) + sl * C::SLAB_BYTES, &tm_v, v_full(s), sl * 64, hk,
-                        (j0 + t) * kTile, it.b);
+            tma_load_4d(v_s(s) + sl * C::KSLAB, &tm_v, v_full(s), sl * 64, hk,
+                        (j0 + t) * kHalf, it.b);
           ++nv;
         }
       }
@@ -384,9 +410,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         mbar_wait(v_full(j % VST), (j / VST) & 1, p.status);
     } else if (warp == 1 && elect_one_sync()) {
       // ----------------------------------------------------------- MMA
-      constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kTile, false, false);
+      constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(kTile, D, false, true);
       int kc = 0, vc = 0, qc = 0;           // key, value and query tiles used
+      int scores[2] = {0, 0};               // products Q K^T issued for tile w
       int steps[2] = {0, 0};                // products P V issued for tile w
       int outs[2] = {0, 0};                 // O_w begun
       bool ok = true;
@@ -402,41 +429,46 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         // Key tile t is j0 + t; query tile w takes part in t of [from, to).
         const int from[2] = {it.lo0 - j0, it.lo1 - j0}, to[2] = {it.hi0 - j0, it.hi1 - j0};
         int left = max(to[0] - from[0], 0) + max(to[1] - from[1], 0);  // scores to issue
-        auto issue_s = [&](int w, int kt) {  // S_w = Q_w K^T
-          const int s = kt % KST;
-          const uint32_t d = tmem + C::S_COL + w * kTile;
+        auto issue_s = [&](int w) {  // S_w = Q_w K^T, with the key tile kc
+          const int s = kc % KST;
+          const uint32_t d = tmem + C::S_COL + w * kTile + (scores[w] & 1) * kHalf;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * C::SLAB_BYTES + (kk & 3) * 32;
-            umma_bf16(d, make_sdesc(q_s(w) + off, 16, 1024, kSw128),
-                      make_sdesc(k_s(s) + off, 16, 1024, kSw128), idesc_s, kk > 0);
-          }
-          umma_commit(s_full(w));
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16(d, make_sdesc(q_s(w) + (kk >> 2) * C::QSLAB + (kk & 3) * 32, 16, 1024, kSw128),
+                      make_sdesc(k_s(s) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024, kSw128),
+                      idesc_s, kk > 0);
+          umma_commit(s_full(w, scores[w]));
+          ++scores[w];
           if (--left == 0) umma_commit(q_empty);
         };
         auto issue_pv = [&](int w, int s, bool begin) {  // O_w += P_w V
+          const uint32_t a = tmem + C::S_COL + w * kTile + (steps[w] & 1) * kHalf;
 #pragma unroll
-          for (int kk = 0; kk < kTile / 16; ++kk)
-            umma_bf16_ts(tmem + C::O_COL + w * D, tmem + C::S_COL + w * kTile + kk * 8,
-                         make_sdesc(v_s(s) + kk * 2048, C::SLAB_BYTES, 1024, kSw128), idesc_o,
+          for (int kk = 0; kk < kHalf / 16; ++kk)
+            umma_bf16_ts(tmem + C::O_COL + w * D, a + kk * 8,
+                         make_sdesc(v_s(s) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_o,
                          (!begin || kk > 0) ? 1u : 0u);
-          umma_commit(o_done(w));
+          umma_commit(o_done(w, steps[w]));
+          ++steps[w];
         };
-        ok = mbar_wait(q_full, qc & 1, p.status) &&
-             mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
+        ok = mbar_wait(q_full, qc & 1, p.status);
         if (!ok) break;
         ++qc;
-        tc_fence_after();
+        for (int t = 0; t < min(n_kv, 2) && ok; ++t) {
+          ok = mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
-          if (from[w] == 0 && to[w] > 0) issue_s(w, kc);
-        umma_commit(k_empty(kc % KST));
-        ++kc;
+          for (int w = 0; w < 2; ++w)
+            if (t >= from[w] && t < to[w]) issue_s(w);
+          umma_commit(k_empty(kc % KST));
+          ++kc;
+        }
         for (int t = 0; t < n_kv && ok; ++t) {
           const int s = vc % VST;
-          const bool next = t + 1 < n_kv;
-          // Two key tiles before the end it is time to look for the next item.
-          if (t == max(n_kv - 2, 0)) mbar_arrive(item_empty(i & 1));
+          const bool next = t + 2 < n_kv;
+          // Four key tiles before the end it is time to look for the next item.
+          if (t == max(n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
           if (next) {
             ok = mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
             if (!ok) break;
@@ -445,19 +477,21 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           if (!ok) break;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            if (!ok || t >= to[w]) continue;
-            if (t >= from[w]) {
-              ok = mbar_wait(p_ready(w), steps[w] & 1, p.status);
+            if (!ok) continue;
+            if (t >= from[w] && t < to[w]) {
+              ok = mbar_wait(p_ready(w, steps[w]), (steps[w] >> 1) & 1, p.status);
               // O_w's last item has been read before it is begun again.
               if (ok && t == from[w] && outs[w] > 0)
                 ok = mbar_wait(o_free(w), (outs[w] - 1) & 1, p.status);
               if (!ok) continue;
               tc_fence_after();
               issue_pv(w, s, t == from[w]);
-              ++steps[w];
               outs[w] += t == from[w];
             }
-            if (t + 1 >= from[w] && t + 1 < to[w]) issue_s(w, kc);
+            if (next && t + 2 >= from[w] && t + 2 < to[w]) {
+              tc_fence_after();
+              issue_s(w);
+            }
           }
           if (!ok) break;
           umma_commit(v_empty(s));
@@ -471,7 +505,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       // Nothing may outlive the CTA's TMEM: wait for each tile's last PV.
 #pragma unroll
       for (int w = 0; w < 2; ++w)
-        if (steps[w] > 0) mbar_wait(o_done(w), (steps[w] - 1) & 1, p.status);
+        if (steps[w] > 0)
+          mbar_wait(o_done(w, steps[w] - 1), ((steps[w] - 1) >> 1) & 1, p.status);
     } else if (warp == 3) {
       // ------------------------------------------------------ scheduler
       const int groups = sh.heads / sh.pack;
@@ -492,10 +527,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           const Span a = span_of_positions(p.first, p.last, it.b, i0, sh.pos128, sh.seq);
           const Span c =
               span_of_positions(p.first, p.last, it.b, i0 + sh.pos128, sh.pos128, sh.seq);
-          it.lo0 = a.lo / kTile;
-          it.hi0 = (a.hi + kTile - 1) / kTile;
-          it.lo1 = c.lo / kTile;
-          it.hi1 = (c.hi + kTile - 1) / kTile;
+          it.lo0 = a.lo / kHalf;
+          it.hi0 = (a.hi + kHalf - 1) / kHalf;
+          it.lo1 = c.lo / kHalf;
+          it.hi1 = (c.hi + kHalf - 1) / kHalf;
         }
         if (lane == 0) {
           items[i & 1] = it;
@@ -513,10 +548,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const bool filled = row < rows;
     const int at = row / sh.pack, head = row % sh.pack;  // position and head within the tile
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t scol = lrow + C::S_COL + w * kTile;
     const uint32_t ocol = lrow + C::O_COL + w * D;
     const float c = sh.scale_log2;
-    const F2 c2 = f2(c, c);
+    const F2 cc2 = f2(c, c);
     const bool wide = wide_rows(p.out);
     bool ok = true;
     int steps = 0;  // key tiles of query tile w, of all items
@@ -533,110 +567,117 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const int jw = w == 0 ? it.lo0 : it.lo1;
       const int nk = (w == 0 ? it.hi0 : it.hi1) - jw;
       const int qpos = (it.t0 + w) * sh.pos128 + at;
-      const unsigned len = sp.hi - sp.lo;
       // What any row of the warp sees, and what every filled row sees.
       const int any_lo = __reduce_min_sync(0xffffffffu, sp.lo < sp.hi ? sp.lo : INT_MAX);
       const int any_hi = __reduce_max_sync(0xffffffffu, sp.hi);
       const int all_lo = __reduce_max_sync(0xffffffffu, filled ? sp.lo : 0);
       const int all_hi = __reduce_min_sync(0xffffffffu, filled ? sp.hi : INT_MAX);
-      float m = -INFINITY;
+      float m = sp.lo < sp.hi ? -INFINITY : 0.0f;  // -inf: has seen nothing yet
       float l = 0.0f;
+      bool begun = __all_sync(0xffffffffu, m != -INFINITY);
       for (int j = 0; j < nk; ++j, ++steps) {
-        ok = mbar_wait(s_full(w), steps & 1, p.status);
+        ok = mbar_wait(s_full(w, steps), (steps >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
-        const int kv0 = (jw + j) * kTile;
-        auto none = [&](int c4) {
-          return kv0 + 32 * c4 + 32 <= any_lo || kv0 + 32 * c4 >= any_hi;
+        const uint32_t scol = lrow + C::S_COL + w * kTile + (steps & 1) * kHalf;
+        const int kv0 = (jw + j) * kHalf;
+        auto none = [&](int c2) {
+          return kv0 + 32 * c2 + 32 <= any_lo || kv0 + 32 * c2 >= any_hi;
         };
-        auto full = [&](int c4) {
-          return kv0 + 32 * c4 >= all_lo && kv0 + 32 * c4 + 32 <= all_hi;
+        auto full = [&](int c2) {
+          return kv0 + 32 * c2 >= all_lo && kv0 + 32 * c2 + 32 <= all_hi;
         };
-        F2 sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+        // Scores that the row does not see become -inf.
+        auto mask = [&](int c2, uint32_t(&r)[32]) {
+          const int k0 = kv0 + 32 * c2;
+          const uint32_t seen =
+              bit_range(min(max(sp.lo - k0, 0), 32), min(max(sp.hi - k0, 0), 32));
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1)) r[e] = 0xFF800000u;
+        };
+        // The largest score of the tile that the row sees.
+        auto tile_max = [&] {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c2 = 0; c2 < 2; ++c2) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(scol + c2 * 32, r);
+            tmem_ld_wait();
+            if (!full(c2)) mask(c2, r);
+            float t[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) t[e & 3] = fmaxf(t[e & 3], __uint_as_float(r[e]));
+            top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          }
+          return top * c;
+        };
+        if (!begun) {
+          const float top = tile_max();
+          if (m == -INFINITY) m = top;
+          begun = __all_sync(0xffffffffu, m != -INFINITY);
+        }
+        const float mref = m == -INFINITY ? 0.0f : m;
+        uint32_t pk[32];
+        F2 sum2 = f2(0.0f, 0.0f);
         uint32_t rb[2][32];
-        if (!none(0)) tmem_ld_32x32b_x32(scol, rb[0]);
 #pragma unroll
-        for (int c4 = 0; c4 < 4; ++c4) {
-          tmem_ld_wait();
-          if (c4 + 1 < 4 && !none(c4 + 1))
-            tmem_ld_32x32b_x32(scol + (c4 + 1) * 32, rb[(c4 + 1) & 1]);
-          uint32_t(&r)[32] = rb[c4 & 1];
-          uint32_t pk[16];
-          if (none(c4)) {
+        for (int c2 = 0; c2 < 2; ++c2)
+          if (!none(c2)) tmem_ld_32x32b_x32(scol + c2 * 32, rb[c2]);
+        tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = 0;
+        for (int c2 = 0; c2 < 2; ++c2) {
+          if (none(c2)) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[c2 * 16 + e] = 0;
           } else {
-            if (!full(c4)) {
-              const int col0 = kv0 + 32 * c4 - sp.lo;
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (static_cast<unsigned>(col0 + e) >= len) r[e] = 0xFF800000u;  // -inf
-            }
-            float m4[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m4[e] = __uint_as_float(r[e]);
-#pragma unroll
-            for (int e = 4; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(r[e]));
-            const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * c;
-            if (m == -INFINITY) m = mx;  // nothing summed yet
-            if (__any_sync(0xffffffffu, mx > m + kGrowLog2)) {
-              // The rows that outgrew their reference take a new one; the
-              // others go through with a factor of 1.
-              const bool grow = mx > m + kGrowLog2;
-              const float f = grow ? ex2_approx(m - mx) : 1.0f;
-              const F2 ff = f2(f, f);
-              if (grow) m = mx;
-              l *= f;
-              sum[0] = sum[0] * ff;
-              sum[1] = sum[1] * ff;
-              tmem_ld_wait();  // the next chunk's scores, ahead of P's here
-              tmem_st_wait();
+            if (!full(c2)) mask(c2, rb[c2]);
+            sum2 = sum2 + exp_chunk(rb[c2], cc2, mref, pk + c2 * 16);
+          }
+        }
+        float2 sum = split(sum2);
+        if (!__any_sync(0xffffffffu, !(sum.x + sum.y <= kMost))) {
+          tmem_st_32x32b_x32(scol, pk);
+        } else {
+          // Some row has outgrown its reference (or holds a NaN, and keeps it).
+          // The scores are still there: those rows take the tile's maximum for a
+          // new one, the others go through with a factor of 1.
+          const float top = tile_max();
+          const bool grow = top > m + kGrowLog2;
+          const float f = grow ? ex2_approx(m - top) : 1.0f;
+          if (grow) m = top;
+          l *= f;
+          if (j > 0) {  // O_w, once its last product is done
+            ok = mbar_wait(o_done(w, steps - 1), ((steps - 1) >> 1) & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
-              for (int cc = 0; cc < c4; ++cc) {
-                uint32_t o[16];
-                tmem_ld_32x32b_x16(scol + cc * 16, o);
-                tmem_ld_wait();
+            for (int cc = 0; cc < D / 16; ++cc) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(ocol + cc * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                  o[e] = pack_bf16x2_f32(__uint_as_float(o[e] << 16) * f,
-                                         __uint_as_float(o[e] & 0xFFFF0000u) * f);
-                tmem_st_32x32b_x16(scol + cc * 16, o);
-              }
-              if (j > 0) {  // O_w, once its last product is done
-                ok = mbar_wait(o_done(w), (steps - 1) & 1, p.status);
-                tc_fence_after();
-#pragma unroll 1
-                for (int cc = 0; cc < D / 16; ++cc) {
-                  uint32_t o[16];
-                  tmem_ld_32x32b_x16(ocol + cc * 16, o);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int e = 0; e < 16; ++e)
-                    o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                  tmem_st_32x32b_x16(ocol + cc * 16, o);
-                }
-              }
-              tmem_st_wait();
-            }
-            // A row that sees nothing yet has only -inf here: 2^-inf = 0.
-            const float mref = m == -INFINITY ? 0.0f : m;
-            const F2 shift = f2(-mref, -mref);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const F2 q = exp2_mufu(fma2(pair_of(r[2 * e], r[2 * e + 1]), c2, shift));
-              sum[e & 1] = sum[e & 1] + q;
-              pk[e] = pack_bf16(q);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st_32x32b_x16(ocol + cc * 16, o);
             }
           }
-          tmem_st_32x32b_x16(scol + c4 * 16, pk);
+          sum2 = f2(0.0f, 0.0f);
+#pragma unroll 1
+          for (int c2 = 0; c2 < 2; ++c2) {
+            uint32_t r[32], pc[16];
+            tmem_ld_32x32b_x32(scol + c2 * 32, r);
+            tmem_ld_wait();
+            mask(c2, r);
+            sum2 = sum2 + exp_chunk(r, cc2, m == -INFINITY ? 0.0f : m, pc);
+            tmem_st_32x32b_x16(scol + c2 * 16, pc);
+          }
+          sum = split(sum2);
         }
-        if (!ok) break;
-        const float2 s = split(sum[0] + sum[1]);
-        l += s.x + s.y;
+        l += sum.x + sum.y;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready(w));
+        if (lane == 0) mbar_arrive(p_ready(w, steps));
       }
       if (!ok) break;
       // The next item's description and span, read while this one ends.
@@ -650,7 +691,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       float* const lse =
           p.lse + (static_cast<size_t>(it.b) * sh.heads + it.h + head) * sh.seq + qpos;
       if (nk > 0) {
-        ok = ok && mbar_wait(o_done(w), (steps - 1) & 1, p.status);
+        ok = ok && mbar_wait(o_done(w, steps - 1), ((steps - 1) >> 1) & 1, p.status);
         if (!ok) break;
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: sees nothing
@@ -1327,12 +1368,6 @@ __device__ __forceinline__ uint32_t transpose_bits(uint32_t x) {
   return x;
 }
 
-// Bits [a, z) of a word, 0 <= a, z <= 32.
-__device__ __forceinline__ uint32_t bit_range(int a, int z) {
-  if (a >= z) return 0;
-  return (z == 32 ? 0xFFFFFFFFu : (1u << z) - 1u) & ~((1u << a) - 1u);
-}
-
 template <int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     span_dkv_kernel(const __grid_constant__ CUtensorMap tm_q,
@@ -1896,8 +1931,8 @@ int launch_fwd(const void* q, const void* k, const void* v, FwdParams p, cudaStr
   if (rc) return rc;
   CUtensorMap tq_, tk, tv;
   if ((rc = map_bshd(&tq_, q, sh.batch, sh.seq, sh.heads, D, sh.pos128, sh.pack))) return rc;
-  if ((rc = map_bshd(&tk, k, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
-  if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D))) return rc;
+  if ((rc = map_bshd(&tk, k, sh.batch, sh.seq, sh.kv_heads, D, kHalf))) return rc;
+  if ((rc = map_bshd(&tv, v, sh.batch, sh.seq, sh.kv_heads, D, kHalf))) return rc;
   p.n_pairs = (sh.tiles128 + 1) / 2;
   const unsigned grid = static_cast<unsigned>(sh.batch) * (sh.heads / sh.pack) * p.n_pairs;
   return launch_kernel(span_fwd_kernel<D>, dim3(grid), dim3(kFwdThreads), C::SMEM,
