@@ -44,9 +44,9 @@ constexpr int kBwdWarps = 8;      // that compute, beside the four of roles
 constexpr int kBwdThreads = 128 + 32 * kBwdWarps;
 constexpr int kParts = kBwdWarps / 4;     // of a streamed 64-wide tile's columns
 constexpr int kPartCols = kHalf / kParts;
-// Who reads a tile's description: TMA, MMA and every computing warp.
-constexpr int kFwdReaders = 2 + 8;
-constexpr int kBwdReaders = 2 + kBwdWarps;
+// Who reads a tile's description: TMA, two of MMA and every computing warp.
+constexpr int kFwdReaders = 3 + 8;
+constexpr int kBwdReaders = 3 + kBwdWarps;
 // A row's exponentials are taken against the maximum of the first tile that it
 // sees until their sum over a tile passes kMost; then against that tile's
 // maximum.  P, l and O keep their relative precision at any exponent, so only
@@ -61,6 +61,17 @@ struct SpanShape {
   // floor(rows / pack) (rows behind pack * positions hold zeros), and the
   // number of such tiles and of 128-key tiles in a sequence.
   int pack, pos128, pos64, tiles128, tiles64, key_tiles;
+};
+
+// A place in a ring of stages and the parity of its phase.
+struct Ring {
+  int stage, phase;
+  __device__ void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
 };
 
 // A query's keys [lo, hi) within [0, seq); 0, 0 when it sees none.
@@ -306,14 +317,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int s = 0; s < KST; ++s) {
       mbar_init(k_full(s), 1);
-      mbar_init(k_empty(s), 1);
+      mbar_init(k_empty(s), 2);
     }
     for (int s = 0; s < VST; ++s) {
       mbar_init(v_full(s), 1);
-      mbar_init(v_empty(s), 1);
+      mbar_init(v_empty(s), 2);
     }
     for (int w = 0; w < 2; ++w) {
       for (int n = 0; n < 2; ++n) {
@@ -408,15 +419,38 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         mbar_wait(k_full(j % KST), (j / KST) & 1, p.status);
       for (int j = nv - VST < 0 ? 0 : nv - VST; j < nv; ++j)
         mbar_wait(v_full(j % VST), (j / VST) & 1, p.status);
-    } else if (warp == 1 && elect_one_sync()) {
-      // ----------------------------------------------------------- MMA
+    } else if (warp >= 1 && warp <= 2 && elect_one_sync()) {
+      // ------------------------------------- MMA of query tile w, a thread each
       constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(kTile, D, false, true);
-      int kc = 0, vc = 0, qc = 0;           // key, value and query tiles used
-      int scores[2] = {0, 0};               // products Q K^T issued for tile w
-      int steps[2] = {0, 0};                // products P V issued for tile w
-      int outs[2] = {0, 0};                 // O_w begun
+      const int w = warp - 1;
+      Ring kr{0, 0}, vr{0, 0};  // the next key and value tile
+      int qc = 0;               // query tiles used
+      int scores = 0;           // products Q K^T issued
+      int steps = 0;            // products P V issued
+      int outs = 0;             // O_w begun
       bool ok = true;
+      auto issue_s = [&] {  // S_w = Q_w K^T
+        const uint32_t d = tmem + C::S_COL + w * kTile + (scores & 1) * kHalf;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma_bf16(d, make_sdesc(q_s(w) + (kk >> 2) * C::QSLAB + (kk & 3) * 32, 16, 1024, kSw128),
+                    make_sdesc(k_s(kr.stage) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
+                               kSw128),
+                    idesc_s, kk > 0);
+        umma_commit(s_full(w, scores));
+        ++scores;
+      };
+      auto issue_pv = [&](bool begin) {  // O_w += P_w V
+        const uint32_t a = tmem + C::S_COL + w * kTile + (steps & 1) * kHalf;
+#pragma unroll
+        for (int kk = 0; kk < kHalf / 16; ++kk)
+          umma_bf16_ts(tmem + C::O_COL + w * D, a + kk * 8,
+                       make_sdesc(v_s(vr.stage) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_o,
+                       (!begin || kk > 0) ? 1u : 0u);
+        umma_commit(o_done(w, steps));
+        ++steps;
+      };
       for (int i = 0; ok; ++i) {
         const FwdItem it = wait_item(i, ok);
         if (it.b < 0) break;
@@ -426,87 +460,47 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           mbar_arrive(item_empty(i & 1));
           continue;
         }
-        // Key tile t is j0 + t; query tile w takes part in t of [from, to).
-        const int from[2] = {it.lo0 - j0, it.lo1 - j0}, to[2] = {it.hi0 - j0, it.hi1 - j0};
-        int left = max(to[0] - from[0], 0) + max(to[1] - from[1], 0);  // scores to issue
-        auto issue_s = [&](int w) {  // S_w = Q_w K^T, with the key tile kc
-          const int s = kc % KST;
-          const uint32_t d = tmem + C::S_COL + w * kTile + (scores[w] & 1) * kHalf;
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16(d, make_sdesc(q_s(w) + (kk >> 2) * C::QSLAB + (kk & 3) * 32, 16, 1024, kSw128),
-                      make_sdesc(k_s(s) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024, kSw128),
-                      idesc_s, kk > 0);
-          umma_commit(s_full(w, scores[w]));
-          ++scores[w];
-          if (--left == 0) umma_commit(q_empty);
-        };
-        auto issue_pv = [&](int w, int s, bool begin) {  // O_w += P_w V
-          const uint32_t a = tmem + C::S_COL + w * kTile + (steps[w] & 1) * kHalf;
-#pragma unroll
-          for (int kk = 0; kk < kHalf / 16; ++kk)
-            umma_bf16_ts(tmem + C::O_COL + w * D, a + kk * 8,
-                         make_sdesc(v_s(s) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_o,
-                         (!begin || kk > 0) ? 1u : 0u);
-          umma_commit(o_done(w, steps[w]));
-          ++steps[w];
-        };
+        // Key tile t is j0 + t; query tile w takes part in t of [from, to).  A
+        // tile is given back by both threads, by the one that leaves it out too
+        // (once it is there: an arrival never runs ahead of its phase).
+        const int from = (w == 0 ? it.lo0 : it.lo1) - j0, to = (w == 0 ? it.hi0 : it.hi1) - j0;
         ok = mbar_wait(q_full, qc & 1, p.status);
         if (!ok) break;
         ++qc;
-        for (int t = 0; t < min(n_kv, 2) && ok; ++t) {
-          ok = mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int w = 0; w < 2; ++w)
-            if (t >= from[w] && t < to[w]) issue_s(w);
-          umma_commit(k_empty(kc % KST));
-          ++kc;
-        }
+        if (to <= from) mbar_arrive(q_empty);
+        auto scores_of = [&](int t) -> bool {
+          if (!mbar_wait(k_full(kr.stage), kr.phase, p.status)) return false;
+          if (t >= from && t < to) {
+            tc_fence_after();
+            issue_s();
+            if (t + 1 == to) umma_commit(q_empty);
+          }
+          umma_commit(k_empty(kr.stage));
+          kr.next(KST);
+          return true;
+        };
+        for (int t = 0; t < min(n_kv, 2) && ok; ++t) ok = scores_of(t);
         for (int t = 0; t < n_kv && ok; ++t) {
-          const int s = vc % VST;
-          const bool next = t + 2 < n_kv;
           // Four key tiles before the end it is time to look for the next item.
           if (t == max(n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
-          if (next) {
-            ok = mbar_wait(k_full(kc % KST), (kc / KST) & 1, p.status);
+          ok = mbar_wait(v_full(vr.stage), vr.phase, p.status);
+          if (!ok) break;
+          if (t >= from && t < to) {
+            ok = mbar_wait(p_ready(w, steps), (steps >> 1) & 1, p.status);
+            // O_w's last item has been read before it is begun again.
+            if (ok && t == from && outs > 0) ok = mbar_wait(o_free(w), (outs - 1) & 1, p.status);
             if (!ok) break;
+            tc_fence_after();
+            issue_pv(t == from);
+            outs += t == from;
           }
-          ok = mbar_wait(v_full(s), (vc / VST) & 1, p.status);
-          if (!ok) break;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (!ok) continue;
-            if (t >= from[w] && t < to[w]) {
-              ok = mbar_wait(p_ready(w, steps[w]), (steps[w] >> 1) & 1, p.status);
-              // O_w's last item has been read before it is begun again.
-              if (ok && t == from[w] && outs[w] > 0)
-                ok = mbar_wait(o_free(w), (outs[w] - 1) & 1, p.status);
-              if (!ok) continue;
-              tc_fence_after();
-              issue_pv(w, s, t == from[w]);
-              outs[w] += t == from[w];
-            }
-            if (next && t + 2 >= from[w] && t + 2 < to[w]) {
-              tc_fence_after();
-              issue_s(w);
-            }
-          }
-          if (!ok) break;
-          umma_commit(v_empty(s));
-          ++vc;
-          if (next) {
-            umma_commit(k_empty(kc % KST));
-            ++kc;
-          }
+          umma_commit(v_empty(vr.stage));
+          vr.next(VST);
+          if (t + 2 < n_kv) ok = scores_of(t + 2);
         }
       }
-      // Nothing may outlive the CTA's TMEM: wait for each tile's last PV.
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-        if (steps[w] > 0)
-          mbar_wait(o_done(w, steps[w] - 1), ((steps[w] - 1) >> 1) & 1, p.status);
+      // Nothing may outlive the CTA's TMEM: wait for the tile's last product.
+      if (steps > 0) mbar_wait(o_done(w, steps - 1), ((steps - 1) >> 1) & 1, p.status);
     } else if (warp == 3) {
       // ------------------------------------------------------ scheduler
       const int groups = sh.heads / sh.pack;
@@ -896,7 +890,7 @@ struct DqCfg {
   static constexpr int KSLAB = kHalf * 128;  // 64 rows x 64 bf16
   static constexpr int KTILE = SLABS * KSLAB;
   static constexpr int KST = D == 128 ? 5 : 8;
-  static constexpr int VST = KST;
+  static constexpr int VST = KST;  // (one stage index for both)
   static constexpr int Q_OFF = 0;
   static constexpr int DO_OFF = QTILE;
   static constexpr int K_OFF = 2 * QTILE;
@@ -976,7 +970,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(v_empty(s), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full(i), 1);
+      mbar_init(s_full(i), 2);
       mbar_init(ds_ready(i), kBwdWarps);
       mbar_init(item_full(i), 1);
       mbar_init(item_empty(i), kBwdReaders);
@@ -1055,11 +1049,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int j = nv - VST < 0 ? 0 : nv - VST; j < nv; ++j)
         mbar_wait(v_full(j % VST), (j / VST) & 1, p.status);
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------- MMA
+  } else if (warp <= 2) {
+    // ------------------------------------- MMA: S and dQ (warp 1), dP (warp 2)
     if (elect_one_sync()) {
       constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
       constexpr uint32_t idesc_dq = make_idesc_bf16(kTile, D, false, true);
+      const bool first = warp == 1;
       int g = 0;   // key tiles, of all items: buffer g & 1, stage g % KST
       int n = 0;   // items with any
       bool ok = true;
@@ -1088,40 +1083,38 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         };
         ok = mbar_wait(a_ready, n & 1, p.status);
         for (int j = 0; j < it.n_kv && ok; ++j, ++g) {
-          const int ks = g % KST, vs = g % VST;
+          const int s = g % KST;
           // Four key tiles before the end it is time to look for the next item.
           if (j == max(it.n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
-          // S_g and dP_g go over dS and dP of two tiles ago: read, and their
-          // product issued before.
-          ok = mbar_wait(k_full(ks), (g / KST) & 1, p.status) &&
-               mbar_wait(v_full(vs), (g / VST) & 1, p.status);
+          // S_g goes over dS of two tiles ago, whose product this thread has
+          // issued; dP_g over that tile's dP, read before its dS was ready.
+          ok = first ? mbar_wait(k_full(s), (g / KST) & 1, p.status)
+                     : mbar_wait(v_full(s), (g / VST) & 1, p.status) &&
+                           (g < 2 || mbar_wait(ds_ready(g & 1), ((g - 2) >> 1) & 1, p.status));
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sd = tmem + C::S_COL + (g & 1) * kHalf;
-          const uint32_t pd = tmem + C::DP_COL + (g & 1) * kHalf;
+          const uint32_t d = tmem + (first ? C::S_COL : C::DP_COL) + (g & 1) * kHalf;
+          const uint32_t a = tmem + (first ? C::Q_COL : C::DO_COL);
+          const uint32_t b = first ? k_s(s) : v_s(s);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16_ts(sd, tmem + C::Q_COL + kk * 8,
-                         make_sdesc(k_s(ks) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
-                                    kSw128),
-                         idesc_s, kk > 0);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            umma_bf16_ts(pd, tmem + C::DO_COL + kk * 8,
-                         make_sdesc(v_s(vs) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
-                                    kSw128),
+            umma_bf16_ts(d, a + kk * 8,
+                         make_sdesc(b + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024, kSw128),
                          idesc_s, kk > 0);
           umma_commit(s_full(g & 1));
-          umma_commit(v_empty(vs));
-          if (j >= 1) ok = issue_dq(g - 1, j == 1);
+          if (!first) umma_commit(v_empty(s));
+          if (first && j >= 1) ok = issue_dq(g - 1, j == 1);
         }
         if (!ok) break;
-        ok = issue_dq(g - 1, it.n_kv == 1);
-        umma_commit(dq_full);
+        if (first) {
+          ok = issue_dq(g - 1, it.n_kv == 1);
+          umma_commit(dq_full);
+        }
         ++n;
       }
       // Nothing may outlive the CTA's TMEM: the last commit covers every MMA.
-      if (n > 0) mbar_wait(dq_full, (n - 1) & 1, p.status);
+      if (n > 0 && first) mbar_wait(dq_full, (n - 1) & 1, p.status);
+      if (n > 0 && !first) mbar_wait(s_full((g - 1) & 1), ((g - 1) >> 1) & 1, p.status);
     }
   } else if (warp == 3) {
     // -------------------------------------------------------- scheduler
@@ -1409,18 +1402,18 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 1);
+    mbar_init(kv_empty, 2);
     for (int s = 0; s < QST; ++s) {
       mbar_init(q_full(s), 1);
-      mbar_init(q_empty(s), 1 + kBwdWarps);  // the MMAs' commit, the warps' stat reads
+      mbar_init(q_empty(s), 2 + kBwdWarps);  // the MMAs' commits, the warps' stat reads
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full(i), 1);
+      mbar_init(s_full(i), 2);
       mbar_init(pds_ready(i), kBwdWarps);
       mbar_init(item_full(i), 1);
       mbar_init(item_empty(i), kBwdReaders);
     }
-    mbar_init(acc_full, 1);
+    mbar_init(acc_full, 2);
     mbar_init(acc_free, kBwdWarps);
     mbar_init(taken, 1);
     fence_mbar_init();
@@ -1491,13 +1484,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int t = issued - QST < 0 ? 0 : issued - QST; t < issued; ++t)
         mbar_wait(q_full(t % QST), (t / QST) & 1, p.status);
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------- MMA
+  } else if (warp <= 2) {
+    // --------------------- MMA: S^T and dV (warp 1), dP^T and dK (warp 2)
     if (elect_one_sync()) {
       constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
       constexpr uint32_t idesc_acc = make_idesc_bf16(kTile, D, false, true);
       int g = 0;  // query tiles, of all items: buffer g & 1, stage g % QST
       int n = 0;  // items with any
+      const bool first = warp == 1;
+      const uint32_t s_col = tmem + (first ? C::S_COL : C::DP_COL);
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const DkvItem it = wait_item(i, ok);
@@ -1515,15 +1510,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           if (begin && n > 0 && !mbar_wait(acc_free, (n - 1) & 1, p.status)) return false;
           tc_fence_after();
           const int s = t % QST;
+          const uint32_t b = first ? do_s(s) : q_s(s);
 #pragma unroll
           for (int kk = 0; kk < kHalf / 16; ++kk)
-            umma_bf16_ts(tmem + C::DV_COL, tmem + C::S_COL + (t & 1) * kHalf + kk * 16,
-                         make_sdesc(do_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
-                         (!begin || kk > 0) ? 1u : 0u);
-#pragma unroll
-          for (int kk = 0; kk < kHalf / 16; ++kk)
-            umma_bf16_ts(tmem + C::DK_COL, tmem + C::DP_COL + (t & 1) * kHalf + kk * 16,
-                         make_sdesc(q_s(s) + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
+            umma_bf16_ts(tmem + (first ? C::DV_COL : C::DK_COL), s_col + (t & 1) * kHalf + kk * 16,
+                         make_sdesc(b + kk * 2048, C::QSLAB, 1024, kSw128), idesc_acc,
                          (!begin || kk > 0) ? 1u : 0u);
           umma_commit(q_empty(s));
           return true;
@@ -1538,22 +1529,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t sd = tmem + C::S_COL + (g & 1) * kHalf;
-          const uint32_t pd = tmem + C::DP_COL + (g & 1) * kHalf;
+          const uint32_t a = first ? k_s : v_s, b = first ? q_s(s) : do_s(s);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
-            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
-            umma_bf16(sd, make_sdesc(k_s + koff, 16, 1024, kSw128),
-                      make_sdesc(q_s(s) + qoff, 16, 1024, kSw128), idesc_s, kk > 0);
-          }
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t koff = (kk >> 2) * C::KSLAB + (kk & 3) * 32;
-            const uint32_t qoff = (kk >> 2) * C::QSLAB + (kk & 3) * 32;
-            umma_bf16(pd, make_sdesc(v_s + koff, 16, 1024, kSw128),
-                      make_sdesc(do_s(s) + qoff, 16, 1024, kSw128), idesc_s, kk > 0);
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma_bf16(s_col + (g & 1) * kHalf,
+                      make_sdesc(a + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024, kSw128),
+                      make_sdesc(b + (kk >> 2) * C::QSLAB + (kk & 3) * 32, 16, 1024, kSw128),
+                      idesc_s, kk > 0);
           umma_commit(s_full(g & 1));
           if (t + 1 == T) umma_commit(kv_empty);
           if (t >= 1) ok = issue_acc(g - 1, t == 1);
