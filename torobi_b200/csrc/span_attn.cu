@@ -243,19 +243,16 @@ struct FwdCfg {
   static constexpr int QTILE = SLABS * QSLAB;
   static constexpr int KSLAB = kHalf * 128;   // 64 rows x 64 bf16
   static constexpr int KTILE = SLABS * KSLAB;
-  // The scores want K two tiles before the product wants V.
-  static constexpr int KST = D == 128 ? 6 : 8;
-  static constexpr int VST = D == 128 ? 4 : 8;
+  // A stage holds K_{t+2} and V_t, which are wanted together.
+  static constexpr int ST = D == 128 ? 5 : 8;
   static constexpr int Q_OFF = 0;  // two query tiles
-  static constexpr int K_OFF = 2 * QTILE;
-  static constexpr int V_OFF = K_OFF + KST * KTILE;
-  static constexpr int ITEM_OFF = V_OFF + VST * KTILE;
+  static constexpr int KV_OFF = 2 * QTILE;
+  static constexpr int ITEM_OFF = KV_OFF + 2 * ST * KTILE;
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(FwdItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
-  // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST],
-  // s_full[2][2], p_ready[2][2], o_done[2][2], o_free[2], item_full[2],
-  // item_empty[2], taken; TMEM slot
-  static constexpr int NBAR = 2 + 2 * KST + 2 * VST + 19;
+  // q_full, q_empty, kv_full[ST], kv_empty[ST], s_full[2][2], p_ready[2][2],
+  // o_done[2][2], o_free[2], item_full[2], item_empty[2], taken; TMEM slot
+  static constexpr int NBAR = 2 + 2 * ST + 19;
   static constexpr int SMEM = 1024 + BAR_OFF + 8 * (NBAR + 1);
   static constexpr int S_COL = 0;    // S_w,b (and P_w,b) at 128 w + 64 b
   static constexpr int O_COL = 256;  // O_w at 256 + D w
@@ -281,22 +278,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
   using C = FwdCfg<D>;
-  constexpr int KST = C::KST;
-  constexpr int VST = C::VST;
+  constexpr int ST = C::ST;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* const gbase = smem_raw + (base - raw);
   auto q_s = [&](int w) { return base + C::Q_OFF + w * C::QTILE; };
-  auto k_s = [&](int s) { return base + C::K_OFF + s * C::KTILE; };
-  auto v_s = [&](int s) { return base + C::V_OFF + s * C::KTILE; };
+  auto k_s = [&](int s) { return base + C::KV_OFF + 2 * s * C::KTILE; };
+  auto v_s = [&](int s) { return base + C::KV_OFF + (2 * s + 1) * C::KTILE; };
   const uint32_t bars = base + C::BAR_OFF;
   const uint32_t q_full = bars, q_empty = bars + 8u;
-  auto k_full = [&](int s) { return bars + 8u * (2 + s); };
-  auto k_empty = [&](int s) { return bars + 8u * (2 + KST + s); };
-  auto v_full = [&](int s) { return bars + 8u * (2 + 2 * KST + s); };
-  auto v_empty = [&](int s) { return bars + 8u * (2 + 2 * KST + VST + s); };
-  constexpr int X = 2 + 2 * KST + 2 * VST;
+  auto kv_full = [&](int s) { return bars + 8u * (2 + s); };
+  auto kv_empty = [&](int s) { return bars + 8u * (2 + ST + s); };
+  constexpr int X = 2 + 2 * ST;
   // n: which of tile w's key tiles it is, counted through all items.
   auto s_full = [&](int w, int n) { return bars + 8u * (X + 2 * w + (n & 1)); };
   auto p_ready = [&](int w, int n) { return bars + 8u * (X + 4 + 2 * w + (n & 1)); };
@@ -318,13 +312,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 2);
-    for (int s = 0; s < KST; ++s) {
-      mbar_init(k_full(s), 1);
-      mbar_init(k_empty(s), 2);
-    }
-    for (int s = 0; s < VST; ++s) {
-      mbar_init(v_full(s), 1);
-      mbar_init(v_empty(s), 2);
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), 2);
     }
     for (int w = 0; w < 2; ++w) {
       for (int n = 0; n < 2; ++n) {
@@ -367,7 +357,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      int nk = 0, nv = 0, nq = 0;  // tiles issued, of all items
+      int ns = 0, nq = 0;  // stages filled, query tiles issued, of all items
       bool ok = true;
       for (int i = 0; ok; ++i) {
         const FwdItem it = wait_item(i, ok);
@@ -377,54 +367,44 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const int j0 = it.hi0 == 0 ? it.lo1 : it.hi1 == 0 ? it.lo0 : min(it.lo0, it.lo1);
         const int n_kv = max(it.hi0, it.hi1) - j0;
         if (n_kv <= 0) continue;
-        auto load_k = [&](int t) -> bool {
-          const int s = nk % KST;
-          if (!mbar_wait(k_empty(s), ((nk / KST) & 1) ^ 1, p.status)) return false;
-          mbar_arrive_expect_tx(k_full(s), C::KTILE);
-          for (int sl = 0; sl < C::SLABS; ++sl)
-            tma_load_4d(k_s(s) + sl * C::KSLAB, &tm_k, k_full(s), sl * 64, hk,
-                        (j0 + t) * kHalf, it.b);
-          ++nk;
-          return true;
-        };
-        // The first key tile needs no room of the last item's query tiles.
-        ok = load_k(0) && mbar_wait(q_empty, (nq & 1) ^ 1, p.status);
-        if (!ok) break;
-        const int tiles = it.t0 + 1 < sh.tiles128 ? 2 : 1;
-        mbar_arrive_expect_tx(q_full, tiles * C::SLABS * rows * 128);
-        for (int w = 0; w < tiles; ++w)
-          for (int sl = 0; sl < C::SLABS; ++sl)
-            tma_load_4d(q_s(w) + sl * C::QSLAB, &tm_q, q_full, sl * 64, it.h,
-                        (it.t0 + w) * sh.pos128, it.b);
-        ++nq;
-        ok = n_kv < 2 || load_k(1);
-        for (int t = 0; t < n_kv && ok; ++t) {
-          if (t + 2 < n_kv && !load_k(t + 2)) {
-            ok = false;
-            break;
-          }
-          const int s = nv % VST;
-          ok = mbar_wait(v_empty(s), ((nv / VST) & 1) ^ 1, p.status);
+        for (int t = 0; t < n_kv + 2 && ok; ++t, ++ns) {  // K_t and V_{t-2}
+          const int s = ns % ST;
+          const bool k = t < n_kv, v = t >= 2;
+          ok = mbar_wait(kv_empty(s), ((ns / ST) & 1) ^ 1, p.status);
           if (!ok) break;
-          mbar_arrive_expect_tx(v_full(s), C::KTILE);
-          for (int sl = 0; sl < C::SLABS; ++sl)
-            tma_load_4d(v_s(s) + sl * C::KSLAB, &tm_v, v_full(s), sl * 64, hk,
-                        (j0 + t) * kHalf, it.b);
-          ++nv;
+          if (k || v)
+            mbar_arrive_expect_tx(kv_full(s), (static_cast<int>(k) + static_cast<int>(v)) * C::KTILE);
+          else
+            mbar_arrive(kv_full(s));
+          for (int sl = 0; sl < C::SLABS && k; ++sl)
+            tma_load_4d(k_s(s) + sl * C::KSLAB, &tm_k, kv_full(s), sl * 64, hk, (j0 + t) * kHalf,
+                        it.b);
+          for (int sl = 0; sl < C::SLABS && v; ++sl)
+            tma_load_4d(v_s(s) + sl * C::KSLAB, &tm_v, kv_full(s), sl * 64, hk,
+                        (j0 + t - 2) * kHalf, it.b);
+          if (t > 0) continue;
+          // The first key tile needs no room of the last item's query tiles.
+          ok = mbar_wait(q_empty, (nq & 1) ^ 1, p.status);
+          if (!ok) break;
+          const int tiles = it.t0 + 1 < sh.tiles128 ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, tiles * C::SLABS * rows * 128);
+          for (int w = 0; w < tiles; ++w)
+            for (int sl = 0; sl < C::SLABS; ++sl)
+              tma_load_4d(q_s(w) + sl * C::QSLAB, &tm_q, q_full, sl * 64, it.h,
+                          (it.t0 + w) * sh.pos128, it.b);
+          ++nq;
         }
       }
       // Never leave a copy in flight.
       if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, p.status);
-      for (int j = nk - KST < 0 ? 0 : nk - KST; j < nk; ++j)
-        mbar_wait(k_full(j % KST), (j / KST) & 1, p.status);
-      for (int j = nv - VST < 0 ? 0 : nv - VST; j < nv; ++j)
-        mbar_wait(v_full(j % VST), (j / VST) & 1, p.status);
+      for (int j = ns - ST < 0 ? 0 : ns - ST; j < ns; ++j)
+        mbar_wait(kv_full(j % ST), (j / ST) & 1, p.status);
     } else if (warp >= 1 && warp <= 2 && elect_one_sync()) {
       // ------------------------------------- MMA of query tile w, a thread each
       constexpr uint32_t idesc_s = make_idesc_bf16(kTile, kHalf, false, false);
       constexpr uint32_t idesc_o = make_idesc_bf16(kTile, D, false, true);
       const int w = warp - 1;
-      Ring kr{0, 0}, vr{0, 0};  // the next key and value tile
+      Ring kv{0, 0};            // the next stage
       int qc = 0;               // query tiles used
       int scores = 0;           // products Q K^T issued
       int steps = 0;            // products P V issued
@@ -435,7 +415,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
           umma_bf16(d, make_sdesc(q_s(w) + (kk >> 2) * C::QSLAB + (kk & 3) * 32, 16, 1024, kSw128),
-                    make_sdesc(k_s(kr.stage) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
+                    make_sdesc(k_s(kv.stage) + (kk >> 2) * C::KSLAB + (kk & 3) * 32, 16, 1024,
                                kSw128),
                     idesc_s, kk > 0);
         umma_commit(s_full(w, scores));
@@ -446,7 +426,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
         for (int kk = 0; kk < kHalf / 16; ++kk)
           umma_bf16_ts(tmem + C::O_COL + w * D, a + kk * 8,
-                       make_sdesc(v_s(vr.stage) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_o,
+                       make_sdesc(v_s(kv.stage) + kk * 2048, C::KSLAB, 1024, kSw128), idesc_o,
                        (!begin || kk > 0) ? 1u : 0u);
         umma_commit(o_done(w, steps));
         ++steps;
@@ -468,35 +448,28 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         if (!ok) break;
         ++qc;
         if (to <= from) mbar_arrive(q_empty);
-        auto scores_of = [&](int t) -> bool {
-          if (!mbar_wait(k_full(kr.stage), kr.phase, p.status)) return false;
+        for (int t = 0; t < n_kv + 2; ++t) {  // S_w(t) and O_w's product t - 2
+          // Four key tiles before the end it is time to look for the next item.
+          if (t == max(n_kv - 2, 2)) mbar_arrive(item_empty(i & 1));
+          ok = mbar_wait(kv_full(kv.stage), kv.phase, p.status);
+          if (!ok) break;
+          if (t - 2 >= from && t - 2 < to) {
+            ok = mbar_wait(p_ready(w, steps), (steps >> 1) & 1, p.status);
+            // O_w's last item has been read before it is begun again.
+            if (ok && t - 2 == from && outs > 0)
+              ok = mbar_wait(o_free(w), (outs - 1) & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t - 2 == from);
+            outs += t - 2 == from;
+          }
           if (t >= from && t < to) {
             tc_fence_after();
             issue_s();
             if (t + 1 == to) umma_commit(q_empty);
           }
-          umma_commit(k_empty(kr.stage));
-          kr.next(KST);
-          return true;
-        };
-        for (int t = 0; t < min(n_kv, 2) && ok; ++t) ok = scores_of(t);
-        for (int t = 0; t < n_kv && ok; ++t) {
-          // Four key tiles before the end it is time to look for the next item.
-          if (t == max(n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
-          ok = mbar_wait(v_full(vr.stage), vr.phase, p.status);
-          if (!ok) break;
-          if (t >= from && t < to) {
-            ok = mbar_wait(p_ready(w, steps), (steps >> 1) & 1, p.status);
-            // O_w's last item has been read before it is begun again.
-            if (ok && t == from && outs > 0) ok = mbar_wait(o_free(w), (outs - 1) & 1, p.status);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(t == from);
-            outs += t == from;
-          }
-          umma_commit(v_empty(vr.stage));
-          vr.next(VST);
-          if (t + 2 < n_kv) ok = scores_of(t + 2);
+          umma_commit(kv_empty(kv.stage));
+          kv.next(ST);
         }
       }
       // Nothing may outlive the CTA's TMEM: wait for the tile's last product.
