@@ -44,6 +44,7 @@ constexpr int kBwdWarps = 8;      // that compute, beside the four of roles
 constexpr int kBwdThreads = 128 + 32 * kBwdWarps;
 constexpr int kParts = kBwdWarps / 4;     // of a streamed 64-wide tile's columns
 constexpr int kPartCols = kHalf / kParts;
+constexpr int kStageBytes = 4096;  // a storing warp's (store_rows)
 // Who reads a tile's description: TMA, two of MMA and every computing warp.
 constexpr int kFwdReaders = 3 + 8;
 constexpr int kBwdReaders = 3 + kBwdWarps;
@@ -184,21 +185,31 @@ __device__ __forceinline__ int take_cta(uint32_t slot, uint32_t bar, int n, int*
   return ok ? static_cast<int>(x) : -1;
 }
 
-// Rows of results: 2 N values a lane, in the widest stores the address allows.
+// Stores 2 N values (bf16 pairs) of a row a lane, through 128 N bytes of the
+// warp's in shared memory: an instruction then writes whole stretches of 4 N
+// bytes (from a row a lane it would write 32 bytes in each of 32 lines, and the
+// warps of a forward tile stood 2000 to 4000 cycles behind their stores).
 template <int N>
-__device__ __forceinline__ void store_row(uint16_t* dst, const uint32_t (&w)[N], bool wide) {
-  static_assert(N % 8 == 0, "whole wide stores");
-  if (wide) {
+__device__ __forceinline__ void store_rows(uint8_t* stage, const uint32_t (&w)[N], uint16_t* row,
+                                           bool valid) {
+  static_assert(N == 16 || N == 32, "64 or 128 bytes a row");
+  constexpr int C = N / 4;  // 16-byte chunks a row, in an order that spreads the banks
+  auto at = [&](int r, int c) {
+    return reinterpret_cast<uint4*>(stage + r * 4 * N + ((c ^ (N == 32 ? r & 7 : r >> 1 & 3)) << 4));
+  };
+  const int lane = threadIdx.x & 31;
+  const uint32_t rows = __ballot_sync(0xffffffffu, valid);
+  __syncwarp();  // what was here has been read
 #pragma unroll
-    for (int i = 0; i < N; i += 8)
-      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i),
-                   "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]),
-                   "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
-                   : "memory");
-  } else {
+  for (int c = 0; c < C; ++c)
+    *at(lane, c) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  __syncwarp();
 #pragma unroll
-    for (int i = 0; i < N; i += 4)
-      *reinterpret_cast<uint4*>(dst + 2 * i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  for (int k = 0; k < C; ++k) {
+    const int r = k * (32 / C) + lane / C, c = lane % C;
+    const uint4 x = *at(r, c);
+    const uint64_t to = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row), r);
+    if (rows >> r & 1) reinterpret_cast<uint4*>(to)[c] = x;
   }
 }
 
@@ -244,10 +255,11 @@ struct FwdCfg {
   static constexpr int KSLAB = kHalf * 128;   // 64 rows x 64 bf16
   static constexpr int KTILE = SLABS * KSLAB;
   // A stage holds K_{t+2} and V_t, which are wanted together.
-  static constexpr int ST = D == 128 ? 5 : 8;
+  static constexpr int ST = D == 128 ? 4 : 8;
   static constexpr int Q_OFF = 0;  // two query tiles
   static constexpr int KV_OFF = 2 * QTILE;
-  static constexpr int ITEM_OFF = KV_OFF + 2 * ST * KTILE;
+  static constexpr int OUT_OFF = KV_OFF + 2 * ST * KTILE;
+  static constexpr int ITEM_OFF = OUT_OFF + 8 * kStageBytes;
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(FwdItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
   // q_full, q_empty, kv_full[ST], kv_empty[ST], s_full[2][2], p_ready[2][2],
@@ -518,7 +530,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     const uint32_t ocol = lrow + C::O_COL + w * D;
     const float c = sh.scale_log2;
     const F2 cc2 = f2(c, c);
-    const bool wide = wide_rows(p.out);
+    uint8_t* const out_s = gbase + C::OUT_OFF + (warp - 4) * kStageBytes;
     bool ok = true;
     int steps = 0;  // key tiles of query tile w, of all items
     FwdItem it = wait_item(0, ok);
@@ -664,27 +676,27 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // 0: sees nothing
         const F2 inv2 = f2(inv, inv);
 #pragma unroll
-        for (int c4 = 0; c4 < D / 32; ++c4) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(ocol + c4 * 32, o);
+        for (int c0 = 0; c0 < D; c0 += 64) {
+          uint32_t o[2][32], wd[32];
+          tmem_ld_32x32b_x32(ocol + c0, o[0]);
+          tmem_ld_32x32b_x32(ocol + c0 + 32, o[1]);
           tmem_ld_wait();
-          if (c4 == D / 32 - 1) {  // O_w may be begun again
+          if (c0 + 64 == D) {  // O_w may be begun again
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(o_free(w));
           }
-          uint32_t wd[16];
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            wd[e] = pack_bf16(pair_of(o[2 * e], o[2 * e + 1]) * inv2);
-          if (valid) store_row(orow + c4 * 32, wd, wide);
+          for (int e = 0; e < 32; ++e)
+            wd[e] = pack_bf16(pair_of(o[e / 16][2 * e % 32], o[e / 16][2 * e % 32 + 1]) * inv2);
+          store_rows(out_s, wd, orow + c0, valid);
         }
         if (valid) *lse = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
-      } else if (valid) {  // no row of the tile sees anything
-        const uint32_t zero[16] = {};
+      } else {  // no row of the tile sees anything
+        const uint32_t zero[32] = {};
 #pragma unroll
-        for (int c4 = 0; c4 < D / 32; ++c4) store_row(orow + c4 * 32, zero, wide);
-        *lse = -INFINITY;
+        for (int c0 = 0; c0 < D; c0 += 64) store_rows(out_s, zero, orow + c0, valid);
+        if (valid) *lse = -INFINITY;
       }
       it = nx;
       sp = nsp;
@@ -862,13 +874,14 @@ struct DqCfg {
   static constexpr int QTILE = SLABS * QSLAB;
   static constexpr int KSLAB = kHalf * 128;  // 64 rows x 64 bf16
   static constexpr int KTILE = SLABS * KSLAB;
-  static constexpr int KST = D == 128 ? 5 : 8;
+  static constexpr int KST = D == 128 ? 4 : 8;
   static constexpr int VST = KST;  // (one stage index for both)
   static constexpr int Q_OFF = 0;
   static constexpr int DO_OFF = QTILE;
   static constexpr int K_OFF = 2 * QTILE;
   static constexpr int V_OFF = K_OFF + KST * KTILE;
-  static constexpr int ITEM_OFF = V_OFF + VST * KTILE;
+  static constexpr int OUT_OFF = V_OFF + VST * KTILE;
+  static constexpr int ITEM_OFF = OUT_OFF + kBwdWarps * kStageBytes;
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DqItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
   // q_full, q_empty, k_full[KST], k_empty[KST], v_full[VST], v_empty[VST], s_full[2],
@@ -1128,7 +1141,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = sh.scale_log2;
     const F2 c2 = f2(c, c), scale2 = f2(p.scale, p.scale);
-    const bool wide = wide_rows(p.dq);
+    uint8_t* const out_s = gbase + C::OUT_OFF + (warp - 4) * kStageBytes;
     bool ok = true;
     int g = 0, n = 0, nq = 0;
     struct RowState {
@@ -1246,26 +1259,22 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         tc_fence_after();
         ++n;
       }
-      constexpr int COLS = D / kParts < 32 ? D / kParts : 32;
+      constexpr int COLS = D / kParts;  // 64 or 32
+      uint32_t wd[COLS / 2] = {};
+      if (it.n_kv > 0) {
+        uint32_t o[COLS / 32][32];
 #pragma unroll
-      for (int e = 0; e < D / kParts / COLS; ++e) {
-        const int c0 = part * (D / kParts) + e * COLS;
-        uint32_t o[COLS];
-        uint32_t w[COLS / 2] = {};
-        if (it.n_kv > 0) {
-          tmem_ld_32x32b_x32(lrow + C::DQ_COL + c0, o);
-          tmem_ld_wait();
-          if (e == D / kParts / COLS - 1) {  // dQ may be begun again
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(dq_free);
-          }
+        for (int e = 0; e < COLS / 32; ++e)
+          tmem_ld_32x32b_x32(lrow + C::DQ_COL + part * COLS + e * 32, o[e]);
+        tmem_ld_wait();
+        tc_fence_before();  // dQ may be begun again
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dq_free);
 #pragma unroll
-          for (int q = 0; q < COLS / 2; ++q)
-            w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * scale2);
-        }
-        if (valid) store_row(orow + c0, w, wide);
+        for (int e = 0; e < COLS / 2; ++e)
+          wd[e] = pack_bf16(pair_of(o[e / 16][2 * e % 32], o[e / 16][2 * e % 32 + 1]) * scale2);
       }
+      store_rows(out_s, wd, orow + part * COLS, valid);
       it = nx;
       st = nst;
     }
@@ -1300,7 +1309,9 @@ struct DkvCfg {
   static constexpr int Q_OFF = 2 * KTILE;
   static constexpr int DO_OFF = Q_OFF + QST * QTILE;
   static constexpr int STAT_OFF = DO_OFF + QST * QTILE;
-  static constexpr int ITEM_OFF = STAT_OFF + QST * STAT_BYTES;
+  static constexpr int OUT_OFF = STAT_OFF + QST * STAT_BYTES;
+  static constexpr int OUT_BYTES = kStageBytes / 2;  // 32 columns at a time: no room for more
+  static constexpr int ITEM_OFF = OUT_OFF + kBwdWarps * OUT_BYTES;
   static constexpr int TAKE_OFF = ITEM_OFF + 2 * static_cast<int>(sizeof(DkvItem));
   static constexpr int BAR_OFF = TAKE_OFF + 16;
   // kv_full, kv_empty, q_full[QST], q_empty[QST], s_full[2], pds_ready[2], acc_full,
@@ -1564,7 +1575,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lrow = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const float c = sh.scale_log2;
     const F2 c2 = f2(c, c);
-    const bool wide = wide_rows(p.dk) && wide_rows(p.dv);
+    uint8_t* const out_s = gbase + C::OUT_OFF + (warp - 4) * C::OUT_BYTES;
     bool ok = true;
     int g = 0, n = 0;
     for (int i = 0; ok; ++i) {
@@ -1663,26 +1674,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const float f = which == 0 ? 1.0f : p.scale;
         const F2 ff = f2(f, f);
         uint16_t* orow = (which == 0 ? p.dv : p.dk) + roff;
-        constexpr int COLS = D / kParts < 32 ? D / kParts : 32;
+        constexpr int COLS = D / kParts;  // 64 or 32
+        uint32_t wd[COLS / 32][16] = {};
+        if (T > 0) {
+          uint32_t o[COLS / 32][32];
 #pragma unroll
-        for (int e = 0; e < D / kParts / COLS; ++e) {
-          const int c0 = part * (D / kParts) + e * COLS;
-          uint32_t o[COLS];
-          uint32_t w[COLS / 2] = {};
-          if (T > 0) {
-            tmem_ld_32x32b_x32(lrow + col + c0, o);
-            tmem_ld_wait();
-            if (which == 1 && e == D / kParts / COLS - 1) {  // dV and dK may begin again
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(acc_free);
-            }
-#pragma unroll
-            for (int q = 0; q < COLS / 2; ++q)
-              w[q] = pack_bf16(pair_of(o[2 * q], o[2 * q + 1]) * ff);
+          for (int e = 0; e < COLS / 32; ++e)
+            tmem_ld_32x32b_x32(lrow + col + part * COLS + e * 32, o[e]);
+          tmem_ld_wait();
+          if (which == 1) {  // dV and dK may begin again
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_free);
           }
-          if (valid) store_row(orow + c0, w, wide);
+#pragma unroll
+          for (int e = 0; e < COLS / 2; ++e)
+            wd[e / 16][e % 16] =
+                pack_bf16(pair_of(o[e / 16][2 * e % 32], o[e / 16][2 * e % 32 + 1]) * ff);
         }
+#pragma unroll
+        for (int e = 0; e < COLS / 32; ++e)
+          store_rows(out_s, wd[e], orow + part * COLS + e * 32, valid);
       }
     }
   }
