@@ -257,7 +257,7 @@ __device__ __forceinline__ void st_chunk(void* p, const uint32_t (&w)[8]) {
 // What a row's sums are of, beside s = sum 2^x: nothing, a = sum x 2^x (the
 // entropy's), or a = sum 2^y, y = (z - m) log2(e) (a second temperature, 1);
 // at temperature 2, 2^y is the square of 2^x, which spares the MUFU unit the
-// second exponential (2046 x 128256: 141 -> 96 us forward).
+// second exponential (2046 x 128256: 89 us forward, 121 at temperature 3).
 enum Mode { kPlain, kEntropy, kTwo, kSquare };
 
 struct Sums {
@@ -697,7 +697,9 @@ struct LogprobParams {
 };
 
 // One CTA per row, or a cluster of `split` CTAs when rows are few, each a
-// contiguous slice of the row's chunks; rank 0 joins them in rank order.
+// contiguous slice of the row's chunks; rank 0 joins them in rank order.  Bound
+// by reading the logits: 2046 x 128256 in 87 us, 6.0 TB/s; 777 x 32003 f32, rows
+// of 16 chunks a thread, 22 us, 4.6 TB/s.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const LogprobParams p) {
   constexpr int U = kInFlight;
@@ -902,6 +904,8 @@ struct LogprobGradParams {
   float c, inv_t;  // log2(e) / temperature, 1 / temperature
 };
 
+// Bound by reading and writing: 2046 x 128256 in 160 us, 6.6 TB/s (in place and
+// behind the forward 150, with rows left in L2).
 template <typename T, bool SAME>
 __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const LogprobGradParams p) {
   griddep_wait();
@@ -1026,7 +1030,9 @@ struct DistillParams {
 };
 
 // kTwo, kSquare: the targets' cross-entropy needs the row's sum at temperature
-// 1 too.
+// 1 too.  Bound by reading the logits: 2046 x 128256 in 88 us with one sum, 89
+// with squares, 121 with both exponentials; 511 x 151936 in 37 us, 4.1 TB/s (511
+// CTAs leave a seventh of 592 places empty; in halves they cost as much more).
 template <typename T, Mode M>
 __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const DistillParams p) {
   constexpr bool TWO = M != kPlain;
@@ -1141,6 +1147,7 @@ struct DistillGradParams {
 // Every element first as if nothing were given (the two softmaxes alone); the
 // few given ones are then written again by the CTA that wrote them, with what
 // all their entries in the row take off (the same id may be given twice).
+// 2046 x 128256 with 64 alternatives: 170 us, 6.2 TB/s.
 template <typename T, bool SAME, Mode M>
 __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGradParams p) {
   __shared__ int ids[kMaxTop + 1];

@@ -29,6 +29,12 @@
 //   SMs idle for a quarter to a third of the time), a little before their own
 //   ends: a scheduler warp reads the next tile's spans, its copies and first
 //   product run while the last one's results are stored.
+// * Two threads issue a CTA's matrix products, each the chains that depend on
+//   themselves only.  A wait costs a thread about 100 cycles even where nothing
+//   is to be waited for, a commit up to 60, and the tensor cores' queue is too
+//   short to hide them: alone, the products of a forward step take 1290 cycles,
+//   with one thread's waits 1800, with two threads' 1340.  (An M = 128, K = 16
+//   product takes 64 cycles at N = 128 and 45 to 50 at N = 64.)
 #include <cuda_bf16.h>
 
 #include <climits>
@@ -222,15 +228,15 @@ __device__ __forceinline__ bool wide_rows(const void* p) {
 // A tile of work is a pair of adjacent packed query tiles of one sequence and
 // key/value head; both share every key/value tile the pair needs.
 //   warp 0       TMA: the query tiles, key and value tiles through a ring
-//   warp 1       one thread issues every tcgen05 MMA
-//   warp 2       allocates / frees the 512 TMEM columns
+//   warps 1, 2   one thread each issues the tcgen05 MMAs of query tile 0, 1;
+//                warp 2 also allocates and frees the 512 TMEM columns
 //   warp 3       scheduler: the next pairs' descriptions, two in shared memory
 //   warps 4-7    softmax of query tile 0 (thread i owns row i, TMEM lane i)
 //   warps 8-11   softmax of query tile 1
 // TMEM: S_w,b (64 f32 columns each: key tiles of 64, two of each query tile) |
-// O_0 | O_1 (dim columns each); P_w,b (bf16 pairs) over S_w,b.  MMA issue order
-// per key tile t, with S of tiles 0 and 1 ahead of the first:
-//   O_0 += P_0(t) V_t,  S_0(t+2) = Q_0 K_{t+2}^T,  O_1 += P_1(t) V_t,  S_1(t+2) ...
+// O_0 | O_1 (dim columns each); P_w,b (bf16 pairs) over S_w,b.  Thread w issues
+// S_w(0), S_w(1) and then, per key tile t,
+//   O_w += P_w(t) V_t,  S_w(t+2) = Q_w K_{t+2}^T
 // and tcgen05.mma operations issued by one thread execute in that order, so
 // S_w(t+2) overwrites P_w(t) right after its product has read it, and a softmax
 // warp has its next scores while it works on these.  (With key tiles of 128 and
@@ -239,6 +245,14 @@ __device__ __forceinline__ bool wide_rows(const void* p) {
 // reference (kMost) and looks at its sum.  Barriers count through all pairs, and
 // no waiter is two phases behind: s_full, p_ready and o_done come in two, by the
 // tile's parity, and S_w(t) complete says that O_w's product t-2 is, too.
+//
+// Four packed rows of 2048 (32 heads over 8 of 128, some six documents a row):
+// 70 us, one row of 8191 with documents of up to 2000: 122 us, 0.62 and 1.0
+// PFLOP/s of what its tiles multiply.  A step of two 64-key products and two of
+// 128 columns takes some 1600 to 1900 cycles of which the tensor cores need 1290
+// and the exponentials 1024; the rest is a tile's end (some 4000 cycles: the last
+// product, O out of tensor memory, the stores), a fifth of the short documents'
+// time.
 
 struct FwdItem {
   int b, h, t0;              // b < 0: no more; first of `pack` heads, first query tile
@@ -721,16 +735,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //   dq     a tile of work is a packed 128-row query tile, key tiles of 64:
 //            S = Q K_j^T, dP = dO V_j^T (tensor memory, double-buffered),
 //            dS = P * (dP - delta), P = exp2(S c - lse2)  (compute warps),
-//            dQ += dS K_j  (dS written back to tensor memory, A from TMEM);
+//            dQ += dS K_j  (dS written over S, A from tensor memory).
+//          Q and dO lie in tensor memory too: read from shared memory for every
+//          key tile they took 94 us where this takes 81;
 //   dkv    a tile of work is a 128-key tile of one key/value head, with the
 //          packed 64-row query tiles that see it:
 //            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, back
 //            into tensor memory), dV += P^T dO_i, dK += dS^T Q_i.
-//          What bounds it is shared memory's 128 bytes a cycle, which feed the
-//          tensor cores: K and Q, V and dO, dO and Q again, 128 KB a tile
-//          and 32 KB of copies -- 1280 cycles; with P^T and dS^T as operands
-//          there too it was 1800.
-// Which CTA does a tile changes no result.
+//          Its products take 1310 cycles a tile and shared memory, which feeds
+//          them 128 KB and takes in 32 KB of copies, 1280 of its 128 bytes a
+//          cycle; with P^T and dS^T as operands there too it was 127 us where
+//          this takes 103.
+// At four packed rows of 2048 (as above): 24, 81 and 103 us.  Which CTA does a
+// tile changes no result.
 
 // The workspace: statistics [batch, heads / pack, tiles64, 64], spans (first
 // key, how many) [batch, tiles64, 64], tiles: what any row of a 64-row packed
@@ -774,7 +791,7 @@ __device__ __forceinline__ void load_16(const uint16_t* p, bool wide, uint32_t (
 }
 
 // A CTA a 64-row tile: two rows a thread, 16 elements of each.  Bound by
-// reading out and dout (packed rows of 2048: 134 MB).
+// reading out and dout (packed rows of 2048: 134 MB in 24 us).
 template <int D>
 __global__ void __launch_bounds__(2 * D) span_prep_kernel(const PrepParams p) {
   constexpr int LANES = D / 16;
@@ -1131,8 +1148,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     // ------------------------------------------------------ compute warps
     // The warpgroups share the 128 rows and split each tile's 64 key columns
     // (the gradient is elementwise given the row's lse and delta), and dQ's
-    // columns at the end.  Two of them: four (96 registers a thread) took 97 us
-    // where two take 94.
+    // columns at the end.  Two of them: four (96 registers a thread) were no
+    // faster.
     const int part = (warp - 4) >> 2;
     const int quad = warp & 3;
     const int row = quad * 32 + lane;
@@ -1508,8 +1525,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int s = g % QST;
           // Four query tiles before the end it is time to look for the next item.
           if (t == max(T - 4, 0)) mbar_arrive(item_empty(i & 1));
-          // S^T_g and dP^T_g go over P^T and dS^T of two tiles ago, whose
-          // products were issued before.
+          // S^T_g (dP^T_g) goes over P^T (dS^T) of two tiles ago, whose product
+          // this thread has issued.
           ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
           if (!ok) break;
           tc_fence_after();
@@ -1716,7 +1733,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // vote a word gives where runs start, bit operations the nearest start of a
 // lane, and one value a warp in shared memory joins the warps.  A row longer
 // than a stretch of 8192 goes stretch by stretch, from the front for the
-// starts and from the back for the ends.
+// starts and from the back for the ends.  Latency is all there is to it: 4 us
+// for one row of 8191, 6 with prefixes.
 
 constexpr int kDocWarps = 32;
 constexpr int kDocWords = 8;
