@@ -232,7 +232,8 @@ class Trainer:
         # one CUDA graph (captured on the first step of a batch shape); the
         # collective and the optimizer stay outside it (AdamW takes the step
         # count from the host).  For small models, whose step the host's
-        # per-launch work would otherwise bound.
+        # per-launch work would otherwise bound.  The objective is captured as
+        # it is: what it reads beside its arguments is read where it lay then.
         self.graph = graph
         self._graphs: dict[tuple, tuple] = {}
         self.opt = opt or AdamWConfig()
