@@ -237,10 +237,10 @@ __device__ __forceinline__ bool wide_rows(const void* p) {
 // O_0 | O_1 (dim columns each); P_w,b (bf16 pairs) over S_w,b.  Thread w issues
 // S_w(0), S_w(1) and then, per key tile t,
 //   O_w += P_w(t) V_t,  S_w(t+2) = Q_w K_{t+2}^T
-// and tcgen05.mma operations issued by one thread execute in that order, so
-// S_w(t+2) overwrites P_w(t) right after its product has read it, and a softmax
-// warp has its next scores while it works on these.  (With key tiles of 128 and
-// one S a query tile it waited 1300 of 4000 cycles for its next scores.)
+// S_w(t+2) overwrites P_w(t), so it is issued when that product is done (the
+// order of two products is given only where shape and accumulator are the same),
+// and a softmax warp has its next scores while it works on these.  (With key
+// tiles of 128 and one S a query tile it waited 1300 of 4000 cycles for them.)
 // A softmax thread needs no maximum before the exponentials: it keeps a
 // reference (kMost) and looks at its sum.  Barriers count through all pairs, and
 // no waiter is two phases behind: s_full, p_ready and o_done come in two, by the
@@ -490,6 +490,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             outs += t - 2 == from;
           }
           if (t >= from && t < to) {
+            // S_w goes over P_w of two tiles ago: its product is done.
+            if (scores >= 2)
+              ok = mbar_wait(o_done(w, scores), ((scores - 2) >> 1) & 1, p.status);
+            if (!ok) break;
             tc_fence_after();
             issue_s();
             if (t + 1 == to) umma_commit(q_empty);
@@ -596,7 +600,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           for (int c2 = 0; c2 < 2; ++c2) {
             uint32_t r[32];
             tmem_ld_32x32b_x32(scol + c2 * 32, r);
-            tmem_ld_wait();
+            tmem_ld_wait(r);
             if (!full(c2)) mask(c2, r);
             float t[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -617,7 +621,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2)
           if (!none(c2)) tmem_ld_32x32b_x32(scol + c2 * 32, rb[c2]);
-        tmem_ld_wait();
+        tmem_ld_wait(rb[0], rb[1]);
 #pragma unroll
         for (int c2 = 0; c2 < 2; ++c2) {
           if (none(c2)) {
@@ -648,7 +652,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             for (int cc = 0; cc < D / 16; ++cc) {
               uint32_t o[16];
               tmem_ld_32x32b_x16(ocol + cc * 16, o);
-              tmem_ld_wait();
+              tmem_ld_wait(o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
               tmem_st_32x32b_x16(ocol + cc * 16, o);
@@ -659,7 +663,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           for (int c2 = 0; c2 < 2; ++c2) {
             uint32_t r[32], pc[16];
             tmem_ld_32x32b_x32(scol + c2 * 32, r);
-            tmem_ld_wait();
+            tmem_ld_wait(r);
             mask(c2, r);
             sum2 = sum2 + exp_chunk(r, cc2, m == -INFINITY ? 0.0f : m, pc);
             tmem_st_32x32b_x16(scol + c2 * 16, pc);
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
           uint32_t o[2][32], wd[32];
           tmem_ld_32x32b_x32(ocol + c0, o[0]);
           tmem_ld_32x32b_x32(ocol + c0 + 32, o[1]);
-          tmem_ld_wait();
+          tmem_ld_wait(o[0], o[1]);
           if (c0 + 64 == D) {  // O_w may be begun again
             tc_fence_before();
             __syncwarp();
@@ -736,8 +740,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //            S = Q K_j^T, dP = dO V_j^T (tensor memory, double-buffered),
 //            dS = P * (dP - delta), P = exp2(S c - lse2)  (compute warps),
 //            dQ += dS K_j  (dS written over S, A from tensor memory).
-//          Q and dO lie in tensor memory too: read from shared memory for every
-//          key tile they took 94 us where this takes 81;
+//          Q and dO lie in tensor memory too (read from shared memory for every
+//          key tile: 94 us where it then took 85);
 //   dkv    a tile of work is a 128-key tile of one key/value head, with the
 //          packed 64-row query tiles that see it:
 //            S^T = K Q_i^T, dP^T = V dO_i^T, P^T and dS^T (compute warps, back
@@ -745,9 +749,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 //          Its products take 1310 cycles a tile and shared memory, which feeds
 //          them 128 KB and takes in 32 KB of copies, 1280 of its 128 bytes a
 //          cycle; with P^T and dS^T as operands there too it was 127 us where
-//          this takes 103.
-// At four packed rows of 2048 (as above): 24, 81 and 103 us.  Which CTA does a
-// tile changes no result.
+//          it then took 103.
+// Scores go over operands of two tiles ago once their product is done (without
+// that wait dq took 81 us and dk/dv 103).  At four packed rows of 2048 (as
+// above): 24, 84 and 108 us.  Which CTA does a tile changes no result.
 
 // The workspace: statistics [batch, heads / pack, tiles64, 64], spans (first
 // key, how many) [batch, tiles64, 64], tiles: what any row of a 64-row packed
@@ -1089,9 +1094,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int s = g % KST;
           // Four key tiles before the end it is time to look for the next item.
           if (j == max(it.n_kv - 4, 0)) mbar_arrive(item_empty(i & 1));
-          // S_g goes over dS of two tiles ago, whose product this thread has
-          // issued; dP_g over that tile's dP, read before its dS was ready.
-          ok = first ? mbar_wait(k_full(s), (g / KST) & 1, p.status)
+          // S_g goes over dS of two tiles ago, whose product is done when it
+          // gives its keys back; dP_g over that tile's dP, read before its dS
+          // was ready.
+          ok = first ? mbar_wait(k_full(s), (g / KST) & 1, p.status) &&
+                           (g < 2 || mbar_wait(k_empty((g - 2) % KST), ((g - 2) / KST) & 1, p.status))
                      : mbar_wait(v_full(s), (g / VST) & 1, p.status) &&
                            (g < 2 || mbar_wait(ds_ready(g & 1), ((g - 2) >> 1) & 1, p.status));
           if (!ok) break;
@@ -1235,7 +1242,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!none) {
           tmem_ld_32x32b_x32(lrow + C::S_COL + (g & 1) * kHalf + part * kPartCols, sv);
           tmem_ld_32x32b_x32(lrow + C::DP_COL + (g & 1) * kHalf + part * kPartCols, dv);
-          tmem_ld_wait();
+          tmem_ld_wait(sv, dv);
         }
         uint32_t pk[kPartCols / 2];
         if (none) {
@@ -1284,6 +1291,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         for (int e = 0; e < COLS / 32; ++e)
           tmem_ld_32x32b_x32(lrow + C::DQ_COL + part * COLS + e * 32, o[e]);
         tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < COLS / 32; ++e) keep_behind(o[e]);
         tc_fence_before();  // dQ may be begun again
         __syncwarp();
         if (lane == 0) mbar_arrive(dq_free);
@@ -1526,8 +1535,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           // Four query tiles before the end it is time to look for the next item.
           if (t == max(T - 4, 0)) mbar_arrive(item_empty(i & 1));
           // S^T_g (dP^T_g) goes over P^T (dS^T) of two tiles ago, whose product
-          // this thread has issued.
-          ok = mbar_wait(q_full(s), (g / QST) & 1, p.status);
+          // is done when its stage is given back.
+          ok = mbar_wait(q_full(s), (g / QST) & 1, p.status) &&
+               (g < 2 || mbar_wait(q_empty((g - 2) % QST), ((g - 2) / QST) & 1, p.status));
           if (!ok) break;
           tc_fence_after();
           const uint32_t a = first ? k_s : v_s, b = first ? q_s(s) : do_s(s);
@@ -1630,7 +1640,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!none) {
           tmem_ld_32x32b_x32(scol, sv);
           tmem_ld_32x32b_x32(dcol, dv);
-          tmem_ld_wait();
+          tmem_ld_wait(sv, dv);
         }
         uint32_t pk[kPartCols / 16][8], dk[kPartCols / 16][8];  // by 16 queries
         if (none) {
@@ -1699,6 +1709,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int e = 0; e < COLS / 32; ++e)
             tmem_ld_32x32b_x32(lrow + col + part * COLS + e * 32, o[e]);
           tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < COLS / 32; ++e) keep_behind(o[e]);
           if (which == 1) {  // dV and dK may begin again
             tc_fence_before();
             __syncwarp();

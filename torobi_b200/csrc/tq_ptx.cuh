@@ -360,6 +360,19 @@ __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The same, with the registers that the loads fill handed through, so that
+// nothing that reads them can be moved ahead of the wait.
+template <int N>
+__device__ __forceinline__ void keep_behind(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+template <typename... Regs>
+__device__ __forceinline__ void tmem_ld_wait(Regs&... r) {
+  tmem_ld_wait();
+  (keep_behind(r), ...);
+}
+
 // Shared-memory matrix descriptor for tcgen05.mma.
 //   bits  0-13  start address >> 4
 //   bits 16-29  leading-dimension byte offset >> 4
