@@ -433,6 +433,46 @@ def test_span_attention_repeats_captured_and_on_another_stream(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 1300, 8, 2, 128), (2, 700, 14, 2, 64), (4, 2100, 4, 4, 64)],
+                         ids=str)
+def test_every_run_writes_every_value(cuda, shape):
+    """Outputs, gradients and workspace full of NaN before each of 20 runs of
+    many tiles an SM, with and without idle gaps: always the same bits."""
+    import ctypes
+    import random
+
+    import torch
+
+    from torobi_b200 import device_status, glue
+    from torobi_b200._lib import lib
+
+    b, s, h, hk, d = shape
+    first, last = _spans(cuda, _random_documents(random.Random(s), b, s, 200))
+    q, k, v, do = _inputs(cuda, s, b, s, h, hk, d, 6.0)
+    o, lse = glue.span_attention_forward(q, k, v, first, last)
+    want = o, lse, *glue.span_attention_backward(q, k, v, first, last, o, do, lse)
+    got = [torch.empty_like(t) for t in want]
+    need = ctypes.c_size_t()
+    assert lib().tq_span_attention_bwd_workspace_bytes(b, s, h, hk, ctypes.byref(need)) == 0
+    ws = torch.empty(need.value, dtype=torch.uint8, device=cuda)
+    stream = torch.cuda.current_stream().cuda_stream
+    at = [t.data_ptr() for t in (q, k, v, first, last)]
+    for run in range(20):
+        for t in got:
+            t.fill_(float("nan"))
+        ws.fill_(255)
+        if run % 3 == 0:
+            torch.cuda.synchronize()
+        assert lib().tq_span_attention_fwd(*at, b, s, h, hk, d, d ** -0.5, got[0].data_ptr(),
+                                           got[1].data_ptr(), stream) == 0
+        assert lib().tq_span_attention_bwd(
+            *at, o.data_ptr(), do.data_ptr(), lse.data_ptr(), b, s, h, hk, d, d ** -0.5,
+            *[t.data_ptr() for t in got[2:]], ws.data_ptr(), need.value, stream) == 0
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+    assert device_status() == 0
+
+
+@pytest.mark.gpu
 def test_span_refusals(cuda):
     import torch
 
