@@ -507,7 +507,9 @@ int tq_distill_fwd(const void* logits, int dtype, const void* teacher_ids, int i
  * Its VJP with respect to the logits (dkl, dce [rows] f32, NULL for none):
  *   dlogits[r, j] = dkl[r] / T (q[j] - sum_{i: ids[i] == j} p[i])
  *                   + dce[r] (softmax(z[r])[j] - [j == targets[r]])
- * dlogits may be the logits buffer itself (then ld_out == ld).
+ * A row whose upstream gradients are 0, or without a distribution, gets zeros
+ * (the given ids and the target too).  dlogits may be the logits buffer itself
+ * (then ld_out == ld).
  */
 int tq_distill_bwd(const void* logits, int dtype, const void* teacher_ids, int ids_bits,
                    const void* teacher_logits, int teacher_dtype, int64_t k,

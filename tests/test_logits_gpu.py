@@ -627,6 +627,41 @@ def test_given_at_minus_infinity_and_dead_rows(cuda):
     assert torch.isfinite(dz).all() and dz[1, 7] == -0.5
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0])
+@pytest.mark.parametrize("vocab, dtype", [(64, "f32"), (1003, "bf16"), (40000, "bf16")])
+def test_a_row_without_a_distribution_passes_no_gradient(cuda, vocab, dtype, temperature, inplace):
+    """A student row of nothing but -inf: kl and ce are +inf and the gradient is
+    0 everywhere, at the given ids and the target too, through kl, through ce
+    and through both; the rows beside it are as they are without it."""
+    import torch
+
+    from torobi_b200 import glue
+
+    z = _logits(cuda, 4, vocab, dtype, 14)
+    ids = torch.tensor([[7, 8, vocab - 1]] * 4, device=cuda)
+    t = torch.tensor([[0.0, 1.0, -1.0]] * 4, device=cuda)
+    targets = torch.tensor([1, 7, 8, vocab - 2], device=cuda)
+    one = torch.ones(4, device=cuda)
+    for ups in ((one, None), (None, one), (one, one)):
+        grads = []
+        for dead in (False, True):
+            x = z.clone()
+            if dead:
+                x[2] = NINF
+            leaf = x.requires_grad_()
+            out = glue.distillation(leaf, ids, t, targets=targets, temperature=temperature,
+                                    inplace=inplace)
+            if dead:
+                assert out[0][2] == math.inf and out[1][2] == math.inf
+            used = [(o, u) for o, u in zip(out, ups) if u is not None]
+            grads += torch.autograd.grad([o for o, _ in used], leaf, [u for _, u in used])
+        clean, dz = grads
+        assert (dz[2] == 0).all() and (clean[2] != 0).any()
+        keep = torch.tensor([0, 1, 3], device=cuda)
+        assert torch.equal(dz[keep], clean[keep])
+
+
 # ------------------------------------------------------------- how it is called --
 
 @pytest.mark.parametrize("temperature", [1.0, 2.0, 3.0])

@@ -1161,9 +1161,9 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGrad
   T* const dz = static_cast<T*>(p.dz) + r * p.ld_out;
   const int k = p.teacher.k;
   float m, ca, cb;
-  bool zero, dead;
+  bool zero;
   auto soft = [&](float f) {
-    if (zero || dead) return 0.0f;
+    if (zero) return 0.0f;
     const float d = f - m;
     const float e = ex2_approx(d * p.c);
     if (M == kSquare) return e * fmaf(cb, e, ca);
@@ -1199,13 +1199,12 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(const DistillGrad
     }
     // Whether anything of the teacher's is given; also orders ids and off.
     const float us = __syncthreads_or(any) ? u : 0.0f;
-    // A row that no gradient reaches gets zeros whatever it holds; one without
-    // a distribution has q = 0.
+    // A row that no gradient reaches gets zeros whatever it holds, and so does
+    // one without a distribution, at its given ids and its target too.
     m = st.x;
-    dead = st.y == -INFINITY;
-    zero = us == 0.0f && v == 0.0f;
-    ca = dead ? 0.0f : us * exp2f(-st.y);
-    cb = dead ? 0.0f : v * exp2f(-st.z);
+    zero = (us == 0.0f && v == 0.0f) || st.y == -INFINITY;
+    ca = us * exp2f(-st.y);
+    cb = v * exp2f(-st.z);
     if (M == kPlain) ca += cb;
     // The given elements' logits, before anything is written over them.
     mine = static_cast<int>(threadIdx.x) <= k ? ids[threadIdx.x] : -1;
