@@ -15,6 +15,8 @@ plus 4 steps of f32 of its own size and of the scores'.
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 
 R = 2.0 ** -8 * 1.1
@@ -469,6 +471,289 @@ def test_every_run_writes_every_value(cuda, shape):
             *at, o.data_ptr(), do.data_ptr(), lse.data_ptr(), b, s, h, hk, d, d ** -0.5,
             *[t.data_ptr() for t in got[2:]], ws.data_ptr(), need.value, stream) == 0
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+    assert device_status() == 0
+
+
+def _outgrown(q, k, first, last, scale):
+    """How often each query's sum over a 64-key tile passes 2^60 against the
+    reference it has by then (the largest score of the first tile it sees, then
+    of the tile where that happened), int [batch, heads, seq], in 64 bits."""
+    import torch
+
+    b, s, h, _ = q.shape
+    group = h // k.shape[2]
+    x = torch.einsum("bihd,bjhd->bhij", q.double(),
+                     k.double().repeat_interleave(group, 2)) * (scale / math.log(2))
+    j = torch.arange(s, device=q.device)
+    see = (j >= first[:, None, :, None]) & (j < last[:, None, :, None])
+    x = x.masked_fill(~see, float("-inf"))
+    m = torch.full((b, h, s), float("-inf"), device=q.device, dtype=torch.float64)
+    times = torch.zeros(b, h, s, dtype=torch.int64, device=q.device)
+    for at in range(0, s, 64):
+        tile = x[..., at:at + 64]
+        top = tile.amax(3)
+        m = torch.where(m == float("-inf"), top, m)
+        total = torch.exp2(tile - m.nan_to_num(neginf=0.0)[..., None]).sum(3)
+        over = total > 2.0 ** 60
+        times += over
+        m = torch.where(over, top, m)
+    return times
+
+
+def _climbing(cuda, seed, b, s, h, hk, d, docs=None):
+    """Operands whose scores climb along a row: the keys lie along one direction,
+    further out every 100 positions, a third of the queries with it, a third
+    twice as far, a third at right angles (beside noise): a step is 70 powers of
+    two for the first third."""
+    import torch
+
+    q, k, v, do = (t.float() for t in _inputs(cuda, seed, b, s, h, hk, d, 0.5))
+    i = torch.arange(s, device=cuda)
+    way = torch.ones(d, device=cuda)
+    way[::2] = -1.0
+    step = 70 * math.log(2) * d ** 0.5 / d
+    far = (i // 100 % 5) * step  # and back to the start, where little weight is left
+    k = 0.25 * k + far[None, :, None, None] * way
+    rows = (i[:, None] + torch.arange(h, device=cuda)) % 3
+    q = q + rows[None, :, :, None] * way
+    return q.bfloat16(), k.bfloat16(), v.bfloat16(), do.bfloat16()
+
+
+def _check_steep(q, k, v, do, first, last):
+    """As _check, for scores so large that their own rounding counts.  A score is
+    a sum of D products in the tensor cores' f32, 16 at a time, each sum off by at
+    most a step (2^-23) of the products' sum `top`, and 4 steps more are the
+    scale's, its product's and the reference's; a probability errs by as much of
+    itself, twice (by its score and by the log-sum-exp)."""
+    import torch
+
+    from torobi_b200 import device_status, glue
+
+    d = q.shape[-1]
+    sc = d ** -0.5
+    ro, ob, rl, g, gb = _reference(q, k, v, first, last, sc, do)
+    top = (q.double().norm(dim=3).amax() * k.double().norm(dim=3).amax() * sc).item()
+    score = (d / 16 + 4) * 2.0 ** -23 * top
+    r = R + 2 * score
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o, lse = glue.span_attention_forward(q, k, v, first, last)
+    got = glue.span_attention_backward(q, k, v, first, last, o, do, lse)
+    assert ((o.double() - ro).abs() <= r * (ob + ro.abs()) + 1e-30).all()
+    assert ((lse.double() - rl).abs()
+            <= score + 2.0 ** -20 + 4 * 2.0 ** -24 * (rl.abs() + top)).all()
+    again = glue.span_attention(*leaves, first, last)
+    assert torch.equal(again, o)
+    for a, c in zip(torch.autograd.grad(again, leaves, do), got):
+        assert torch.equal(a, c)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        off = (t.double() - g[name]).abs() - r * (gb[name] + g[name].abs()) - 1e-6 * top
+        assert off.max().item() <= 0, (name, off.max().item())
+    assert device_status() == 0
+
+
+STEEP = [
+    # batch, seq, heads, kv_heads, dim, positions a document (0: the whole row)
+    (1, 500, 4, 2, 64, 0),
+    (1, 500, 4, 2, 128, 0),
+    (2, 777, 8, 2, 128, 0),
+    (2, 777, 14, 2, 64, 333),     # documents that start inside a tile of others
+    (1, 1025, 3, 1, 64, 420),
+    (1, 900, 6, 6, 128, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", STEEP, ids=str)
+def test_scores_that_outgrow_their_reference(cuda, case):
+    """Scores that climb past 2^60 of the first tile's maximum, several times
+    along a row, for some rows of a warp and not for others: O in tensor memory
+    is scaled in place and the tile done again."""
+    import torch
+
+    b, s, h, hk, d, length = case
+    i = torch.arange(s, device=cuda, dtype=torch.int32).expand(b, s)
+    first = (i // length * length if length else torch.zeros_like(i)).contiguous()
+    last = (i + 1).contiguous()
+    q, k, v, do = _climbing(cuda, 50 + s, b, s, h, hk, d)
+    times = _outgrown(q, k, first, last, d ** -0.5)
+    # The first third of queries two to four times, the last third never.
+    for n in (0, 1, 2, 3):
+        assert (times == n).sum().item() >= 20, (n, times.unique(return_counts=True))
+    _check_steep(q, k, v, do, first, last)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_steep_random_scores(cuda, dim):
+    """Queries 40 times as long as a trained model's: hundreds of rows outgrow
+    their reference, here and there."""
+    import torch
+
+    b, s, h, hk = 2, 777, 4, 2
+    i = torch.arange(s, device=cuda, dtype=torch.int32).expand(b, s).contiguous()
+    first, last = (i // 300) * 300, i + 1
+    q, k, v, do = _inputs(cuda, 5 + dim, b, s, h, hk, dim, 40.0)
+    assert (_outgrown(q, k, first, last, dim ** -0.5) > 0).sum().item() >= 200
+    _check_steep(q, k, v, do, first, last)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 1300, 8, 2, 128), (2, 700, 14, 2, 64)], ids=str)
+def test_rows_that_outgrow_their_reference_repeat(cuda, shape):
+    """The same over outputs full of NaN, 20 times: always the same bits."""
+    import torch
+
+    from torobi_b200 import device_status
+    from torobi_b200._lib import lib
+
+    b, s, h, hk, d = shape
+    i = torch.arange(s, device=cuda, dtype=torch.int32).expand(b, s).contiguous()
+    first, last = (i // 450) * 450, i + 1
+    q, k, v, _ = _climbing(cuda, s, b, s, h, hk, d)
+    assert (_outgrown(q, k, first, last, d ** -0.5) > 1).sum().item() >= 200
+    stream = torch.cuda.current_stream().cuda_stream
+    want = None
+    for run in range(20):
+        o = torch.full_like(q, float("nan"))
+        lse = torch.full((b, h, s), float("nan"), device=cuda)
+        if run % 3 == 0:
+            torch.cuda.synchronize()
+        assert lib().tq_span_attention_fwd(
+            *[t.data_ptr() for t in (q, k, v, first, last)], b, s, h, hk, d, d ** -0.5,
+            o.data_ptr(), lse.data_ptr(), stream) == 0
+        if want is None:
+            want = o, lse
+            assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    assert device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_every_visible_key_counts_once(cuda, case):
+    """Queries of zero weigh all their keys alike: the sum is their number
+    exactly, the log-sum-exp its logarithm (log2f is off by at most a step, its
+    product with ln 2 by half a step each of the factor and the result: 2 steps
+    of 2^-23), and o the mean of their values (sums in f32 and one rounding)."""
+    import random
+
+    import torch
+
+    from torobi_b200 import glue
+
+    b, s, h, hk, d, mean, _, causal = case
+    docs = _random_documents(random.Random(s + 1), b, s, mean)
+    first, last = _spans(cuda, docs, None, causal)
+    q, k, v, _ = _inputs(cuda, s + d + 1, b, s, h, hk, d)
+    o, lse = glue.span_attention_forward(torch.zeros_like(q), k, v, first, last)
+    n = (last - first).double()
+    want = n.log()[:, None].expand_as(lse)
+    fine = want.isfinite()
+    assert torch.equal(lse[~fine].double(), want[~fine])
+    assert ((lse.double() - want).abs()[fine] <= 2 * 2.0 ** -23 * want[fine]).all()
+    sums = torch.zeros(b, s + 1, hk, d, device=cuda, dtype=torch.float64)
+    size = sums.clone()
+    sums[:, 1:] = v.double().cumsum(1)
+    size[:, 1:] = v.double().abs().cumsum(1)
+
+    def mean_of(c):
+        at = lambda i: c.gather(1, i.long()[..., None, None].expand(b, s, hk, d))  # noqa: E731
+        return ((at(last) - at(first)) / n.clamp(min=1)[..., None, None]).repeat_interleave(
+            h // hk, 2)
+
+    ro = mean_of(sums)
+    # s additions in f32, and two roundings more, beside that to bf16.
+    assert ((o.double() - ro).abs()
+            <= 2.0 ** -8 * 1.01 * ro.abs() + (s + 2) * 2.0 ** -24 * mean_of(size) + 1e-30).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_log_sum_exp_to_f32(cuda, case):
+    """lse by its own arithmetic.  A score is a sum of D products in the tensor
+    cores' f32 (16 at a time, each sum off by at most a step, 2^-23, of the
+    products' sum so far; 4 steps for the scale, its product and the reference's);
+    the exponentials are off by 2^-22, their sum by half a step an addition (n /
+    64 tiles, 16 in a tile, 3 joins), log2f by a step and the last sum and
+    product by half a step each of the result."""
+    import random
+
+    import torch
+
+    from torobi_b200 import glue
+
+    b, s, h, hk, d, mean, _, causal = case
+    docs = _random_documents(random.Random(s + 2), b, s, mean)
+    first, last = _spans(cuda, docs, None, causal)
+    q, k, v, _ = _inputs(cuda, s + d + 2, b, s, h, hk, d)
+    sc = d ** -0.5
+    _, lse = glue.span_attention_forward(q, k, v, first, last)
+    _, _, want, _, _ = _reference(q, k, v, first, last, sc)
+    kk = k.double().abs().repeat_interleave(h // hk, 2)
+    size = torch.einsum("bihd,bjhd->bhij", q.double().abs(), kk).amax(3) * sc
+    fine = want.isfinite()
+    assert torch.equal(lse[~fine].double(), want[~fine])
+    tol = ((d / 16 + 4) * 2.0 ** -23 * size + 2.0 ** -22 + (s / 64 + 19) * 2.0 ** -24
+           + 4 * 2.0 ** -24 * (want.abs() + size))
+    off = ((lse.double() - want).abs() - tol)[fine]
+    assert off.numel() == 0 or off.max().item() <= 0, off.max().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_causal_document_is_causal_attention_everywhere(cuda, dim):
+    """One document a row against ``attention``, element by element: both err by
+    at most R of their products' sizes and of the value (see above; R has room for
+    the polynomial of attn.cu, 7.5e-5), so they differ by at most twice that."""
+    import torch
+
+    from torobi_b200 import glue
+
+    q, k, v, do = _inputs(cuda, 4, 2, 413, 8, 2, dim)
+    first, last = _spans(cuda, [[0] * 413] * 2)
+    ro, ob, _, g, gb = _reference(q, k, v, first, last, dim ** -0.5, do)
+    a = [t.clone().requires_grad_() for t in (q, k, v)]
+    c = [t.clone().requires_grad_() for t in (q, k, v)]
+    x, y = glue.span_attention(*a, first, last), glue.attention(*c, True)
+    want = (ro, g["dq"], g["dk"], g["dv"])
+    size = (ob, gb["dq"], gb["dk"], gb["dv"])
+    for n, (s, t) in enumerate(zip((x, *torch.autograd.grad(x, a, do)),
+                                   (y, *torch.autograd.grad(y, c, do)))):
+        # 1e-4: dq and dk of the first position, where zero is what is left.
+        assert ((s - t).double().abs()
+                <= 2 * R * (size[n] + want[n].abs()) + (1e-4 if n in (1, 2) else 0)).all(), n
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(cuda):
+    """Forward and backward on two streams side by side, of different shapes,
+    beside one another for a while: the bits of each alone."""
+    import torch
+
+    from torobi_b200 import device_status, glue
+
+    work = []
+    for n, (b, s, h, hk, d) in enumerate([(2, 1300, 8, 2, 128), (3, 900, 14, 2, 64)]):
+        docs = torch.arange(s, device=cuda).expand(b, s) // (170 + 60 * n)
+        work.append((*_inputs(cuda, 60 + n, b, s, h, hk, d), docs.contiguous()))
+
+    def run(q, k, v, do, docs):
+        first, last = glue.document_spans(docs)
+        o, lse = glue.span_attention_forward(q, k, v, first, last)
+        return o, lse, *glue.span_attention_backward(q, k, v, first, last, o, do, lse)
+
+    want = [run(*w) for w in work]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = ([], [])
+    for _ in range(15):
+        for n in (0, 1):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(run(*work[n]))
+    torch.cuda.synchronize()
+    for n in (0, 1):
+        for out in got[n]:
+            assert all(torch.equal(a, c) for a, c in zip(out, want[n]))
     assert device_status() == 0
 
 
