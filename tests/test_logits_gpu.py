@@ -425,6 +425,36 @@ def test_gradient_with_another_pitch(cuda, dtype):
     assert torch.equal(*outs)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [1, 1000, 1003, 1024])
+def test_gradient_of_a_slice_takes_its_own_room(cuda, vocab, dtype):
+    """The last positions of [batch, seq, vocab] logits, rows of a pitch of seq *
+    vocab: the gradient holds the rows read and at most a chunk of 32 bytes more
+    a row, not the whole tensor's room, and is right."""
+    import torch
+
+    from torobi_b200 import glue
+
+    batch, seq = 5, 67
+    full = _logits(cuda, batch * seq, vocab, dtype, 33).contiguous().view(batch, seq, vocab)
+    z = full[:, -1]
+    assert z.stride(0) == seq * vocab
+    tokens = _tokens(cuda, batch, vocab, 33)
+    ids, t = _teacher(cuda, batch, vocab, min(3, vocab), 33, torch.int64, "f32")
+    g, h = torch.randn(batch, device=cuda), torch.randn(batch, device=cuda)
+    leaf = z.detach().requires_grad_()
+    r = glue.token_logprobs(leaf, tokens)
+    kl, ce = glue.distillation(leaf, ids, t, targets=tokens, temperature=1.5)
+    a, = torch.autograd.grad((r.logprobs, r.entropy), leaf, (g, h))
+    b, = torch.autograd.grad((kl, ce), leaf, (g, h))
+    *_, want, size, reach = _distill_reference(z, ids, t, tokens, 1.5, g, h)
+    _check_gradient(a, *_logprob_grad(z, tokens, 1.0, g, h), dtype)
+    _check_gradient(b, want, 2 * size, reach, dtype)
+    for dz in (a, b):
+        assert dz.shape == z.shape
+        assert dz.untyped_storage().nbytes() <= batch * (vocab * z.element_size() + 32)
+
+
 def test_rows_without_upstream_gradient(cuda):
     """A padding position (no gradient reaches it) gets zeros even where its
     logits are NaN."""

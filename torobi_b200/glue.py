@@ -484,12 +484,17 @@ def _logit_rows(op: str, z: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
     return z, rows, vocab, max(pitch, vocab)
 
 
-def _gradient_like(z: torch.Tensor, rows: int, vocab: int, pitch: int) -> torch.Tensor:
-    """Room for a gradient of logits, with their rows' pitch."""
-    if pitch == vocab:
-        return torch.empty_like(z, memory_format=torch.contiguous_format)
-    wide = torch.empty(rows, pitch, dtype=z.dtype, device=z.device)
-    return wide.view(*z.shape[:-1], pitch)[..., :vocab]
+def _gradient_like(z: torch.Tensor, rows: int, vocab: int,
+                   pitch: int) -> tuple[torch.Tensor, int]:
+    """Room for a gradient of logits, and its rows' pitch: the least that moves
+    on in the 32-byte chunks of memory as the logits' does (the kernels then read
+    and write whole chunks; a slice of a larger tensor has a pitch far above its
+    rows)."""
+    least = vocab + (pitch - vocab) % (32 // z.element_size())
+    if least == vocab:
+        return torch.empty_like(z, memory_format=torch.contiguous_format), vocab
+    wide = torch.empty(rows, least, dtype=z.dtype, device=z.device)
+    return wide.view(*z.shape[:-1], least)[..., :vocab], least
 
 
 def _positions(op: str, name: str, t: torch.Tensor, z: torch.Tensor) -> torch.Tensor:
@@ -563,23 +568,23 @@ class _TokenLogprobs(torch.autograd.Function):
     def backward(ctx, dlogprobs, dentropy, _top, _ids):
         _once("token_logprobs")
         z, tokens, stats = ctx.saved_tensors
-        dz = _gradient_room(ctx, "token_logprobs", z)
+        dz, ld_out = _gradient_room(ctx, "token_logprobs", z)
         rows, vocab, pitch = ctx.shape
         dlogprobs, dentropy = _upstream(dlogprobs), _upstream(dentropy)
         _on(z.device, "token_logprobs", lambda stream: lib().tq_token_logprobs_bwd(
             _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), _ptr(stats), rows, vocab, pitch,
-            ctx.temperature, _ptr(dlogprobs), _ptr(dentropy), _ptr(dz), pitch, stream))
+            ctx.temperature, _ptr(dlogprobs), _ptr(dentropy), _ptr(dz), ld_out, stream))
         return dz, None, None, None, None
 
 
-def _gradient_room(ctx, op: str, z: torch.Tensor) -> torch.Tensor:
+def _gradient_room(ctx, op: str, z: torch.Tensor) -> tuple[torch.Tensor, int]:
     if not ctx.inplace:
         return _gradient_like(z, *ctx.shape)
     if ctx.spent:
         raise RuntimeError(f"[{op}] inplace=True wrote the gradient over the logits: this graph "
                            "cannot be run backward twice")
     ctx.spent = True
-    return z
+    return z, ctx.shape[2]
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
@@ -641,13 +646,13 @@ class _Distillation(torch.autograd.Function):
     def backward(ctx, dkl, dce=None):
         _once("distillation")
         z, ids, logits, targets, stats = ctx.saved_tensors
-        dz = _gradient_room(ctx, "distillation", z)
+        dz, ld_out = _gradient_room(ctx, "distillation", z)
         rows, vocab, pitch = ctx.shape
         dkl, dce = _upstream(dkl), _upstream(dce)
         _on(z.device, "distillation", lambda stream: lib().tq_distill_bwd(
             _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
             _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), _ptr(stats), rows,
-            vocab, pitch, ctx.temperature, _ptr(dkl), _ptr(dce), _ptr(dz), pitch, stream))
+            vocab, pitch, ctx.temperature, _ptr(dkl), _ptr(dce), _ptr(dz), ld_out, stream))
         return dz, None, None, None, None, None
 
 
