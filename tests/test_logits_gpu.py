@@ -451,8 +451,55 @@ def test_gradient_of_a_slice_takes_its_own_room(cuda, vocab, dtype):
     _check_gradient(a, *_logprob_grad(z, tokens, 1.0, g, h), dtype)
     _check_gradient(b, want, 2 * size, reach, dtype)
     for dz in (a, b):
-        assert dz.shape == z.shape
-        assert dz.untyped_storage().nbytes() <= batch * (vocab * z.element_size() + 32)
+        taken, row = dz.untyped_storage().nbytes(), vocab * z.element_size()
+        assert dz.shape == z.shape and taken <= batch * (row + 32)
+
+
+@pytest.mark.parametrize("writer", ["token_logprobs", "distillation", "cross_entropy"])
+def test_logits_written_over_are_refused_to_other_backward_passes(cuda, writer):
+    """inplace=True with another op of the same logits: where the writer's
+    backward pass comes first, the other's raises instead of reading a gradient
+    for logits; where it comes last, the sum is the sum of both gradients."""
+    import torch
+
+    from torobi_b200 import glue
+
+    base = _logits(cuda, 9, 500, "bf16", 34).contiguous()
+    tokens = _tokens(cuda, 9, 500, 34).clamp(0, 499)
+    ids, t = _teacher(cuda, 9, 500, 4, 34, torch.int64, "f32")
+    calls = {
+        "token_logprobs": lambda z, w: glue.token_logprobs(z, tokens, inplace=w).logprobs.sum(),
+        "distillation": lambda z, w: glue.distillation(z, ids, t, inplace=w).sum(),
+        "cross_entropy": lambda z, w: glue.cross_entropy(z, tokens, inplace=w).sum(),
+        "torch": lambda z, w: (z.float() * z).sum(),
+    }
+
+    def logits():
+        leaf = base.clone().requires_grad_()
+        return leaf, leaf * 1.0  # not a leaf, and nothing that its own backward reads
+
+    for other in calls:
+        if other == writer:
+            continue
+        # The later op's backward pass runs first.
+        leaf, z = logits()
+        loss = calls[other](z, False) + calls[writer](z, True)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        leaf, z = logits()
+        (calls[writer](z, True) + calls[other](z, False)).backward()
+        apart = []
+        for name in (other, writer):
+            l2, z2 = logits()
+            calls[name](z2, False).backward()
+            apart.append(l2.grad)
+        # bf16 gradients, added in bf16 by autograd.
+        assert torch.equal(leaf.grad, apart[0] + apart[1])
+    leaf, z = logits()
+    loss = calls[writer](z, True)
+    loss.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="backward twice"):
+        loss.backward()
 
 
 def test_rows_without_upstream_gradient(cuda):

@@ -16,6 +16,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .ops import _launch, _need_cuda, _ptr, _stream
 from ._lib import TQ_DTYPE_BF16, TQ_DTYPE_F32, check, lib
@@ -379,6 +380,16 @@ def swiglu(g: torch.Tensor, u: torch.Tensor) -> torch.Tensor:
     return _SwiGLU.apply(g, u)
 
 
+def _spend(ctx, op: str) -> None:
+    """Ahead of a backward pass that writes over the logits it reads: once only.
+    After it the logits' version moves on (``increment_version``), so that
+    autograd refuses them to every other backward pass that needs them."""
+    if ctx.inplace and ctx.spent:
+        raise RuntimeError(f"[{op}] inplace=True wrote the gradient over the logits: this graph "
+                           "cannot be run backward twice")
+    ctx.spent = True
+
+
 class _CrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, targets, inplace):
@@ -395,10 +406,12 @@ class _CrossEntropy(torch.autograd.Function):
             _ptr(z), _ptr(t), rows, vocab, vocab, _ptr(lse), _ptr(loss), _stream()))
         ctx.save_for_backward(z, t, lse)
         ctx.inplace = inplace
+        ctx.spent = False
         return loss.view(z.shape[:-1])
 
     @staticmethod
     def backward(ctx, dloss):
+        _spend(ctx, "cross_entropy")
         z, t, lse = ctx.saved_tensors
         vocab = z.shape[-1]
         rows = z.numel() // vocab
@@ -406,6 +419,8 @@ class _CrossEntropy(torch.autograd.Function):
         dz = z if ctx.inplace else torch.empty_like(z)
         _launch("cross_entropy", lambda: lib().tq_cross_entropy_bwd(
             _ptr(z), _ptr(t), _ptr(lse), rows, vocab, vocab, _ptr(dl), 1.0, _ptr(dz), _stream()))
+        if ctx.inplace:
+            increment_version(z)
         return dz, None, None
 
 
@@ -414,7 +429,8 @@ def cross_entropy(logits: torch.Tensor, targets: torch.Tensor,
     """Per-position ``logsumexp(logits) - logits[target]`` in f32 (no
     reduction, as the reference's loss node), logits bf16 [..., vocab].
     ``inplace=True`` writes the gradient over the logits in backward (no
-    second [rows, vocab] buffer); the graph then cannot be run backward twice."""
+    second [rows, vocab] buffer); the graph then cannot be run backward twice,
+    nor another op of the same logits after it (autograd raises)."""
     return _CrossEntropy.apply(logits, targets, inplace)
 
 
@@ -567,24 +583,17 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dlogprobs, dentropy, _top, _ids):
         _once("token_logprobs")
+        _spend(ctx, "token_logprobs")
         z, tokens, stats = ctx.saved_tensors
-        dz, ld_out = _gradient_room(ctx, "token_logprobs", z)
         rows, vocab, pitch = ctx.shape
+        dz, ld_out = (z, pitch) if ctx.inplace else _gradient_like(z, *ctx.shape)
         dlogprobs, dentropy = _upstream(dlogprobs), _upstream(dentropy)
         _on(z.device, "token_logprobs", lambda stream: lib().tq_token_logprobs_bwd(
             _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(tokens), _ptr(stats), rows, vocab, pitch,
             ctx.temperature, _ptr(dlogprobs), _ptr(dentropy), _ptr(dz), ld_out, stream))
+        if ctx.inplace:
+            increment_version(z)
         return dz, None, None, None, None
-
-
-def _gradient_room(ctx, op: str, z: torch.Tensor) -> tuple[torch.Tensor, int]:
-    if not ctx.inplace:
-        return _gradient_like(z, *ctx.shape)
-    if ctx.spent:
-        raise RuntimeError(f"[{op}] inplace=True wrote the gradient over the logits: this graph "
-                           "cannot be run backward twice")
-    ctx.spent = True
-    return z, ctx.shape[2]
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
@@ -645,14 +654,17 @@ class _Distillation(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dkl, dce=None):
         _once("distillation")
+        _spend(ctx, "distillation")
         z, ids, logits, targets, stats = ctx.saved_tensors
-        dz, ld_out = _gradient_room(ctx, "distillation", z)
         rows, vocab, pitch = ctx.shape
+        dz, ld_out = (z, pitch) if ctx.inplace else _gradient_like(z, *ctx.shape)
         dkl, dce = _upstream(dkl), _upstream(dce)
         _on(z.device, "distillation", lambda stream: lib().tq_distill_bwd(
             _ptr(z), _LOGIT_DTYPES[z.dtype], _ptr(ids), 8 * ids.element_size(), _ptr(logits),
             _LOGIT_DTYPES[logits.dtype], ids.shape[-1], _ptr(targets), _ptr(stats), rows,
             vocab, pitch, ctx.temperature, _ptr(dkl), _ptr(dce), _ptr(dz), ld_out, stream))
+        if ctx.inplace:
+            increment_version(z)
         return dz, None, None, None, None, None
 
 
