@@ -598,6 +598,39 @@ def test_steep_random_scores(cuda, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("jump", [100, 130, 140, 150, 165])
+def test_small_weights_outlive_a_jump(cuda, jump, dim):
+    """A second tile of keys 50 powers of two above the first, a third `jump`
+    above it with values of 0: o is the second's share, 2^(50 - jump) of its
+    values, a normal number although the factor that takes O to the third tile's
+    reference is not one."""
+    import torch
+
+    from torobi_b200 import glue
+
+    b, s, h, hk = 2, 192, 4, 2
+    q, k, v, _ = (t.float() for t in _inputs(cuda, 90 + dim, b, s, h, hk, dim))
+    way = torch.ones(dim, device=cuda)
+    way[::2] = -1.0
+    i = torch.arange(s, device=cuda)
+    step = math.log(2) / dim ** 0.5  # a power of two
+    height = torch.where(i < 64, 0.0, torch.where(i < 128, 50.0, float(jump))) * step
+    q = way.expand_as(q).bfloat16()
+    k = (height[None, :, None, None] * way + 0.0 * k).bfloat16()
+    v = torch.where(i[None, :, None, None] < 128, v, 0.0).bfloat16()
+    last = (i + 1).to(torch.int32).expand(b, s).contiguous()
+    first = torch.zeros_like(last)
+    o, lse = glue.span_attention_forward(q, k, v, first, last)
+    ro, ob, rl, _, _ = _reference(q, k, v, first, last, dim ** -0.5)
+    assert 2.0 ** (45 - jump) < ro[:, 128:].abs().amax() < 2.0 ** (58 - jump)
+    score = (dim / 16 + 4) * 2.0 ** -23 * jump * math.log(2) * 1.01  # as in _check_steep
+    assert ((o.double() - ro).abs() <= (R + 2 * score) * (ob + ro.abs())).all()
+    assert ((lse.double() - rl).abs()
+            <= score + 2.0 ** -20 + 4 * 2.0 ** -24 * (rl.abs() + jump)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(3, 1300, 8, 2, 128), (2, 700, 14, 2, 64)], ids=str)
 def test_rows_that_outgrow_their_reference_repeat(cuda, shape):
     """The same over outputs full of NaN, 20 times: always the same bits."""

@@ -638,12 +638,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         } else {
           // Some row has outgrown its reference (or holds a NaN, and keeps it).
           // The scores are still there: those rows take the tile's maximum for a
-          // new one, the others go through with a factor of 1.
+          // new one, the others go through with a factor of 1.  It is applied as
+          // the square of its root: itself it may be below 2^-126, which is 0
+          // here, where l and O are as much as 2^60 above their first terms.
           const float top = tile_max();
           const bool grow = top > m + kGrowLog2;
-          const float f = grow ? ex2_approx(m - top) : 1.0f;
+          const float f = grow ? ex2_approx(0.5f * (m - top)) : 1.0f;
           if (grow) m = top;
-          l *= f;
+          l = l * f * f;
           if (j > 0) {  // O_w, once its last product is done
             ok = mbar_wait(o_done(w, steps - 1), ((steps - 1) >> 1) & 1, p.status);
             if (!ok) break;
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
               tmem_ld_32x32b_x16(ocol + cc * 16, o);
               tmem_ld_wait(o);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f * f);
               tmem_st_32x32b_x16(ocol + cc * 16, o);
             }
           }
