@@ -758,6 +758,40 @@ def test_one_causal_document_is_causal_attention_everywhere(cuda, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("op", ["span_attention", "attention"])
+def test_operands_and_gradients_off_the_16_byte_boundary(cuda, op):
+    """Views that start at an odd element, and a result joined behind an odd
+    number of elements, whose gradient then is such a view: the bits of the
+    aligned call."""
+    import torch
+
+    from torobi_b200 import glue
+
+    q, k, v, do = _inputs(cuda, 12, 2, 150, 4, 2, 64)
+    first, last = _spans(cuda, [[0] * 150] * 2)
+
+    def call(*t):
+        return glue.span_attention(*t, first, last) if op == "span_attention" else glue.attention(*t)
+
+    def off(t):
+        room = torch.empty(t.numel() + 1, device=cuda, dtype=t.dtype)
+        room[1:] = t.flatten()
+        return room[1:].view_as(t)
+
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    o = call(*leaves)
+    want = [o, *torch.autograd.grad(o, leaves, do)]
+    leaves = [off(t).requires_grad_() for t in (q, k, v)]
+    assert all(t.data_ptr() % 16 for t in leaves)
+    o = call(*leaves)
+    head = torch.ones(3, device=cuda, dtype=torch.bfloat16)
+    joined = torch.cat([head, o.flatten()])
+    up = torch.cat([head, do.flatten()])
+    for a, c in zip([o, *torch.autograd.grad(joined, leaves, up)], want):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(cuda):
     """Forward and backward on two streams side by side, of different shapes,
     beside one another for a while: the bits of each alone."""

@@ -28,6 +28,14 @@ def _bf16_contig(name: str, t: torch.Tensor) -> torch.Tensor:
     return t.contiguous()
 
 
+def _bf16_tile(name: str, t: torch.Tensor) -> torch.Tensor:
+    """For the kernels that copy tiles: contiguous, and on the 16-byte boundary
+    that those copies start on (a view may lie off it: the gradient of a tensor
+    joined behind an odd number of elements)."""
+    t = _bf16_contig(name, t)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _RMSNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, eps):
@@ -142,9 +150,9 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal:
     or 128).  Returns o in q's layout and lse [batch, heads, seq] f32 (the
     natural-log log-sum-exp of each query row's scaled scores)."""
     _need_cuda("attention", q=q, k=k, v=v)
-    q = _bf16_contig("q", q)
-    k = _bf16_contig("k", k)
-    v = _bf16_contig("v", v)
+    q = _bf16_tile("q", q)
+    k = _bf16_tile("k", k)
+    v = _bf16_tile("v", v)
     if q.dim() != 4 or k.shape != v.shape or k.dim() != 4:
         raise ValueError(f"[attention] q {tuple(q.shape)}, k {tuple(k.shape)}, v "
                          f"{tuple(v.shape)}: want [batch, seq, heads, dim] and equal k/v")
@@ -167,8 +175,8 @@ def attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: tor
     """dq, dk, dv of ``attention_forward`` given the upstream gradient do
     (q's layout) and the forward's o and lse."""
     _need_cuda("attention", q=q, k=k, v=v, o=o, do=do, lse=lse)
-    q, k, v, o = (_bf16_contig(n, t) for n, t in (("q", q), ("k", k), ("v", v), ("o", o)))
-    do = _bf16_contig("do", do)
+    q, k, v, o = (_bf16_tile(n, t) for n, t in (("q", q), ("k", k), ("v", v), ("o", o)))
+    do = _bf16_tile("do", do)
     if o.shape != q.shape or do.shape != q.shape:
         raise ValueError("[attention] o and do must have q's shape")
     b, s, h, d = q.shape
@@ -248,7 +256,7 @@ def document_spans(documents: torch.Tensor, prefix: torch.Tensor | None = None,
 
 
 def _span_operands(op: str, q, k, v, first, last):
-    q, k, v = (_bf16_contig(n, t) for n, t in (("q", q), ("k", k), ("v", v)))
+    q, k, v = (_bf16_tile(n, t) for n, t in (("q", q), ("k", k), ("v", v)))
     if q.dim() != 4 or k.shape != v.shape or k.dim() != 4:
         raise ValueError(f"[{op}] q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: "
                          "want [batch, seq, heads, dim] and equal k/v")
@@ -311,7 +319,7 @@ def span_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     op = "span_attention"
     _one_device(op, q=q, k=k, v=v, first=first, last=last, o=o, do=do, lse=lse)
     q, k, v, first, last = _span_operands(op, q, k, v, first, last)
-    o, do = _bf16_contig("o", o), _bf16_contig("do", do)
+    o, do = _bf16_tile("o", o), _bf16_tile("do", do)
     if o.shape != q.shape or do.shape != q.shape:
         raise ValueError(f"[{op}] o and do must have q's shape")
     b, s, h, d = q.shape
@@ -332,7 +340,7 @@ class _SpanAttention(torch.autograd.Function):
     def backward(ctx, do):
         _once("span_attention")
         q, k, v, first, last, o, lse = ctx.saved_tensors
-        do = _bf16_contig("do", do)
+        do = _bf16_tile("do", do)
         return *_span_backward(q, k, v, first, last, o, do, lse, ctx.scale), None, None, None
 
 
