@@ -157,6 +157,38 @@ def test_a_student_distilled_from_a_teachers_alternatives(cuda, graph):
         trainer.step(ids, docs[:1])
 
 
+def test_an_objective_that_weighs_every_target_alike(cuda):
+    """A sum over the micro-batch by the whole step's targets, times the number
+    of micro-batches: the same loss and gradients however the rows are split."""
+    import torch
+
+    from torobi_b200.train import AdamWConfig, Trainer
+
+    ids, docs, _ = _rows(cuda, [[40, 60, 20], [5], [64, 64], [128]], 128)
+    total = ((docs[:, 1:] == docs[:, :-1]) & (docs[:, 1:] >= 0)).sum()
+    seen = []
+    for micro in (1, 2, 4):
+        model = _model(8)
+
+        def objective(rows, documents):
+            lp = model.token_logprobs(rows, documents=documents).logprobs
+            return -lp.sum() * ((4 // micro) / total)
+
+        trainer = Trainer(model, AdamWConfig(lr=1e-3), micro_batch=micro, objective=objective)
+        loss = trainer.step(ids, docs).item()
+        # The trainer's own division by the micro-batches is left to the optimizer.
+        seen.append((loss, model.store.grads.clone() / (4 // micro)))
+    plain = _model(8)
+    with torch.no_grad():
+        lp = plain.token_logprobs(ids, documents=docs).logprobs
+    want = -(lp.double().sum() / total).item()
+    for loss, grads in seen:
+        # f32 sums of 340 log probabilities of size 7.
+        assert abs(loss - want) <= 1e-5 * abs(want)
+        # bf16 gradients of the logits at other scales: a power of two apart.
+        assert ((grads - seen[0][1]).norm() / seen[0][1].norm()).item() <= 2 ** -8
+
+
 def test_a_captured_step_beside_a_score_that_keeps_its_graph(cuda):
     """The teacher's answer is held with its graph while the student's step is
     captured and replayed; the teacher's own backward still runs after."""

@@ -286,7 +286,10 @@ class Trainer:
         ids, a teacher's alternatives), handed to the objective beside the
         micro-batch's ids in this order.  Returns the global mean loss as a
         device tensor: the mean of the micro-batches' losses, each a mean over
-        what counts in it."""
+        what counts in it.  Where packed rows leave a different number of
+        targets in each, a target of a sparse micro-batch weighs more; an
+        objective that sums and divides by the whole step's count, times the
+        micro-batches (of all ranks), weighs every target alike."""
         st = self.store
         for t in more:
             if t.shape[0] != ids.shape[0]:
