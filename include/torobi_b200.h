@@ -373,7 +373,9 @@ int tq_attention_bwd(const void* q, const void* k, const void* v, const void* ou
  * gets o = 0, lse = -inf and no gradient.  Layouts, types and determinism as
  * above; the work of key tiles that no query of a tile sees is not done.
  * What a query does not see still enters products with 0: k, v, and q and
- * dout of queries that see nothing, must be finite.  No counterpart in the
+ * dout of queries that see nothing, must be finite (and values above 1e14 in
+ * size may overflow where scores rise steeply along a row: probabilities are
+ * summed against a reference up to 2^60 below).  No counterpart in the
  * reference (its node takes a causal mode or a mask tensor,
  * engine/src/interp.rs:405-432).
  * workspace: tq_span_attention_bwd_workspace_bytes() bytes, 256-byte aligned.

@@ -257,7 +257,7 @@ __device__ __forceinline__ void st_chunk(void* p, const uint32_t (&w)[8]) {
 // What a row's sums are of, beside s = sum 2^x: nothing, a = sum x 2^x (the
 // entropy's), or a = sum 2^y, y = (z - m) log2(e) (a second temperature, 1);
 // at temperature 2, 2^y is the square of 2^x, which spares the MUFU unit the
-// second exponential (2046 x 128256: 89 us forward, 121 at temperature 3).
+// second exponential (2046 x 128256: 85 us forward, 118 at temperature 3).
 enum Mode { kPlain, kEntropy, kTwo, kSquare };
 
 struct Sums {
@@ -560,8 +560,8 @@ __device__ __forceinline__ void gather(const Row<T>& row, int l0, int l1, uint32
 // candidates than the pool holds are gone through in parts.  It is latency
 // behind the pass over the row -- one barrier to share the maxima, one scan of
 // the keys, one reading of the chunks, one ranking -- and the SM's other three
-// CTAs cover only part of it: 4092 x 151936 takes 185 us without alternatives,
-// 219 with one, 247 with 64, 293 with 128.
+// CTAs cover only part of it: 4092 x 151936 takes 184 us without alternatives,
+// 213 with one, 238 with 64, 267 with 128.
 template <typename T>
 __device__ void slice_top(const Row<T>& row, int c0, int n, int top, ChunkKey<T>* keys, float mine,
                           bool any, uint64_t* pool, TopShared& sh) {
@@ -698,8 +698,9 @@ struct LogprobParams {
 
 // One CTA per row, or a cluster of `split` CTAs when rows are few, each a
 // contiguous slice of the row's chunks; rank 0 joins them in rank order.  Bound
-// by reading the logits: 2046 x 128256 in 87 us, 6.0 TB/s; 777 x 32003 f32, rows
-// of 16 chunks a thread, 22 us, 4.6 TB/s.
+// by reading the logits: 2046 x 128256 in 84 us, 6.2 TB/s, one call behind the
+// other (behind a backward pass, whose last writes leave L2 meanwhile, 97 to 105);
+// 777 x 32003 f32, rows of 16 chunks a thread, 22 us, 4.6 TB/s.
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads, kPerSm) logprobs_fwd_kernel(const LogprobParams p) {
   constexpr int U = kInFlight;
@@ -1030,8 +1031,9 @@ struct DistillParams {
 };
 
 // kTwo, kSquare: the targets' cross-entropy needs the row's sum at temperature
-// 1 too.  Bound by reading the logits: 2046 x 128256 in 88 us with one sum, 89
-// with squares, 121 with both exponentials; 511 x 151936 in 37 us, 4.1 TB/s (511
+// 1 too.  Bound by reading the logits: 2046 x 128256 in 84 us with one sum, 85
+// with squares, 118 with both exponentials, one call behind the other (behind a
+// backward pass 100 to 114 with squares); 511 x 151936 in 37 us, 4.1 TB/s (511
 // CTAs leave a seventh of 592 places empty; in halves they cost as much more).
 template <typename T, Mode M>
 __global__ void __launch_bounds__(kThreads, kPerSm) distill_fwd_kernel(const DistillParams p) {
@@ -1278,6 +1280,11 @@ int parts_for(int64_t rows, int64_t vocab, int ch, int least) {
 // What a CTA of a backward kernel reads before its chunks can be finished is
 // hidden behind about so many of them: a few numbers, or the alternatives and
 // their softmax (four CTAs a row of 2046 x 128256 170 us, one 188, eight 189).
+// What the two give elsewhere, with one, two, four and eight CTAs a row and by
+// the rule, us: log probabilities 47, 47, 45, 57 and 45 at 2046 x 32000, 92, 88,
+// 86, 83 and 86 at 2046 x 65536, 207, 203, 196, 191 and 191 at 2046 x 151936, 90,
+// 88, 86, 84 and 86 at 2046 x 32003 f32; distillation 55, 57, 72, 107 and 55, 100,
+// 96, 102, 127 and 96, 219, 209, 201, 219 and 201, and 98, 92, 96, 119 and 92.
 constexpr int kLeastLogprobs = 900;
 constexpr int kLeastDistill = 1800;
 

@@ -57,7 +57,8 @@ constexpr int kBwdReaders = 3 + kBwdWarps;
 // A row's exponentials are taken against the maximum of the first tile that it
 // sees until their sum over a tile passes kMost; then against that tile's
 // maximum.  P, l and O keep their relative precision at any exponent, so only
-// their range counts.
+// their range counts: O is up to kMost, times the key tiles, above the values it
+// sums, which at 2^20 tiles is within f32 for values up to 2^47.
 constexpr float kMost = 1.152921504606846976e18f;  // 2^60
 constexpr float kGrowLog2 = 50.0f;  // below 60 by more than the log of a tile's keys
 
@@ -798,7 +799,10 @@ __device__ __forceinline__ void load_16(const uint16_t* p, bool wide, uint32_t (
 }
 
 // A CTA a 64-row tile: two rows a thread, 16 elements of each.  Bound by
-// reading out and dout (packed rows of 2048: 134 MB in 24 us).
+// reading out and dout (packed rows of 2048: 134 MB in 24 us).  delta is summed
+// in f32 of the stored output, which is rounded to bf16 (delta is off by 2^-8 of
+// sum |dO O| at most, the order of dS's own rounding): an f32 copy of O would cost
+// the forward twice the bytes of its result and this kernel as many again.
 template <int D>
 __global__ void __launch_bounds__(2 * D) span_prep_kernel(const PrepParams p) {
   constexpr int LANES = D / 16;

@@ -353,7 +353,9 @@ def span_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, first: tor
     dim] bf16, dim 64 or 128; first/last int32 [batch, seq]; output in q's
     layout; the scale defaults to dim^-1/2.  A query that sees nothing gets 0
     and passes no gradient.  What a query does not see still enters products
-    with 0, so k and v, and q of queries that see nothing, must be finite."""
+    with 0, so k and v, and q and the upstream gradient of queries that see
+    nothing, must be finite (and v below 1e14 in size: probabilities are summed
+    against a reference up to 2^60 below)."""
     op = "span_attention"
     _one_device(op, q=q, k=k, v=v, first=first, last=last)
     q, k, v, first, last = _span_operands(op, q, k, v, first, last)
@@ -616,9 +618,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     id: ``top_logprobs`` f32 and ``top_ids`` int64 [..., top] (None for none).
 
     Differentiable through logprobs and entropy.  ``inplace=True`` writes the
-    gradient over the logits in backward, as ``cross_entropy`` does.  A -inf
-    logit has probability 0; a position of nothing else has no distribution
-    (log probabilities -inf, entropy 0, gradient 0)."""
+    gradient over the logits in backward, as ``cross_entropy`` does: a backward
+    pass that needs the logits after it raises.  A -inf logit has probability 0;
+    a position of nothing else has no distribution (log probabilities -inf,
+    entropy 0, gradient 0)."""
     op = "token_logprobs"
     _one_device(op, logits=logits, tokens=tokens)
     tokens = _positions(op, "tokens", tokens, logits)
@@ -693,7 +696,9 @@ def distillation(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     ``ce`` is the targets' cross-entropy at temperature 1, 0 where a target is
     outside [0, vocab); both gradients come from one pass.  A loss that mixes
     them is ``(1 - a) * ce + a * temperature**2 * kl``.  ``inplace=True``
-    writes the gradient over the logits in backward."""
+    writes the gradient over the logits in backward, as ``cross_entropy`` does.
+    Where the logits of a position are all -inf, kl and ce are +inf and the
+    gradient is 0."""
     op = "distillation"
     _one_device(op, logits=logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits,
                 targets=targets)
